@@ -774,6 +774,59 @@ int tpw_knn_mask_euclidean(const void *x1, const void *x2, int dtype, int64_t n,
                            const float *aux1, const float *aux2, int64_t count, uint8_t *mask,
                            void *workspace, void *stream);
 
+/* ---- attention ------------------------------------------------------------------------
+ * out[b, h, i, :] = sum_j p_ij value[b, h / group, j, :], p_ij = exp(s_ij) / sum_j exp(s_ij),
+ * s_ij = scale query[b, h, i, :] . key[b, h / group, j, :] (+ mask), over the keys that are left;
+ * group = heads / key_heads.  A row that no key is left to gives zeros.  Left are the keys
+ *   - j < lengths[b] (clamped to 0 .. m; null: m); later keys and values are not read,
+ *   - causal: j - i <= length - n (the last query sees every key),
+ *   - TPW_MASK_KEEP: whose mask byte is not 0; TPW_MASK_ADD_*: whose added value is not -inf.
+ * A key that a mask leaves out has no weight in the row, whatever its score; its value row must be
+ * finite all the same (0 * inf is NaN in the products).
+ * Element strides are of [batch, heads, rows], features dense; the mask's are of [batch, heads,
+ * n, m] (0 where it is broadcast).  key and value (in the backward query and grad_out too) need a
+ * row stride of at least their width and at most 8 MiB.  stats [2, batch, heads, n] (fp32) carries
+ * each row's maximum and sum from the forward (null: not wanted) to the backward and has no other
+ * meaning.  out and stats are read by the backward. */
+#define TPW_MASK_NONE 0
+#define TPW_MASK_KEEP 1     /* bool bytes */
+#define TPW_MASK_ADD_F32 2  /* added to the scaled scores */
+#define TPW_MASK_ADD_BF16 3
+typedef struct tpw_attention_desc {
+    int32_t dtype; /* TPW_F32 or TPW_BF16: query, key, value, out and their gradients */
+    int32_t causal;
+    int32_t mask_type;
+    int32_t reserved;
+    int64_t batch, heads, key_heads, n, m, d, dv; /* 1 <= d, dv <= 256 */
+    double scale;
+    const void *query, *key, *value, *mask;
+    const int64_t *lengths; /* [batch] or null */
+    void *out;
+    float *stats;
+    const void *grad_out; /* backward only, as the following three */
+    void *grad_query, *grad_key, *grad_value;
+    int64_t query_strides[3], key_strides[3], value_strides[3], out_strides[3];
+    int64_t grad_out_strides[3], grad_query_strides[3], grad_key_strides[3], grad_value_strides[3];
+    int64_t mask_strides[4];
+} tpw_attention_desc;
+
+size_t tpw_attention_workspace_size(const tpw_attention_desc *desc);
+int tpw_attention(const tpw_attention_desc *desc, void *workspace, void *stream);
+/* grad_query, grad_key and grad_value (every element is written) for an upstream grad_out. */
+size_t tpw_attention_backward_workspace_size(const tpw_attention_desc *desc);
+int tpw_attention_backward(const tpw_attention_desc *desc, void *workspace, void *stream);
+
+/* ---- rotary positions -----------------------------------------------------------------
+ * Turns the first 2 * pairs features of every row of x [batch, heads, n, d] (float32 or bfloat16)
+ * by the angles t = position * frequencies[pair] (positions [batch, n] int64 with strides in
+ * elements, frequencies [pairs] float64): (u, w) -> scale (u cos t - w sin t, u sin t + w cos t),
+ * t negated where inverse != 0 (the gradient).  A pair is features (2 p, 2 p + 1) where
+ * interleaved != 0, else (p, p + pairs).  The other features are copied.  Angles are reduced to
+ * one turn in 64 bits.  Strides of x and out are of [batch, heads, n], features dense; out may be x. */
+int tpw_rotary(const void *x, int dtype, int64_t batch, int64_t heads, int64_t n, int64_t d, const int64_t *x_strides,
+               const int64_t *positions, const int64_t *position_strides, const double *frequencies, int64_t pairs,
+               int interleaved, int inverse, double scale, void *out, const int64_t *out_strides, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,483 @@
+"""attention and rotary_embedding: forward, gradients, masks, lengths, layouts and refusals, against
+the plain 64-bit forms of tests/_attention.py with bounds derived there."""
+import math
+
+import pytest
+import torch
+
+import torchpairwise as tp
+from tests._attention import reference, rotate
+from tests._util import assert_close, assert_equal, gen, randn
+
+F32, BF16 = torch.float32, torch.bfloat16
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+TINY = 1e-30
+
+
+def rows(b, h, n, d, seed, dtype=F32, rows_first=False):
+    x = torch.randn(b, n, h, d, generator=gen(seed)) if rows_first else torch.randn(b, h, n, d, generator=gen(seed))
+    x = x.to(dtype)
+    return x.transpose(1, 2) if rows_first else x
+
+
+def on(device, *xs):
+    """Copies on the device with the same strides."""
+    out = []
+    for x in xs:
+        if x is None:
+            out.append(None)
+            continue
+        y = torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=device)
+        y.copy_(x)
+        out.append(y)
+    return out
+
+
+def check(device, q, k, v, mask=None, causal=False, scale=None, lengths=None, grad=None, what=""):
+    want = reference(q, k, v, mask, causal, scale, lengths, grad)
+    dq, dk, dv, dm, dl, dg = on(device, q, k, v, None, lengths, grad)
+    dm = None if mask is None else mask.to(device)
+    if grad is not None:
+        for x in (dq, dk, dv):
+            x.requires_grad_()
+    out = tp.attention(dq, dk, dv, dm, causal=causal, scale=scale, lengths=dl)
+    assert out.dtype == q.dtype and out.shape == (*q.shape[:-1], v.shape[-1])
+    assert_close(out, want["out"], rtol=0.0, atol=want["tol_out"] + TINY, what=f"{what} out")
+    if grad is None:
+        return out
+    grads = torch.autograd.grad(out, (dq, dk, dv), dg)
+    for name, g, x in zip(("dq", "dk", "dv"), grads, (q, k, v)):
+        assert g.dtype == x.dtype and g.shape == x.shape
+        assert_close(g, want[name], rtol=0.0, atol=want["tol_" + name] + TINY, what=f"{what} {name}")
+    return out, grads
+
+
+# b, heads, key heads, n, m, d, dv, rows first
+SIZES = [
+    (1, 1, 1, 1, 1, 1, 1, False),
+    (1, 2, 1, 1, 7, 8, 8, False),
+    (2, 3, 3, 5, 33, 50, 50, True),
+    (1, 4, 2, 31, 64, 64, 64, False),
+    (2, 4, 1, 65, 129, 96, 96, True),
+    (1, 2, 2, 128, 128, 128, 128, False),
+    (1, 6, 2, 130, 257, 128, 128, True),
+    (3, 2, 2, 70, 40, 80, 16, False),
+    (1, 2, 1, 100, 75, 33, 200, True),
+    (1, 2, 2, 97, 161, 256, 256, False),
+    (1, 2, 1, 64, 100, 203, 256, True),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_forward_and_gradients(device, dtype, causal, size):
+    b, h, hk, n, m, d, dv, rf = size
+    check(device, rows(b, h, n, d, 1, dtype, rf), rows(b, hk, m, d, 2, dtype, rf), rows(b, hk, m, dv, 3, dtype, rf),
+          causal=causal, grad=rows(b, h, n, dv, 4, dtype, rf))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 90, 128, 256])
+@pytest.mark.parametrize("kind", ["keep", "keep_keys", "bias", "bias_heads", "bias_bf16", "keep_strided"])
+def test_masks(device, dtype, d, kind):
+    b, h, hk, n, m = 2, 4, 2, 45, 91
+    g = gen(7)
+    if kind == "keep":
+        mask = torch.rand(n, m, generator=g) < 0.4
+        mask[3] = False  # a row that nothing is left to
+        mask[40:] = False
+        mask[5] = torch.arange(m) == 17  # one key
+    elif kind == "keep_keys":
+        mask = (torch.rand(b, 1, 1, m, generator=g) < 0.5)
+        mask[1] = False
+    elif kind == "keep_strided":
+        mask = (torch.rand(b, h, m, n, generator=g) < 0.5).mT
+    elif kind == "bias":
+        mask = torch.randn(n, m, generator=g)
+        mask[torch.rand(n, m, generator=g) < 0.3] = -math.inf
+        mask[2] = -math.inf
+        mask[4] = torch.finfo(torch.float32).min  # the lowest value: every key weighs the same
+        mask[6, 1:] = torch.finfo(torch.float32).min
+    elif kind == "bias_heads":
+        mask = torch.randn(h, 1, m, generator=g) * 3
+    else:
+        mask = torch.randn(1, h, n, m + 1, generator=g).to(BF16)[..., 1:]
+    check(device, rows(b, h, n, d, 1, dtype), rows(b, hk, m, d, 2, dtype), rows(b, hk, m, d, 3, dtype), mask,
+          grad=rows(b, h, n, d, 4, dtype), what=kind)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_lengths_and_what_lies_behind_them(device, dtype, causal):
+    """Lengths of 0 and 1, past m and below 0; rows behind them hold NaN and infinities and are not
+    read; their gradients are zeros."""
+    b, h, hk, n, m, d = 6, 2, 1, 9, 150, 64
+    lengths = torch.tensor([0, 1, 64, 149, 999, -5])
+    q, k, v = rows(b, h, n, d, 1, dtype), rows(b, hk, m, d, 2, dtype), rows(b, hk, m, d, 3, dtype)
+    for i, l in enumerate(lengths.clamp(0, m).tolist()):
+        k[i, :, l:] = math.nan
+        v[i, :, l:] = math.inf
+    out, (dq, dk, dv) = check(device, q, k, v, causal=causal, lengths=lengths, grad=rows(b, h, n, d, 4, dtype))
+    for i in (0, 5):
+        for x in (out, dq, dk, dv):
+            assert not x[i].any()
+    assert not dk[1, :, 1:].any() and not dv[2, :, 64:].any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("additive", [False, True])
+def test_keys_that_a_mask_leaves_out_may_score_nan(device, dtype, additive):
+    b, h, n, m, d = 1, 2, 40, 70, 64
+    q, k, v = rows(b, h, n, d, 1, dtype), rows(b, h, m, d, 2, dtype), rows(b, h, m, d, 3, dtype)
+    off = torch.zeros(m, dtype=torch.bool)
+    off[[0, 33, 69]] = True
+    mask = torch.where(off, -math.inf, 0.0).expand(n, m) if additive else ~off.expand(n, m)
+    want = reference(q, k, v, mask)
+    k = k.clone()
+    k[:, :, 0] = math.nan
+    k[:, :, 33] = math.inf
+    k[:, :, 69] = -math.inf
+    out = tp.attention(*on(device, q, k, v), mask.to(device))
+    assert_close(out, want["out"], rtol=0.0, atol=want["tol_out"])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_nan_and_infinite_scores_stay_in_their_row(device):
+    q, k, v = rows(1, 1, 40, 64, 1), rows(1, 1, 70, 64, 2), rows(1, 1, 70, 64, 3)
+    want = reference(q, k, v)
+    q[0, 0, 3, 5] = math.nan
+    out = tp.attention(*on(device, q, k, v)).cpu()
+    assert out[0, 0, 3].isnan().all()
+    others = torch.arange(40) != 3
+    assert_close(out[:, :, others], want["out"][:, :, others], rtol=0.0, atol=want["tol_out"][:, :, others])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 3.0])
+def test_scales(device, dtype, scale):
+    check(device, rows(1, 2, 33, 40, 1, dtype), rows(1, 2, 65, 40, 2, dtype), rows(1, 2, 65, 40, 3, dtype), scale=scale,
+          grad=rows(1, 2, 33, 40, 4, dtype))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strides_and_alignment(device, dtype):
+    """Sliced features (rows not dense), a column offset that breaks 16-byte alignment, transposed
+    features, rows a stride apart, broadcast batch and heads, an expanded gradient."""
+    b, h, n, m, d = 2, 4, 37, 83, 64
+    base = rows(b, h, m, 3 * d + 5, 1, dtype)
+    q = rows(b, h, n, d + 3, 2, dtype)[..., 3:]
+    grad = rows(b, h, n, d, 4, dtype)
+    k, v = base[..., 1:1 + d], base[..., 1 + d:1 + 2 * d]
+    check(device, q, k, v, grad=grad, what="offset")
+    check(device, rows(b, h, 2 * n, d, 2, dtype)[:, :, ::2], rows(b, h, d, m, 5, dtype).mT, base[..., ::3][..., :d],
+          grad=grad, what="strided")
+    one = rows(1, 1, m, d, 6, dtype)
+    kk = one.expand(b, h, m, d)
+    want = reference(q, kk, kk, grad=grad)
+    dq, dk, dg = on(device, q, one, grad)
+    dk.requires_grad_()
+    x = dk.expand(b, h, m, d)
+    out = tp.attention(dq, x, x)
+    assert_close(out, want["out"], rtol=0.0, atol=want["tol_out"], what="broadcast")
+    (got,) = torch.autograd.grad(out, dk, dg)
+    tol = (want["tol_dk"] + want["tol_dv"]).sum((0, 1), keepdim=True)
+    both = want["dk"] + want["dv"]
+    # autograd adds the two and sums over b and h in the data type
+    steps = b * h + 2
+    tol = tol + steps * torch.finfo(dtype).eps / 2 * both.abs().sum((0, 1), keepdim=True)
+    assert_close(got, both.sum((0, 1), keepdim=True), rtol=0.0, atol=tol, what="broadcast gradient")
+    ones = torch.ones(1, dtype=dtype).expand(b, h, n, d)
+    want = reference(q, k, v, grad=ones)
+    leaves = [x.detach().requires_grad_() for x in on(device, q, k, v)]
+    got = torch.autograd.grad(tp.attention(*leaves), leaves, torch.ones(1, dtype=dtype, device=device).expand(b, h, n, d))
+    for name, x in zip(("dq", "dk", "dv"), got):
+        assert_close(x, want[name], rtol=0.0, atol=want["tol_" + name] + TINY, what=f"expanded gradient {name}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_two_and_three_dimensions(device):
+    q, k, v = randn(2, 30, 48, seed=1), randn(2, 50, 48, seed=2), randn(2, 50, 20, seed=3)
+    mask = torch.rand(2, 30, 50, generator=gen(4)) < 0.7
+    full = tp.attention(q[:, None], k[:, None], v[:, None], mask[:, None])[:, 0]
+    for x, got in ((full, tp.attention(*on(device, q, k, v), mask.to(device))),
+                   (full[0], tp.attention(*on(device, q[0], k[0], v[0]), mask[0].to(device)))):
+        assert got.shape == x.shape
+        assert_close(got, x, rtol=1e-4, atol=1e-5)
+    shape = tp.attention(*on(device, rows(2, 4, 9, 16, 1, F32, True), rows(2, 2, 9, 16, 2), rows(2, 2, 9, 8, 3)))
+    assert shape.transpose(1, 2).is_contiguous()  # rows before heads, as the queries have them
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_empty_sizes(device):
+    for b, h, n, m in ((0, 2, 3, 4), (2, 0, 3, 4), (2, 2, 0, 4), (2, 2, 3, 0)):
+        q = torch.zeros(b, h, n, 8, device=device, requires_grad=True)
+        k = torch.ones(b, 2, m, 8, device=device, requires_grad=True)
+        v = torch.ones(b, 2, m, 5, device=device, requires_grad=True)
+        out = tp.attention(q, k, v)
+        assert out.shape == (b, h, n, 5) and not out.any()
+        for g, x in zip(torch.autograd.grad(out.sum(), (q, k, v)), (q, k, v)):
+            assert g.shape == x.shape and not g.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    q, k, v = (x.to(device) for x in (randn(2, 4, 5, 8, seed=1), randn(2, 2, 6, 8, seed=2), randn(2, 2, 6, 3, seed=3)))
+    at = tp.attention
+
+    def refuses(message, *args, **kw):
+        with pytest.raises(RuntimeError, match=message):
+            at(*args, **kw)
+
+    refuses("2-D, 3-D or 4-D", q[0, 0, 0], k, v)
+    refuses("same number of dimensions", q, k[0], v[0])
+    refuses("dtypes differ", q, k.to(BF16), v)
+    refuses("supports float32 and bfloat16", q.half(), k.half(), v.half())
+    refuses("batch_size", q[:1], k, v)
+    refuses("feature dimension", q[..., :7], k, v)
+    refuses("keys and values", q, k[:, :, :5], v)
+    refuses("heads of key and value", q, k, v[:, :1])
+    refuses("multiple of the number of key heads", q[:, :3], k, v)
+    refuses("1 to 256 features", torch.zeros(1, 1, 2, 257, device=device), torch.zeros(1, 1, 2, 257, device=device),
+            torch.zeros(1, 1, 2, 8, device=device))
+    refuses("does not broadcast", q, k, v, torch.ones(4, 6, dtype=torch.bool, device=device))
+    refuses("mask must be bool", q, k, v, torch.ones(5, 6, dtype=torch.int32, device=device))
+    refuses("mask has no gradient", q, k, v, torch.zeros(5, 6, device=device, requires_grad=True))
+    refuses("lengths must have shape", q, k, v, lengths=torch.tensor([1], device=device))
+    refuses("lengths must be int64", q, k, v, lengths=torch.tensor([1.0, 2.0], device=device))
+    refuses("scale must be finite", q, k, v, scale=math.inf)
+    leaf = q.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(at(leaf, k, v).sum(), leaf, create_graph=True)
+    x, pos, f = q, torch.arange(5, device=device), torch.ones(4, dtype=torch.float64, device=device)
+    for message, args in (("2-D, 3-D or 4-D", (x[0, 0, 0], pos, f)), ("positions must have", (x, pos[:4], f)),
+                          ("positions must be int64", (x, pos.float(), f)), ("do not fit", (x, pos, f.repeat(2))),
+                          ("frequencies must be", (x, pos, f.long())), ("supports float32", (x.half(), pos, f))):
+        with pytest.raises(RuntimeError, match=message):
+            tp.rotary_embedding(*args)
+    with pytest.raises(RuntimeError, match="scale must be finite"):
+        tp.rotary_embedding(x, pos, f, scale=math.nan)
+    with pytest.raises(RuntimeError, match="frequencies have no gradient"):
+        tp.rotary_embedding(x, pos, f.clone().requires_grad_())
+
+
+def test_gradients_against_differences():
+    g = gen(3)
+    q, k, v = (torch.randn(*s, generator=g, dtype=torch.float64, requires_grad=True)
+               for s in ((2, 4, 6, 5), (2, 2, 9, 5), (2, 2, 9, 3)))
+    mask = torch.rand(6, 9, generator=g) < 0.6
+    mask[2] = False
+    bias = torch.randn(2, 1, 6, 9, generator=g, dtype=torch.float64)
+    for kw in ({}, {"causal": True, "scale": -0.7}, {"mask": mask}, {"mask": bias, "lengths": torch.tensor([9, 4])}):
+        assert torch.autograd.gradcheck(lambda *x: tp.attention(*x, **kw), (q, k, v)), kw
+    f, s = tp.rotary_frequencies(4, scaling="parts", factor=4.0, original_length=100)
+    for inter in (False, True):
+        assert torch.autograd.gradcheck(
+            lambda x: tp.rotary_embedding(x, torch.arange(6) * 11, f, interleaved=inter, scale=s), (q,))
+
+
+# ---------------------------------------------------------------- single tokens, long rows of keys
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,h,hk,m,d,dv", [(1, 1, 1, 5000, 64, 64), (1, 16, 2, 4097, 128, 128), (1, 8, 1, 3001, 256, 256),
+                                          (4, 8, 2, 2050, 96, 128), (3, 40, 1, 1030, 128, 64), (1, 3, 3, 700, 50, 50),
+                                          (2, 16, 1, 9000, 128, 128)])
+def test_few_rows_over_many_keys(dtype, n, h, hk, m, d, dv):
+    lengths = torch.tensor([m, m // 3, 1])
+    check("cuda", rows(3, h, n, d, 1, dtype), rows(3, hk, m, d, 2, dtype, True), rows(3, hk, m, dv, 3, dtype),
+          causal=n > 1, lengths=lengths, grad=rows(3, h, n, dv, 4, dtype) if m < 3000 else None)
+    g = torch.rand(3, h, n, m, generator=gen(5)) < 0.3
+    check("cuda", rows(3, h, n, d, 1, dtype), rows(3, hk, m, d, 2, dtype), rows(3, hk, m, dv, 3, dtype), g, lengths=lengths)
+    bias = torch.randn(h, 1, m, generator=gen(6))
+    bias[:, :, ::5] = -math.inf
+    check("cuda", rows(3, h, n, d, 1, dtype), rows(3, hk, m, d, 2, dtype), rows(3, hk, m, dv, 3, dtype), bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_longer_sequences(dtype, causal, d):
+    b, h, hk, n = 1, 4, 2, 700
+    check("cuda", rows(b, h, n, d, 1, dtype), rows(b, hk, n, d, 2, dtype), rows(b, hk, n, d, 3, dtype), causal=causal,
+          grad=rows(b, h, n, d, 4, dtype))
+
+
+@pytest.mark.gpu
+def test_chunk_over_a_cache_equals_the_whole():
+    """Queries in chunks over a growing cache with lengths give the rows of one causal call."""
+    h, hk, n, d = 4, 2, 300, 64
+    q, k, v = on("cuda", rows(1, h, n, d, 1, BF16), rows(1, hk, n, d, 2, BF16), rows(1, hk, n, d, 3, BF16))
+    whole = tp.attention(q, k, v, causal=True).float().cpu()
+    got = [tp.attention(q[:, :, a:b], k, v, causal=True, lengths=torch.tensor([b], device="cuda"))
+           for a, b in ((0, 1), (1, 130), (130, 131), (131, 300))]
+    bound = reference(*(x.cpu() for x in (q, k, v)), causal=True)["tol_out"]
+    assert_close(torch.cat(got, 2), whole, rtol=0.0, atol=2 * bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_repeats_and_other_streams(dtype):
+    """The same call gives the same bits, on another stream too."""
+    args = on("cuda", rows(2, 8, 200, 128, 1, dtype), rows(2, 2, 333, 128, 2, dtype), rows(2, 2, 333, 128, 3, dtype))
+    grad = rows(2, 8, 200, 128, 4, dtype).cuda()
+    leaves = [x.requires_grad_() for x in args]
+
+    def call():
+        out = tp.attention(*leaves, causal=True)
+        return out, *torch.autograd.grad(out, leaves, grad)
+
+    first = call()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(2):
+        with torch.cuda.stream(side):
+            again = call()
+        side.synchronize()
+        for a, b in zip(first, again):
+            assert_equal(a, b)
+
+
+@pytest.mark.gpu
+def test_replays_of_a_graph():
+    q, k, v = on("cuda", rows(2, 8, 1, 128, 1, BF16), rows(2, 2, 1500, 128, 2, BF16), rows(2, 2, 1500, 128, 3, BF16))
+    lengths = torch.tensor([700, 1500], device="cuda")
+    f, _ = tp.rotary_frequencies(128, device="cuda")
+    pos = torch.tensor([[699], [1499]], device="cuda")
+
+    def call():
+        return tp.attention(tp.rotary_embedding(q, pos, f), k, v, lengths=lengths)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        q.add_(0.25)
+        lengths[0] = 100 * i
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_equal(out, call(), f"replay {i}")
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Keys and values whose rows lie 6 GiB apart in all, in one head."""
+    m, d, stride = 800, 64, 1 << 22  # 8 MiB between rows
+    k, v = rows(1, 1, m, d, 2, BF16), rows(1, 1, m, d, 3, BF16)
+    buf = torch.zeros(m * stride, dtype=BF16, device="cuda")
+    view = buf.view(1, 1, m, stride)
+    view[..., :d] = k.cuda()
+    view[..., d:2 * d] = v.cuda()
+    for n in (1, 70):
+        q, grad = rows(1, 1, n, d, 1, BF16), rows(1, 1, n, d, 4, BF16)
+        want = reference(q, k, v, grad=grad)
+        dq = q.cuda().requires_grad_()
+        out = tp.attention(dq, view[..., :d], view[..., d:2 * d])
+        assert_close(out, want["out"], rtol=0.0, atol=want["tol_out"])
+        (g,) = torch.autograd.grad(out, dq, grad.cuda())
+        assert_close(g, want["dq"], rtol=0.0, atol=want["tol_dq"])
+
+
+@pytest.mark.gpu
+def test_neighbour_mask_feeds_attention():
+    """Attention over a neighbour graph of the framework's own masks; isolated points give zeros."""
+    x = randn(300, 32, seed=1).cuda()
+    x[7] += 1000.0
+    mask = tp.radius_neighbors_mask(x, epsilon=6.0)
+    if mask.shape == (300, 300):
+        mask = mask & ~torch.eye(300, dtype=torch.bool, device="cuda")
+    want = reference(*(x.cpu()[None, None],) * 3, mask.cpu(), scale=0.05)
+    out = tp.attention(x, x, x, mask, scale=0.05)
+    assert not out[7].any()
+    assert_close(out, want["out"][0, 0], rtol=0.0, atol=want["tol_out"][0, 0] + TINY)
+
+
+# ---------------------------------------------------------------- rotary
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("b,h,n,d,width,rf", [(1, 1, 1, 2, 2, False), (2, 3, 5, 64, 64, True), (16, 8, 1, 128, 128, False),
+                                             (3, 5, 103, 118, 50, True), (1, 2, 33, 96, 32, False), (2, 2, 7, 9, 6, False),
+                                             (1, 4, 300, 256, 128, True), (2, 2, 4, 20, 0, False)])
+def test_rotary(device, dtype, interleaved, b, h, n, d, width, rf):
+    x, grad = rows(b, h, n, d, 1, dtype, rf), rows(b, h, n, d, 2, dtype, rf)
+    f = 10000.0 ** (-torch.arange(width // 2, dtype=torch.float64) / max(width // 2, 1))
+    pos = torch.randint(0, 1 << 20, (b, n), generator=gen(3))
+    dx, dg = on(device, x, grad)
+    dx.requires_grad_()
+    # cos, sin (2 u each), two products and a sum in fp32, the result's rounding
+    b_round = torch.finfo(dtype).eps / 2
+    for p, scale in ((pos, 1.0), (pos[:1], 1.3), (pos[0], 1.0)):
+        y = tp.rotary_embedding(dx, p.to(device), f.to(device), interleaved=interleaved, scale=scale)
+        assert y.shape == x.shape and y.dtype == dtype
+        want = rotate(x, p, f, interleaved, scale)
+        size = rotate(x.abs(), torch.zeros_like(p), f, interleaved, scale)
+        pair = _partner(x.abs().double(), width, interleaved, scale)
+        assert_close(y, want, rtol=b_round, atol=8 * 2.0 ** -24 * (size + pair), what="rotary")
+        assert_equal(y[..., width:], x[..., width:], "features past the width")
+        (g,) = torch.autograd.grad(y, dx, dg)
+        want = rotate(grad, p, f, interleaved, scale, inverse=True)
+        size = rotate(grad.abs(), torch.zeros_like(p), f, interleaved, scale)
+        pair = _partner(grad.abs().double(), width, interleaved, scale)
+        assert_close(g, want, rtol=b_round, atol=8 * 2.0 ** -24 * (size + pair), what="rotary gradient")
+
+
+def _partner(x, width, interleaved, scale):
+    """Each rotated feature's partner, times scale."""
+    r = x[..., :width]
+    if interleaved:
+        y = r.unflatten(-1, (width // 2, 2)).flip(-1).flatten(-2)
+    else:
+        y = r.roll(width // 2, -1) if width else r
+    return torch.cat([y * scale, torch.zeros_like(x[..., width:])], -1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rotary_strides(device):
+    f = torch.rand(8, dtype=torch.float64, generator=gen(1))
+    base = randn(2, 3, 11, 45, seed=2)
+    pos = torch.arange(22).view(1, 22)[:, ::2]
+    for x in (base[..., 1:33], base[..., 5:37:2], base[:, :, ::2, :17][:, :, :, 1:], base.mT[:, :, :16, :11].mT):
+        want = rotate(x, pos[:, :x.shape[2]], f)
+        got = tp.rotary_embedding(on(device, x)[0], pos.to(device)[:, :x.shape[2]], f.to(device))
+        assert_close(got, want, rtol=2.0 ** -22, atol=2.0 ** -20)
+    y = tp.rotary_embedding(on(device, randn(11, 16, seed=3))[0], pos[0].to(device).int(), f.float().to(device))
+    assert_close(y, rotate(randn(11, 16, seed=3)[None, None], pos, f.float())[0, 0], rtol=2.0 ** -22, atol=2.0 ** -20)
+
+
+def test_rotary_makes_products_depend_on_the_distance():
+    f, _ = tp.rotary_frequencies(32)
+    q, k = randn(1, 32, seed=1).double(), randn(1, 32, seed=2).double()
+    at = [(tp.rotary_embedding(q, torch.tensor([a]), f) @ tp.rotary_embedding(k, torch.tensor([a + 5]), f).T).item()
+          for a in (0, 17, 100000)]
+    assert max(at) - min(at) < 1e-9
+
+
+def test_rotary_frequencies():
+    f, s = tp.rotary_frequencies(8)
+    assert f.dtype == torch.float64 and s == 1.0
+    assert_close(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-14, atol=0.0)
+    lin, s = tp.rotary_frequencies(8, scaling="linear", factor=4.0)
+    assert_close(lin, f / 4, rtol=1e-14, atol=0.0)
+    b, s = tp.rotary_frequencies(8, scaling="base", factor=4.0)
+    assert abs(b[0] - 1) < 1e-14 and abs(b[-1] / f[-1] - 0.25) < 1e-12 and s == 1.0
+    p, s = tp.rotary_frequencies(64, scaling="parts", factor=8.0, original_length=4096)
+    f = tp.rotary_frequencies(64)[0]
+    turns = 4096 * f / (2 * math.pi)
+    assert_close(p[turns > 40], f[turns > 40], rtol=1e-14, atol=0.0)
+    assert_close(p[turns < 0.8], f[turns < 0.8] / 8, rtol=1e-14, atol=0.0)
+    assert ((p <= f) & (p >= f / 8 * (1 - 1e-14))).all() and abs(s - (0.1 * math.log(8.0) + 1)) < 1e-15
+    for bad in ({"width": 7}, {"width": 8, "base": 1.0}, {"width": 8, "scaling": "x"}, {"width": 8, "factor": 2.0},
+                {"width": 8, "scaling": "linear", "factor": 0.5}, {"width": 8, "scaling": "parts", "factor": 2.0},
+                {"width": 8, "scaling": "parts", "factor": 2.0, "original_length": 64, "fast": 1.0}):
+        with pytest.raises(ValueError):
+            tp.rotary_frequencies(**bad)

@@ -25,7 +25,24 @@ FAM_PPMINKOWSKI, FAM_WMINKOWSKI, FAM_CANBERRA, FAM_BRAYCURTIS, FAM_CHI2, FAM_JS 
 
 _i64, _p, _i, _d, _sz = C.c_int64, C.c_void_p, C.c_int, C.c_double, C.c_size_t
 
+
+class AttentionDesc(C.Structure):
+    """``tpw_attention_desc``."""
+    _fields_ = [("dtype", C.c_int32), ("causal", C.c_int32), ("mask_type", C.c_int32), ("reserved", C.c_int32),
+                *[(f, _i64) for f in ("batch", "heads", "key_heads", "n", "m", "d", "dv")], ("scale", _d),
+                *[(f, _p) for f in ("query", "key", "value", "mask", "lengths", "out", "stats", "grad_out",
+                                    "grad_query", "grad_key", "grad_value")],
+                *[(f + "_strides", _i64 * 3) for f in ("query", "key", "value", "out", "grad_out", "grad_query",
+                                                       "grad_key", "grad_value")],
+                ("mask_strides", _i64 * 4)]
+
+
 _SIGNATURES = {
+    "tpw_attention_workspace_size": (_sz, [_p]),
+    "tpw_attention": (_i, [_p, _p, _p]),
+    "tpw_attention_backward_workspace_size": (_sz, [_p]),
+    "tpw_attention_backward": (_i, [_p, _p, _p]),
+    "tpw_rotary": (_i, [_p, _i, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _i, _i, _d, _p, _p, _p]),
     "tpw_last_error": (C.c_char_p, []),
     "tpw_runtime_version": (_i, []),
     "tpw_launch_timer_arm": (_i, [C.c_char_p, _i]),

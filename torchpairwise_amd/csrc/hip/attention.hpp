@@ -1,0 +1,450 @@
+// Shared pieces of the attention kernels (attention.hip, attention_backward.hip).
+//
+//   s_ij = scale q_i . k_j (+ mask_ij),  p_ij = exp(s_ij - m_i) / l_i,  o_i = sum_j p_ij v_j
+//
+// with the row maximum m_i and sum l_i over the keys that the mask, the causal limit and the
+// lengths leave; a row that none is left to gives zeros.  No [n, m] matrix is written.
+//
+// Products run on the matrix cores, transposed so that a lane owns one row: a block of W x W
+// scores is K (first operand, from LDS) times Q (second operand, in registers), and its
+// accumulator holds row c = lane % W, keys 4 NG a + 4 g + e in register 4 a + e, g = lane / W,
+// NG = 64 / W.  Each row's softmax is then a loop over the lane's own registers and one exchange
+// between its NG lanes.  The probabilities are the second operand of the next product as they
+// lie: in a step of KS = 8 NG keys a lane holds quads 2 t and 2 t + 1, and the order of keys
+// within a step is free as long as both operands agree, so V is read in that order (rows
+// 4 NG (2 t + u) + 4 g .. + 3: one transposing LDS read for bf16, four dwords for fp32).
+//
+//   bf16: v_mfma_f32_32x32x16_bf16, W = 32;  fp32: 8 x v_mfma_f32_16x16x4_f32 per step, W = 16.
+#pragma once
+
+#include "tile_mfma.hpp"
+
+namespace tpw {
+namespace attn {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+enum MaskMode { kNoMask = 0, kKeep = 1, kBias = 2 };
+
+// One operand: element strides of [batch, heads, rows, features] (features dense).
+struct View {
+    const void *p;
+    int64_t b, h, n;
+};
+
+struct Args {
+    View q, k, v;
+    View o, go;          // output; upstream gradient (backward)
+    View gq, gk, gv;     // gradients (backward)
+    float *stats;        // [2, b, h, n]: row maxima, row sums
+    float *rows;         // [3, b, h, n] (backward): base and 1 / sum of the softmax, delta
+    const void *mask;    // bool bytes (kKeep) or fp32 / bf16 (kBias)
+    int64_t mb, mh, mn, mm;
+    int mask_bf16, mask_vec;
+    const int64_t *lengths;  // [b] or null
+    int64_t batch, heads, key_heads, group, n, m, d, dv;
+    float scale;   // |scale| * log2(e) (kBias: |scale|), 1 where scale is 0
+    float qsign;   // -1, 0 or 1: the sign of scale, folded into q as it is loaded
+    float gscale;  // scale (backward)
+    int causal;
+    int vec;       // rows of q, k, v (and do, o) are whole 16-byte pieces at 16-byte aligned addresses
+    int vec_out;   // the outputs' rows take stores of four features
+    int64_t tiles;  // row tiles (dk / dv: key tiles) per (batch, key head)
+    int splits;     // parts of the summed axis
+    float *part;    // [splits, ...] partial results where splits > 1
+    float *part_stats;
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int W>
+struct Mma;
+
+// Eight consecutive elements of a lane, as the matrix instructions take them.
+template <typename T>
+struct Frag;
+template <>
+struct Frag<uint16_t> {
+    uint4 v;
+};
+template <>
+struct Frag<float> {
+    f32x4 v[2];
+};
+
+template <int W_>
+struct Shape {
+    static constexpr int W = W_, NG = 64 / W_, KS = 8 * NG, Q = W_ / (4 * NG);  // quads per block
+};
+
+template <>
+struct Mma<uint16_t, 32> : Shape<32> {
+    typedef floatx16 Acc;
+    static __device__ __forceinline__ void mma(Acc &acc, const Frag<uint16_t> &a, const Frag<uint16_t> &b) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v),
+                                                      acc, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<uint16_t, 16> : Shape<16> {
+    typedef f32x4 Acc;
+    static __device__ __forceinline__ void mma(Acc &acc, const Frag<uint16_t> &a, const Frag<uint16_t> &b) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v),
+                                                      acc, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<float, 16> : Shape<16> {
+    typedef f32x4 Acc;
+    // element e of every lane makes one instruction: its four k are elements e of the four groups
+    static __device__ __forceinline__ void mma(Acc &acc, const Frag<float> &a, const Frag<float> &b) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e >> 2][e & 3], b.v[e >> 2][e & 3], acc, 0, 0, 0);
+    }
+};
+
+__device__ __forceinline__ Frag<uint16_t> pack8(const float (&x)[8], uint16_t) {
+    return {make_uint4(f32x2_to_bf16x2_rne(x[0], x[1]), f32x2_to_bf16x2_rne(x[2], x[3]),
+                       f32x2_to_bf16x2_rne(x[4], x[5]), f32x2_to_bf16x2_rne(x[6], x[7]))};
+}
+__device__ __forceinline__ Frag<float> pack8(const float (&x)[8], float) {
+    return {{{x[0], x[1], x[2], x[3]}, {x[4], x[5], x[6], x[7]}}};
+}
+__device__ __forceinline__ void unpack8(const Frag<uint16_t> &f, float (&x)[8]) {
+    const uint32_t w[4] = {f.v.x, f.v.y, f.v.z, f.v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack8(const Frag<float> &f, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f.v[i >> 2][i & 3];
+}
+
+// ---- LDS tiles -----------------------------------------------------------------------------
+// A tile of ROWS rows of DP features lies as 16-byte pieces, piece c of row r at position
+// c ^ swz(r): eight consecutive rows put one piece into eight different 16-byte slots (row
+// fragments), and four consecutive rows put a pair of pieces into four different pairs
+// (transposing reads), so neither read meets a bank twice.
+__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+
+template <typename T, int DP>
+struct Tile {
+    static constexpr int E = 16 / (int)sizeof(T);  // elements per piece
+    static constexpr int C = DP / E;               // pieces per row
+    static constexpr int kRowBytes = DP * (int)sizeof(T);
+};
+
+constexpr uint32_t kRange = 0x7ffffff0u;  // bytes a tile's buffer resource spans at most
+constexpr uint32_t kBeyond = 0xfffffff0u;  // an offset that no range holds: the load gives zeros
+
+// 16 bytes per lane from the resource into LDS at lds_base + 16 * lane, zeros where the offset is
+// past the range.  Inline asm for the reason given at tile::dma16.
+__device__ __forceinline__ void dma16(tpw_u32x4 rsrc, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds_base)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ tpw_u32x4 resource(const void *base, int64_t bytes) {
+    const uint64_t a = (uint64_t)(uintptr_t)base;
+    const uint32_t num = bytes <= 0 ? 0u : bytes > (int64_t)kRange ? kRange : (uint32_t)bytes;
+    return tpw_u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu)),
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)num), 0x00020000u};
+}
+
+// The same address in every lane, in scalar registers.
+__device__ __forceinline__ const void *uniform(const void *p) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+    return reinterpret_cast<const void *>((uintptr_t)((uint64_t)hi << 32 | lo));
+}
+
+// Moves rows [0, ROWS) of a tile into LDS; rows at or past `rows` and features at or past `d`
+// become zeros and are not read.
+template <typename T, int DP, int ROWS, int WAVES>
+struct Stager {
+    using L = Tile<T, DP>;
+    static constexpr int kSlots = ROWS * L::C / (64 * WAVES);
+    static_assert(ROWS * L::C % (64 * WAVES) == 0, "whole instructions");
+    uint32_t off[kSlots];
+    int64_t stride;  // bytes between rows
+    int d, vec, wave, lane;
+
+    __device__ __forceinline__ void init(int64_t row_stride, int d_, int vec_, int wave_, int lane_) {
+        stride = row_stride * (int64_t)sizeof(T);
+        d = d_;
+        vec = vec_;
+        wave = wave_;
+        lane = lane_;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+            const int s = (i * WAVES + wave) * 64 + lane, r = s / L::C, c = (s % L::C) ^ swz(r);
+            off[i] = c * L::E < d ? (uint32_t)(r * stride + c * 16) : kBeyond;
+        }
+    }
+    __device__ __forceinline__ void load(const T *base, int64_t rows, uint32_t lds) const {
+        if (vec) {
+            const tpw_u32x4 r = resource(base, rows * stride);
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) dma16(r, off[i], lds + (uint32_t)((i * WAVES + wave) * 1024));
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < kSlots; ++i) {
+                const int s = (i * WAVES + wave) * 64 + lane, r = s / L::C, c = (s % L::C) ^ swz(r);
+                T x[L::E];
+#pragma unroll
+                for (int e = 0; e < L::E; ++e) {
+                    const int f = c * L::E + e;
+                    x[e] = r < rows && f < d ? base[r * (stride / (int64_t)sizeof(T)) + f] : T(0);
+                }
+                uint4 w;
+                __builtin_memcpy(&w, x, 16);
+                *reinterpret_cast<__attribute__((address_space(3))) tpw_u32x4 *>((uintptr_t)(lds + (uint32_t)s * 16)) =
+                    tpw_u32x4{w.x, w.y, w.z, w.w};
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ tpw_u32x4 lds_read16(uint32_t a) {
+    return *reinterpret_cast<__attribute__((address_space(3))) const tpw_u32x4 *>((uintptr_t)a);
+}
+
+// Row fragment: features KS s + 8 g .. + 7 of row r.
+template <typename T, int DP, int W>
+struct RowReader {
+    using L = Tile<T, DP>;
+    using S = Shape<W>;
+    uint32_t row;
+    int x, g;
+    __device__ __forceinline__ RowReader(int lane) : row((uint32_t)((lane % W) * L::kRowBytes)), x(swz(lane % W)), g(lane / W) {}
+    // block `blk` of W rows; swz(r) depends on r mod 8 only, and W is a multiple of 8
+    __device__ __forceinline__ Frag<T> read(uint32_t tile, int blk, int s) const {
+        const uint32_t base = tile + (uint32_t)(blk * W * L::kRowBytes) + row;
+        Frag<T> f;
+        if constexpr (sizeof(T) == 2) {
+            f.v = __builtin_bit_cast(uint4, lds_read16(base + (uint32_t)(((S::NG * s + g) ^ x) * 16)));
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                f.v[u] = __builtin_bit_cast(f32x4, lds_read16(base + (uint32_t)(((2 * (S::NG * s + g) + u) ^ x) * 16)));
+        }
+        return f;
+    }
+};
+
+// Column fragment (first operand of the second products): feature W b + lane % W of rows
+// 4 NG (2 t + u) + 4 g + e, element 4 u + e.
+template <typename T, int DP, int W>
+struct ColReader {
+    using L = Tile<T, DP>;
+    using S = Shape<W>;
+    int lane, g;
+    __device__ __forceinline__ ColReader(int l) : lane(l), g(l / W) {}
+    __device__ __forceinline__ Frag<T> read(uint32_t tile, int t, int b) const {
+        Frag<T> f;
+        if constexpr (sizeof(T) == 2) {
+            // lane i of a group of 16 points at four features of row i / 4; it receives feature i % 16
+            // of the four rows
+            const int i = lane & 15, r0 = 4 * g + (i >> 2), x = swz(r0);
+            const int col = W * b + 16 * ((lane % W) >> 4) + 4 * (i & 3);
+            uint2 v[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t a = tile + (uint32_t)((4 * S::NG * (2 * t + u) + r0) * L::kRowBytes) +
+                                   (uint32_t)((((col >> 3) ^ x) * 16) + (col & 4) * 2);
+                v[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     (__attribute__((address_space(3))) s16x4 *)(uintptr_t)a));
+            }
+            f.v = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
+        } else {
+            const int col = W * b + lane % W;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r0 = 4 * g + e;
+                    const uint32_t a = tile + (uint32_t)((4 * S::NG * (2 * t + u) + r0) * L::kRowBytes) +
+                                       (uint32_t)((((col >> 2) ^ swz(r0)) * 16) + (col & 3) * 4);
+                    f.v[u][e] = *reinterpret_cast<__attribute__((address_space(3))) const float *>((uintptr_t)a);
+                }
+        }
+        return f;
+    }
+};
+// (4 NG (2 t + u) is a multiple of 8, so swz of the whole row index is swz(r0).)
+
+// Features KS s + 8 g .. + 7 of a row in global memory (null: zeros).
+template <typename T>
+__device__ __forceinline__ Frag<T> load_row8(const T *row, int f, int d, int vec) {
+    T x[8];
+    if (vec) {
+        // d is whole 16-byte pieces
+        constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int u = 0; u < 8 / E; ++u) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (row && f + u * E < d) w = *reinterpret_cast<const uint4 *>(row + f + u * E);
+            __builtin_memcpy(x + u * E, &w, 16);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = row && f + e < d ? row[f + e] : T(0);
+    }
+    Frag<T> r;
+    __builtin_memcpy(&r, x, sizeof(r));
+    return r;
+}
+
+// Four consecutive features of an output row.
+__device__ __forceinline__ void store4(float *row, int f, int d, int vec, f32x4 v) {
+    if (vec) {
+        if (f < d) *reinterpret_cast<f32x4 *>(row + f) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (f + e < d) row[f + e] = v[e];
+    }
+}
+__device__ __forceinline__ void store4(uint16_t *row, int f, int d, int vec, f32x4 v) {
+    if (vec) {
+        if (f < d)
+            *reinterpret_cast<uint2 *>(row + f) = make_uint2(f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (f + e < d) row[f + e] = f32_to_bf16_rne(v[e]);
+    }
+}
+
+template <int W>
+__device__ __forceinline__ float over_groups_max(float v) {
+#pragma unroll
+    for (int o = W; o < 64; o <<= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+template <int W>
+__device__ __forceinline__ float over_groups_sum(float v) {
+#pragma unroll
+    for (int o = W; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// Row r of the n * group query rows that share a key head: its head and row, and the keys it
+// sees: j < lim.
+struct RowOf {
+    int64_t head, i;
+};
+__device__ __forceinline__ int64_t key_end(const Args &a, int64_t b) {
+    if (!a.lengths) return a.m;
+    const int64_t l = a.lengths[b];
+    return l < 0 ? 0 : l > a.m ? a.m : l;
+}
+// Keys that query i sees, of `len`: the last query sees all of them.
+__device__ __forceinline__ int64_t row_limit(const Args &a, int64_t len, int64_t i) {
+    if (!a.causal) return len;
+    const int64_t l = i + 1 + len - a.n;
+    return l < 0 ? 0 : l;
+}
+
+// Mask entries of keys j .. j + 3 (j + 3 may pass the end; entries past m are not read) of one
+// row.  keep: a bit per key; bias: four values.
+__device__ __forceinline__ uint32_t mask_keep4(const Args &a, const uint8_t *row, int64_t j) {
+    if (a.mask_vec && j + 3 < a.m) return *reinterpret_cast<const uint32_t *>(row + j);
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < a.m && row[(j + e) * a.mm]) w |= 1u << (8 * e);
+    return w;
+}
+__device__ __forceinline__ f32x4 mask_bias4(const Args &a, const void *row, int64_t j) {
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.mask_bf16) {
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
+        if (a.mask_vec && j + 3 < a.m) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(p + j);
+            v = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                      __uint_as_float(w.y & 0xffff0000u)};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < a.m) v[e] = bf16_to_f32(p[(j + e) * a.mm]);
+        }
+    } else {
+        const float *p = reinterpret_cast<const float *>(row);
+        if (a.mask_vec && j + 3 < a.m) {
+            v = *reinterpret_cast<const f32x4 *>(p + j);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < a.m) v[e] = p[(j + e) * a.mm];
+        }
+    }
+    return v;
+}
+__device__ __forceinline__ const void *mask_row(const Args &a, int64_t b, int64_t h, int64_t i, int bytes) {
+    return reinterpret_cast<const uint8_t *>(a.mask) + (b * a.mb + h * a.mh + i * a.mn) * bytes;
+}
+
+__device__ __forceinline__ int64_t cdiv_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Block id -> (tile, batch * key_heads + key head): ids go round-robin over the 8 XCDs, so where
+// they divide, each XCD gets a contiguous range: the blocks that share keys share an L2.
+__device__ __forceinline__ int64_t xcd_linear(int64_t bid, int64_t total) {
+    return (total & 7) == 0 ? (bid & 7) * (total >> 3) + (bid >> 3) : bid;
+}
+
+// Keys per tile in LDS (rows per tile of the dk / dv kernel): two buffers of two tiles stay within
+// 64 KiB, so two blocks share a CU (fp32 at 256 features: 128 KiB).
+template <typename T, int DP>
+struct Tiles {
+    static constexpr int kWidth = sizeof(T) == 2 ? 32 : 16;  // W of the matrix instructions
+    static constexpr int kKeys = DP * (int)sizeof(T) <= 256 ? 64 : 32;
+    static constexpr int kRows = 32;
+};
+
+// Host side: reads a descriptor into the kernels' arguments (attention.hip).
+int read_args(const tpw_attention_desc *d, bool backward, Args &a);
+
+// Runs f(type tag, DP, mask mode) for the arguments' types and widths.
+template <int V>
+struct Const {
+    static constexpr int value = V;
+};
+template <typename T, typename F>
+int by_width(const Args &a, int mode, F &&f) {
+    const int64_t w = a.d > a.dv ? a.d : a.dv;
+    const auto by_mode = [&](auto dp) {
+        if (mode == kNoMask) return f(T{}, dp, Const<kNoMask>{});
+        if (mode == kKeep) return f(T{}, dp, Const<kKeep>{});
+        return f(T{}, dp, Const<kBias>{});
+    };
+    if (w <= 64) return by_mode(Const<64>{});
+    if (w <= 128) return by_mode(Const<128>{});
+    return by_mode(Const<256>{});
+}
+template <typename F>
+int by_type(const Args &a, int dtype, int mode, F &&f) {
+    return dtype == TPW_BF16 ? by_width<uint16_t>(a, mode, f) : by_width<float>(a, mode, f);
+}
+inline int mask_mode(const tpw_attention_desc *d) {
+    return d->mask_type == TPW_MASK_NONE ? kNoMask : d->mask_type == TPW_MASK_KEEP ? kKeep : kBias;
+}
+// Parts of a summed axis of `steps` tiles for `blocks` blocks: none where the blocks fill 256 CUs
+// twice, else as many as fill them, each of two steps at least.
+inline int64_t parts_for(int64_t blocks, int64_t steps) {
+    if (blocks >= 384 || blocks <= 0) return 1;
+    int64_t p = cdiv(512, blocks), most = steps / 2 > 1 ? steps / 2 : 1;
+    p = p < most ? p : most;
+    return p < 64 ? p : 64;
+}
+
+}  // namespace attn
+}  // namespace tpw

@@ -27,8 +27,11 @@ _INTERNALS = [
     "pwand_sum", "pwor_sum", "pwxor_sum", "pweq_sum", "pwne_sum", "pweq_mean", "pwne_mean",
     "prf_div", "prf_ldiv", "prf_div_", "prf_ldiv_",
 ]
+_ATTENTION = ["attention", "rotary_embedding"]
 
-for _name in _METRICS + _CPDIST + _INTERNALS:
+for _name in _METRICS + _CPDIST + _INTERNALS + _ATTENTION:
     globals()[_name] = getattr(torch.ops.torchpairwise, _name)
 
-__all__ = list(_METRICS) + list(_CPDIST) + list(_INTERNALS)
+from .rotary import rotary_frequencies  # noqa: E402
+
+__all__ = list(_METRICS) + list(_CPDIST) + list(_INTERNALS) + list(_ATTENTION) + ["rotary_frequencies"]
