@@ -12,6 +12,7 @@ template <typename T, int W, int DP, int BN, int MM>
 struct Forward {
     using M = Mma<T, W>;
     using Acc = typename M::Acc;
+    using CR = ColReader<T, DP, W>;
     static constexpr int NB = BN / W, NQ = NB * M::Q, DB = DP / W, QS = DP / M::KS;
 
     Frag<T> q[QS];
@@ -40,7 +41,7 @@ struct Forward {
         const T *row = live ? reinterpret_cast<const T *>(a.q.p) + b * a.q.b + qh * a.q.h + qi * a.q.n : nullptr;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
-            q[s] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d, a.vec);
+            q[s] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d);
             if (a.qsign != 1.0f) {
                 float x[8];
                 unpack8(q[s], x);
@@ -60,7 +61,7 @@ struct Forward {
         if (j0 >= wlim_max) return;
         const int g = lane / W;
         const RowReader<T, DP, W> rr(lane);
-        const ColReader<T, DP, W> cr(lane);
+        const CR cr(lane);
         Acc s[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) s[i] = Acc{};
@@ -70,7 +71,7 @@ struct Forward {
             for (int i = 0; i < NB; ++i) M::mma(s[i], rr.read(kt, i, k), q[k]);
 
         if constexpr (MM == kBias) {
-            const void *mr = mask_row(a, b, qh, qi, a.mask_bf16 ? 2 : 4);
+            const void *mr = mask_row(a, b, qh, qi);
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -86,20 +87,21 @@ struct Forward {
                 }
         }
         if constexpr (MM == kKeep) {
-            const uint8_t *mr = reinterpret_cast<const uint8_t *>(mask_row(a, b, qh, qi, 1));
+            const uint32_t *mr = mask_words(a, b, qh, qi) + j0 / 32;
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+            for (int u = 0; u < BN / 32; ++u) {
+                const uint32_t keep = j0 + 32 * u < lim ? mr[u] >> (4 * g) : 0;
 #pragma unroll
-                for (int w = 0; w < M::Q; ++w) {
-                    const int j = j0 + W * i + 4 * M::NG * w + 4 * g;
-                    uint32_t keep = 0;
-                    if (j < lim) keep = mask_keep4(a, mr, j);
+                for (int x = 0; x < 32 / (4 * M::NG); ++x)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!(keep & (0xffu << (8 * e)))) s[i][4 * w + e] = -INFINITY;
-                }
+                    for (int e = 0; e < 4; ++e) {
+                        const int at = 32 * u + 4 * M::NG * x;  // of the tile's keys
+                        if (!(keep & (1u << (4 * M::NG * x + e)))) s[at / W][4 * (at % W / (4 * M::NG)) + e] = -INFINITY;
+                    }
+            }
         }
         if (j0 + BN > wlim_min) {
+            asm volatile("");  // a branch: most tiles skip this
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -150,14 +152,14 @@ struct Forward {
                 for (int e = 0; e < 4; ++e) x[4 * u + e] = s[(2 * t + u) / M::Q][4 * ((2 * t + u) % M::Q) + e];
             const Frag<T> p = pack8(x, T{});
 #pragma unroll
-            for (int i = 0; i < DB; ++i) M::mma(o[i], cr.read(vt, t, i), p);
+            for (int c = 0; c < CR::kPieces; ++c) CR::use(o, c, cr.read(vt, t, c), p);
         }
     }
 };
 
-// One block: kWaves x W query rows of the rows that share a key head, over the keys of one part.
-template <typename T, int W, int DP, int BN, int MM, int OCC>
-__global__ __launch_bounds__(kThreads, OCC) void attention_kernel(const Args a) {
+// One block: kWaves * W query rows of the rows that share a key head, over the keys of one part.
+template <typename T, int W, int DP, int BN, int MM, int kWaves, int OCC>
+__global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args a) {
     using F = Forward<T, W, DP, BN, MM>;
     using M = typename F::M;
     constexpr uint32_t kTileBytes = BN * DP * sizeof(T);
@@ -182,8 +184,8 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_kernel(const Args a) 
 
     const uint32_t lds = tile::lds_addr(smem);
     Stager<T, DP, BN, kWaves> sk, sv;
-    sk.init(a.k.n, (int)a.d, a.vec, wave, lane);
-    sv.init(a.v.n, (int)a.dv, a.vec, wave, lane);
+    sk.init(a.k.n, (int)a.d, wave, lane);
+    sv.init(a.v.n, (int)a.dv, wave, lane);
     const T *kb = reinterpret_cast<const T *>(a.k.p) + b * a.k.b + kh * a.k.h;
     const T *vb = reinterpret_cast<const T *>(a.v.p) + b * a.v.b + kh * a.v.h;
     const auto fetch = [&](int i) {
@@ -213,15 +215,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_kernel(const Args a) 
             st[all + row] = sum;
         }
         float *p = a.part + (part * all + row) * a.dv;
-#pragma unroll
-        for (int i = 0; i < F::DB; ++i)
-#pragma unroll
-            for (int w = 0; w < M::Q; ++w) {
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = f.o[i][4 * w + e];
-                store4(p, W * i + 4 * M::NG * w + 4 * g, (int)a.dv, a.dv % 4 == 0, v);
-            }
+        F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.dv, a.dv % 4 == 0, v); });
         return;
     }
     if (g == 0 && a.stats) {
@@ -229,52 +223,65 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_kernel(const Args a) 
         a.stats[a.batch * a.heads * a.n + row] = sum;
     }
     T *p = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + b * a.o.b + f.qh * a.o.h + f.qi * a.o.n;
-#pragma unroll
-    for (int i = 0; i < F::DB; ++i)
-#pragma unroll
-        for (int w = 0; w < M::Q; ++w) {
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = f.o[i][4 * w + e] * inv;
-            store4(p, W * i + 4 * M::NG * w + 4 * g, (int)a.dv, a.vec_out, v);
-        }
+    F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.dv, a.vec_out, v * inv); });
 }
 
-// Joins the parts of every row: m = max m_s, l = sum l_s 2^(m_s - m), o = sum o_s 2^(m_s - m) / l,
-// in the order of the parts.  One thread per four features.
-template <typename T, bool BIAS>
-__global__ void attention_join_kernel(const Args a) {
-    const int64_t rows = a.batch * a.heads * a.n, quads = (a.dv + 3) / 4;
-    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (id >= rows * quads) return;
-    const int64_t row = id / quads;
-    const int f = (int)(id % quads) * 4;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = __builtin_fmaxf(top, a.part_stats[2 * s * rows + row]);
+// Joins the parts of every row: m = max m_s, l = sum l_s 2^(m_s - m), o = sum o_s 2^(m_s - m) / l.
+// One wave per row: lane s holds part s's weight; then LANES lanes of four features each, 64 / LANES
+// parts at a time, in an order that the sizes fix.
+template <typename T, bool BIAS, int LANES>
+__global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
+    const int64_t rows = a.batch * a.heads * a.n, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63, f = lane % LANES * 4;
+    const float top_s = lane < a.splits ? a.part_stats[2 * lane * rows + row] : -INFINITY;
+    const float sum_s = lane < a.splits ? a.part_stats[(2 * lane + 1) * rows + row] : 0.0f;
+    const float top = over_groups_max<1>(top_s);
     const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    const float w = __builtin_amdgcn_exp2f(BIAS ? (top_s - base) * kLog2e : top_s - base);
+    const float sum = over_groups_sum<1>(lane < a.splits ? w * sum_s : 0.0f);
+    constexpr int G = 64 / LANES, U = 8;
+    const float *p = a.part + row * a.dv + f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; ++s) {
-        const float d = a.part_stats[2 * s * rows + row] - base;
-        const float w = __builtin_amdgcn_exp2f(BIAS ? d * kLog2e : d);
-        sum += w * a.part_stats[(2 * s + 1) * rows + row];
-        const float *p = a.part + (s * rows + row) * a.dv + f;
+    for (int s0 = 0; s0 < a.splits; s0 += G * U) {
+        f32x4 x[U];
+        float c[U];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (f + e < a.dv) o[e] += w * p[e];
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + G * u + lane / LANES;
+            const bool in = s < a.splits;
+            c[u] = __shfl(w, in ? s : 0, 64);
+            x[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (in) {
+                const float *q = p + s * rows * a.dv;
+                if (a.dv % 4 == 0) {
+                    if (f < a.dv) x[u] = *reinterpret_cast<const f32x4 *>(q);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (f + e < a.dv) x[u][e] = q[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) o += x[u] * c[u];
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = over_groups_sum<LANES>(o[e]);
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    if (f == 0 && a.stats) {
+    if (lane == 0 && a.stats) {
         a.stats[row] = top;
         a.stats[rows + row] = sum;
     }
+    if (lane >= LANES) return;
     const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
-    T *p = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + b * a.o.b + h * a.o.h + i * a.o.n;
-    o *= inv;
-    store4(p, f, (int)a.dv, a.vec_out, o);
+    T *out = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + b * a.o.b + h * a.o.h + i * a.o.n;
+    store4(out, f, (int)a.dv, a.vec_out, o * inv);
 }
 
 namespace {
+
+int64_t round_up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 
 bool whole_pieces(const View &v, int64_t width, int64_t size) {
     return aligned16(v.p) && width * size % 16 == 0 && v.b * size % 16 == 0 && v.h * size % 16 == 0 && v.n * size % 16 == 0;
@@ -283,16 +290,152 @@ View view_of(const void *p, const int64_t *strides, int64_t rows, int64_t width)
     return {p, strides[0], strides[1], rows == 1 ? width : strides[2]};
 }
 
-int64_t forward_parts(const Args &a, int64_t keys) { return parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, keys)); }
+constexpr int kPadded = 5;  // q, k, v, do, o
+struct PadArgs {
+    View from[kPadded];
+    void *to[kPadded];
+    int64_t heads[kPadded], rows[kPadded], width[kPadded], pieces[kPadded], first[kPadded + 1];
+    int count;
+};
+
+// Dense copies [batch, heads, rows, whole pieces] of operands, zeros past their width; one thread per
+// 16-byte piece.
+template <typename T>
+__global__ void pad_kernel(const PadArgs a) {
+    constexpr int E = 16 / (int)sizeof(T);
+    int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (id >= a.first[a.count]) return;
+    int t = 0;
+    while (id >= a.first[t + 1]) ++t;
+    id -= a.first[t];
+    const int64_t c = id % a.pieces[t], r = id / a.pieces[t], i = r % a.rows[t], bh = r / a.rows[t];
+    const View v = a.from[t];
+    const T *row = reinterpret_cast<const T *>(v.p) + bh / a.heads[t] * v.b + bh % a.heads[t] * v.h + i * v.n;
+    T x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = c * E + e < a.width[t] ? row[c * E + e] : T(0);
+    uint4 w;
+    __builtin_memcpy(&w, x, 16);
+    reinterpret_cast<uint4 *>(a.to[t])[id] = w;
+}
+
+// The operands to copy, their addresses from `at` on; returns the bytes they take.
+size_t plan_padding(Args &a, int dtype, bool backward, uint8_t *at, PadArgs *p) {
+    const int64_t size = dtype == TPW_F32 ? 4 : 2, e = 16 / size;
+    size_t bytes = 0;
+    const auto take = [&](View &v, int64_t heads, int64_t rows, int64_t width) {
+        if (whole_pieces(v, width, size) || a.batch * heads * rows == 0) return;
+        const int64_t pieces = cdiv(width, e), n = a.batch * heads * rows * pieces;
+        if (p) {
+            const int t = p->count++;
+            p->from[t] = v;
+            p->to[t] = at + bytes;
+            p->heads[t] = heads, p->rows[t] = rows, p->width[t] = width, p->pieces[t] = pieces;
+            p->first[t + 1] = p->first[t] + n;
+            v = {p->to[t], heads * rows * pieces * e, rows * pieces * e, pieces * e};
+        }
+        bytes += (size_t)n * 16;
+    };
+    take(a.q, a.heads, a.n, a.d);
+    take(a.k, a.key_heads, a.m, a.d);
+    take(a.v, a.key_heads, a.m, a.dv);
+    if (backward) {
+        take(a.go, a.heads, a.n, a.dv);
+        take(a.o, a.heads, a.n, a.dv);
+    }
+    return bytes;
+}
+
+struct BitArgs {
+    const uint8_t *mask;
+    uint32_t *bits, *cols;
+    int64_t mb, mh, mn, mm, heads, n, m, lead, words;
+};
+
+// Bits of a boolean mask, one row of words for each of its distinct rows (a broadcast dimension
+// counts once): the kernels test a bit of a word where they would load a byte, and the heads that
+// share a mask read an eighth of it.  For the backward also by column: word (i / 32, j) holds rows
+// 32 (i / 32) .. + 31 of key j.  One wave per 64 keys x 32 rows; all of its loads are in flight at once.
+__global__ __launch_bounds__(256) void pack_mask_kernel(const BitArgs a) {
+    const int64_t pairs = a.words / 2, steps = cdiv_dev(a.n, 32), id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t w = id % pairs * 2, t = id / pairs, i0 = t % steps * 32, bh = t / steps;
+    if (bh >= a.lead) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t j = 32 * w + lane;
+    const uint8_t *p = a.mask + bh / a.heads * a.mb + bh % a.heads * a.mh + i0 * a.mn + j * a.mm;
+    const int rows = a.n - i0 < 32 ? (int)(a.n - i0) : 32;
+    uint8_t x[32];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) x[r] = r < rows && j < a.m ? p[r * a.mn] : 0;
+    uint32_t col = 0, mine = 0;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+        const uint64_t all = __ballot(x[r] != 0);
+        if (lane % 32 == r) mine = lane < 32 ? (uint32_t)all : (uint32_t)(all >> 32);
+        col |= x[r] != 0 ? 1u << r : 0u;
+    }
+    if (lane % 32 < rows) a.bits[(bh * a.n + i0 + lane % 32) * a.words + w + lane / 32] = mine;
+    // one row for all: every row of the column
+    if (a.cols && j < a.m) a.cols[(bh * steps + i0 / 32) * a.m + j] = a.mn ? col : col ? 0xffffffffu : 0u;
+}
+
+// The bits' layout, its strides into the arguments; returns the bytes they take.
+int64_t plan_bits(Args &a, bool backward, uint8_t *at, BitArgs *p) {
+    const int64_t words = round_up(cdiv(a.m, 32), 2);  // whole tiles of 64 keys
+    const int64_t n = a.mn ? a.n : 1, heads = a.mh ? a.heads : 1, lead = heads * (a.mb ? a.batch : 1), steps = cdiv(n, 32);
+    const int64_t rows = round_up(lead * n * words * 4, 16);
+    if (p)
+        *p = {reinterpret_cast<const uint8_t *>(a.mask), reinterpret_cast<uint32_t *>(at),
+              backward ? reinterpret_cast<uint32_t *>(at + rows) : nullptr, a.mb, a.mh, a.mn, a.mm, heads, n, a.m, lead, words};
+    a.mask = at;
+    a.mask_cols = backward ? reinterpret_cast<uint32_t *>(at + rows) : nullptr;
+    a.cn = a.mn ? a.m : 0;
+    a.ch = a.mh ? steps * a.m : 0;
+    a.cb = a.mb ? heads * steps * a.m : 0;
+    a.mb = a.mb ? heads * n * words : 0;
+    a.mh = a.mh ? n * words : 0;
+    a.mn = a.mn ? words : 0;
+    a.mm = 0;
+    return rows + (backward ? round_up(lead * steps * a.m * 4, 16) : 0);
+}
 
 // Sets tiles and splits for the element type and width.
 template <typename T, int DP>
 void plan(Args &a) {
-    a.tiles = cdiv(a.n * a.group, (int64_t)kWaves * Tiles<T, DP>::kWidth);
-    a.splits = (int)forward_parts(a, Tiles<T, DP>::kKeys);
+    a.tiles = cdiv(a.n * a.group, (int64_t)Tiles<T, DP>::kWaves * Tiles<T, DP>::kWidth);
+    a.splits = (int)parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, Tiles<T, DP>::kKeys), Tiles<T, DP>::kPerCu);
 }
 
 }  // namespace
+
+size_t prepared_bytes(const Args &a, const tpw_attention_desc *d, bool backward) {
+    Args b = a;
+    return plan_padding(b, d->dtype, backward, nullptr, nullptr) + (mask_mode(d) == kKeep ? (size_t)plan_bits(b, backward, nullptr, nullptr) : 0);
+}
+int prepare_operands(Args &a, const tpw_attention_desc *d, bool backward, void *at, hipStream_t s) {
+    PadArgs p = {};
+    uint8_t *next = reinterpret_cast<uint8_t *>(at);
+    if (const size_t bytes = plan_padding(a, d->dtype, backward, next, &p)) {
+        const int64_t blocks = cdiv(p.first[p.count], 256);
+        TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: too many rows");
+        if (d->dtype == TPW_F32)
+            hipLaunchKernelGGL((pad_kernel<uint32_t>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+        else
+            hipLaunchKernelGGL((pad_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+        if (const int rc = check_launch("pad_kernel")) return rc;
+        next += bytes;
+    }
+    if (mask_mode(d) == kKeep) {
+        BitArgs m = {};
+        plan_bits(a, backward, next, &m);
+        if (m.lead * m.n * m.words == 0) return TPW_OK;
+        const int64_t blocks = cdiv(m.lead * cdiv(m.n, 32) * (m.words / 2), 4);
+        TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: mask too large");
+        hipLaunchKernelGGL(pack_mask_kernel, dim3((unsigned)blocks), dim3(256), 0, s, m);
+        return check_launch("pack_mask_kernel");
+    }
+    return TPW_OK;
+}
 
 int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
     TPW_REQUIRE(d, "null descriptor");
@@ -325,14 +468,10 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
     a.mn = d->mask_strides[2];
     a.mm = d->mask_strides[3];
     a.mask_bf16 = d->mask_type == TPW_MASK_ADD_BF16;
-    const int64_t quad = d->mask_type == TPW_MASK_KEEP ? 4 : a.mask_bf16 ? 8 : 16, unit = quad / 4;
-    a.mask_vec = a.mm == 1 && reinterpret_cast<uintptr_t>(a.mask) % quad == 0 && a.mb * unit % quad == 0 &&
-                 a.mh * unit % quad == 0 && a.mn * unit % quad == 0;
     const bool bias = mask_mode(d) == kBias;
     a.qsign = d->scale > 0 ? 1.0f : d->scale < 0 ? -1.0f : 0.0f;
     a.scale = d->scale == 0 ? 1.0f : (float)(fabs(d->scale) * (bias ? 1.0 : 1.4426950408889634));
     a.gscale = (float)d->scale;
-    a.vec = whole_pieces(a.q, a.d, size) && whole_pieces(a.k, a.d, size) && whole_pieces(a.v, a.dv, size);
     a.vec_out = whole_pieces(a.o, a.dv, size);
     const auto streamed = [&](const View &v, int64_t rows, int64_t width) {
         return a.batch * a.heads * a.n * a.m == 0 || rows <= 1 || (v.n >= width && v.n * size <= (int64_t(1) << 23));
@@ -343,7 +482,6 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
         a.gq = view_of(d->grad_query, d->grad_query_strides, d->n, d->d);
         a.gk = view_of(d->grad_key, d->grad_key_strides, d->m, d->d);
         a.gv = view_of(d->grad_value, d->grad_value_strides, d->m, d->dv);
-        a.vec = a.vec && whole_pieces(a.go, a.dv, size) && whole_pieces(a.o, a.dv, size);
         a.vec_out = whole_pieces(a.gq, a.d, size) && whole_pieces(a.gk, a.d, size) && whole_pieces(a.gv, a.dv, size);
         ok = ok && streamed(a.q, d->n, d->d) && streamed(a.go, d->n, d->dv);
     }
@@ -371,7 +509,7 @@ extern "C" size_t tpw_attention_workspace_size(const tpw_attention_desc *d) {
     size_t bytes = 0;
     by_type(a, d->dtype, kNoMask, [&](auto t, auto dp, auto) {
         plan<decltype(t), decltype(dp)::value>(a);
-        bytes = forward_workspace(a);
+        bytes = prepared_bytes(a, d, false) + forward_workspace(a);
         return TPW_OK;
     });
     return bytes;
@@ -384,6 +522,11 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
     TPW_REQUIRE(a.q.p && a.o.p && (a.m == 0 || (a.k.p && a.v.p)), "attention: null operand");
     TPW_REQUIRE(d->mask_type == TPW_MASK_NONE || a.mask || a.m == 0, "attention: null mask");
     hipStream_t s = as_stream(stream);
+    const size_t prepared = prepared_bytes(a, d, false);
+    if (prepared) {
+        TPW_REQUIRE(workspace && aligned16(workspace), "attention: null or unaligned workspace");
+        if (const int rc = prepare_operands(a, d, false, workspace, s)) return rc;
+    }
     return by_type(a, d->dtype, mask_mode(d), [&](auto t, auto dp, auto mode) {
         using T = decltype(t);
         constexpr int DP = decltype(dp)::value, MM = decltype(mode)::value, W = Tiles<T, DP>::kWidth;
@@ -392,16 +535,16 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
         TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: too many rows");
         if (a.splits > 1) {
             TPW_REQUIRE(workspace && aligned16(workspace), "attention: null or unaligned workspace");
-            a.part = reinterpret_cast<float *>(workspace);
+            a.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + prepared);
             a.part_stats = a.part + a.splits * rows * a.dv;
         }
-        constexpr int kOcc = sizeof(T) == 4 && DP == 256 ? 1 : 2;
-        hipLaunchKernelGGL((attention_kernel<T, W, DP, Tiles<T, DP>::kKeys, MM, kOcc>), dim3((unsigned)blocks),
-                           dim3(attn::kThreads), 0, s, a);
+        constexpr int kOcc = 2;
+        constexpr int kWaves = Tiles<T, DP>::kWaves;
+        hipLaunchKernelGGL((attention_kernel<T, W, DP, Tiles<T, DP>::kKeys, MM, kWaves, kOcc>), dim3((unsigned)blocks),
+                           dim3(64 * kWaves), 0, s, a);
         if (const int rc = check_launch("attention_kernel")) return rc;
         if (a.splits > 1) {
-            const int64_t quads = rows * cdiv(a.dv, 4);
-            hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias>), dim3((unsigned)cdiv(quads, 256)), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, DP / 4>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a);
             return check_launch("attention_join_kernel");
         }
         return TPW_OK;

@@ -22,13 +22,13 @@
 namespace tpw {
 namespace attn {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 enum MaskMode { kNoMask = 0, kKeep = 1, kBias = 2 };
 
-// One operand: element strides of [batch, heads, rows, features] (features dense).
+// One operand: element strides of [batch, heads, rows, features] (features dense).  The kernels read
+// rows as 16-byte pieces at 16-byte aligned addresses, a last partial piece filled up with zeros:
+// operands that do not lie so are copied first (pad_kernel).
 struct View {
     const void *p;
     int64_t b, h, n;
@@ -40,16 +40,17 @@ struct Args {
     View gq, gk, gv;     // gradients (backward)
     float *stats;        // [2, b, h, n]: row maxima, row sums
     float *rows;         // [3, b, h, n] (backward): base and 1 / sum of the softmax, delta
-    const void *mask;    // bool bytes (kKeep) or fp32 / bf16 (kBias)
-    int64_t mb, mh, mn, mm;
-    int mask_bf16, mask_vec;
+    const void *mask;    // kKeep: words of 32 keys' bits (pack_mask_kernel); kBias: fp32 or bf16 values
+    int64_t mb, mh, mn, mm;  // its strides, in words or values (0: broadcast; words: mm is 0)
+    int mask_bf16;
+    const uint32_t *mask_cols;  // kKeep, backward: bits by column, word (row / 32, key)
+    int64_t cb, ch, cn;         // its strides over batch, heads and row / 32
     const int64_t *lengths;  // [b] or null
     int64_t batch, heads, key_heads, group, n, m, d, dv;
     float scale;   // |scale| * log2(e) (kBias: |scale|), 1 where scale is 0
     float qsign;   // -1, 0 or 1: the sign of scale, folded into q as it is loaded
     float gscale;  // scale (backward)
     int causal;
-    int vec;       // rows of q, k, v (and do, o) are whole 16-byte pieces at 16-byte aligned addresses
     int vec_out;   // the outputs' rows take stores of four features
     int64_t tiles;  // row tiles (dk / dv: key tiles) per (batch, key head)
     int splits;     // parts of the summed axis
@@ -175,14 +176,11 @@ struct Stager {
     static_assert(ROWS * L::C % (64 * WAVES) == 0, "whole instructions");
     uint32_t off[kSlots];
     int64_t stride;  // bytes between rows
-    int d, vec, wave, lane;
+    int wave;
 
-    __device__ __forceinline__ void init(int64_t row_stride, int d_, int vec_, int wave_, int lane_) {
+    __device__ __forceinline__ void init(int64_t row_stride, int d, int wave_, int lane) {
         stride = row_stride * (int64_t)sizeof(T);
-        d = d_;
-        vec = vec_;
         wave = wave_;
-        lane = lane_;
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
             const int s = (i * WAVES + wave) * 64 + lane, r = s / L::C, c = (s % L::C) ^ swz(r);
@@ -190,26 +188,9 @@ struct Stager {
         }
     }
     __device__ __forceinline__ void load(const T *base, int64_t rows, uint32_t lds) const {
-        if (vec) {
-            const tpw_u32x4 r = resource(base, rows * stride);
+        const tpw_u32x4 r = resource(base, rows * stride);
 #pragma unroll
-            for (int i = 0; i < kSlots; ++i) dma16(r, off[i], lds + (uint32_t)((i * WAVES + wave) * 1024));
-        } else {
-#pragma unroll 1
-            for (int i = 0; i < kSlots; ++i) {
-                const int s = (i * WAVES + wave) * 64 + lane, r = s / L::C, c = (s % L::C) ^ swz(r);
-                T x[L::E];
-#pragma unroll
-                for (int e = 0; e < L::E; ++e) {
-                    const int f = c * L::E + e;
-                    x[e] = r < rows && f < d ? base[r * (stride / (int64_t)sizeof(T)) + f] : T(0);
-                }
-                uint4 w;
-                __builtin_memcpy(&w, x, 16);
-                *reinterpret_cast<__attribute__((address_space(3))) tpw_u32x4 *>((uintptr_t)(lds + (uint32_t)s * 16)) =
-                    tpw_u32x4{w.x, w.y, w.z, w.w};
-            }
-        }
+        for (int i = 0; i < kSlots; ++i) dma16(r, off[i], lds + (uint32_t)((i * WAVES + wave) * 1024));
     }
 };
 
@@ -217,86 +198,140 @@ __device__ __forceinline__ tpw_u32x4 lds_read16(uint32_t a) {
     return *reinterpret_cast<__attribute__((address_space(3))) const tpw_u32x4 *>((uintptr_t)a);
 }
 
-// Row fragment: features KS s + 8 g .. + 7 of row r.
+// Row fragments: features KS s + 8 g .. + 7 of row lane % W of a block of W rows.  Of the piece's
+// index only the low three bits meet swz, so a few lane addresses and immediate offsets reach all.
 template <typename T, int DP, int W>
 struct RowReader {
     using L = Tile<T, DP>;
     using S = Shape<W>;
-    uint32_t row;
-    int x, g;
-    __device__ __forceinline__ RowReader(int lane) : row((uint32_t)((lane % W) * L::kRowBytes)), x(swz(lane % W)), g(lane / W) {}
-    // block `blk` of W rows; swz(r) depends on r mod 8 only, and W is a multiple of 8
+    static constexpr int P = 8 / L::E, kStep = S::NG * P;           // pieces per fragment, per step
+    static constexpr int kAddr = kStep < 8 ? 8 / kStep : 1;         // steps until the low bits repeat
+    uint32_t at[kAddr][P];
+    __device__ __forceinline__ RowReader(int lane) {
+        const int r = lane % W, x = swz(r), g = lane / W;
+#pragma unroll
+        for (int s = 0; s < kAddr; ++s)
+#pragma unroll
+            for (int u = 0; u < P; ++u)
+                at[s][u] = (uint32_t)(r * L::kRowBytes + ((kStep * s + P * g + u) ^ x) * 16);
+    }
+    // block `blk` of the tile at `tile` (swz(r) depends on r mod 8 only, and W is a multiple of 8)
     __device__ __forceinline__ Frag<T> read(uint32_t tile, int blk, int s) const {
-        const uint32_t base = tile + (uint32_t)(blk * W * L::kRowBytes) + row;
+        const uint32_t far = (uint32_t)(blk * W * L::kRowBytes + s / kAddr * kAddr * kStep * 16);
         Frag<T> f;
         if constexpr (sizeof(T) == 2) {
-            f.v = __builtin_bit_cast(uint4, lds_read16(base + (uint32_t)(((S::NG * s + g) ^ x) * 16)));
+            f.v = __builtin_bit_cast(uint4, lds_read16(tile + at[s % kAddr][0] + far));
         } else {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-                f.v[u] = __builtin_bit_cast(f32x4, lds_read16(base + (uint32_t)(((2 * (S::NG * s + g) + u) ^ x) * 16)));
+            for (int u = 0; u < 2; ++u) f.v[u] = __builtin_bit_cast(f32x4, lds_read16(tile + at[s % kAddr][u] + far));
         }
         return f;
     }
 };
 
-// Column fragment (first operand of the second products): feature W b + lane % W of rows
-// 4 NG (2 t + u) + 4 g + e, element 4 u + e.
+// Column pieces, the first operands of the second products (sums over rows): a step t covers KS rows
+// in kPieces pieces, each of which `use` multiplies into the accumulators of its feature blocks.
+// Element 4 u + e of the second operand is row 4 NG (2 t + u) + 4 g + e of the tile.
+//   bf16: piece c is block c of W features, by two transposing reads: lane i of a group of 16 points
+//   at four features of row i / 4 and receives feature i % 16 of the four rows.
+//   fp32: piece c is rows u = c % 2 of features 64 (c / 2) .. + 63.  A lane reads features 4 (lane %
+//   16) .. + 3 of each row, so block 4 B + k holds features 64 B + 4 i + k: one 16-byte read feeds
+//   four products.
+// `each` gives the results back as quads of consecutive features.
 template <typename T, int DP, int W>
-struct ColReader {
-    using L = Tile<T, DP>;
-    using S = Shape<W>;
-    int lane, g;
-    __device__ __forceinline__ ColReader(int l) : lane(l), g(l / W) {}
-    __device__ __forceinline__ Frag<T> read(uint32_t tile, int t, int b) const {
-        Frag<T> f;
-        if constexpr (sizeof(T) == 2) {
-            // lane i of a group of 16 points at four features of row i / 4; it receives feature i % 16
-            // of the four rows
-            const int i = lane & 15, r0 = 4 * g + (i >> 2), x = swz(r0);
+struct ColReader;
+template <int DP, int W>
+struct ColReader<uint16_t, DP, W> {
+    using L = Tile<uint16_t, DP>;
+    using M = Mma<uint16_t, W>;
+    static constexpr int kBlocks = DP / W, kPieces = kBlocks, kAddr = 64 / W;  // blocks until the low bits repeat
+    typedef uint4 Piece;
+    uint32_t at[kAddr];
+    __device__ __forceinline__ ColReader(int lane) {
+        const int i = lane & 15, r0 = 4 * (lane / W) + (i >> 2), x = swz(r0);
+#pragma unroll
+        for (int b = 0; b < kAddr; ++b) {
             const int col = W * b + 16 * ((lane % W) >> 4) + 4 * (i & 3);
-            uint2 v[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t a = tile + (uint32_t)((4 * S::NG * (2 * t + u) + r0) * L::kRowBytes) +
-                                   (uint32_t)((((col >> 3) ^ x) * 16) + (col & 4) * 2);
-                v[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                     (__attribute__((address_space(3))) s16x4 *)(uintptr_t)a));
-            }
-            f.v = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
-        } else {
-            const int col = W * b + lane % W;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r0 = 4 * g + e;
-                    const uint32_t a = tile + (uint32_t)((4 * S::NG * (2 * t + u) + r0) * L::kRowBytes) +
-                                       (uint32_t)((((col >> 2) ^ swz(r0)) * 16) + (col & 3) * 4);
-                    f.v[u][e] = *reinterpret_cast<__attribute__((address_space(3))) const float *>((uintptr_t)a);
-                }
+            at[b] = (uint32_t)(r0 * L::kRowBytes + ((col >> 3) ^ x) * 16 + (col & 4) * 2);
         }
-        return f;
+    }
+    // (4 NG (2 t + u) is a multiple of 8, so swz of the whole row index is swz(r0))
+    __device__ __forceinline__ Piece read(uint32_t tile, int t, int c) const {
+        uint2 v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t a = tile + at[c % kAddr] +
+                               (uint32_t)(4 * M::NG * (2 * t + u) * L::kRowBytes + c / kAddr * kAddr * W * 2);
+            v[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                 (__attribute__((address_space(3))) s16x4 *)(uintptr_t)a));
+        }
+        return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
+    }
+    static __device__ __forceinline__ void use(typename M::Acc *acc, int c, const Piece &a, const Frag<uint16_t> &p) {
+        M::mma(acc[c], Frag<uint16_t>{a}, p);
+    }
+    template <typename F>
+    static __device__ __forceinline__ void each(const typename M::Acc *acc, int lane, F &&f) {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int w = 0; w < M::Q; ++w)
+                f(W * i + 4 * M::NG * w + 4 * (lane / W),
+                  f32x4{acc[i][4 * w], acc[i][4 * w + 1], acc[i][4 * w + 2], acc[i][4 * w + 3]});
     }
 };
-// (4 NG (2 t + u) is a multiple of 8, so swz of the whole row index is swz(r0).)
-
-// Features KS s + 8 g .. + 7 of a row in global memory (null: zeros).
-template <typename T>
-__device__ __forceinline__ Frag<T> load_row8(const T *row, int f, int d, int vec) {
-    T x[8];
-    if (vec) {
-        // d is whole 16-byte pieces
-        constexpr int E = 16 / (int)sizeof(T);
+template <int DP>
+struct ColReader<float, DP, 16> {
+    using L = Tile<float, DP>;
+    using M = Mma<float, 16>;
+    static constexpr int kBlocks = DP / 16, kPieces = DP / 32;
+    struct Piece {
+        f32x4 v[4];
+    };
+    uint32_t at[4];
+    __device__ __forceinline__ ColReader(int lane) {
 #pragma unroll
-        for (int u = 0; u < 8 / E; ++u) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (row && f + u * E < d) w = *reinterpret_cast<const uint4 *>(row + f + u * E);
-            __builtin_memcpy(x + u * E, &w, 16);
+        for (int e = 0; e < 4; ++e) {
+            const int r0 = 4 * (lane / 16) + e;
+            at[e] = (uint32_t)(r0 * L::kRowBytes + ((lane % 16) ^ swz(r0)) * 16);
         }
-    } else {
+    }
+    __device__ __forceinline__ Piece read(uint32_t tile, int t, int c) const {
+        Piece p;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = row && f + e < d ? row[f + e] : T(0);
+        for (int e = 0; e < 4; ++e)
+            p.v[e] = __builtin_bit_cast(
+                f32x4, lds_read16(tile + at[e] + (uint32_t)(16 * (2 * t + c % 2) * L::kRowBytes + c / 2 * 256)));
+        return p;
+    }
+    static __device__ __forceinline__ void use(M::Acc *acc, int c, const Piece &a, const Frag<float> &p) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                acc[4 * (c / 2) + k] = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e][k], p.v[c % 2][e], acc[4 * (c / 2) + k], 0, 0, 0);
+    }
+    template <typename F>
+    static __device__ __forceinline__ void each(const M::Acc *acc, int lane, F &&f) {
+#pragma unroll
+        for (int b = 0; b < kBlocks / 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                f(64 * b + 16 * (lane / 16) + 4 * r,
+                  f32x4{acc[4 * b][r], acc[4 * b + 1][r], acc[4 * b + 2][r], acc[4 * b + 3][r]});
+    }
+};
+
+// Features f .. f + 7 of a row in global memory (null: zeros).
+template <typename T>
+__device__ __forceinline__ Frag<T> load_row8(const T *row, int f, int d) {
+    constexpr int E = 16 / (int)sizeof(T);
+    T x[8];
+#pragma unroll
+    for (int u = 0; u < 8 / E; ++u) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (row && f + u * E < d) w = *reinterpret_cast<const uint4 *>(row + f + u * E);
+        __builtin_memcpy(x + u * E, &w, 16);
     }
     Frag<T> r;
     __builtin_memcpy(&r, x, sizeof(r));
@@ -354,22 +389,22 @@ __device__ __forceinline__ int64_t row_limit(const Args &a, int64_t len, int64_t
     return l < 0 ? 0 : l;
 }
 
-// Mask entries of keys j .. j + 3 (j + 3 may pass the end; entries past m are not read) of one
-// row.  keep: a bit per key; bias: four values.
-__device__ __forceinline__ uint32_t mask_keep4(const Args &a, const uint8_t *row, int64_t j) {
-    if (a.mask_vec && j + 3 < a.m) return *reinterpret_cast<const uint32_t *>(row + j);
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (j + e < a.m && row[(j + e) * a.mm]) w |= 1u << (8 * e);
-    return w;
+// kKeep: bits of keys 32 w .. 32 w + 31 of a row.  kBias: values of keys j .. j + 3 (any alignment;
+// keys past m are not read).
+__device__ __forceinline__ const uint32_t *mask_words(const Args &a, int64_t b, int64_t h, int64_t i) {
+    return reinterpret_cast<const uint32_t *>(a.mask) + b * a.mb + h * a.mh + i * a.mn;
+}
+__device__ __forceinline__ const void *mask_row(const Args &a, int64_t b, int64_t h, int64_t i) {
+    return reinterpret_cast<const uint8_t *>(a.mask) + (b * a.mb + h * a.mh + i * a.mn) * (a.mask_bf16 ? 2 : 4);
 }
 __device__ __forceinline__ f32x4 mask_bias4(const Args &a, const void *row, int64_t j) {
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool run = a.mm == 1 && j + 3 < a.m;
     if (a.mask_bf16) {
         const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
-        if (a.mask_vec && j + 3 < a.m) {
-            const uint2 w = *reinterpret_cast<const uint2 *>(p + j);
+        if (run) {
+            uint2 w;
+            __builtin_memcpy(&w, p + j, 8);
             v = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
                       __uint_as_float(w.y & 0xffff0000u)};
         } else {
@@ -379,8 +414,8 @@ __device__ __forceinline__ f32x4 mask_bias4(const Args &a, const void *row, int6
         }
     } else {
         const float *p = reinterpret_cast<const float *>(row);
-        if (a.mask_vec && j + 3 < a.m) {
-            v = *reinterpret_cast<const f32x4 *>(p + j);
+        if (run) {
+            __builtin_memcpy(&v, p + j, 16);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -388,9 +423,6 @@ __device__ __forceinline__ f32x4 mask_bias4(const Args &a, const void *row, int6
         }
     }
     return v;
-}
-__device__ __forceinline__ const void *mask_row(const Args &a, int64_t b, int64_t h, int64_t i, int bytes) {
-    return reinterpret_cast<const uint8_t *>(a.mask) + (b * a.mb + h * a.mh + i * a.mn) * bytes;
 }
 
 __device__ __forceinline__ int64_t cdiv_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -401,17 +433,28 @@ __device__ __forceinline__ int64_t xcd_linear(int64_t bid, int64_t total) {
     return (total & 7) == 0 ? (bid & 7) * (total >> 3) + (bid >> 3) : bid;
 }
 
-// Keys per tile in LDS (rows per tile of the dk / dv kernel): two buffers of two tiles stay within
-// 64 KiB, so two blocks share a CU (fp32 at 256 features: 128 KiB).
+// Blocks and tiles: waves per block, keys per LDS tile (rows per tile of the dk / dv kernel).  Two
+// buffers of two tiles stay within 64 KiB, so two blocks of four waves share a CU; fp32 at 256
+// features takes 128 KiB, and eight waves share them.
 template <typename T, int DP>
 struct Tiles {
     static constexpr int kWidth = sizeof(T) == 2 ? 32 : 16;  // W of the matrix instructions
+    static constexpr int kWaves = DP * (int)sizeof(T) == 1024 ? 8 : 4;
     static constexpr int kKeys = DP * (int)sizeof(T) <= 256 ? 64 : 32;
-    static constexpr int kRows = 32;
+    static constexpr int kRowWaves = 4, kRows = 32;          // dk / dv kernel
+    // blocks that share a CU: forward, dq, dk / dv
+    static constexpr bool kNarrow = DP * (int)sizeof(T) == 128;  // bf16 at 64 features
+    static constexpr int kPerCu = kNarrow ? 4 : kWaves == 8 ? 1 : 2;
+    static constexpr int kPerCuQ = kNarrow ? 4 : DP == 256 ? 1 : 2;
+    static constexpr int kPerCuK = DP == 256 || (DP == 128 && sizeof(T) == 4) ? 1 : 2;
 };
 
-// Host side: reads a descriptor into the kernels' arguments (attention.hip).
+// Host side (attention.hip): reads a descriptor into the kernels' arguments; bytes that a call's
+// prepared operands take (padded copies of those that need one, the bits of a boolean mask), and the
+// launches that prepare them at `at` (16-byte aligned) and point the arguments to them.
 int read_args(const tpw_attention_desc *d, bool backward, Args &a);
+size_t prepared_bytes(const Args &a, const tpw_attention_desc *d, bool backward);
+int prepare_operands(Args &a, const tpw_attention_desc *d, bool backward, void *at, hipStream_t s);
 
 // Runs f(type tag, DP, mask mode) for the arguments' types and widths.
 template <int V>
@@ -437,13 +480,15 @@ int by_type(const Args &a, int dtype, int mode, F &&f) {
 inline int mask_mode(const tpw_attention_desc *d) {
     return d->mask_type == TPW_MASK_NONE ? kNoMask : d->mask_type == TPW_MASK_KEEP ? kKeep : kBias;
 }
-// Parts of a summed axis of `steps` tiles for `blocks` blocks: none where the blocks fill 256 CUs
-// twice, else as many as fill them, each of two steps at least.
-inline int64_t parts_for(int64_t blocks, int64_t steps) {
-    if (blocks >= 384 || blocks <= 0) return 1;
-    int64_t p = cdiv(512, blocks), most = steps / 2 > 1 ? steps / 2 : 1;
-    p = p < most ? p : most;
-    return p < 64 ? p : 64;
+// Parts of a summed axis of `steps` tiles for `blocks` blocks where a CU holds `per_cu` of them: as
+// many as still run all at once on 256 CUs (one more would start a second round), at most one per
+// step and kMaxParts.
+constexpr int kMaxParts = 64;  // the join gives each part a lane
+inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu) {
+    if (blocks <= 0 || steps <= 1) return 1;
+    int64_t p = 256 * per_cu / blocks;
+    p = p < steps ? p : steps;
+    return p < 1 ? 1 : p < kMaxParts ? p : kMaxParts;
 }
 
 }  // namespace attn

@@ -14,12 +14,28 @@
 namespace tpw {
 namespace attn {
 
+// Runs N steps of `use` on fragments that `load` reads from LDS, the next step's reads issued before
+// this step's products.  The compiler may not move the reads further ahead: left alone it hoists
+// them all and spills the accumulators.
+template <int N, int F, typename Piece, typename Load, typename Use>
+__device__ __forceinline__ void stream_steps(Load load, Use use) {
+    Piece f[2][F];
+    load(0, f[0]);
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        if (x + 1 < N) load(x + 1, f[(x + 1) & 1]);
+        asm volatile("" ::: "memory");
+        use(x, f[x & 1]);
+    }
+}
+
 constexpr int kUnit = 32;  // rows (keys) of the streamed operand that are worked on at a time
 
-template <typename T, int W, int DP, int BN, int MM, int OCC>
-__global__ __launch_bounds__(kThreads, OCC) void attention_dq_kernel(const Args a) {
+template <typename T, int W, int DP, int BN, int MM, int kWaves, int OCC>
+__global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Args a) {
     using M = Mma<T, W>;
     using Acc = typename M::Acc;
+    using CR = ColReader<T, DP, W>;
     constexpr int DB = DP / W, QS = DP / M::KS, NU = kUnit / W, ST = kUnit / M::KS;
     constexpr uint32_t kTileBytes = BN * DP * sizeof(T);
     __shared__ uint4 smem[4 * kTileBytes / 16];
@@ -55,8 +71,8 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dq_kernel(const Args 
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
             const int f = M::KS * s + 8 * g;
-            q[s] = load_row8(qr, f, (int)a.d, a.vec);
-            go[s] = load_row8(gr, f, (int)a.dv, a.vec);
+            q[s] = load_row8(qr, f, (int)a.d);
+            go[s] = load_row8(gr, f, (int)a.dv);
             float x[8], y[8];
             if (a.qsign != 1.0f) {
                 unpack8(q[s], x);
@@ -65,7 +81,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dq_kernel(const Args 
                 q[s] = pack8(x, T{});
             }
             unpack8(go[s], x);
-            unpack8(load_row8(orow, f, (int)a.dv, a.vec), y);
+            unpack8(load_row8(orow, f, (int)a.dv), y);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
         }
@@ -95,8 +111,8 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dq_kernel(const Args 
 
     const uint32_t lds = tile::lds_addr(smem);
     Stager<T, DP, BN, kWaves> sk, sv;
-    sk.init(a.k.n, (int)a.d, a.vec, wave, lane);
-    sv.init(a.v.n, (int)a.dv, a.vec, wave, lane);
+    sk.init(a.k.n, (int)a.d, wave, lane);
+    sv.init(a.v.n, (int)a.dv, wave, lane);
     const T *kb = reinterpret_cast<const T *>(a.k.p) + b * a.k.b + kh * a.k.h;
     const T *vb = reinterpret_cast<const T *>(a.v.p) + b * a.v.b + kh * a.v.h;
     const auto fetch = [&](int i) {
@@ -106,7 +122,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dq_kernel(const Args 
         sv.load(vb + j0 * a.v.n, len - j0, buf + kTileBytes);
     };
     const RowReader<T, DP, W> rr(lane);
-    const ColReader<T, DP, W> cr(lane);
+    const CR cr(lane);
     if (t0 < t1) fetch(t0);
     for (int it = t0; it < t1; ++it) {
         tile::barrier_all();
@@ -127,7 +143,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dq_kernel(const Args 
                     M::mma(dp[i], rr.read(vt, u * NU + i, k), go[k]);
                 }
             if constexpr (MM == kBias) {
-                const void *mr = mask_row(a, b, qh, qi, a.mask_bf16 ? 2 : 4);
+                const void *mr = mask_row(a, b, qh, qi);
 #pragma unroll
                 for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -144,23 +160,19 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dq_kernel(const Args 
                     }
             }
             if constexpr (MM == kKeep) {
-                const uint8_t *mr = reinterpret_cast<const uint8_t *>(mask_row(a, b, qh, qi, 1));
+                const uint32_t keep = j0 < lim ? mask_words(a, b, qh, qi)[j0 / 32] >> (4 * g) : 0;
 #pragma unroll
-                for (int i = 0; i < NU; ++i)
+                for (int x = 0; x < 32 / (4 * M::NG); ++x)
 #pragma unroll
-                    for (int w = 0; w < M::Q; ++w) {
-                        const int j = j0 + W * i + 4 * M::NG * w + 4 * g;
-                        uint32_t keep = 0;
-                        if (j < lim) keep = mask_keep4(a, mr, j);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!(keep & (0xffu << (8 * e)))) {
-                                s[i][4 * w + e] = -INFINITY;
-                                dp[i][4 * w + e] = 0.0f;
-                            }
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        if (!(keep & (1u << (4 * M::NG * x + e)))) {
+                            const int at = 4 * M::NG * x;
+                            s[at / W][4 * (at % W / (4 * M::NG)) + e] = -INFINITY;
+                            dp[at / W][4 * (at % W / (4 * M::NG)) + e] = 0.0f;
+                        }
             }
             if (j0 + kUnit > wmin) {
+                asm volatile("");  // a branch: most units skip this
 #pragma unroll
                 for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -190,62 +202,53 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dq_kernel(const Args 
                     for (int e = 0; e < 4; ++e) x[4 * v + e] = s[(2 * st + v) / M::Q][4 * ((2 * st + v) % M::Q) + e];
                 const Frag<T> ds = pack8(x, T{});
 #pragma unroll
-                for (int i = 0; i < DB; ++i) M::mma(dq[i], cr.read(kt, u * ST + st, i), ds);
+                for (int c = 0; c < CR::kPieces; ++c) CR::use(dq, c, cr.read(kt, u * ST + st, c), ds);
             }
         }
     }
     if (!live) return;
     if (a.splits > 1) {
         float *p = a.part + (part * all + row) * a.d;
-#pragma unroll
-        for (int i = 0; i < DB; ++i)
-#pragma unroll
-            for (int w = 0; w < M::Q; ++w) {
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = dq[i][4 * w + e];
-                store4(p, W * i + 4 * M::NG * w + 4 * g, (int)a.d, a.d % 4 == 0, v);
-            }
+        CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.d, a.d % 4 == 0, v); });
         return;
     }
     T *p = reinterpret_cast<T *>(const_cast<void *>(a.gq.p)) + b * a.gq.b + qh * a.gq.h + qi * a.gq.n;
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int w = 0; w < M::Q; ++w) {
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = dq[i][4 * w + e] * a.gscale;
-            store4(p, W * i + 4 * M::NG * w + 4 * g, (int)a.d, a.vec_out, v);
-        }
+    CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.d, a.vec_out, v * a.gscale); });
 }
 
-template <typename T, int W, int DP, int BM, int MM, int OCC>
-__global__ __launch_bounds__(kThreads, OCC) void attention_dkv_kernel(const Args a) {
+template <typename T, int W, int DP, int BM, int MM, int kWaves, int OCC, bool VLDS, int OUT>
+__global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const Args a) {
     using M = Mma<T, W>;
     using Acc = typename M::Acc;
+    using CR = ColReader<T, DP, W>;
     constexpr int DB = DP / W, QS = DP / M::KS, NU = kUnit / W, ST = kUnit / M::KS;
     constexpr uint32_t kTileBytes = BM * DP * sizeof(T), kBuf = 2 * kTileBytes + 3 * 64 * 4;
     static_assert(BM <= 64, "one DMA of row values per array");
-    __shared__ uint4 smem[2 * kBuf / 16];  // two buffers of a q tile, a do tile and the row values
+    constexpr uint32_t kValues = VLDS ? kWaves * W * DP * sizeof(T) : 0;
+    // two buffers of a q tile, a do tile and the row values; the block's value rows
+    __shared__ uint4 smem[(2 * kBuf + kValues) / 16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane / W;
     int64_t t = xcd_linear(blockIdx.x, gridDim.x);
     const int64_t part = t % a.splits;
     t /= a.splits;
-    const int64_t tile = t % a.tiles;  // first keys of a causal call first: most rows see them
+    // A causal call's first keys are seen by the most rows.  They come first, and the second half of the
+    // tiles comes in reverse, so that where two blocks share a CU a long one and a short one do.
+    const int64_t half = (a.tiles + 1) / 2, tt = t % a.tiles, tile = tt < half ? tt : a.tiles - 1 - (tt - half);
     const int64_t bk = t / a.tiles, b = bk / a.key_heads, kh = bk % a.key_heads;
     const int64_t len = key_end(a, b), all = a.batch * a.heads * a.n;
+    const int rows = (int)a.n;
     const int64_t key0 = tile * (kWaves * W), j = key0 + wave * W + lane % W;
     const bool live = j < len, stored = j < a.m;
 
-    Frag<T> k[QS], v[QS];
+    constexpr bool DK = (OUT & 1) != 0, DV = (OUT & 2) != 0, VREG = DK && !VLDS;
+    Frag<T> k[QS], v[VREG ? QS : 1];
     {
         const T *kr = live ? reinterpret_cast<const T *>(a.k.p) + b * a.k.b + kh * a.k.h + j * a.k.n : nullptr;
         const T *vr = live ? reinterpret_cast<const T *>(a.v.p) + b * a.v.b + kh * a.v.h + j * a.v.n : nullptr;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
-            k[s] = load_row8(kr, M::KS * s + 8 * g, (int)a.d, a.vec);
-            v[s] = load_row8(vr, M::KS * s + 8 * g, (int)a.dv, a.vec);
+            k[s] = load_row8(kr, M::KS * s + 8 * g, (int)a.d);
+            if constexpr (VREG) v[s] = load_row8(vr, M::KS * s + 8 * g, (int)a.dv);
             if (a.qsign != 1.0f) {
                 float x[8];
                 unpack8(k[s], x);
@@ -268,9 +271,12 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dkv_kernel(const Args
     wfirst = __builtin_amdgcn_readfirstlane(wfirst);
     wlast = __builtin_amdgcn_readfirstlane(wlast);
 
-    Acc dk[DB], dv[DB];
+    Acc dk[DK ? DB : 1], dv[DV ? DB : 1];
 #pragma unroll
-    for (int i = 0; i < DB; ++i) dk[i] = dv[i] = Acc{};
+    for (int i = 0; i < DB; ++i) {
+        if constexpr (DK) dk[i] = Acc{};
+        if constexpr (DV) dv[i] = Acc{};
+    }
 
     // row tiles of each head from the first that sees a key of this block
     const int nt = (int)cdiv_dev(a.n, BM);
@@ -282,8 +288,8 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dkv_kernel(const Args
 
     const uint32_t lds = tile::lds_addr(smem);
     Stager<T, DP, BM, kWaves> sq, sg;
-    sq.init(a.q.n, (int)a.d, a.vec, wave, lane);
-    sg.init(a.go.n, (int)a.dv, a.vec, wave, lane);
+    sq.init(a.q.n, (int)a.d, wave, lane);
+    sg.init(a.go.n, (int)a.dv, wave, lane);
     int hd = per ? (int)(i0 / per) : 0, rt = per ? tf + (int)(i0 % per) : 0;  // the next tile to fetch
     const auto fetch = [&](int64_t it) {
         const int64_t qh = kh * a.group + hd, r0 = (int64_t)rt * BM;
@@ -298,7 +304,13 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dkv_kernel(const Args
         }
     };
     const RowReader<T, DP, W> rr(lane);
-    const ColReader<T, DP, W> cr(lane);
+    const CR cr(lane);
+    const uint32_t vt = lds + 2 * kBuf;
+    if constexpr (VLDS) {
+        Stager<T, DP, kWaves * W, kWaves> sv;
+        sv.init(a.v.n, (int)a.dv, wave, lane);
+        sv.load(reinterpret_cast<const T *>(a.v.p) + b * a.v.b + kh * a.v.h + key0 * a.v.n, len - key0, vt);
+    }
     if (i0 < i1) fetch(i0);
     for (int64_t it = i0; it < i1; ++it) {
         const int64_t qh = kh * a.group + hd;
@@ -313,45 +325,38 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dkv_kernel(const Args
 #pragma unroll
         for (int u = 0; u < BM / kUnit; ++u) {
             const int u0 = r0 + u * kUnit;
-            if (u0 + kUnit <= wfirst || u0 >= a.n) continue;
+            if (u0 + kUnit <= wfirst || u0 >= rows) continue;
+            // the mask's bits of this key, rows u0 .. u0 + 31
+            const uint32_t word = MM == kKeep && live ? a.mask_cols[b * a.cb + qh * a.ch + u0 / 32 * a.cn + j] : 0;
             Acc s[NU], dp[NU];
 #pragma unroll
             for (int i = 0; i < NU; ++i) s[i] = dp[i] = Acc{};
+            constexpr int F1 = DK ? VLDS ? 3 : 2 : 1, F2 = DK && DV ? 2 : 1;
+            stream_steps<QS * NU, F1, Frag<T>>(
+                [&](int x, Frag<T>(&f)[F1]) {
+                    f[0] = rr.read(qt, u * NU + x % NU, x / NU);
+                    if constexpr (DK) f[1] = rr.read(gt, u * NU + x % NU, x / NU);
+                    if constexpr (DK && VLDS) f[2] = rr.read(vt, wave, x / NU);
+                },
+                [&](int x, const Frag<T>(&f)[F1]) {
+                    M::mma(s[x % NU], f[0], k[x / NU]);
+                    if constexpr (VREG) M::mma(dp[x % NU], f[1], v[x / NU]);
+                    if constexpr (DK && VLDS) M::mma(dp[x % NU], f[1], f[2]);
+                });
+            if constexpr (MM == kKeep) {
+                const uint32_t keep = word >> (4 * g);
 #pragma unroll
-            for (int f = 0; f < QS; ++f)
+                for (int x = 0; x < 32 / (4 * M::NG); ++x)
 #pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    M::mma(s[i], rr.read(qt, u * NU + i, f), k[f]);
-                    M::mma(dp[i], rr.read(gt, u * NU + i, f), v[f]);
-                }
-            if constexpr (MM != kNoMask) {
-                const uint8_t *mr = reinterpret_cast<const uint8_t *>(
-                    mask_row(a, b, qh, 0, MM == kKeep ? 1 : a.mask_bf16 ? 2 : 4));
-#pragma unroll
-                for (int i = 0; i < NU; ++i)
-#pragma unroll
-                    for (int w = 0; w < M::Q; ++w)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int64_t r = u0 + W * i + 4 * M::NG * w + 4 * g + e;
-                            const bool in = live && r < a.n;
-                            const int64_t at = r * a.mn + j * a.mm;
-                            float x = s[i][4 * w + e];
-                            bool off;
-                            if constexpr (MM == kKeep) {
-                                off = !in || !mr[at];
-                            } else {
-                                const float add = !in ? 0.0f
-                                                  : a.mask_bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(mr)[at])
-                                                                : reinterpret_cast<const float *>(mr)[at];
-                                off = add == -INFINITY;
-                                x = x * a.scale + add;
-                            }
-                            s[i][4 * w + e] = off ? -INFINITY : x;
-                            if (off) dp[i][4 * w + e] = 0.0f;
+                    for (int e = 0; e < 4; ++e)
+                        if (!(keep & (1u << (4 * M::NG * x + e)))) {
+                            const int at = 4 * M::NG * x;
+                            s[at / W][4 * (at % W / (4 * M::NG)) + e] = -INFINITY;
+                            dp[at / W][4 * (at % W / (4 * M::NG)) + e] = 0.0f;
                         }
             }
-            if (u0 < wlast || u0 + kUnit > a.n) {
+            if constexpr (MM == kBias) {
+                const uint8_t *mr = reinterpret_cast<const uint8_t *>(mask_row(a, b, qh, 0));
 #pragma unroll
                 for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -359,7 +364,25 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dkv_kernel(const Args
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = u0 + W * i + 4 * M::NG * w + 4 * g + e;
-                            if (r < first || r >= a.n) {
+                            const int64_t at = r * a.mn + j * a.mm;
+                            const float add = !(live && r < rows) ? 0.0f
+                                              : a.mask_bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(mr)[at])
+                                                            : reinterpret_cast<const float *>(mr)[at];
+                            const bool off = add == -INFINITY;
+                            s[i][4 * w + e] = off ? -INFINITY : s[i][4 * w + e] * a.scale + add;
+                            if (off) dp[i][4 * w + e] = 0.0f;
+                        }
+            }
+            if (u0 < wlast || u0 + kUnit > rows) {
+                asm volatile("");  // a branch: most units skip this
+#pragma unroll
+                for (int i = 0; i < NU; ++i)
+#pragma unroll
+                    for (int w = 0; w < M::Q; ++w)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = u0 + W * i + 4 * M::NG * w + 4 * g + e;
+                            if (r < first || r >= rows) {
                                 s[i][4 * w + e] = -INFINITY;
                                 dp[i][4 * w + e] = 0.0f;
                             }
@@ -383,6 +406,7 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dkv_kernel(const Args
                         s[i][4 * w + e] = p * (dp[i][4 * w + e] - delta[e]);
                     }
                 }
+            Frag<T> p[ST], ds[ST];
 #pragma unroll
             for (int st = 0; st < ST; ++st) {
                 float y[8], z[8];
@@ -393,73 +417,80 @@ __global__ __launch_bounds__(kThreads, OCC) void attention_dkv_kernel(const Args
                         y[4 * h + e] = x[2 * st + h][e];
                         z[4 * h + e] = s[(2 * st + h) / M::Q][4 * ((2 * st + h) % M::Q) + e];
                     }
-                const Frag<T> p = pack8(y, T{}), ds = pack8(z, T{});
-#pragma unroll
-                for (int i = 0; i < DB; ++i) {
-                    M::mma(dv[i], cr.read(gt, u * ST + st, i), p);
-                    M::mma(dk[i], cr.read(qt, u * ST + st, i), ds);
-                }
+                p[st] = pack8(y, T{});
+                ds[st] = pack8(z, T{});
             }
+            constexpr int kPieces = CR::kPieces;
+            stream_steps<ST * kPieces, F2, typename CR::Piece>(
+                [&](int x, typename CR::Piece(&f)[F2]) {
+                    if constexpr (DV) f[0] = cr.read(gt, u * ST + x / kPieces, x % kPieces);
+                    if constexpr (DK) f[F2 - 1] = cr.read(qt, u * ST + x / kPieces, x % kPieces);
+                },
+                [&](int x, const typename CR::Piece(&f)[F2]) {
+                    if constexpr (DV) CR::use(dv, x % kPieces, f[0], p[x / kPieces]);
+                    if constexpr (DK) CR::use(dk, x % kPieces, f[F2 - 1], ds[x / kPieces]);
+                });
         }
     }
     if (!stored) return;
-    if (a.splits > 1) {
-        const int64_t keys = a.batch * a.key_heads * a.m, row = (b * a.key_heads + kh) * a.m + j;
-        float *pk = a.part + (part * keys + row) * (a.d + a.dv), *pv = pk + a.d;
-#pragma unroll
-        for (int i = 0; i < DB; ++i)
-#pragma unroll
-            for (int w = 0; w < M::Q; ++w) {
-                f32x4 x, y;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[e] = dk[i][4 * w + e];
-                    y[e] = dv[i][4 * w + e];
-                }
-                const int f = W * i + 4 * M::NG * w + 4 * g;
-                const int v4 = a.d % 4 == 0 && a.dv % 4 == 0;
-                store4(pk, f, (int)a.d, v4, x);
-                store4(pv, f, (int)a.dv, v4, y);
-            }
-        return;
-    }
-    T *pk = reinterpret_cast<T *>(const_cast<void *>(a.gk.p)) + b * a.gk.b + kh * a.gk.h + j * a.gk.n;
-    T *pv = reinterpret_cast<T *>(const_cast<void *>(a.gv.p)) + b * a.gv.b + kh * a.gv.h + j * a.gv.n;
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int w = 0; w < M::Q; ++w) {
-            f32x4 x, y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = dk[i][4 * w + e] * a.gscale;
-                y[e] = dv[i][4 * w + e];
-            }
-            const int f = W * i + 4 * M::NG * w + 4 * g;
-            store4(pk, f, (int)a.d, a.vec_out, x);
-            store4(pv, f, (int)a.dv, a.vec_out, y);
-        }
+    const int64_t keys = a.batch * a.key_heads * a.m, row = (b * a.key_heads + kh) * a.m + j;
+    const auto store = [&](const Acc *acc, int64_t width, int64_t at, const View &out, float scale) {
+        float *part_row = a.part + (part * keys + row) * (a.d + a.dv) + at;
+        T *out_row = reinterpret_cast<T *>(const_cast<void *>(out.p)) + b * out.b + kh * out.h + j * out.n;
+        CR::each(acc, lane, [&](int f, f32x4 x) {
+            if (a.splits > 1)
+                store4(part_row, f, (int)width, a.d % 4 == 0 && a.dv % 4 == 0, x);
+            else
+                store4(out_row, f, (int)width, a.vec_out, x * scale);
+        });
+    };
+    if constexpr (DK) store(dk, a.d, 0, a.gk, a.gscale);
+    if constexpr (DV) store(dv, a.dv, a.d, a.gv, 1.0f);
 }
 
-// Sums the parts of the gradients, in their order, one thread per four features: rows of `width`
-// fp32 values of which this output takes `d` from `at`, times `scale`.
+// Sums the parts of one or two gradients, in their order, one thread per four features: rows of fp32
+// values, the first output's features, then the second's.
+struct SumArgs {
+    const float *part;
+    View out[2];
+    int64_t width[2];
+    float scale[2];
+    int64_t rows, heads, n;
+    int splits, vec_out;
+};
 template <typename T>
-__global__ void attention_sum_kernel(const float *part, int splits, int64_t rows, int64_t width, int64_t at, int64_t d,
-                                     float scale, View out, int64_t heads, int64_t n, int vec) {
-    const int64_t quads = (d + 3) / 4, id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (id >= rows * quads) return;
-    const int64_t row = id / quads;
-    const int f = (int)(id % quads) * 4;
+__global__ __launch_bounds__(256) void attention_sum_kernel(const SumArgs a) {
+    constexpr int U = 8;
+    const int64_t q0 = cdiv_dev(a.width[0], 4), quads = q0 + cdiv_dev(a.width[1], 4);
+    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, row = id / quads;
+    if (row >= a.rows) return;
+    const int which = id % quads >= q0, f = (int)(id % quads - (which ? q0 : 0)) * 4;
+    const int64_t all = a.width[0] + a.width[1], d = which ? a.width[1] : a.width[0];
+    const float *p = a.part + row * all + (which ? a.width[0] : 0) + f;
+    const bool vec = a.width[0] % 4 == 0 && a.width[1] % 4 == 0;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < splits; ++s) {
-        const float *p = part + (s * rows + row) * width + at + f;
+    for (int s0 = 0; s0 < a.splits; s0 += U) {
+        f32x4 y[U];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (f + e < d) x[e] += p[e];
+        for (int u = 0; u < U; ++u) {
+            y[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (s0 + u >= a.splits) continue;
+            const float *q = p + (s0 + u) * a.rows * all;
+            if (vec) {
+                y[u] = *reinterpret_cast<const f32x4 *>(q);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (f + e < d) y[u][e] = q[e];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) x += y[u];
     }
-    const int64_t i = row % n, h = row / n % heads, b = row / n / heads;
-    x *= scale;
-    store4(reinterpret_cast<T *>(const_cast<void *>(out.p)) + b * out.b + h * out.h + i * out.n, f, (int)d, vec, x);
+    const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
+    const View out = which ? a.out[1] : a.out[0];
+    store4(reinterpret_cast<T *>(const_cast<void *>(out.p)) + b * out.b + h * out.h + i * out.n, f, (int)d, a.vec_out,
+           x * (which ? a.scale[1] : a.scale[0]));
 }
 
 }  // namespace attn
@@ -477,11 +508,12 @@ struct BackwardPlan {
 template <typename T, int DP>
 BackwardPlan backward_plan(const Args &a) {
     BackwardPlan p;
-    const int64_t own = (int64_t)kWaves * Tiles<T, DP>::kWidth, bk = a.batch * a.key_heads;
-    p.q_tiles = cdiv(a.n * a.group, own);
-    p.k_tiles = cdiv(a.m, own);
-    p.q_splits = (int)parts_for(bk * p.q_tiles, cdiv(a.m, Tiles<T, DP>::kKeys));
-    p.k_splits = (int)parts_for(bk * p.k_tiles, a.group * cdiv(a.n, Tiles<T, DP>::kRows));
+    using L = Tiles<T, DP>;
+    const int64_t bk = a.batch * a.key_heads;
+    p.q_tiles = cdiv(a.n * a.group, (int64_t)L::kWaves * L::kWidth);
+    p.k_tiles = cdiv(a.m, (int64_t)L::kRowWaves * L::kWidth);
+    p.q_splits = (int)parts_for(bk * p.q_tiles, cdiv(a.m, L::kKeys), L::kPerCuQ);
+    p.k_splits = (int)parts_for(bk * p.k_tiles, a.group * cdiv(a.n, L::kRows), L::kPerCuK);
     return p;
 }
 int64_t round4(int64_t x) { return (x + 3) / 4 * 4; }
@@ -493,10 +525,9 @@ size_t backward_workspace(const Args &a, const BackwardPlan &p) {
 }
 
 template <typename T>
-int sum_parts(const Args &a, int64_t rows, int64_t width, int64_t at, int64_t d, float scale, const View &out,
-              int64_t heads, int64_t n, hipStream_t s) {
-    hipLaunchKernelGGL((attention_sum_kernel<T>), dim3((unsigned)cdiv(rows * cdiv(d, 4), 256)), dim3(256), 0, s, a.part,
-                       a.splits, rows, width, at, d, scale, out, heads, n, a.vec_out);
+int sum_parts(const SumArgs &a, hipStream_t s) {
+    const int64_t threads = a.rows * (cdiv(a.width[0], 4) + cdiv(a.width[1], 4));
+    hipLaunchKernelGGL((attention_sum_kernel<T>), dim3((unsigned)cdiv(threads, 256)), dim3(256), 0, s, a);
     return check_launch("attention_sum_kernel");
 }
 
@@ -507,7 +538,7 @@ extern "C" size_t tpw_attention_backward_workspace_size(const tpw_attention_desc
     if (read_args(d, true, a) != TPW_OK) return 0;
     size_t bytes = 0;
     by_type(a, d->dtype, kNoMask, [&](auto t, auto dp, auto) {
-        bytes = backward_workspace(a, backward_plan<decltype(t), decltype(dp)::value>(a));
+        bytes = prepared_bytes(a, d, true) + backward_workspace(a, backward_plan<decltype(t), decltype(dp)::value>(a));
         return TPW_OK;
     });
     return bytes;
@@ -523,35 +554,49 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
     TPW_REQUIRE(d->mask_type == TPW_MASK_NONE || a.mask || a.m == 0, "attention: null mask");
     TPW_REQUIRE(workspace && aligned16(workspace), "attention backward: null or unaligned workspace");
     hipStream_t s = as_stream(stream);
+    const size_t prepared = prepared_bytes(a, d, true);
+    if (prepared)
+        if (const int rc = prepare_operands(a, d, true, workspace, s)) return rc;
     return by_type(a, d->dtype, mask_mode(d), [&](auto t, auto dp, auto mode) {
         using T = decltype(t);
         constexpr int DP = decltype(dp)::value, MM = decltype(mode)::value, W = Tiles<T, DP>::kWidth;
-        constexpr int kOcc = DP == 256 ? 1 : 2;
+        constexpr int kOcc = sizeof(T) == 2 && DP == 256 ? 1 : 2, kOccKv = DP == 256 ? 1 : 2;
         const BackwardPlan p = backward_plan<T, DP>(a);
         const int64_t bk = a.batch * a.key_heads;
         TPW_REQUIRE(bk * p.q_tiles * p.q_splits < (int64_t(1) << 31) && bk * p.k_tiles * p.k_splits < (int64_t(1) << 31),
                     "attention: too many rows");
-        a.rows = reinterpret_cast<float *>(workspace);
+        a.rows = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + prepared);
         a.part = a.rows + round4(3 * rows);
         if (rows) {
             a.tiles = p.q_tiles;
             a.splits = p.q_splits;
-            hipLaunchKernelGGL((attention_dq_kernel<T, W, DP, Tiles<T, DP>::kKeys, MM, kOcc>),
-                               dim3((unsigned)(bk * a.tiles * a.splits)), dim3(attn::kThreads), 0, s, a);
+            constexpr int kWaves = Tiles<T, DP>::kWaves;
+            hipLaunchKernelGGL((attention_dq_kernel<T, W, DP, Tiles<T, DP>::kKeys, MM, kWaves, kOcc>),
+                               dim3((unsigned)(bk * a.tiles * a.splits)), dim3(64 * kWaves), 0, s, a);
             if (const int rc = check_launch("attention_dq_kernel")) return rc;
             if (a.splits > 1)
-                if (const int rc = sum_parts<T>(a, rows, a.d, 0, a.d, a.gscale, a.gq, a.heads, a.n, s)) return rc;
+                if (const int rc = sum_parts<T>(
+                        {a.part, {a.gq, {}}, {a.d, 0}, {a.gscale, 0.0f}, rows, a.heads, a.n, a.splits, a.vec_out}, s))
+                    return rc;
         }
         if (keys) {
             a.tiles = p.k_tiles;
             a.splits = p.k_splits;
-            hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, Tiles<T, DP>::kRows, MM, kOcc>),
-                               dim3((unsigned)(bk * a.tiles * a.splits)), dim3(attn::kThreads), 0, s, a);
-            if (const int rc = check_launch("attention_dkv_kernel")) return rc;
-            if (a.splits > 1) {
-                if (const int rc = sum_parts<T>(a, keys, a.d + a.dv, 0, a.d, a.gscale, a.gk, a.key_heads, a.m, s)) return rc;
-                return sum_parts<T>(a, keys, a.d + a.dv, a.d, a.dv, 1.0f, a.gv, a.key_heads, a.m, s);
+            const dim3 grid((unsigned)(bk * a.tiles * a.splits)), block(64 * Tiles<T, DP>::kRowWaves);
+            // bf16 at 256 features: dk and dv would take all 256 accumulation registers and leave none for
+            // the scores, so each is a launch of its own
+            constexpr bool kApart = sizeof(T) == 2 && DP == 256;
+            constexpr int kRows = Tiles<T, DP>::kRows, kWaves = Tiles<T, DP>::kRowWaves;
+            if constexpr (kApart) {
+                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, 2, false, 2>), grid, block, 0, s, a);
+                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, 1, false, 1>), grid, block, 0, s, a);
+            } else {
+                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, kOccKv, DP == 128, 3>), grid, block, 0, s, a);
             }
+            if (const int rc = check_launch("attention_dkv_kernel")) return rc;
+            if (a.splits > 1)
+                return sum_parts<T>({a.part, {a.gk, a.gv}, {a.d, a.dv}, {a.gscale, 1.0f}, keys, a.key_heads, a.m, a.splits,
+                                     a.vec_out}, s);
         }
         return TPW_OK;
     });
