@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
     using F = Forward<T, W, DP, BN, MM>;
     using M = typename F::M;
     constexpr uint32_t kTileBytes = BN * DP * sizeof(T);
-    __shared__ uint4 smem[4 * kTileBytes / 16];  // two buffers of a key tile and a value tile
+    __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];  // two buffers of a key tile and a value tile
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     int64_t t = xcd_linear(blockIdx.x, gridDim.x);
     const int64_t part = t % a.splits;
@@ -214,8 +214,8 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
             st[row] = f.top;
             st[all + row] = sum;
         }
-        float *p = a.part + (part * all + row) * a.dv;
-        F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.dv, a.dv % 4 == 0, v); });
+        float *p = a.part + (part * all + row) * quads4(a.dv);
+        F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.dv, 1, v); });
         return;
     }
     if (g == 0 && a.stats) {
@@ -227,53 +227,89 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
 }
 
 // Joins the parts of every row: m = max m_s, l = sum l_s 2^(m_s - m), o = sum o_s 2^(m_s - m) / l.
-// One wave per row: lane s holds part s's weight; then LANES lanes of four features each, 64 / LANES
-// parts at a time, in an order that the sizes fix.
+// One block per row: lane s of every wave holds part s's weight; then LANES lanes of four features
+// each, 256 / LANES parts at a time, in an order that the sizes fix.
 template <typename T, bool BIAS, int LANES>
 __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
-    const int64_t rows = a.batch * a.heads * a.n, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 63, f = lane % LANES * 4;
+    constexpr int G = 256 / LANES, U = kMaxParts / G < 8 ? kMaxParts / G : 8;
+    __shared__ f32x4 waves[3][LANES];
+    const int64_t rows = a.batch * a.heads * a.n, row = blockIdx.x, pitch = quads4(a.dv);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, f = lane % LANES * 4;
     const float top_s = lane < a.splits ? a.part_stats[2 * lane * rows + row] : -INFINITY;
     const float sum_s = lane < a.splits ? a.part_stats[(2 * lane + 1) * rows + row] : 0.0f;
     const float top = over_groups_max<1>(top_s);
     const float base = top == -INFINITY ? 0.0f : top;
     const float w = __builtin_amdgcn_exp2f(BIAS ? (top_s - base) * kLog2e : top_s - base);
     const float sum = over_groups_sum<1>(lane < a.splits ? w * sum_s : 0.0f);
-    constexpr int G = 64 / LANES, U = 8;
-    const float *p = a.part + row * a.dv + f;
+    const float *p = a.part + row * pitch + f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < a.splits; s0 += G * U) {
         f32x4 x[U];
         float c[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = s0 + G * u + lane / LANES;
+            const int s = s0 + G * u + (int)threadIdx.x / LANES;
             const bool in = s < a.splits;
             c[u] = __shfl(w, in ? s : 0, 64);
-            x[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (in) {
-                const float *q = p + s * rows * a.dv;
-                if (a.dv % 4 == 0) {
-                    if (f < a.dv) x[u] = *reinterpret_cast<const f32x4 *>(q);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (f + e < a.dv) x[u][e] = q[e];
-                }
-            }
+            x[u] = in && f < a.dv ? *reinterpret_cast<const f32x4 *>(p + s * rows * pitch) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) o += x[u] * c[u];
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = over_groups_sum<LANES>(o[e]);
+    if (wave > 0 && lane < LANES) waves[wave - 1][lane] = o;
+    __syncthreads();
+    if ((int)threadIdx.x >= LANES) return;
+#pragma unroll
+    for (int v = 0; v < 3; ++v) o += waves[v][lane];
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     if (lane == 0 && a.stats) {
         a.stats[row] = top;
         a.stats[rows + row] = sum;
     }
-    if (lane >= LANES) return;
+    const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
+    T *out = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + b * a.o.b + h * a.o.h + i * a.o.n;
+    store4(out, f, (int)a.dv, a.vec_out, o * inv);
+}
+
+// The same for at most kFew parts: one thread per four features, every load in flight at once
+// (32 x 4096 rows of 64 features in two parts: 30 us, where a wave per row takes 80).
+constexpr int kFew = 8;
+template <typename T, bool BIAS>
+__global__ __launch_bounds__(256) void attention_join_few_kernel(const Args a) {
+    const int64_t rows = a.batch * a.heads * a.n, quads = cdiv_dev(a.dv, 4);
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / quads;
+    if (row >= rows) return;
+    const int f = (int)(id % quads) * 4;
+    float top_s[kFew], sum_s[kFew];
+    f32x4 x[kFew];
+#pragma unroll
+    for (int s = 0; s < kFew; ++s) {
+        top_s[s] = -INFINITY;
+        sum_s[s] = 0.0f;
+        x[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (s >= a.splits) continue;
+        top_s[s] = a.part_stats[2 * s * rows + row];
+        sum_s[s] = a.part_stats[(2 * s + 1) * rows + row];
+        x[s] = *reinterpret_cast<const f32x4 *>(a.part + (s * rows + row) * (4 * quads) + f);
+    }
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kFew; ++s) top = __builtin_fmaxf(top, top_s[s]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < kFew; ++s) {
+        const float w = __builtin_amdgcn_exp2f(BIAS ? (top_s[s] - base) * kLog2e : top_s[s] - base);
+        sum += w * sum_s[s];
+        o += x[s] * w;
+    }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    if (f == 0 && a.stats) {
+        a.stats[row] = top;
+        a.stats[rows + row] = sum;
+    }
     const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
     T *out = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + b * a.o.b + h * a.o.h + i * a.o.n;
     store4(out, f, (int)a.dv, a.vec_out, o * inv);
@@ -403,7 +439,7 @@ int64_t plan_bits(Args &a, bool backward, uint8_t *at, BitArgs *p) {
 template <typename T, int DP>
 void plan(Args &a) {
     a.tiles = cdiv(a.n * a.group, (int64_t)Tiles<T, DP>::kWaves * Tiles<T, DP>::kWidth);
-    a.splits = (int)parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, Tiles<T, DP>::kKeys), Tiles<T, DP>::kPerCu);
+    a.splits = (int)parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, Tiles<T, DP>::kKeys), Tiles<T, DP>::kPerCu, uneven(a));
 }
 
 }  // namespace
@@ -498,7 +534,7 @@ using namespace tpw::attn;
 namespace {
 
 size_t forward_workspace(const Args &a) {
-    return a.splits > 1 ? (size_t)a.splits * a.batch * a.heads * a.n * (a.dv + 2) * 4 : 0;
+    return a.splits > 1 ? (size_t)a.splits * a.batch * a.heads * a.n * (quads4(a.dv) + 2) * 4 : 0;
 }
 
 }  // namespace
@@ -536,7 +572,7 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
         if (a.splits > 1) {
             TPW_REQUIRE(workspace && aligned16(workspace), "attention: null or unaligned workspace");
             a.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + prepared);
-            a.part_stats = a.part + a.splits * rows * a.dv;
+            a.part_stats = a.part + a.splits * rows * quads4(a.dv);
         }
         constexpr int kOcc = 2;
         constexpr int kWaves = Tiles<T, DP>::kWaves;
@@ -544,7 +580,11 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
                            dim3(64 * kWaves), 0, s, a);
         if (const int rc = check_launch("attention_kernel")) return rc;
         if (a.splits > 1) {
-            hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, DP / 4>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a);
+            if (a.splits <= kFew)
+                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias>), dim3((unsigned)cdiv(rows * cdiv(a.dv, 4), 256)),
+                                   dim3(256), 0, s, a);
+            else
+                hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, DP / 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
             return check_launch("attention_join_kernel");
         }
         return TPW_OK;

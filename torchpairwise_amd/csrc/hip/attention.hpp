@@ -54,8 +54,8 @@ struct Args {
     int vec_out;   // the outputs' rows take stores of four features
     int64_t tiles;  // row tiles (dk / dv: key tiles) per (batch, key head)
     int splits;     // parts of the summed axis
-    float *part;    // [splits, ...] partial results where splits > 1
-    float *part_stats;
+    float *part;    // [splits, rows, features] partial results where splits > 1, rows of whole quads
+    float *part_stats;  // [splits, 2, rows]
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -86,14 +86,6 @@ struct Mma<uint16_t, 32> : Shape<32> {
     typedef floatx16 Acc;
     static __device__ __forceinline__ void mma(Acc &acc, const Frag<uint16_t> &a, const Frag<uint16_t> &b) {
         acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v),
-                                                      acc, 0, 0, 0);
-    }
-};
-template <>
-struct Mma<uint16_t, 16> : Shape<16> {
-    typedef f32x4 Acc;
-    static __device__ __forceinline__ void mma(Acc &acc, const Frag<uint16_t> &a, const Frag<uint16_t> &b) {
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v),
                                                       acc, 0, 0, 0);
     }
 };
@@ -130,16 +122,25 @@ __device__ __forceinline__ void unpack8(const Frag<float> &f, float (&x)[8]) {
 
 // ---- LDS tiles -----------------------------------------------------------------------------
 // A tile of ROWS rows of DP features lies as 16-byte pieces, piece c of row r at position
-// c ^ swz(r): eight consecutive rows put one piece into eight different 16-byte slots (row
-// fragments), and four consecutive rows put a pair of pieces into four different pairs
-// (transposing reads), so neither read meets a bank twice.
-__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
-
+// c ^ swz(r).  Every 16 consecutive rows put one piece into the 16 different 16-byte slots of the 64
+// banks (row fragments), and four consecutive rows put a run of four pieces into four different
+// quarters of them (transposing reads), so that either read moves 256 bytes a cycle.
 template <typename T, int DP>
 struct Tile {
     static constexpr int E = 16 / (int)sizeof(T);  // elements per piece
     static constexpr int C = DP / E;               // pieces per row
     static constexpr int kRowBytes = DP * (int)sizeof(T);
+    static constexpr int kMask = C >= 16 ? 15 : 7;  // bits of a piece's index that swz reaches
+    static_assert(C >= 8, "rows of 128 bytes at least");
+    // rows of 128 bytes: two rows share the banks, so the pairs of rows take turns
+    static __host__ __device__ constexpr int swz(int r) {
+        return C >= 16 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    }
+    // Address of piece c ^ (what `base` holds): base is 256-byte aligned but for a lane's own bits of
+    // the piece, which differ from c's.
+    static __device__ __forceinline__ uint32_t piece(uint32_t base, int c, int far) {
+        return (base ^ (uint32_t)((c & kMask) * 16)) + (uint32_t)((c & ~kMask) * 16 + far);
+    }
 };
 
 constexpr uint32_t kRange = 0x7ffffff0u;  // bytes a tile's buffer resource spans at most
@@ -183,7 +184,7 @@ struct Stager {
         wave = wave_;
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
-            const int s = (i * WAVES + wave) * 64 + lane, r = s / L::C, c = (s % L::C) ^ swz(r);
+            const int s = (i * WAVES + wave) * 64 + lane, r = s / L::C, c = (s % L::C) ^ L::swz(r);
             off[i] = c * L::E < d ? (uint32_t)(r * stride + c * 16) : kBeyond;
         }
     }
@@ -198,32 +199,27 @@ __device__ __forceinline__ tpw_u32x4 lds_read16(uint32_t a) {
     return *reinterpret_cast<__attribute__((address_space(3))) const tpw_u32x4 *>((uintptr_t)a);
 }
 
-// Row fragments: features KS s + 8 g .. + 7 of row lane % W of a block of W rows.  Of the piece's
-// index only the low three bits meet swz, so a few lane addresses and immediate offsets reach all.
+// Row fragments: features KS s + 8 g .. + 7 of row lane % W of a block of W rows.  A lane's own part
+// of the address is one register; pieces differ from it by an exclusive or of a constant.
 template <typename T, int DP, int W>
 struct RowReader {
     using L = Tile<T, DP>;
     using S = Shape<W>;
-    static constexpr int P = 8 / L::E, kStep = S::NG * P;           // pieces per fragment, per step
-    static constexpr int kAddr = kStep < 8 ? 8 / kStep : 1;         // steps until the low bits repeat
-    uint32_t at[kAddr][P];
+    static constexpr int P = 8 / L::E;  // pieces per fragment
+    uint32_t at;
     __device__ __forceinline__ RowReader(int lane) {
-        const int r = lane % W, x = swz(r), g = lane / W;
-#pragma unroll
-        for (int s = 0; s < kAddr; ++s)
-#pragma unroll
-            for (int u = 0; u < P; ++u)
-                at[s][u] = (uint32_t)(r * L::kRowBytes + ((kStep * s + P * g + u) ^ x) * 16);
+        const int r = lane % W;
+        at = (uint32_t)(r * L::kRowBytes + ((P * (lane / W)) ^ L::swz(r)) * 16);
     }
-    // block `blk` of the tile at `tile` (swz(r) depends on r mod 8 only, and W is a multiple of 8)
+    // block `blk` of the tile at `tile` (swz(r) depends on r mod 16 only, and W is a multiple of 16)
     __device__ __forceinline__ Frag<T> read(uint32_t tile, int blk, int s) const {
-        const uint32_t far = (uint32_t)(blk * W * L::kRowBytes + s / kAddr * kAddr * kStep * 16);
         Frag<T> f;
         if constexpr (sizeof(T) == 2) {
-            f.v = __builtin_bit_cast(uint4, lds_read16(tile + at[s % kAddr][0] + far));
+            f.v = __builtin_bit_cast(uint4, lds_read16(L::piece(tile + at, S::NG * s, blk * W * L::kRowBytes)));
         } else {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) f.v[u] = __builtin_bit_cast(f32x4, lds_read16(tile + at[s % kAddr][u] + far));
+            for (int u = 0; u < 2; ++u)
+                f.v[u] = __builtin_bit_cast(f32x4, lds_read16(L::piece(tile + at, 2 * S::NG * s + u, blk * W * L::kRowBytes)));
         }
         return f;
     }
@@ -240,28 +236,24 @@ struct RowReader {
 // `each` gives the results back as quads of consecutive features.
 template <typename T, int DP, int W>
 struct ColReader;
-template <int DP, int W>
-struct ColReader<uint16_t, DP, W> {
+template <int DP>
+struct ColReader<uint16_t, DP, 32> {
+    static constexpr int W = 32;
     using L = Tile<uint16_t, DP>;
     using M = Mma<uint16_t, W>;
-    static constexpr int kBlocks = DP / W, kPieces = kBlocks, kAddr = 64 / W;  // blocks until the low bits repeat
+    static constexpr int kBlocks = DP / W, kPieces = kBlocks;
     typedef uint4 Piece;
-    uint32_t at[kAddr];
+    uint32_t at;
     __device__ __forceinline__ ColReader(int lane) {
-        const int i = lane & 15, r0 = 4 * (lane / W) + (i >> 2), x = swz(r0);
-#pragma unroll
-        for (int b = 0; b < kAddr; ++b) {
-            const int col = W * b + 16 * ((lane % W) >> 4) + 4 * (i & 3);
-            at[b] = (uint32_t)(r0 * L::kRowBytes + ((col >> 3) ^ x) * 16 + (col & 4) * 2);
-        }
+        const int i = lane & 15, r0 = 4 * (lane / W) + (i >> 2), col = 16 * ((lane % W) >> 4) + 4 * (i & 3);
+        at = (uint32_t)(r0 * L::kRowBytes + ((col >> 3) ^ L::swz(r0)) * 16 + (col & 4) * 2);
     }
-    // (4 NG (2 t + u) is a multiple of 8, so swz of the whole row index is swz(r0))
     __device__ __forceinline__ Piece read(uint32_t tile, int t, int c) const {
         uint2 v[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const uint32_t a = tile + at[c % kAddr] +
-                               (uint32_t)(4 * M::NG * (2 * t + u) * L::kRowBytes + c / kAddr * kAddr * W * 2);
+            // swz(8 (2 t + u) + r0) = swz(r0) ^ 2 u
+            const uint32_t a = L::piece(tile + at, (4 * c) ^ (2 * u), 8 * (2 * t + u) * L::kRowBytes);
             v[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                  (__attribute__((address_space(3))) s16x4 *)(uintptr_t)a));
         }
@@ -288,20 +280,17 @@ struct ColReader<float, DP, 16> {
     struct Piece {
         f32x4 v[4];
     };
-    uint32_t at[4];
+    uint32_t at;
     __device__ __forceinline__ ColReader(int lane) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int r0 = 4 * (lane / 16) + e;
-            at[e] = (uint32_t)(r0 * L::kRowBytes + ((lane % 16) ^ swz(r0)) * 16);
-        }
+        const int r0 = 4 * (lane / 16);
+        at = (uint32_t)(r0 * L::kRowBytes + ((lane % 16) ^ L::swz(r0)) * 16);
     }
     __device__ __forceinline__ Piece read(uint32_t tile, int t, int c) const {
         Piece p;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e)  // swz(r0 + e) = swz(r0) ^ 4 e
             p.v[e] = __builtin_bit_cast(
-                f32x4, lds_read16(tile + at[e] + (uint32_t)(16 * (2 * t + c % 2) * L::kRowBytes + c / 2 * 256)));
+                f32x4, lds_read16(L::piece(tile + at, (c / 2 * 16) ^ (4 * e), (16 * (2 * t + c % 2) + e) * L::kRowBytes)));
         return p;
     }
     static __device__ __forceinline__ void use(M::Acc *acc, int c, const Piece &a, const Frag<float> &p) {
@@ -426,6 +415,7 @@ __device__ __forceinline__ f32x4 mask_bias4(const Args &a, const void *row, int6
 }
 
 __device__ __forceinline__ int64_t cdiv_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__host__ __device__ inline int64_t quads4(int64_t x) { return (x + 3) / 4 * 4; }
 
 // Block id -> (tile, batch * key_heads + key head): ids go round-robin over the 8 XCDs, so where
 // they divide, each XCD gets a contiguous range: the blocks that share keys share an L2.
@@ -445,7 +435,7 @@ struct Tiles {
     // blocks that share a CU: forward, dq, dk / dv
     static constexpr bool kNarrow = DP * (int)sizeof(T) == 128;  // bf16 at 64 features
     static constexpr int kPerCu = kNarrow ? 4 : kWaves == 8 ? 1 : 2;
-    static constexpr int kPerCuQ = kNarrow ? 4 : DP == 256 ? 1 : 2;
+    static constexpr int kPerCuQ = kNarrow ? 3 : DP == 256 ? 1 : 2;
     static constexpr int kPerCuK = DP == 256 || (DP == 128 && sizeof(T) == 4) ? 1 : 2;
 };
 
@@ -482,11 +472,14 @@ inline int mask_mode(const tpw_attention_desc *d) {
 }
 // Parts of a summed axis of `steps` tiles for `blocks` blocks where a CU holds `per_cu` of them: as
 // many as still run all at once on 256 CUs (one more would start a second round), at most one per
-// step and kMaxParts.
+// step and kMaxParts.  Where blocks differ in length (a square causal call's longest takes
+// twice the mean) twice as many, longest first, so that short ones fill up behind long ones (dk / dv of causal 2 x 4 key heads x 8192 keys x 128: 1.76 ms in 512 blocks,
+// 1.23 in 1024 and 0.035 for the sum of their parts).
+inline bool uneven(const Args &a) { return a.causal && 2 * a.n > a.m; }
 constexpr int kMaxParts = 64;  // the join gives each part a lane
-inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu) {
+inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu, bool uneven) {
     if (blocks <= 0 || steps <= 1) return 1;
-    int64_t p = 256 * per_cu / blocks;
+    int64_t p = uneven ? cdiv(2 * 256 * per_cu, blocks) : 256 * per_cu / blocks;
     p = p < steps ? p : steps;
     return p < 1 ? 1 : p < kMaxParts ? p : kMaxParts;
 }

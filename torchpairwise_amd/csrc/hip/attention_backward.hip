@@ -38,7 +38,7 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
     using CR = ColReader<T, DP, W>;
     constexpr int DB = DP / W, QS = DP / M::KS, NU = kUnit / W, ST = kUnit / M::KS;
     constexpr uint32_t kTileBytes = BN * DP * sizeof(T);
-    __shared__ uint4 smem[4 * kTileBytes / 16];
+    __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane / W;
     int64_t t = xcd_linear(blockIdx.x, gridDim.x);
     const int64_t part = t % a.splits;
@@ -208,8 +208,8 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
     }
     if (!live) return;
     if (a.splits > 1) {
-        float *p = a.part + (part * all + row) * a.d;
-        CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.d, a.d % 4 == 0, v); });
+        float *p = a.part + (part * all + row) * quads4(a.d);
+        CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.d, 1, v); });
         return;
     }
     T *p = reinterpret_cast<T *>(const_cast<void *>(a.gq.p)) + b * a.gq.b + qh * a.gq.h + qi * a.gq.n;
@@ -226,14 +226,12 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
     static_assert(BM <= 64, "one DMA of row values per array");
     constexpr uint32_t kValues = VLDS ? kWaves * W * DP * sizeof(T) : 0;
     // two buffers of a q tile, a do tile and the row values; the block's value rows
-    __shared__ uint4 smem[(2 * kBuf + kValues) / 16];
+    __shared__ __attribute__((aligned(256))) uint4 smem[(2 * kBuf + kValues) / 16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane / W;
     int64_t t = xcd_linear(blockIdx.x, gridDim.x);
     const int64_t part = t % a.splits;
     t /= a.splits;
-    // A causal call's first keys are seen by the most rows.  They come first, and the second half of the
-    // tiles comes in reverse, so that where two blocks share a CU a long one and a short one do.
-    const int64_t half = (a.tiles + 1) / 2, tt = t % a.tiles, tile = tt < half ? tt : a.tiles - 1 - (tt - half);
+    const int64_t tile = t % a.tiles;  // first keys of a causal call first: most rows see them
     const int64_t bk = t / a.tiles, b = bk / a.key_heads, kh = bk % a.key_heads;
     const int64_t len = key_end(a, b), all = a.batch * a.heads * a.n;
     const int rows = (int)a.n;
@@ -435,21 +433,21 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
     if (!stored) return;
     const int64_t keys = a.batch * a.key_heads * a.m, row = (b * a.key_heads + kh) * a.m + j;
     const auto store = [&](const Acc *acc, int64_t width, int64_t at, const View &out, float scale) {
-        float *part_row = a.part + (part * keys + row) * (a.d + a.dv) + at;
+        float *part_row = a.part + (part * keys + row) * (quads4(a.d) + quads4(a.dv)) + at;
         T *out_row = reinterpret_cast<T *>(const_cast<void *>(out.p)) + b * out.b + kh * out.h + j * out.n;
         CR::each(acc, lane, [&](int f, f32x4 x) {
             if (a.splits > 1)
-                store4(part_row, f, (int)width, a.d % 4 == 0 && a.dv % 4 == 0, x);
+                store4(part_row, f, (int)width, 1, x);
             else
                 store4(out_row, f, (int)width, a.vec_out, x * scale);
         });
     };
     if constexpr (DK) store(dk, a.d, 0, a.gk, a.gscale);
-    if constexpr (DV) store(dv, a.dv, a.d, a.gv, 1.0f);
+    if constexpr (DV) store(dv, a.dv, quads4(a.d), a.gv, 1.0f);
 }
 
 // Sums the parts of one or two gradients, in their order, one thread per four features: rows of fp32
-// values, the first output's features, then the second's.
+// quads, the first output's features, then the second's.
 struct SumArgs {
     const float *part;
     View out[2];
@@ -465,31 +463,22 @@ __global__ __launch_bounds__(256) void attention_sum_kernel(const SumArgs a) {
     const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, row = id / quads;
     if (row >= a.rows) return;
     const int which = id % quads >= q0, f = (int)(id % quads - (which ? q0 : 0)) * 4;
-    const int64_t all = a.width[0] + a.width[1], d = which ? a.width[1] : a.width[0];
-    const float *p = a.part + row * all + (which ? a.width[0] : 0) + f;
-    const bool vec = a.width[0] % 4 == 0 && a.width[1] % 4 == 0;
+    const int64_t pitch = 4 * quads;
+    const float *p = a.part + row * pitch + (which ? 4 * q0 : 0) + f;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < a.splits; s0 += U) {
         f32x4 y[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            y[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (s0 + u >= a.splits) continue;
-            const float *q = p + (s0 + u) * a.rows * all;
-            if (vec) {
-                y[u] = *reinterpret_cast<const f32x4 *>(q);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (f + e < d) y[u][e] = q[e];
-            }
-        }
+        for (int u = 0; u < U; ++u)
+            y[u] = s0 + u < a.splits ? *reinterpret_cast<const f32x4 *>(p + (s0 + u) * a.rows * pitch)
+                                     : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int u = 0; u < U; ++u) x += y[u];
     }
     const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
     const View out = which ? a.out[1] : a.out[0];
-    store4(reinterpret_cast<T *>(const_cast<void *>(out.p)) + b * out.b + h * out.h + i * out.n, f, (int)d, a.vec_out,
+    store4(reinterpret_cast<T *>(const_cast<void *>(out.p)) + b * out.b + h * out.h + i * out.n, f,
+           (int)(which ? a.width[1] : a.width[0]), a.vec_out,
            x * (which ? a.scale[1] : a.scale[0]));
 }
 
@@ -512,16 +501,15 @@ BackwardPlan backward_plan(const Args &a) {
     const int64_t bk = a.batch * a.key_heads;
     p.q_tiles = cdiv(a.n * a.group, (int64_t)L::kWaves * L::kWidth);
     p.k_tiles = cdiv(a.m, (int64_t)L::kRowWaves * L::kWidth);
-    p.q_splits = (int)parts_for(bk * p.q_tiles, cdiv(a.m, L::kKeys), L::kPerCuQ);
-    p.k_splits = (int)parts_for(bk * p.k_tiles, a.group * cdiv(a.n, L::kRows), L::kPerCuK);
+    p.q_splits = (int)parts_for(bk * p.q_tiles, cdiv(a.m, L::kKeys), L::kPerCuQ, uneven(a));
+    p.k_splits = (int)parts_for(bk * p.k_tiles, a.group * cdiv(a.n, L::kRows), L::kPerCuK, uneven(a));
     return p;
 }
-int64_t round4(int64_t x) { return (x + 3) / 4 * 4; }
 size_t backward_workspace(const Args &a, const BackwardPlan &p) {
     const int64_t rows = a.batch * a.heads * a.n;
-    const int64_t q = p.q_splits > 1 ? p.q_splits * rows * a.d : 0;
-    const int64_t k = p.k_splits > 1 ? p.k_splits * a.batch * a.key_heads * a.m * (a.d + a.dv) : 0;
-    return (size_t)(round4(3 * rows) + (q > k ? q : k)) * 4;
+    const int64_t q = p.q_splits > 1 ? p.q_splits * rows * quads4(a.d) : 0;
+    const int64_t k = p.k_splits > 1 ? p.k_splits * a.batch * a.key_heads * a.m * (quads4(a.d) + quads4(a.dv)) : 0;
+    return (size_t)(quads4(3 * rows) + (q > k ? q : k)) * 4;
 }
 
 template <typename T>
@@ -566,7 +554,7 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
         TPW_REQUIRE(bk * p.q_tiles * p.q_splits < (int64_t(1) << 31) && bk * p.k_tiles * p.k_splits < (int64_t(1) << 31),
                     "attention: too many rows");
         a.rows = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + prepared);
-        a.part = a.rows + round4(3 * rows);
+        a.part = a.rows + quads4(3 * rows);
         if (rows) {
             a.tiles = p.q_tiles;
             a.splits = p.q_splits;
