@@ -310,6 +310,38 @@ def test_longer_sequences(dtype, causal, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d,dv", [(128, 128), (90, 72), (256, 256), (140, 256)])
+@pytest.mark.parametrize("kind", ["all", "causal", "keep", "bias", "ragged"])
+def test_many_heads_of_wide_rows(kind, d, dv):
+    """fp32 calls that fill the GPU keep the scores' gradients for the products."""
+    b, h, hk, n, m = 8, 16, 8, 170, 330
+    g = gen(9)
+    mask = None
+    if kind == "keep":
+        mask = torch.rand(n, m, generator=g) < 0.3
+        mask[17] = False
+    elif kind == "bias":
+        mask = torch.randn(h, n, m, generator=g)
+        mask[:, :, 40:90] = -math.inf
+    lengths = torch.tensor([330, 0, 1, 31, 128, 129, 300, 64]) if kind == "ragged" else None
+    check("cuda", rows(b, h, n, d, 1, F32, True), rows(b, hk, m, d, 2), rows(b, hk, m, dv, 3, F32, True), mask,
+          causal=kind in ("causal", "ragged"), lengths=lengths, grad=rows(b, h, n, dv, 4), what=kind)
+
+
+@pytest.mark.gpu
+def test_heads_in_several_rounds():
+    """More kept gradients than the workspace holds at a time: first and last heads of 20."""
+    h, n, d = 20, 4096, 72
+    q, k, v, grad = (rows(1, h, n, d, i, F32) for i in range(1, 5))
+    leaves = [x.cuda().requires_grad_() for x in (q, k, v)]
+    got = torch.autograd.grad(tp.attention(*leaves, causal=True), leaves, grad.cuda())
+    for i in (0, 19):
+        want = reference(*(x[:, i:i + 1] for x in (q, k, v)), causal=True, grad=grad[:, i:i + 1])
+        for name, x in zip(("dq", "dk", "dv"), got):
+            assert_close(x[:, i:i + 1], want[name], rtol=0.0, atol=want["tol_" + name] + TINY, what=f"head {i} {name}")
+
+
+@pytest.mark.gpu
 def test_chunk_over_a_cache_equals_the_whole():
     """Queries in chunks over a growing cache with lengths give the rows of one causal call."""
     h, hk, n, d = 4, 2, 300, 64

@@ -66,9 +66,20 @@ struct Forward {
 #pragma unroll
         for (int i = 0; i < NB; ++i) s[i] = Acc{};
 #pragma unroll
-        for (int k = 0; k < QS; ++k)
+        for (int k = 0; k < QS; ++k) {
+            if constexpr (sizeof(T) == 4) {  // independent products side by side
+                Frag<T> f[NB];
 #pragma unroll
-            for (int i = 0; i < NB; ++i) M::mma(s[i], rr.read(kt, i, k), q[k]);
+                for (int i = 0; i < NB; ++i) f[i] = rr.read(kt, i, k);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) M::mma1(s[i], f[i], q[k], e);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) M::mma(s[i], rr.read(kt, i, k), q[k]);
+            }
+        }
 
         if constexpr (MM == kBias) {
             const void *mr = mask_row(a, b, qh, qi);

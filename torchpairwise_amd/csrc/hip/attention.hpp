@@ -54,6 +54,8 @@ struct Args {
     int vec_out;   // the outputs' rows take stores of four features
     int64_t tiles;  // row tiles (dk / dv: key tiles) per (batch, key head)
     int splits;     // parts of the summed axis
+    float *ds;      // kept score gradients (backward of wide fp32 rows): [key heads' heads, m, ds_pitch]
+    int64_t ds_pitch, first_bk;  // rows rounded up to whole units; first (batch, key head) of this launch
     float *part;    // [splits, rows, features] partial results where splits > 1, rows of whole quads
     float *part_stats;  // [splits, 2, rows]
 };
@@ -93,10 +95,12 @@ template <>
 struct Mma<float, 16> : Shape<16> {
     typedef f32x4 Acc;
     // element e of every lane makes one instruction: its four k are elements e of the four groups
+    static __device__ __forceinline__ void mma1(Acc &acc, const Frag<float> &a, const Frag<float> &b, int e) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e >> 2][e & 3], b.v[e >> 2][e & 3], acc, 0, 0, 0);
+    }
     static __device__ __forceinline__ void mma(Acc &acc, const Frag<float> &a, const Frag<float> &b) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e >> 2][e & 3], b.v[e >> 2][e & 3], acc, 0, 0, 0);
+        for (int e = 0; e < 8; ++e) mma1(acc, a, b, e);
     }
 };
 
@@ -480,6 +484,7 @@ constexpr int kMaxParts = 64;  // the join gives each part a lane
 inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu, bool uneven) {
     if (blocks <= 0 || steps <= 1) return 1;
     int64_t p = uneven ? cdiv(2 * 256 * per_cu, blocks) : 256 * per_cu / blocks;
+    if (steps < 4) p = 1;  // a tile or two take less than the join's launch
     p = p < steps ? p : steps;
     return p < 1 ? 1 : p < kMaxParts ? p : kMaxParts;
 }

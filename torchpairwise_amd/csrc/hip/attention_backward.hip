@@ -6,7 +6,9 @@
 //   dq_i = scale sum_j ds_ij k_j                    attention_dq_kernel: a wave owns query rows
 //   dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij do_i   attention_dkv_kernel: a wave owns keys
 // Seven products where five would do with dq summed in memory: the two scores' products are formed
-// in both kernels.
+// in both kernels.  On the fp32 matrix cores two products of wide rows cost more than writing and
+// reading ds: there (see keeps_ds) the kernel that owns keys keeps ds in the workspace, for as many heads
+// at a time as 1 GiB holds, and dk and dq are one product each (attention_ds_product_kernel).
 #include <math.h>
 
 #include "attention.hpp"
@@ -136,12 +138,29 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
 #pragma unroll
             for (int i = 0; i < NU; ++i) s[i] = dp[i] = Acc{};
 #pragma unroll
-            for (int k = 0; k < QS; ++k)
+            for (int k = 0; k < QS; ++k) {
+                Frag<T> fk[NU], fv[NU];
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    M::mma(s[i], rr.read(kt, u * NU + i, k), q[k]);
-                    M::mma(dp[i], rr.read(vt, u * NU + i, k), go[k]);
+                    fk[i] = rr.read(kt, u * NU + i, k);
+                    fv[i] = rr.read(vt, u * NU + i, k);
                 }
+                if constexpr (sizeof(T) == 4) {  // independent products side by side
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+#pragma unroll
+                        for (int i = 0; i < NU; ++i) {
+                            M::mma1(s[i], fk[i], q[k], e);
+                            M::mma1(dp[i], fv[i], go[k], e);
+                        }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NU; ++i) {
+                        M::mma(s[i], fk[i], q[k]);
+                        M::mma(dp[i], fv[i], go[k]);
+                    }
+                }
+            }
             if constexpr (MM == kBias) {
                 const void *mr = mask_row(a, b, qh, qi);
 #pragma unroll
@@ -232,13 +251,14 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
     const int64_t part = t % a.splits;
     t /= a.splits;
     const int64_t tile = t % a.tiles;  // first keys of a causal call first: most rows see them
-    const int64_t bk = t / a.tiles, b = bk / a.key_heads, kh = bk % a.key_heads;
+    const int64_t bk = a.first_bk + t / a.tiles, b = bk / a.key_heads, kh = bk % a.key_heads;
     const int64_t len = key_end(a, b), all = a.batch * a.heads * a.n;
     const int rows = (int)a.n;
     const int64_t key0 = tile * (kWaves * W), j = key0 + wave * W + lane % W;
     const bool live = j < len, stored = j < a.m;
 
-    constexpr bool DK = (OUT & 1) != 0, DV = (OUT & 2) != 0, VREG = DK && !VLDS;
+    // OUT: 1 dk, 2 dv, 4 ds kept in a.ds
+    constexpr bool DK = (OUT & 1) != 0, DV = (OUT & 2) != 0, DS = (OUT & 5) != 0, VREG = DS && !VLDS;
     Frag<T> k[QS], v[VREG ? QS : 1];
     {
         const T *kr = live ? reinterpret_cast<const T *>(a.k.p) + b * a.k.b + kh * a.k.h + j * a.k.n : nullptr;
@@ -329,17 +349,33 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
             Acc s[NU], dp[NU];
 #pragma unroll
             for (int i = 0; i < NU; ++i) s[i] = dp[i] = Acc{};
-            constexpr int F1 = DK ? VLDS ? 3 : 2 : 1, F2 = DK && DV ? 2 : 1;
-            stream_steps<QS * NU, F1, Frag<T>>(
+            constexpr int R = DS ? 2 : 1, F1 = R * NU + (DS && VLDS), F2 = DK && DV ? 2 : 1;
+            stream_steps<QS, F1, Frag<T>>(
                 [&](int x, Frag<T>(&f)[F1]) {
-                    f[0] = rr.read(qt, u * NU + x % NU, x / NU);
-                    if constexpr (DK) f[1] = rr.read(gt, u * NU + x % NU, x / NU);
-                    if constexpr (DK && VLDS) f[2] = rr.read(vt, wave, x / NU);
+#pragma unroll
+                    for (int i = 0; i < NU; ++i) {
+                        f[R * i] = rr.read(qt, u * NU + i, x);
+                        if constexpr (DS) f[R * i + 1] = rr.read(gt, u * NU + i, x);
+                    }
+                    if constexpr (DS && VLDS) f[F1 - 1] = rr.read(vt, wave, x);
                 },
                 [&](int x, const Frag<T>(&f)[F1]) {
-                    M::mma(s[x % NU], f[0], k[x / NU]);
-                    if constexpr (VREG) M::mma(dp[x % NU], f[1], v[x / NU]);
-                    if constexpr (DK && VLDS) M::mma(dp[x % NU], f[1], f[2]);
+                    const Frag<T> &vv = VLDS ? f[F1 - 1] : v[VREG ? x : 0];
+                    if constexpr (sizeof(T) == 4) {  // independent products side by side
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+#pragma unroll
+                            for (int i = 0; i < NU; ++i) {
+                                M::mma1(s[i], f[R * i], k[x], e);
+                                if constexpr (DS) M::mma1(dp[i], f[R * i + R - 1], vv, e);
+                            }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NU; ++i) {
+                            M::mma(s[i], f[R * i], k[x]);
+                            if constexpr (DS) M::mma(dp[i], f[R * i + R - 1], vv);
+                        }
+                    }
                 });
             if constexpr (MM == kKeep) {
                 const uint32_t keep = word >> (4 * g);
@@ -404,6 +440,20 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
                         s[i][4 * w + e] = p * (dp[i][4 * w + e] - delta[e]);
                     }
                 }
+            if constexpr ((OUT & 4) != 0) {
+                if (live) {
+                    float *kept = a.ds + (((bk - a.first_bk) * a.group + (qh - kh * a.group)) * a.m + j) * a.ds_pitch + u0 + 4 * g;
+#pragma unroll
+                    for (int i = 0; i < NU; ++i)
+#pragma unroll
+                        for (int w = 0; w < M::Q; ++w) {
+                            f32x4 y;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) y[e] = s[i][4 * w + e];
+                            *reinterpret_cast<f32x4 *>(kept + W * i + 4 * M::NG * w) = y;
+                        }
+                }
+            }
             Frag<T> p[ST], ds[ST];
 #pragma unroll
             for (int st = 0; st < ST; ++st) {
@@ -444,6 +494,122 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
     };
     if constexpr (DK) store(dk, a.d, 0, a.gk, a.gscale);
     if constexpr (DV) store(dv, a.dv, quads4(a.d), a.gv, 1.0f);
+}
+
+// base, 1 / sum and delta of every row, one wave per row (the dq kernel forms them where it runs).
+template <typename T>
+__global__ __launch_bounds__(256) void attention_rows_kernel(const Args a) {
+    const int64_t all = a.batch * a.heads * a.n, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= all) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
+    const T *o = reinterpret_cast<const T *>(a.o.p) + b * a.o.b + h * a.o.h + i * a.o.n;
+    const T *g = reinterpret_cast<const T *>(a.go.p) + b * a.go.b + h * a.go.h + i * a.go.n;
+    float delta = 0.0f;
+    for (int f = lane; f < a.dv; f += 64) delta = __builtin_fmaf(to_f32(o[f]), to_f32(g[f]), delta);
+    delta = over_groups_sum<1>(delta);
+    if (lane) return;
+    const float top = a.stats[row], sum = a.stats[all + row];
+    a.rows[row] = top == -INFINITY ? 0.0f : top;
+    a.rows[all + row] = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    a.rows[2 * all + row] = delta;
+}
+
+// dk (KEYS) or dq from the kept ds: a wave owns 16 keys (query rows) and streams q (k) through LDS.
+// Only units that the kernel above wrote are read; what no row sees counts as zero.
+template <int DP, bool KEYS>
+__global__ __launch_bounds__(512, 2) void attention_ds_product_kernel(const Args a) {
+    constexpr int W = 16, kWaves = 8;
+    using M = Mma<float, W>;
+    using CR = ColReader<float, DP, W>;
+    constexpr uint32_t kTileBytes = kUnit * DP * 4;
+    __shared__ __attribute__((aligned(256))) uint4 smem[2 * kTileBytes / 16];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane / W;
+    const int64_t t = xcd_linear(blockIdx.x, gridDim.x), own_tiles = cdiv_dev(KEYS ? a.m : a.n, kWaves * W);
+    // longest first: a causal call's first keys and last rows
+    const int64_t tile = KEYS ? t % own_tiles : own_tiles - 1 - t % own_tiles;
+    const int64_t head = KEYS ? 0 : t / own_tiles % a.group, local = KEYS ? t / own_tiles : t / own_tiles / a.group;
+    const int64_t bk = a.first_bk + local, b = bk / a.key_heads, kh = bk % a.key_heads;
+    const int64_t len = key_end(a, b), own0 = tile * (kWaves * W), o = own0 + wave * W + lane % W;
+
+    // KEYS: the first row that sees the key; else the keys that the row sees
+    int bound;
+    if (KEYS) {
+        const int64_t first = o >= len ? 0x7fffffff : a.causal ? o - (len - a.n) : 0;
+        bound = (int)(first < 0 ? 0 : first);
+    } else {
+        bound = o < a.n ? (int)row_limit(a, len, o) : 0;
+    }
+    int far = bound;  // over the wave: KEYS the least, else the greatest
+#pragma unroll
+    for (int s = 1; s < W; s <<= 1) {
+        const int x = __shfl_xor(far, s, 64);
+        far = (KEYS ? x < far : x > far) ? x : far;
+    }
+    far = __builtin_amdgcn_readfirstlane(far);
+
+    // units of the streamed rows: KEYS of every head of the group, from the first that sees a key
+    int64_t skip = own0 >= len ? a.n : a.causal ? own0 - (len - a.n) : 0;
+    skip = skip < 0 ? 0 : skip > a.n ? a.n : skip;
+    const int64_t last = own0 + kWaves * W < a.n ? own0 + kWaves * W - 1 : a.n - 1;
+    const int nt = (int)cdiv_dev(KEYS ? a.n : row_limit(a, len, last), kUnit);
+    const int tf = !KEYS ? 0 : skip >= a.n ? nt : (int)(skip / kUnit), per = nt - tf;
+    const int total = KEYS ? (int)a.group * per : per;
+
+    const uint32_t lds = tile::lds_addr(smem);
+    Stager<float, DP, kUnit, kWaves> st;
+    const View &x = KEYS ? a.q : a.k;
+    st.init(x.n, (int)a.d, wave, lane);
+    const float *xb = reinterpret_cast<const float *>(x.p) + b * x.b + kh * (KEYS ? a.group : 1) * x.h;
+    const float *db = a.ds + (local * a.group + head) * a.m * a.ds_pitch;
+    int fh = 0, ft = tf;  // head and unit to fetch next
+    Frag<float> next = {}, now = {};
+    const auto fetch = [&](int i) {
+        const int64_t r0 = (int64_t)ft * kUnit;
+        st.load(xb + fh * x.h + r0 * x.n, (KEYS ? a.n : len) - r0, lds + (uint32_t)(i & 1) * kTileBytes);
+        next = Frag<float>{};
+        if (KEYS) {
+            if (o < len && r0 + kUnit > far) {
+                const float *p = db + (fh * a.m + o) * a.ds_pitch + r0 + 4 * g;
+                next.v[0] = *reinterpret_cast<const f32x4 *>(p);
+                next.v[1] = *reinterpret_cast<const f32x4 *>(p + 16);
+            }
+        } else if (r0 < far) {
+            const float *p = db + (o < a.n ? o : 0);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int64_t key = r0 + 16 * (e >> 2) + 4 * g + (e & 3);
+                const float y = p[(key < bound ? key : 0) * a.ds_pitch];
+                next.v[e >> 2][e & 3] = key < bound ? y : 0.0f;
+            }
+        }
+        if (++ft == nt) {
+            ft = tf;
+            ++fh;
+        }
+    };
+    M::Acc acc[CR::kBlocks];
+#pragma unroll
+    for (int i = 0; i < CR::kBlocks; ++i) acc[i] = M::Acc{};
+    const CR cr(lane);
+    if (total > 0) fetch(0);
+    int ct = tf;
+    for (int i = 0; i < total; ++i) {
+        tile::barrier_all();
+        now = next;
+        const int r0 = ct * kUnit;
+        if (++ct == nt) ct = tf;
+        if (i + 1 < total) fetch(i + 1);
+        if (KEYS ? r0 + kUnit <= far : r0 >= far) continue;
+        const uint32_t at = lds + (uint32_t)(i & 1) * kTileBytes;
+#pragma unroll
+        for (int c = 0; c < CR::kPieces; ++c) CR::use(acc, c, cr.read(at, 0, c), now);
+    }
+    if (o >= (KEYS ? a.m : a.n)) return;
+    const View &out = KEYS ? a.gk : a.gq;
+    float *row = reinterpret_cast<float *>(const_cast<void *>(out.p)) + b * out.b +
+                 (KEYS ? kh : kh * a.group + head) * out.h + o * out.n;
+    CR::each(acc, lane, [&](int f, f32x4 v) { store4(row, f, (int)a.d, a.vec_out, v * a.gscale); });
 }
 
 // Sums the parts of one or two gradients, in their order, one thread per four features: rows of fp32
@@ -493,7 +659,18 @@ namespace {
 struct BackwardPlan {
     int64_t q_tiles, k_tiles;
     int q_splits, k_splits;
+    int64_t kept;  // (batch, key head)s whose ds is kept at a time; 0: formed again
 };
+// fp32 rows of more than 64 features keep ds where a 1 GiB workspace holds enough heads for a block on
+// most CUs (8 x 8192^2 x 256: 11.3 ms where forming them again takes 15.5; 8 x 4096^2 x 128: 1.56, 2.07)
+constexpr int64_t kKeptBytes = int64_t(1) << 30, kKeptKeys = 128;
+int64_t ds_bytes(const Args &a) { return a.group * a.m * (cdiv(a.n, kUnit) * kUnit) * 4; }  // of one key head
+template <typename T, int DP>
+int64_t keeps_ds(const Args &a) {
+    if (sizeof(T) != 4 || DP == 64 || a.n == 0 || a.m == 0 || ds_bytes(a) > kKeptBytes) return 0;
+    const int64_t bk = a.batch * a.key_heads, most = kKeptBytes / ds_bytes(a), rounds = cdiv(bk, most), kept = cdiv(bk, rounds);
+    return kept * cdiv(a.m, kKeptKeys) >= 192 && kept * a.group * cdiv(a.n, kKeptKeys) >= 192 ? kept : 0;
+}
 template <typename T, int DP>
 BackwardPlan backward_plan(const Args &a) {
     BackwardPlan p;
@@ -503,10 +680,12 @@ BackwardPlan backward_plan(const Args &a) {
     p.k_tiles = cdiv(a.m, (int64_t)L::kRowWaves * L::kWidth);
     p.q_splits = (int)parts_for(bk * p.q_tiles, cdiv(a.m, L::kKeys), L::kPerCuQ, uneven(a));
     p.k_splits = (int)parts_for(bk * p.k_tiles, a.group * cdiv(a.n, L::kRows), L::kPerCuK, uneven(a));
+    p.kept = keeps_ds<T, DP>(a);
     return p;
 }
 size_t backward_workspace(const Args &a, const BackwardPlan &p) {
     const int64_t rows = a.batch * a.heads * a.n;
+    if (p.kept) return (size_t)(quads4(3 * rows) * 4 + p.kept * ds_bytes(a));
     const int64_t q = p.q_splits > 1 ? p.q_splits * rows * quads4(a.d) : 0;
     const int64_t k = p.k_splits > 1 ? p.k_splits * a.batch * a.key_heads * a.m * (quads4(a.d) + quads4(a.dv)) : 0;
     return (size_t)(quads4(3 * rows) + (q > k ? q : k)) * 4;
@@ -517,6 +696,26 @@ int sum_parts(const SumArgs &a, hipStream_t s) {
     const int64_t threads = a.rows * (cdiv(a.width[0], 4) + cdiv(a.width[1], 4));
     hipLaunchKernelGGL((attention_sum_kernel<T>), dim3((unsigned)cdiv(threads, 256)), dim3(256), 0, s, a);
     return check_launch("attention_sum_kernel");
+}
+
+template <int DP, int MM>
+int backward_kept(Args &a, int64_t kept, int64_t rows, hipStream_t s) {
+    const int64_t bk = a.batch * a.key_heads, k_tiles = cdiv(a.m, kKeptKeys), q_tiles = cdiv(a.n, kKeptKeys);
+    hipLaunchKernelGGL((attention_rows_kernel<float>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a);
+    if (const int rc = check_launch("attention_rows_kernel")) return rc;
+    a.ds = a.part;
+    a.ds_pitch = cdiv(a.n, kUnit) * kUnit;
+    a.tiles = k_tiles;
+    a.splits = 1;
+    for (a.first_bk = 0; a.first_bk < bk; a.first_bk += kept) {
+        const int64_t now = bk - a.first_bk < kept ? bk - a.first_bk : kept;
+        const dim3 keys((unsigned)(now * k_tiles)), queries((unsigned)(now * a.group * q_tiles));
+        hipLaunchKernelGGL((attention_dkv_kernel<float, 16, DP, 32, MM, 8, 2, false, 6>), keys, dim3(512), 0, s, a);
+        hipLaunchKernelGGL((attention_ds_product_kernel<DP, true>), keys, dim3(512), 0, s, a);
+        hipLaunchKernelGGL((attention_ds_product_kernel<DP, false>), queries, dim3(512), 0, s, a);
+        if (const int rc = check_launch("attention_ds_product_kernel")) return rc;
+    }
+    return TPW_OK;
 }
 
 }  // namespace
@@ -555,6 +754,9 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
                     "attention: too many rows");
         a.rows = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + prepared);
         a.part = a.rows + quads4(3 * rows);
+        if constexpr (sizeof(T) == 4 && DP > 64) {
+            if (p.kept) return backward_kept<DP, MM>(a, p.kept, rows, s);
+        }
         if (rows) {
             a.tiles = p.q_tiles;
             a.splits = p.q_splits;
