@@ -787,7 +787,9 @@ int tpw_knn_mask_euclidean(const void *x1, const void *x2, int dtype, int64_t n,
  * n, m] (0 where it is broadcast).  key and value (in the backward query and grad_out too) need a
  * row stride of at least their width and at most 8 MiB.  stats [2, batch, heads, n] (fp32) carries
  * each row's maximum and sum from the forward (null: not wanted) to the backward and has no other
- * meaning.  out and stats are read by the backward. */
+ * meaning.  out_rest (bfloat16 only, or null) takes what rounding left of out's values: with it the
+ * backward's gradients of rows that rest on few keys keep their precision.  out, out_rest and stats are
+ * read by the backward. */
 #define TPW_MASK_NONE 0
 #define TPW_MASK_KEEP 1     /* bool bytes */
 #define TPW_MASK_ADD_F32 2  /* added to the scaled scores */
@@ -802,6 +804,7 @@ typedef struct tpw_attention_desc {
     const void *query, *key, *value, *mask;
     const int64_t *lengths; /* [batch] or null */
     void *out;
+    void *out_rest; /* strides of out; or null */
     float *stats;
     const void *grad_out; /* backward only, as the following three */
     void *grad_query, *grad_key, *grad_value;

@@ -202,6 +202,24 @@ def test_strides_and_alignment(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n,causal,density", [(32, True, 1.0), (96, True, 1.0), (200, False, 0.02), (20, False, 0.25)])
+def test_bf16_gradients_of_rows_on_few_keys(device, n, causal, density):
+    """dq and dk of bfloat16 rows that rest on few keys: two roundings of the same size (the scores'
+    gradients for the matrix cores, the result) make sqrt(2) of what rounding the exact result costs;
+    from a rounded output alone delta would make it up to 1.7."""
+    h, d = 16, 64
+    mask = torch.rand(n, n, generator=gen(5)) < density
+    mask[torch.arange(n), torch.arange(n)] = True
+    q, k, v, grad = (rows(1, h, n, d, i, BF16) for i in range(1, 5))
+    want = reference(q, k, v, mask, causal, grad=grad)
+    leaves = [x.requires_grad_() for x in on(device, q, k, v)]
+    got = torch.autograd.grad(tp.attention(*leaves, mask.to(device), causal=causal), leaves, grad.to(device))
+    for name, x in zip(("dq", "dk"), got):
+        exact = want[name]
+        assert (x.cpu().double() - exact).norm() <= 1.5 * (exact.to(BF16).double() - exact).norm(), name
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_two_and_three_dimensions(device):
     q, k, v = randn(2, 30, 48, seed=1), randn(2, 50, 48, seed=2), randn(2, 50, 20, seed=3)
     mask = torch.rand(2, 30, 50, generator=gen(4)) < 0.7

@@ -30,7 +30,7 @@ class AttentionDesc(C.Structure):
     """``tpw_attention_desc``."""
     _fields_ = [("dtype", C.c_int32), ("causal", C.c_int32), ("mask_type", C.c_int32), ("reserved", C.c_int32),
                 *[(f, _i64) for f in ("batch", "heads", "key_heads", "n", "m", "d", "dv")], ("scale", _d),
-                *[(f, _p) for f in ("query", "key", "value", "mask", "lengths", "out", "stats", "grad_out",
+                *[(f, _p) for f in ("query", "key", "value", "mask", "lengths", "out", "out_rest", "stats", "grad_out",
                                     "grad_query", "grad_key", "grad_value")],
                 *[(f + "_strides", _i64 * 3) for f in ("query", "key", "value", "out", "grad_out", "grad_query",
                                                        "grad_key", "grad_value")],

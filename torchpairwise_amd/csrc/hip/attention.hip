@@ -233,8 +233,8 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
         a.stats[row] = f.top;
         a.stats[a.batch * a.heads * a.n + row] = sum;
     }
-    T *p = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + b * a.o.b + f.qh * a.o.h + f.qi * a.o.n;
-    F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.dv, a.vec_out, v * inv); });
+    const OutRow<T> out(a, b, f.qh, f.qi);
+    F::CR::each(f.o, lane, [&](int at, f32x4 v) { out.store(at, v * inv); });
 }
 
 // Joins the parts of every row: m = max m_s, l = sum l_s 2^(m_s - m), o = sum o_s 2^(m_s - m) / l.
@@ -280,8 +280,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
         a.stats[rows + row] = sum;
     }
     const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
-    T *out = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + b * a.o.b + h * a.o.h + i * a.o.n;
-    store4(out, f, (int)a.dv, a.vec_out, o * inv);
+    OutRow<T>(a, b, h, i).store(f, o * inv);
 }
 
 // The same for at most kFew parts: one thread per four features, every load in flight at once
@@ -322,8 +321,7 @@ __global__ __launch_bounds__(256) void attention_join_few_kernel(const Args a) {
         a.stats[rows + row] = sum;
     }
     const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
-    T *out = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + b * a.o.b + h * a.o.h + i * a.o.n;
-    store4(out, f, (int)a.dv, a.vec_out, o * inv);
+    OutRow<T>(a, b, h, i).store(f, o * inv);
 }
 
 namespace {
@@ -337,7 +335,7 @@ View view_of(const void *p, const int64_t *strides, int64_t rows, int64_t width)
     return {p, strides[0], strides[1], rows == 1 ? width : strides[2]};
 }
 
-constexpr int kPadded = 5;  // q, k, v, do, o
+constexpr int kPadded = 6;  // q, k, v, do, o and its rest
 struct PadArgs {
     View from[kPadded];
     void *to[kPadded];
@@ -370,8 +368,8 @@ __global__ void pad_kernel(const PadArgs a) {
 size_t plan_padding(Args &a, int dtype, bool backward, uint8_t *at, PadArgs *p) {
     const int64_t size = dtype == TPW_F32 ? 4 : 2, e = 16 / size;
     size_t bytes = 0;
-    const auto take = [&](View &v, int64_t heads, int64_t rows, int64_t width) {
-        if (whole_pieces(v, width, size) || a.batch * heads * rows == 0) return;
+    const auto take = [&](View &v, int64_t heads, int64_t rows, int64_t width, bool always = false) {
+        if ((!always && whole_pieces(v, width, size)) || a.batch * heads * rows == 0) return;
         const int64_t pieces = cdiv(width, e), n = a.batch * heads * rows * pieces;
         if (p) {
             const int t = p->count++;
@@ -388,7 +386,11 @@ size_t plan_padding(Args &a, int dtype, bool backward, uint8_t *at, PadArgs *p) 
     take(a.v, a.key_heads, a.m, a.dv);
     if (backward) {
         take(a.go, a.heads, a.n, a.dv);
-        take(a.o, a.heads, a.n, a.dv);
+        View rest = {a.rest, a.o.b, a.o.h, a.o.n};
+        const bool both = a.rest && !(whole_pieces(a.o, a.dv, size) && whole_pieces(rest, a.dv, size));
+        take(a.o, a.heads, a.n, a.dv, both);
+        if (both) take(rest, a.heads, a.n, a.dv, both);  // strides of o
+        a.rest = const_cast<void *>(rest.p);
     }
     return bytes;
 }
@@ -519,7 +521,8 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
     a.qsign = d->scale > 0 ? 1.0f : d->scale < 0 ? -1.0f : 0.0f;
     a.scale = d->scale == 0 ? 1.0f : (float)(fabs(d->scale) * (bias ? 1.0 : 1.4426950408889634));
     a.gscale = (float)d->scale;
-    a.vec_out = whole_pieces(a.o, a.dv, size);
+    a.rest = d->dtype == TPW_BF16 ? d->out_rest : nullptr;
+    a.vec_out = whole_pieces(a.o, a.dv, size) && aligned16(a.rest);
     const auto streamed = [&](const View &v, int64_t rows, int64_t width) {
         return a.batch * a.heads * a.n * a.m == 0 || rows <= 1 || (v.n >= width && v.n * size <= (int64_t(1) << 23));
     };

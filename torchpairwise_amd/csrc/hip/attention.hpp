@@ -39,6 +39,7 @@ struct Args {
     View o, go;          // output; upstream gradient (backward)
     View gq, gk, gv;     // gradients (backward)
     float *stats;        // [2, b, h, n]: row maxima, row sums
+    void *rest;          // bf16: what the outputs' rounding left, strides of o; or null
     float *rows;         // [3, b, h, n] (backward): base and 1 / sum of the softmax, delta
     const void *mask;    // kKeep: words of 32 keys' bits (pack_mask_kernel); kBias: fp32 or bf16 values
     int64_t mb, mh, mn, mm;  // its strides, in words or values (0: broadcast; words: mm is 0)
@@ -351,6 +352,31 @@ __device__ __forceinline__ void store4(uint16_t *row, int f, int d, int vec, f32
             if (f + e < d) row[f + e] = f32_to_bf16_rne(v[e]);
     }
 }
+
+// What rounding the four values above left, rounded in turn.  delta = do . o of a row that rests on few
+// keys meets ds = p (dp - delta) with everything cancelled: from o alone, 2^-8 of each value off, dq and
+// dk of short or sparse rows would lose a quarter of their precision.
+__device__ __forceinline__ void store_rest4(uint16_t *row, int f, int d, int vec, f32x4 v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] -= bf16_to_f32(f32_to_bf16_rne(v[e]));
+    store4(row, f, d, vec, v);
+}
+// Output row of head h, row i: values, and their rest where it is wanted.
+template <typename T>
+struct OutRow {
+    T *row, *rest;
+    int d, vec;
+    __device__ __forceinline__ OutRow(const Args &a, int64_t b, int64_t h, int64_t i) : d((int)a.dv), vec(a.vec_out) {
+        const int64_t at = b * a.o.b + h * a.o.h + i * a.o.n;
+        row = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + at;
+        rest = a.rest ? reinterpret_cast<T *>(a.rest) + at : nullptr;
+    }
+    __device__ __forceinline__ void store(int f, f32x4 v) const {
+        store4(row, f, d, vec, v);
+        if constexpr (sizeof(T) == 2)
+            if (rest) store_rest4(rest, f, d, vec, v);
+    }
+};
 
 template <int W>
 __device__ __forceinline__ float over_groups_max(float v) {

@@ -69,7 +69,9 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
     {
         const T *qr = live ? reinterpret_cast<const T *>(a.q.p) + b * a.q.b + qh * a.q.h + qi * a.q.n : nullptr;
         const T *gr = live ? reinterpret_cast<const T *>(a.go.p) + b * a.go.b + qh * a.go.h + qi * a.go.n : nullptr;
-        const T *orow = live ? reinterpret_cast<const T *>(a.o.p) + b * a.o.b + qh * a.o.h + qi * a.o.n : nullptr;
+        const int64_t oat = b * a.o.b + qh * a.o.h + qi * a.o.n;
+        const T *orow = live ? reinterpret_cast<const T *>(a.o.p) + oat : nullptr;
+        const T *rest = live && a.rest ? reinterpret_cast<const T *>(a.rest) + oat : nullptr;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
             const int f = M::KS * s + 8 * g;
@@ -86,6 +88,11 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
             unpack8(load_row8(orow, f, (int)a.dv), y);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+            if constexpr (sizeof(T) == 2) {
+                unpack8(load_row8(rest, f, (int)a.dv), y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+            }
         }
         delta = over_groups_sum<W>(delta);
     }

@@ -145,29 +145,35 @@ at::Tensor masked_scores(const at::Tensor &q, const at::Tensor &k, const Operand
 }
 at::ScalarType compute_type(const at::Tensor &x) { return x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
 
-std::tuple<at::Tensor, at::Tensor> attention_cpu(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value,
-                                                 const OptTensor &mask, const OptTensor &lengths, bool causal,
-                                                 double scale) {
+using Results = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+
+Results attention_cpu(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value, const OptTensor &mask,
+                      const OptTensor &lengths, bool causal, double scale, bool train) {
     const Operands o = check_attention(query, key, value, mask, lengths);
     const auto t = compute_type(query);
     auto stats = at::zeros({2, o.batch, o.heads, o.n}, query.options().dtype(t));
     auto out = empty_rows({o.batch, o.heads, o.n, o.dv}, o.q);
-    if (out.numel() == 0 || o.m == 0) return {like_dims(out.zero_(), query), stats};
+    auto rest = at::empty({0}, out.options());
+    if (train && out.scalar_type() == at::kBFloat16) rest = at::zeros_like(out);
+    if (out.numel() == 0 || o.m == 0) return {like_dims(out.zero_(), query), stats, rest};
     auto s = masked_scores(grouped(o.q, o, t), live_rows(o.k, o, t), o, causal, scale);
     auto top = s.amax(-1, true);
     auto base = top.masked_fill(top == -std::numeric_limits<double>::infinity(), 0.0);
     auto p = (s - base).exp_();
     auto sum = p.sum(-1, true);
     auto acc = at::matmul(p.reshape({o.batch, o.key_heads, -1, o.m}), live_rows(o.v, o, t)).view(out.sizes());
-    out.copy_(acc / sum.masked_fill(sum == 0, 1.0));
+    acc = acc / sum.masked_fill(sum == 0, 1.0);
+    out.copy_(acc);
+    if (rest.numel() > 0) rest.copy_(acc - out);
     stats.select(0, 0).copy_(base.squeeze(-1));
     stats.select(0, 1).copy_(sum.squeeze(-1));
-    return {like_dims(out, query), stats};
+    return {like_dims(out, query), stats, rest};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward_cpu(
+Results attention_backward_cpu(
     const at::Tensor &grad, const at::Tensor &query, const at::Tensor &key, const at::Tensor &value, const at::Tensor &out,
-    const at::Tensor &stats, const OptTensor &mask, const OptTensor &lengths, bool causal, double scale) {
+    const at::Tensor &stats, const at::Tensor &rest, const OptTensor &mask, const OptTensor &lengths, bool causal,
+    double scale) {
     const Operands o = check_attention(query, key, value, mask, lengths);
     TORCH_CHECK(grad.sizes() == out.sizes(), "attention: gradient of shape ", grad.sizes(), " for an output of ", out.sizes());
     const auto t = compute_type(query);
@@ -180,7 +186,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward_cpu(
     auto p = (s - base).exp_().div_(sum.masked_fill(sum == 0, 1.0));
     auto g4 = as4(grad).to(t);
     auto g = grouped(g4, o, t);
-    auto delta = (g4 * as4(out).to(t)).sum(-1, true);
+    auto o4 = as4(out).to(t);
+    if (rest.numel() > 0) o4 = o4 + rest;
+    auto delta = (g4 * o4).sum(-1, true);
     auto dp = at::matmul(g, v.transpose(-1, -2)).view(p.sizes());
     auto ds = (p * (dp - delta)).masked_fill_(off, 0.0).mul_(scale).reshape({o.batch, o.key_heads, -1, o.m});
     auto pg = p.reshape(ds.sizes());
@@ -273,13 +281,16 @@ tpw_attention_desc describe(const Operands &o, bool causal, double scale) {
     return a;
 }
 
-std::tuple<at::Tensor, at::Tensor> attention_cuda(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value,
-                                                  const OptTensor &mask, const OptTensor &lengths, bool causal,
-                                                  double scale) {
+Results attention_cuda(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value, const OptTensor &mask,
+                       const OptTensor &lengths, bool causal, double scale, bool train) {
     Operands o = check_attention(query, key, value, mask, lengths);
     DeviceGuard guard(query.device());
     auto out = empty_rows({o.batch, o.heads, o.n, o.dv}, o.q);
-    auto stats = at::empty({2, o.batch, o.heads, o.n}, query.options().dtype(at::kFloat));
+    // what only the backward reads
+    at::Tensor stats = train ? at::empty({2, o.batch, o.heads, o.n}, query.options().dtype(at::kFloat))
+                             : at::empty({0}, query.options().dtype(at::kFloat));
+    at::Tensor rest = train && out.scalar_type() == at::kBFloat16 ? at::empty_strided(out.sizes(), out.strides(), out.options())
+                                                                  : at::empty({0}, out.options());
     if (out.numel() > 0) {
         o.q = dense_rows(o.q, false);
         o.k = dense_rows(o.k, true);
@@ -287,18 +298,20 @@ std::tuple<at::Tensor, at::Tensor> attention_cuda(const at::Tensor &query, const
         auto a = describe(o, causal, scale);
         a.out = out.data_ptr();
         set_strides(a.out_strides, out);
-        a.stats = stats.data_ptr<float>();
+        if (train) a.stats = stats.data_ptr<float>();
+        if (rest.numel() > 0) a.out_rest = rest.data_ptr();
         const size_t bytes = tpw_attention_workspace_size(&a);
         at::Tensor ws;
         if (bytes > 0) ws = workspace(bytes, query);
         check_rc(tpw_attention(&a, bytes > 0 ? ws.data_ptr() : nullptr, current_stream()), "_attention");
     }
-    return {like_dims(out, query), stats};
+    return {like_dims(out, query), stats, rest};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward_cuda(
+Results attention_backward_cuda(
     const at::Tensor &grad, const at::Tensor &query, const at::Tensor &key, const at::Tensor &value, const at::Tensor &out,
-    const at::Tensor &stats, const OptTensor &mask, const OptTensor &lengths, bool causal, double scale) {
+    const at::Tensor &stats, const at::Tensor &rest, const OptTensor &mask, const OptTensor &lengths, bool causal,
+    double scale) {
     Operands o = check_attention(query, key, value, mask, lengths);
     TORCH_CHECK(grad.sizes() == out.sizes(), "attention: gradient of shape ", grad.sizes(), " for an output of ", out.sizes());
     TORCH_CHECK(out.scalar_type() == query.scalar_type() && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
@@ -311,12 +324,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward_cuda(
         o.q = dense_rows(o.q, true);
         o.k = dense_rows(o.k, true);
         o.v = dense_rows(o.v, true);
-        auto g4 = dense_rows(as4(grad.to(query.scalar_type())), true), o4 = dense_rows(as4(out), false);
+        auto g4 = dense_rows(as4(grad.to(query.scalar_type())), true), o4 = as4(out);
+        TORCH_CHECK((rest.numel() == 0 || (rest.sizes() == o4.sizes() && rest.strides() == o4.strides() &&
+                                           rest.scalar_type() == out.scalar_type() && rest.device() == out.device())) &&
+                        (o4.size(3) == 1 || o4.stride(3) == 1),
+                    "_attention_backward: out and rest must be what the forward returned");
         TORCH_CHECK(o4.size(0) == o.batch && o4.size(1) == o.heads && o4.size(2) == o.n && o4.size(3) == o.dv,
                     "_attention_backward: out must be what the forward returned");
         auto a = describe(o, causal, scale);
         a.out = o4.data_ptr();
         set_strides(a.out_strides, o4);
+        if (rest.numel() > 0) a.out_rest = rest.data_ptr();
         a.stats = stats.data_ptr<float>();
         a.grad_out = g4.data_ptr();
         set_strides(a.grad_out_strides, g4);
@@ -353,25 +371,23 @@ at::Tensor rotary_cuda(const at::Tensor &x, const at::Tensor &positions, const a
 }
 
 // ------------------------------------------------------------------ dispatch
-std::tuple<at::Tensor, at::Tensor> attention_op(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
-                                                const OptTensor &mask, const OptTensor &lengths, bool causal,
-                                                double scale) {
+Results attention_op(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const OptTensor &mask,
+                     const OptTensor &lengths, bool causal, double scale, bool train) {
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("torchpairwise::_attention", "")
-                         .typed<std::tuple<at::Tensor, at::Tensor>(const at::Tensor &, const at::Tensor &, const at::Tensor &,
-                                                                   const OptTensor &, const OptTensor &, bool, double)>();
-    return op.call(q, k, v, mask, lengths, causal, scale);
+                         .typed<Results(const at::Tensor &, const at::Tensor &, const at::Tensor &, const OptTensor &,
+                                        const OptTensor &, bool, double, bool)>();
+    return op.call(q, k, v, mask, lengths, causal, scale, train);
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward_op(
-    const at::Tensor &grad, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &out,
-    const at::Tensor &stats, const OptTensor &mask, const OptTensor &lengths, bool causal, double scale) {
-    static auto op =
-        c10::Dispatcher::singleton()
-            .findSchemaOrThrow("torchpairwise::_attention_backward", "")
-            .typed<std::tuple<at::Tensor, at::Tensor, at::Tensor>(
-                const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
-                const at::Tensor &, const OptTensor &, const OptTensor &, bool, double)>();
-    return op.call(grad, q, k, v, out, stats, mask, lengths, causal, scale);
+Results attention_backward_op(const at::Tensor &grad, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                              const at::Tensor &out, const at::Tensor &stats, const at::Tensor &rest, const OptTensor &mask,
+                              const OptTensor &lengths, bool causal, double scale) {
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("torchpairwise::_attention_backward", "")
+                         .typed<Results(const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                        const at::Tensor &, const at::Tensor &, const at::Tensor &, const OptTensor &,
+                                        const OptTensor &, bool, double)>();
+    return op.call(grad, q, k, v, out, stats, rest, mask, lengths, causal, scale);
 }
 at::Tensor rotary_op(const at::Tensor &x, const at::Tensor &positions, const at::Tensor &frequencies, bool interleaved,
                      double scale, bool inverse) {
@@ -387,7 +403,8 @@ at::Tensor attention(const at::Tensor &query, const at::Tensor &key, const at::T
                      : query.dim() > 0 && query.size(-1) > 0 ? 1.0 / std::sqrt((double)query.size(-1))
                                                              : 1.0;
     TORCH_CHECK(std::isfinite(s) && std::fabs(s) <= 1e30, "attention: scale must be finite, got ", s);
-    return std::get<0>(attention_op(query, key, value, mask, lengths, causal, s));
+    const bool train = at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad());
+    return std::get<0>(attention_op(query, key, value, mask, lengths, causal, s, train));
 }
 
 at::Tensor rotary_embedding(const at::Tensor &x, const at::Tensor &positions, const at::Tensor &frequencies,
@@ -403,21 +420,21 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
         TORCH_CHECK(!(mask.has_value() && mask->defined() && mask->requires_grad()),
                     "attention: the mask has no gradient; pass mask.detach()");
         at::AutoDispatchBelowADInplaceOrView g;
-        auto r = attention_op(query, key, value, mask, lengths, causal, scale);
-        auto out = std::get<0>(r), stats = std::get<1>(r);
-        ctx->save_for_backward({query, key, value, out, stats, mask.has_value() ? *mask : at::Tensor(),
+        auto r = attention_op(query, key, value, mask, lengths, causal, scale, true);
+        auto out = std::get<0>(r), stats = std::get<1>(r), rest = std::get<2>(r);
+        ctx->save_for_backward({query, key, value, out, stats, rest, mask.has_value() ? *mask : at::Tensor(),
                                 lengths.has_value() ? *lengths : at::Tensor()});
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["scale"] = scale;
-        ctx->mark_non_differentiable({stats});
-        return {out, stats};
+        ctx->mark_non_differentiable({stats, rest});
+        return {out, stats, rest};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "attention: second derivatives are not implemented");
         auto s = ctx->get_saved_variables();
         const auto opt = [](const at::Tensor &x) { return x.defined() ? OptTensor(x) : OptTensor(); };
         auto grad = grads[0].defined() ? grads[0] : at::zeros_like(s[3]);
-        auto g = attention_backward_op(grad, s[0], s[1], s[2], s[3], s[4], opt(s[5]), opt(s[6]),
+        auto g = attention_backward_op(grad, s[0], s[1], s[2], s[3], s[4], s[5], opt(s[6]), opt(s[7]),
                                        ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
         return {std::get<0>(g), std::get<1>(g), std::get<2>(g), Variable(), Variable(), Variable(), Variable()};
     }
@@ -443,11 +460,16 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     }
 };
 
-std::tuple<at::Tensor, at::Tensor> attention_autograd(const at::Tensor &query, const at::Tensor &key,
-                                                      const at::Tensor &value, const OptTensor &mask,
-                                                      const OptTensor &lengths, bool causal, double scale) {
+Results attention_autograd(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value, const OptTensor &mask,
+                           const OptTensor &lengths, bool causal, double scale, bool train) {
+    if (!train) {
+        TORCH_CHECK(!(at::GradMode::is_enabled() && mask.has_value() && mask->defined() && mask->requires_grad()),
+                    "attention: the mask has no gradient; pass mask.detach()");
+        at::AutoDispatchBelowADInplaceOrView g;
+        return attention_op(query, key, value, mask, lengths, causal, scale, false);
+    }
     auto r = AttentionFunction::apply(query, key, value, mask, lengths, causal, scale);
-    return {r[0], r[1]};
+    return {r[0], r[1], r[2]};
 }
 at::Tensor rotary_autograd(const at::Tensor &x, const at::Tensor &positions, const at::Tensor &frequencies,
                            bool interleaved, double scale, bool inverse) {
@@ -464,9 +486,9 @@ TORCH_LIBRARY_FRAGMENT(torchpairwise, m) {
           "float scale=1.0) -> Tensor",
           TORCH_FN(rotary_embedding));
     m.def("_attention(Tensor query, Tensor key, Tensor value, Tensor? mask, Tensor? lengths, bool causal, "
-          "float scale) -> (Tensor out, Tensor stats)");
+          "float scale, bool train) -> (Tensor out, Tensor stats, Tensor rest)");
     m.def("_attention_backward(Tensor grad, Tensor query, Tensor key, Tensor value, Tensor out, Tensor stats, "
-          "Tensor? mask, Tensor? lengths, bool causal, float scale) -> (Tensor, Tensor, Tensor)");
+          "Tensor rest, Tensor? mask, Tensor? lengths, bool causal, float scale) -> (Tensor, Tensor, Tensor)");
     m.def("_rotary(Tensor x, Tensor positions, Tensor frequencies, bool interleaved, float scale, bool inverse) -> Tensor");
 }
 
