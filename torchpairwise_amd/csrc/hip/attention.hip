@@ -173,7 +173,7 @@ template <typename T, int W, int DP, int BN, int MM, int kWaves, int OCC>
 __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args a) {
     using F = Forward<T, W, DP, BN, MM>;
     using M = typename F::M;
-    constexpr uint32_t kTileBytes = BN * DP * sizeof(T);
+    constexpr uint32_t kTileBytes = BN * Tile<T, DP>::kRowBytes;
     __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];  // two buffers of a key tile and a value tile
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     int64_t t = xcd_linear(blockIdx.x, gridDim.x);
@@ -225,8 +225,9 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
             st[row] = f.top;
             st[all + row] = sum;
         }
-        float *p = a.part + (part * all + row) * quads4(a.dv);
-        F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.dv, 1, v); });
+        const int width = (int)quads4(a.dv);
+        float *p = a.part + (part * all + row) * width;
+        F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, width, v); });
         return;
     }
     if (g == 0 && a.stats) {
@@ -451,8 +452,12 @@ int64_t plan_bits(Args &a, bool backward, uint8_t *at, BitArgs *p) {
 // Sets tiles and splits for the element type and width.
 template <typename T, int DP>
 void plan(Args &a) {
-    a.tiles = cdiv(a.n * a.group, (int64_t)Tiles<T, DP>::kWaves * Tiles<T, DP>::kWidth);
-    a.splits = (int)parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, Tiles<T, DP>::kKeys), Tiles<T, DP>::kPerCu, uneven(a));
+    using L = Tiles<T, DP>;
+    constexpr int64_t kOwn = L::kWaves * L::kWidth;
+    a.tiles = cdiv(a.n * a.group, kOwn);
+    a.splits = (int)parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, L::kKeys), L::kPerCu, uneven(a),
+                              step_us<T, DP>(kOwn, L::kKeys, 2, L::kPerCu),
+                              part_us(a.batch * a.heads * a.n, quads4(a.dv)));
 }
 
 }  // namespace
@@ -467,7 +472,15 @@ int prepare_operands(Args &a, const tpw_attention_desc *d, bool backward, void *
     if (const size_t bytes = plan_padding(a, d->dtype, backward, next, &p)) {
         const int64_t blocks = cdiv(p.first[p.count], 256);
         TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: too many rows");
-        if (d->dtype == TPW_F32)
+        bool pairs = d->dtype == TPW_BF16;  // bf16 rows of whole dwords: copied by dwords
+        for (int t = 0; t < p.count; ++t)
+            pairs = pairs && p.width[t] % 2 == 0 && p.from[t].b % 2 == 0 && p.from[t].h % 2 == 0 && p.from[t].n % 2 == 0 &&
+                    reinterpret_cast<uintptr_t>(p.from[t].p) % 4 == 0;
+        for (int t = 0; pairs && t < p.count; ++t) {
+            p.width[t] /= 2;
+            p.from[t].b /= 2, p.from[t].h /= 2, p.from[t].n /= 2;
+        }
+        if (d->dtype == TPW_F32 || pairs)
             hipLaunchKernelGGL((pad_kernel<uint32_t>), dim3((unsigned)blocks), dim3(256), 0, s, p);
         else
             hipLaunchKernelGGL((pad_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, s, p);
@@ -522,7 +535,6 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
     a.scale = d->scale == 0 ? 1.0f : (float)(fabs(d->scale) * (bias ? 1.0 : 1.4426950408889634));
     a.gscale = (float)d->scale;
     a.rest = d->dtype == TPW_BF16 ? d->out_rest : nullptr;
-    a.vec_out = whole_pieces(a.o, a.dv, size) && aligned16(a.rest);
     const auto streamed = [&](const View &v, int64_t rows, int64_t width) {
         return a.batch * a.heads * a.n * a.m == 0 || rows <= 1 || (v.n >= width && v.n * size <= (int64_t(1) << 23));
     };
@@ -532,7 +544,6 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
         a.gq = view_of(d->grad_query, d->grad_query_strides, d->n, d->d);
         a.gk = view_of(d->grad_key, d->grad_key_strides, d->m, d->d);
         a.gv = view_of(d->grad_value, d->grad_value_strides, d->m, d->dv);
-        a.vec_out = whole_pieces(a.gq, a.d, size) && whole_pieces(a.gk, a.d, size) && whole_pieces(a.gv, a.dv, size);
         ok = ok && streamed(a.q, d->n, d->d) && streamed(a.go, d->n, d->dv);
     }
     TPW_REQUIRE(ok, "attention: rows of an operand overlap or lie more than 8 MiB apart");
@@ -598,7 +609,7 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
                 hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias>), dim3((unsigned)cdiv(rows * cdiv(a.dv, 4), 256)),
                                    dim3(256), 0, s, a);
             else
-                hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, DP / 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
+                hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, Tile<T, DP>::P / 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
             return check_launch("attention_join_kernel");
         }
         return TPW_OK;

@@ -52,7 +52,6 @@ struct Args {
     float qsign;   // -1, 0 or 1: the sign of scale, folded into q as it is loaded
     float gscale;  // scale (backward)
     int causal;
-    int vec_out;   // the outputs' rows take stores of four features
     int64_t tiles;  // row tiles (dk / dv: key tiles) per (batch, key head)
     int splits;     // parts of the summed axis
     float *ds;      // kept score gradients (backward of wide fp32 rows): [key heads' heads, m, ds_pitch]
@@ -126,15 +125,16 @@ __device__ __forceinline__ void unpack8(const Frag<float> &f, float (&x)[8]) {
 }
 
 // ---- LDS tiles -----------------------------------------------------------------------------
-// A tile of ROWS rows of DP features lies as 16-byte pieces, piece c of row r at position
-// c ^ swz(r).  Every 16 consecutive rows put one piece into the 16 different 16-byte slots of the 64
+// A tile of ROWS rows of DP features, with room for a power of two of them, lies as 16-byte pieces,
+// piece c of row r at position c ^ swz(r).  Every 16 consecutive rows put one piece into the 16 different 16-byte slots of the 64
 // banks (row fragments), and four consecutive rows put a run of four pieces into four different
 // quarters of them (transposing reads), so that either read moves 256 bytes a cycle.
 template <typename T, int DP>
 struct Tile {
-    static constexpr int E = 16 / (int)sizeof(T);  // elements per piece
-    static constexpr int C = DP / E;               // pieces per row
-    static constexpr int kRowBytes = DP * (int)sizeof(T);
+    static constexpr int P = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;  // features a row has room for
+    static constexpr int E = 16 / (int)sizeof(T);                    // elements per piece
+    static constexpr int C = P / E;                                  // pieces per row
+    static constexpr int kRowBytes = P * (int)sizeof(T);
     static constexpr int kMask = C >= 16 ? 15 : 7;  // bits of a piece's index that swz reaches
     static_assert(C >= 8, "rows of 128 bytes at least");
     // rows of 128 bytes: two rows share the banks, so the pairs of rows take turns
@@ -332,23 +332,24 @@ __device__ __forceinline__ Frag<T> load_row8(const T *row, int f, int d) {
     return r;
 }
 
-// Four consecutive features of an output row.
-__device__ __forceinline__ void store4(float *row, int f, int d, int vec, f32x4 v) {
-    if (vec) {
-        if (f < d) *reinterpret_cast<f32x4 *>(row + f) = v;
+// Four consecutive features of an output row: one store of any alignment (global memory takes it),
+// element by element past the last whole quad.
+__device__ __forceinline__ void store4(float *row, int f, int d, f32x4 v) {
+    if (f + 4 <= d) {
+        __builtin_memcpy(row + f, &v, 16);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 3; ++e)
             if (f + e < d) row[f + e] = v[e];
     }
 }
-__device__ __forceinline__ void store4(uint16_t *row, int f, int d, int vec, f32x4 v) {
-    if (vec) {
-        if (f < d)
-            *reinterpret_cast<uint2 *>(row + f) = make_uint2(f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]));
+__device__ __forceinline__ void store4(uint16_t *row, int f, int d, f32x4 v) {
+    if (f + 4 <= d) {
+        const uint2 w = make_uint2(f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]));
+        __builtin_memcpy(row + f, &w, 8);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 3; ++e)
             if (f + e < d) row[f + e] = f32_to_bf16_rne(v[e]);
     }
 }
@@ -356,25 +357,25 @@ __device__ __forceinline__ void store4(uint16_t *row, int f, int d, int vec, f32
 // What rounding the four values above left, rounded in turn.  delta = do . o of a row that rests on few
 // keys meets ds = p (dp - delta) with everything cancelled: from o alone, 2^-8 of each value off, dq and
 // dk of short or sparse rows would lose a quarter of their precision.
-__device__ __forceinline__ void store_rest4(uint16_t *row, int f, int d, int vec, f32x4 v) {
+__device__ __forceinline__ void store_rest4(uint16_t *row, int f, int d, f32x4 v) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] -= bf16_to_f32(f32_to_bf16_rne(v[e]));
-    store4(row, f, d, vec, v);
+    store4(row, f, d, v);
 }
 // Output row of head h, row i: values, and their rest where it is wanted.
 template <typename T>
 struct OutRow {
     T *row, *rest;
-    int d, vec;
-    __device__ __forceinline__ OutRow(const Args &a, int64_t b, int64_t h, int64_t i) : d((int)a.dv), vec(a.vec_out) {
+    int d;
+    __device__ __forceinline__ OutRow(const Args &a, int64_t b, int64_t h, int64_t i) : d((int)a.dv) {
         const int64_t at = b * a.o.b + h * a.o.h + i * a.o.n;
         row = reinterpret_cast<T *>(const_cast<void *>(a.o.p)) + at;
         rest = a.rest ? reinterpret_cast<T *>(a.rest) + at : nullptr;
     }
     __device__ __forceinline__ void store(int f, f32x4 v) const {
-        store4(row, f, d, vec, v);
+        store4(row, f, d, v);
         if constexpr (sizeof(T) == 2)
-            if (rest) store_rest4(rest, f, d, vec, v);
+            if (rest) store_rest4(rest, f, d, v);
     }
 };
 
@@ -459,14 +460,15 @@ __device__ __forceinline__ int64_t xcd_linear(int64_t bid, int64_t total) {
 template <typename T, int DP>
 struct Tiles {
     static constexpr int kWidth = sizeof(T) == 2 ? 32 : 16;  // W of the matrix instructions
-    static constexpr int kWaves = DP * (int)sizeof(T) == 1024 ? 8 : 4;
-    static constexpr int kKeys = DP * (int)sizeof(T) <= 256 ? 64 : 32;
+    static constexpr int kRowBytes = Tile<T, DP>::kRowBytes;
+    static constexpr int kWaves = kRowBytes == 1024 ? 8 : 4;
+    static constexpr int kKeys = kRowBytes <= 256 ? 64 : 32;
     static constexpr int kRowWaves = 4, kRows = 32;          // dk / dv kernel
-    // blocks that share a CU: forward, dq, dk / dv
-    static constexpr bool kNarrow = DP * (int)sizeof(T) == 128;  // bf16 at 64 features
+    // blocks that share a CU (waves per SIMD, for the compiler): forward, dq, dk / dv
+    static constexpr bool kNarrow = kRowBytes == 128;  // bf16 up to 64 features
     static constexpr int kPerCu = kNarrow ? 4 : kWaves == 8 ? 1 : 2;
-    static constexpr int kPerCuQ = kNarrow ? 3 : DP == 256 ? 1 : 2;
-    static constexpr int kPerCuK = DP == 256 || (DP == 128 && sizeof(T) == 4) ? 1 : 2;
+    static constexpr int kPerCuQ = kNarrow ? 3 : kWaves == 8 || DP == 256 ? 1 : 2;
+    static constexpr int kPerCuK = DP == 256 || (DP > 64 && sizeof(T) == 4) ? 1 : 2;
 };
 
 // Host side (attention.hip): reads a descriptor into the kernels' arguments; bytes that a call's
@@ -489,8 +491,13 @@ int by_width(const Args &a, int mode, F &&f) {
         if (mode == kKeep) return f(T{}, dp, Const<kKeep>{});
         return f(T{}, dp, Const<kBias>{});
     };
+    // widths between the powers of two, where a third of the products would be of zeros (the fp32 column
+    // pieces are of 64 features)
     if (w <= 64) return by_mode(Const<64>{});
+    if constexpr (sizeof(T) == 2)
+        if (w <= 96) return by_mode(Const<96>{});
     if (w <= 128) return by_mode(Const<128>{});
+    if (w <= 192) return by_mode(Const<192>{});
     return by_mode(Const<256>{});
 }
 template <typename F>
@@ -500,20 +507,42 @@ int by_type(const Args &a, int dtype, int mode, F &&f) {
 inline int mask_mode(const tpw_attention_desc *d) {
     return d->mask_type == TPW_MASK_NONE ? kNoMask : d->mask_type == TPW_MASK_KEEP ? kKeep : kBias;
 }
-// Parts of a summed axis of `steps` tiles for `blocks` blocks where a CU holds `per_cu` of them: as
-// many as still run all at once on 256 CUs (one more would start a second round), at most one per
-// step and kMaxParts.  Where blocks differ in length (a square causal call's longest takes
-// twice the mean) twice as many, longest first, so that short ones fill up behind long ones (dk / dv of causal 2 x 4 key heads x 8192 keys x 128: 1.76 ms in 512 blocks,
-// 1.23 in 1024 and 0.035 for the sum of their parts).
-inline bool uneven(const Args &a) { return a.causal && 2 * a.n > a.m; }
+// Parts of a summed axis of `steps` tiles for `blocks` blocks, `per_cu` of which share a CU: the least
+// of the time that this model gives.
+//   - A tile takes a block step_us with its CU full and about half of that alone (fp32-masked bf16 at 128
+//     features: 3.3 us two by two, 2.4 alone).
+//   - Blocks run in rounds of 256 per_cu.  A square causal call's differ in length, the longest twice
+//     the mean, and start with the longest: the rounds run into one another.
+//   - Parts cost the launch that joins them (6 us, host and device) and their bytes, written and read (part_us each).
+// dk / dv of causal 2 x 4 key heads x 8192 keys x 128: 1.76 ms in 512 blocks, 1.23 + 0.035 in 1024;
+// forward of causal 8 x 4 (2) x 587 x 128: 28 + 24 us in seven parts.
 constexpr int kMaxParts = 64;  // the join gives each part a lane
-inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu, bool uneven) {
-    if (blocks <= 0 || steps <= 1) return 1;
-    int64_t p = uneven ? cdiv(2 * 256 * per_cu, blocks) : 256 * per_cu / blocks;
-    if (steps < 4) p = 1;  // a tile or two take less than the join's launch
-    p = p < steps ? p : steps;
-    return p < 1 ? 1 : p < kMaxParts ? p : kMaxParts;
+inline bool uneven(const Args &a) { return a.causal && 2 * a.n > a.m; }
+inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu, bool uneven, double step_us, double part_us) {
+    if (blocks <= 0) return 1;
+    int64_t best = 1;
+    double least = 0;
+    for (int64_t p = 1; p <= steps && p <= kMaxParts; ++p) {
+        const int64_t n = blocks * p, slots = 256 * per_cu, sharing = cdiv(n, 256) < per_cu ? cdiv(n, 256) : per_cu;
+        const double step = step_us * (0.5 + 0.5 * (double)sharing / (double)per_cu), len = (double)cdiv(steps, p);
+        const double flow = 0.5 * (double)steps * (double)blocks / (double)slots + 0.125 * len;
+        double t = step * (!uneven ? (double)cdiv(n, slots) * len : len > flow ? len : flow);
+        if (p > 1) t += 6.0 + (double)p * part_us;
+        if (p == 1 || t < least) {
+            least = t;
+            best = p;
+        }
+        if (n >= 4 * slots) break;
+    }
+    return best;
 }
+// Microseconds of one tile with its CU full: `products` products of own x streamed x DP at the rate
+// the kernels reach (0.9 PFLOP/s bf16, 120 TFLOP/s fp32).
+template <typename T, int DP>
+double step_us(int64_t own, int64_t streamed, int products, int64_t per_cu) {
+    return 2.0 * products * (double)own * (double)streamed * DP * (double)per_cu * 256.0 / (sizeof(T) == 2 ? 0.9e9 : 0.12e9);
+}
+inline double part_us(int64_t rows, int64_t width) { return 2.0 * 4.0 * (double)rows * (double)width / 4.5e6; }
 
 }  // namespace attn
 }  // namespace tpw

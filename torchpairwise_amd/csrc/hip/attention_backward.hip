@@ -17,16 +17,16 @@ namespace tpw {
 namespace attn {
 
 // Runs N steps of `use` on fragments that `load` reads from LDS, the next step's reads issued before
-// this step's products.  The compiler may not move the reads further ahead: left alone it hoists
-// them all and spills the accumulators.
-template <int N, int F, typename Piece, typename Load, typename Use>
+// this step's products.  FENCED: the compiler may not move the reads further ahead; left alone it hoists
+// them all, which spills the accumulators where registers are scarce.
+template <int N, int F, typename Piece, bool FENCED = true, typename Load, typename Use>
 __device__ __forceinline__ void stream_steps(Load load, Use use) {
     Piece f[2][F];
     load(0, f[0]);
 #pragma unroll
     for (int x = 0; x < N; ++x) {
         if (x + 1 < N) load(x + 1, f[(x + 1) & 1]);
-        asm volatile("" ::: "memory");
+        if constexpr (FENCED) asm volatile("" ::: "memory");
         use(x, f[x & 1]);
     }
 }
@@ -39,7 +39,8 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
     using Acc = typename M::Acc;
     using CR = ColReader<T, DP, W>;
     constexpr int DB = DP / W, QS = DP / M::KS, NU = kUnit / W, ST = kUnit / M::KS;
-    constexpr uint32_t kTileBytes = BN * DP * sizeof(T);
+    constexpr bool kFenced = DP == 192 || sizeof(T) == 4;
+    constexpr uint32_t kTileBytes = BN * Tile<T, DP>::kRowBytes;
     __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane / W;
     int64_t t = xcd_linear(blockIdx.x, gridDim.x);
@@ -144,30 +145,31 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
             Acc s[NU], dp[NU];
 #pragma unroll
             for (int i = 0; i < NU; ++i) s[i] = dp[i] = Acc{};
-#pragma unroll
-            for (int k = 0; k < QS; ++k) {
-                Frag<T> fk[NU], fv[NU];
-#pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    fk[i] = rr.read(kt, u * NU + i, k);
-                    fv[i] = rr.read(vt, u * NU + i, k);
-                }
-                if constexpr (sizeof(T) == 4) {  // independent products side by side
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-#pragma unroll
-                        for (int i = 0; i < NU; ++i) {
-                            M::mma1(s[i], fk[i], q[k], e);
-                            M::mma1(dp[i], fv[i], go[k], e);
-                        }
-                } else {
+            stream_steps<QS, 2 * NU, Frag<T>, kFenced>(
+                [&](int x, Frag<T>(&f)[2 * NU]) {
 #pragma unroll
                     for (int i = 0; i < NU; ++i) {
-                        M::mma(s[i], fk[i], q[k]);
-                        M::mma(dp[i], fv[i], go[k]);
+                        f[2 * i] = rr.read(kt, u * NU + i, x);
+                        f[2 * i + 1] = rr.read(vt, u * NU + i, x);
                     }
-                }
-            }
+                },
+                [&](int x, const Frag<T>(&f)[2 * NU]) {
+                    if constexpr (sizeof(T) == 4) {  // independent products side by side
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+#pragma unroll
+                            for (int i = 0; i < NU; ++i) {
+                                M::mma1(s[i], f[2 * i], q[x], e);
+                                M::mma1(dp[i], f[2 * i + 1], go[x], e);
+                            }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NU; ++i) {
+                            M::mma(s[i], f[2 * i], q[x]);
+                            M::mma(dp[i], f[2 * i + 1], go[x]);
+                        }
+                    }
+                });
             if constexpr (MM == kBias) {
                 const void *mr = mask_row(a, b, qh, qi);
 #pragma unroll
@@ -219,6 +221,7 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
                     s[i][e] = p * inv * (dp[i][e] - delta);
                 }
             // ds of bf16 inputs is rounded to bf16 for the matrix cores, as p is
+            Frag<T> ds[ST];
 #pragma unroll
             for (int st = 0; st < ST; ++st) {
                 float x[8];
@@ -226,20 +229,22 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
                 for (int v = 0; v < 2; ++v)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[4 * v + e] = s[(2 * st + v) / M::Q][4 * ((2 * st + v) % M::Q) + e];
-                const Frag<T> ds = pack8(x, T{});
-#pragma unroll
-                for (int c = 0; c < CR::kPieces; ++c) CR::use(dq, c, cr.read(kt, u * ST + st, c), ds);
+                ds[st] = pack8(x, T{});
             }
+            stream_steps<ST * CR::kPieces, 1, typename CR::Piece, kFenced>(
+                [&](int x, typename CR::Piece(&f)[1]) { f[0] = cr.read(kt, u * ST + x / CR::kPieces, x % CR::kPieces); },
+                [&](int x, const typename CR::Piece(&f)[1]) { CR::use(dq, x % CR::kPieces, f[0], ds[x / CR::kPieces]); });
         }
     }
     if (!live) return;
     if (a.splits > 1) {
-        float *p = a.part + (part * all + row) * quads4(a.d);
-        CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.d, 1, v); });
+        const int width = (int)quads4(a.d);
+        float *p = a.part + (part * all + row) * width;
+        CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, width, v); });
         return;
     }
     T *p = reinterpret_cast<T *>(const_cast<void *>(a.gq.p)) + b * a.gq.b + qh * a.gq.h + qi * a.gq.n;
-    CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.d, a.vec_out, v * a.gscale); });
+    CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.d, v * a.gscale); });
 }
 
 template <typename T, int W, int DP, int BM, int MM, int kWaves, int OCC, bool VLDS, int OUT>
@@ -248,9 +253,9 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
     using Acc = typename M::Acc;
     using CR = ColReader<T, DP, W>;
     constexpr int DB = DP / W, QS = DP / M::KS, NU = kUnit / W, ST = kUnit / M::KS;
-    constexpr uint32_t kTileBytes = BM * DP * sizeof(T), kBuf = 2 * kTileBytes + 3 * 64 * 4;
+    constexpr uint32_t kTileBytes = BM * Tile<T, DP>::kRowBytes, kBuf = 2 * kTileBytes + 3 * 64 * 4;
     static_assert(BM <= 64, "one DMA of row values per array");
-    constexpr uint32_t kValues = VLDS ? kWaves * W * DP * sizeof(T) : 0;
+    constexpr uint32_t kValues = VLDS ? kWaves * W * Tile<T, DP>::kRowBytes : 0;
     // two buffers of a q tile, a do tile and the row values; the block's value rows
     __shared__ __attribute__((aligned(256))) uint4 smem[(2 * kBuf + kValues) / 16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane / W;
@@ -494,9 +499,9 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
         T *out_row = reinterpret_cast<T *>(const_cast<void *>(out.p)) + b * out.b + kh * out.h + j * out.n;
         CR::each(acc, lane, [&](int f, f32x4 x) {
             if (a.splits > 1)
-                store4(part_row, f, (int)width, 1, x);
+                store4(part_row, f, (int)quads4(width), x);
             else
-                store4(out_row, f, (int)width, a.vec_out, x * scale);
+                store4(out_row, f, (int)width, x * scale);
         });
     };
     if constexpr (DK) store(dk, a.d, 0, a.gk, a.gscale);
@@ -529,7 +534,7 @@ __global__ __launch_bounds__(512, 2) void attention_ds_product_kernel(const Args
     constexpr int W = 16, kWaves = 8;
     using M = Mma<float, W>;
     using CR = ColReader<float, DP, W>;
-    constexpr uint32_t kTileBytes = kUnit * DP * 4;
+    constexpr uint32_t kTileBytes = kUnit * Tile<float, DP>::kRowBytes;
     __shared__ __attribute__((aligned(256))) uint4 smem[2 * kTileBytes / 16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane / W;
     const int64_t t = xcd_linear(blockIdx.x, gridDim.x), own_tiles = cdiv_dev(KEYS ? a.m : a.n, kWaves * W);
@@ -616,7 +621,7 @@ __global__ __launch_bounds__(512, 2) void attention_ds_product_kernel(const Args
     const View &out = KEYS ? a.gk : a.gq;
     float *row = reinterpret_cast<float *>(const_cast<void *>(out.p)) + b * out.b +
                  (KEYS ? kh : kh * a.group + head) * out.h + o * out.n;
-    CR::each(acc, lane, [&](int f, f32x4 v) { store4(row, f, (int)a.d, a.vec_out, v * a.gscale); });
+    CR::each(acc, lane, [&](int f, f32x4 v) { store4(row, f, (int)a.d, v * a.gscale); });
 }
 
 // Sums the parts of one or two gradients, in their order, one thread per four features: rows of fp32
@@ -627,7 +632,7 @@ struct SumArgs {
     int64_t width[2];
     float scale[2];
     int64_t rows, heads, n;
-    int splits, vec_out;
+    int splits;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void attention_sum_kernel(const SumArgs a) {
@@ -651,7 +656,7 @@ __global__ __launch_bounds__(256) void attention_sum_kernel(const SumArgs a) {
     const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
     const View out = which ? a.out[1] : a.out[0];
     store4(reinterpret_cast<T *>(const_cast<void *>(out.p)) + b * out.b + h * out.h + i * out.n, f,
-           (int)(which ? a.width[1] : a.width[0]), a.vec_out,
+           (int)(which ? a.width[1] : a.width[0]),
            x * (which ? a.scale[1] : a.scale[0]));
 }
 
@@ -685,8 +690,12 @@ BackwardPlan backward_plan(const Args &a) {
     const int64_t bk = a.batch * a.key_heads;
     p.q_tiles = cdiv(a.n * a.group, (int64_t)L::kWaves * L::kWidth);
     p.k_tiles = cdiv(a.m, (int64_t)L::kRowWaves * L::kWidth);
-    p.q_splits = (int)parts_for(bk * p.q_tiles, cdiv(a.m, L::kKeys), L::kPerCuQ, uneven(a));
-    p.k_splits = (int)parts_for(bk * p.k_tiles, a.group * cdiv(a.n, L::kRows), L::kPerCuK, uneven(a));
+    p.q_splits = (int)parts_for(bk * p.q_tiles, cdiv(a.m, L::kKeys), L::kPerCuQ, uneven(a),
+                                step_us<T, DP>((int64_t)L::kWaves * L::kWidth, L::kKeys, 3, L::kPerCuQ),
+                                part_us(a.batch * a.heads * a.n, quads4(a.d)));
+    p.k_splits = (int)parts_for(bk * p.k_tiles, a.group * cdiv(a.n, L::kRows), L::kPerCuK, uneven(a),
+                                step_us<T, DP>((int64_t)L::kRowWaves * L::kWidth, L::kRows, 4, L::kPerCuK),
+                                part_us(bk * a.m, quads4(a.d) + quads4(a.dv)));
     p.kept = keeps_ds<T, DP>(a);
     return p;
 }
@@ -754,7 +763,8 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
     return by_type(a, d->dtype, mask_mode(d), [&](auto t, auto dp, auto mode) {
         using T = decltype(t);
         constexpr int DP = decltype(dp)::value, MM = decltype(mode)::value, W = Tiles<T, DP>::kWidth;
-        constexpr int kOcc = sizeof(T) == 2 && DP == 256 ? 1 : 2, kOccKv = DP == 256 ? 1 : 2;
+        constexpr int kOcc = sizeof(T) == 2 && DP == 256 ? 1 : 2, kOccKv = Tile<T, DP>::P == 256 ? 1 : 2;
+        constexpr bool kValuesInLds = Tile<T, DP>::P == 128;
         const BackwardPlan p = backward_plan<T, DP>(a);
         const int64_t bk = a.batch * a.key_heads;
         TPW_REQUIRE(bk * p.q_tiles * p.q_splits < (int64_t(1) << 31) && bk * p.k_tiles * p.k_splits < (int64_t(1) << 31),
@@ -773,7 +783,7 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
             if (const int rc = check_launch("attention_dq_kernel")) return rc;
             if (a.splits > 1)
                 if (const int rc = sum_parts<T>(
-                        {a.part, {a.gq, {}}, {a.d, 0}, {a.gscale, 0.0f}, rows, a.heads, a.n, a.splits, a.vec_out}, s))
+                        {a.part, {a.gq, {}}, {a.d, 0}, {a.gscale, 0.0f}, rows, a.heads, a.n, a.splits}, s))
                     return rc;
         }
         if (keys) {
@@ -782,18 +792,17 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
             const dim3 grid((unsigned)(bk * a.tiles * a.splits)), block(64 * Tiles<T, DP>::kRowWaves);
             // bf16 at 256 features: dk and dv would take all 256 accumulation registers and leave none for
             // the scores, so each is a launch of its own
-            constexpr bool kApart = sizeof(T) == 2 && DP == 256;
+            constexpr bool kApart = sizeof(T) == 2 && DP > 128;
             constexpr int kRows = Tiles<T, DP>::kRows, kWaves = Tiles<T, DP>::kRowWaves;
             if constexpr (kApart) {
                 hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, 2, false, 2>), grid, block, 0, s, a);
-                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, 1, false, 1>), grid, block, 0, s, a);
+                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, DP == 256 ? 1 : 2, false, 1>), grid, block, 0, s, a);
             } else {
-                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, kOccKv, DP == 128, 3>), grid, block, 0, s, a);
+                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, kOccKv, kValuesInLds, 3>), grid, block, 0, s, a);
             }
             if (const int rc = check_launch("attention_dkv_kernel")) return rc;
             if (a.splits > 1)
-                return sum_parts<T>({a.part, {a.gk, a.gv}, {a.d, a.dv}, {a.gscale, 1.0f}, keys, a.key_heads, a.m, a.splits,
-                                     a.vec_out}, s);
+                return sum_parts<T>({a.part, {a.gk, a.gv}, {a.d, a.dv}, {a.gscale, 1.0f}, keys, a.key_heads, a.m, a.splits}, s);
         }
         return TPW_OK;
     });
