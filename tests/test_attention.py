@@ -451,6 +451,22 @@ def test_neighbour_mask_feeds_attention():
     assert_close(out, want["out"][0, 0], rtol=0.0, atol=want["tol_out"][0, 0] + TINY)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_example(device):
+    """The example's parts together: training lowers the loss, tokens over a cache give what one call
+    gives, neighbours correct labels."""
+    import importlib.util
+    from pathlib import Path
+
+    spec = importlib.util.spec_from_file_location("example", Path(__file__).parent.parent / "examples" / "attention.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    r = example.main(device, steps=60)
+    assert r["last_loss"] < 0.5 * r["first_loss"]
+    assert r["decode_gap"] < 1e-3  # logits of order 10 in fp32
+    assert r["labels_after"] > r["labels_before"]
+
+
 # ---------------------------------------------------------------- rotary
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -1,3 +1,4 @@
+"""Attention and rotary positions (not in the reference)."""
 import torch
 
 from torchpairwise_amd.ops.rotary import rotary_frequencies  # noqa: F401

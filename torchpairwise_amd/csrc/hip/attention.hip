@@ -332,8 +332,9 @@ int64_t round_up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 bool whole_pieces(const View &v, int64_t width, int64_t size) {
     return aligned16(v.p) && width * size % 16 == 0 && v.b * size % 16 == 0 && v.h * size % 16 == 0 && v.n * size % 16 == 0;
 }
-View view_of(const void *p, const int64_t *strides, int64_t rows, int64_t width) {
-    return {p, strides[0], strides[1], rows == 1 ? width : strides[2]};
+// Strides of dimensions of one entry reach nothing: whatever they are, they ask for no copy.
+View view_of(const void *p, const int64_t *strides, int64_t batch, int64_t heads, int64_t rows, int64_t width, int64_t size) {
+    return {p, batch == 1 ? 0 : strides[0], heads == 1 ? 0 : strides[1], rows == 1 ? cdiv(width * size, 16) * 16 / size : strides[2]};
 }
 
 constexpr int kPadded = 6;  // q, k, v, do, o and its rest
@@ -518,10 +519,10 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
     a.d = d->d;
     a.dv = d->dv;
     a.causal = d->causal != 0;
-    a.q = view_of(d->query, d->query_strides, d->n, d->d);
-    a.k = view_of(d->key, d->key_strides, d->m, d->d);
-    a.v = view_of(d->value, d->value_strides, d->m, d->dv);
-    a.o = view_of(d->out, d->out_strides, d->n, d->dv);
+    a.q = view_of(d->query, d->query_strides, d->batch, d->heads, d->n, d->d, size);
+    a.k = view_of(d->key, d->key_strides, d->batch, d->key_heads, d->m, d->d, size);
+    a.v = view_of(d->value, d->value_strides, d->batch, d->key_heads, d->m, d->dv, size);
+    a.o = view_of(d->out, d->out_strides, d->batch, d->heads, d->n, d->dv, size);
     a.stats = d->stats;
     a.lengths = d->lengths;
     a.mask = d->mask_type == TPW_MASK_NONE ? nullptr : d->mask;
@@ -540,10 +541,10 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
     };
     bool ok = streamed(a.k, d->m, d->d) && streamed(a.v, d->m, d->dv);
     if (backward) {
-        a.go = view_of(d->grad_out, d->grad_out_strides, d->n, d->dv);
-        a.gq = view_of(d->grad_query, d->grad_query_strides, d->n, d->d);
-        a.gk = view_of(d->grad_key, d->grad_key_strides, d->m, d->d);
-        a.gv = view_of(d->grad_value, d->grad_value_strides, d->m, d->dv);
+        a.go = view_of(d->grad_out, d->grad_out_strides, d->batch, d->heads, d->n, d->dv, size);
+        a.gq = view_of(d->grad_query, d->grad_query_strides, d->batch, d->heads, d->n, d->d, size);
+        a.gk = view_of(d->grad_key, d->grad_key_strides, d->batch, d->key_heads, d->m, d->d, size);
+        a.gv = view_of(d->grad_value, d->grad_value_strides, d->batch, d->key_heads, d->m, d->dv, size);
         ok = ok && streamed(a.q, d->n, d->d) && streamed(a.go, d->n, d->dv);
     }
     TPW_REQUIRE(ok, "attention: rows of an operand overlap or lie more than 8 MiB apart");
