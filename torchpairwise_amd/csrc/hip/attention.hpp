@@ -511,8 +511,9 @@ inline int mask_mode(const tpw_attention_desc *d) {
 // of the time that this model gives.
 //   - A tile takes a block step_us with its CU full and about half of that alone (fp32-masked bf16 at 128
 //     features: 3.3 us two by two, 2.4 alone).
-//   - Blocks run in rounds of 256 per_cu.  A square causal call's differ in length, the longest twice
-//     the mean, and start with the longest: the rounds run into one another.
+//   - Up to 256 per_cu blocks run at once, more as places come free, with a tail of a third of a block.
+//     A square causal call's differ in length, the longest twice the mean; they start with the longest,
+//     which speeds up as it is left alone.
 //   - Parts cost the launch that joins them (6 us, host and device) and their bytes, written and read (part_us each).
 // dk / dv of causal 2 x 4 key heads x 8192 keys x 128: 1.76 ms in 512 blocks, 1.23 + 0.035 in 1024;
 // forward of causal 8 x 4 (2) x 587 x 128: 28 + 24 us in seven parts.
@@ -526,7 +527,7 @@ inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu, bool une
         const int64_t n = blocks * p, slots = 256 * per_cu, sharing = cdiv(n, 256) < per_cu ? cdiv(n, 256) : per_cu;
         const double step = step_us * (0.5 + 0.5 * (double)sharing / (double)per_cu), len = (double)cdiv(steps, p);
         const double flow = 0.5 * (double)steps * (double)blocks / (double)slots + 0.125 * len;
-        double t = step * (!uneven ? (double)cdiv(n, slots) * len : len > flow ? len : flow);
+        double t = step * (uneven ? (0.85 * len > flow ? 0.85 * len : flow) : n <= slots ? len : len * ((double)n / (double)slots + 0.35));
         if (p > 1) t += 6.0 + (double)p * part_us;
         if (p == 1 || t < least) {
             least = t;
