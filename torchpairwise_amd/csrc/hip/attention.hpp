@@ -61,6 +61,7 @@ struct Args {
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <typename T, int W>
@@ -237,7 +238,7 @@ struct RowReader {
 //   at four features of row i / 4 and receives feature i % 16 of the four rows.
 //   fp32: piece c is rows u = c % 2 of features 64 (c / 2) .. + 63.  A lane reads features 4 (lane %
 //   16) .. + 3 of each row, so block 4 B + k holds features 64 B + 4 i + k: one 16-byte read feeds
-//   four products.
+//   four products.  The last 32 of 96 features go two by two.
 // `each` gives the results back as quads of consecutive features.
 template <typename T, int DP, int W>
 struct ColReader;
@@ -281,38 +282,54 @@ template <int DP>
 struct ColReader<float, DP, 16> {
     using L = Tile<float, DP>;
     using M = Mma<float, 16>;
-    static constexpr int kBlocks = DP / 16, kPieces = DP / 32;
+    static constexpr int kWhole = DP / 64, kHalf = DP % 64 / 32;
+    static constexpr int kBlocks = DP / 16, kPieces = 2 * (kWhole + kHalf);
+    static_assert(DP % 32 == 0, "pieces of 64 features and one of 32");
     struct Piece {
         f32x4 v[4];
     };
-    uint32_t at;
+    uint32_t at, half;
     __device__ __forceinline__ ColReader(int lane) {
-        const int r0 = 4 * (lane / 16);
-        at = (uint32_t)(r0 * L::kRowBytes + ((lane % 16) ^ L::swz(r0)) * 16);
+        const int r0 = 4 * (lane / 16), i = lane % 16;
+        at = (uint32_t)(r0 * L::kRowBytes + (i ^ L::swz(r0)) * 16);
+        half = (uint32_t)(r0 * L::kRowBytes + ((i >> 1) ^ L::swz(r0)) * 16 + (i & 1) * 8);
     }
     __device__ __forceinline__ Piece read(uint32_t tile, int t, int c) const {
         Piece p;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)  // swz(r0 + e) = swz(r0) ^ 4 e
-            p.v[e] = __builtin_bit_cast(
-                f32x4, lds_read16(L::piece(tile + at, (c / 2 * 16) ^ (4 * e), (16 * (2 * t + c % 2) + e) * L::kRowBytes)));
+        for (int e = 0; e < 4; ++e) {  // swz(r0 + e) = swz(r0) ^ 4 e
+            const int index = (c / 2 * 16) ^ (4 * e), far = (16 * (2 * t + c % 2) + e) * L::kRowBytes;
+            if (c / 2 < kWhole) {
+                p.v[e] = __builtin_bit_cast(f32x4, lds_read16(L::piece(tile + at, index, far)));
+            } else {
+                const f32x2 x = *reinterpret_cast<__attribute__((address_space(3))) const f32x2 *>(
+                    (uintptr_t)L::piece(tile + half, index, far));
+                p.v[e] = f32x4{x[0], x[1], 0.0f, 0.0f};
+            }
+        }
         return p;
     }
     static __device__ __forceinline__ void use(M::Acc *acc, int c, const Piece &a, const Frag<float> &p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < (c / 2 < kWhole ? 4 : 2); ++k)
                 acc[4 * (c / 2) + k] = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e][k], p.v[c % 2][e], acc[4 * (c / 2) + k], 0, 0, 0);
     }
     template <typename F>
     static __device__ __forceinline__ void each(const M::Acc *acc, int lane, F &&f) {
 #pragma unroll
-        for (int b = 0; b < kBlocks / 4; ++b)
+        for (int b = 0; b < kWhole; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 f(64 * b + 16 * (lane / 16) + 4 * r,
                   f32x4{acc[4 * b][r], acc[4 * b + 1][r], acc[4 * b + 2][r], acc[4 * b + 3][r]});
+        if constexpr (kHalf)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const auto &x = acc[4 * kWhole], &y = acc[4 * kWhole + 1];
+                f(64 * kWhole + 8 * (lane / 16) + 4 * h, f32x4{x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1]});
+            }
     }
 };
 
@@ -491,11 +508,9 @@ int by_width(const Args &a, int mode, F &&f) {
         if (mode == kKeep) return f(T{}, dp, Const<kKeep>{});
         return f(T{}, dp, Const<kBias>{});
     };
-    // widths between the powers of two, where a third of the products would be of zeros (the fp32 column
-    // pieces are of 64 features)
+    // widths between the powers of two too, where up to half of the products would be of zeros
     if (w <= 64) return by_mode(Const<64>{});
-    if constexpr (sizeof(T) == 2)
-        if (w <= 96) return by_mode(Const<96>{});
+    if (w <= 96) return by_mode(Const<96>{});
     if (w <= 128) return by_mode(Const<128>{});
     if (w <= 192) return by_mode(Const<192>{});
     return by_mode(Const<256>{});
