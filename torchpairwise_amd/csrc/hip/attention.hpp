@@ -526,7 +526,7 @@ inline int mask_mode(const tpw_attention_desc *d) {
 // of the time that this model gives.
 //   - A tile takes a block step_us with its CU full and about half of that alone (fp32-masked bf16 at 128
 //     features: 3.3 us two by two, 2.4 alone).
-//   - Up to 256 per_cu blocks run at once, more as places come free, with a tail of a third of a block.
+//   - Up to 256 per_cu blocks run at once, more as places come free: a started round costs a third of one.
 //     A square causal call's differ in length, the longest twice the mean; they start with the longest,
 //     which speeds up as it is left alone.
 //   - Parts cost the launch that joins them (6 us, host and device) and their bytes, written and read (part_us each).
@@ -542,7 +542,9 @@ inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu, bool une
         const int64_t n = blocks * p, slots = 256 * per_cu, sharing = cdiv(n, 256) < per_cu ? cdiv(n, 256) : per_cu;
         const double step = step_us * (0.5 + 0.5 * (double)sharing / (double)per_cu), len = (double)cdiv(steps, p);
         const double flow = 0.5 * (double)steps * (double)blocks / (double)slots + 0.125 * len;
-        double t = step * (uneven ? (0.85 * len > flow ? 0.85 * len : flow) : n <= slots ? len : len * ((double)n / (double)slots + 0.35));
+        const double rounds = (double)(n / slots), over = (double)(n % slots) / (double)slots;
+        const double even = len * (rounds == 0 ? 1.0 : rounds + (over > 0 ? 0.35 + 0.65 * over : 0.0));
+        double t = step * (!uneven ? even : 0.85 * len > flow ? 0.85 * len : flow);
         if (p > 1) t += 6.0 + (double)p * part_us;
         if (p == 1 || t < least) {
             least = t;
