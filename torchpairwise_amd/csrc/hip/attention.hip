@@ -168,7 +168,14 @@ struct Forward {
     }
 };
 
-// One block: kWaves * W query rows of the rows that share a key head, over the keys of one part.
+// One block: kWaves * W query rows of the rows that share a key head, over the keys of one part.  The
+// next tile of keys and values travels by DMA while this one is worked on, one barrier a tile.
+// Bound by the matrix cores beside the softmax: a 32 x 64 tile of scores at 128 features is 1024 cycles
+// of products and about 900 of maxima, exponentials, sums and packing, which the two waves of a SIMD
+// overlap.  bf16, not causal: 2 x 16 (4) x 8192^2 x 128 in 1.09 to 1.19 ms (0.92 to 1.01 PFLOP/s), 8 x
+// 8192^2 x 256 in 0.55 (0.99), 32 x 4096^2 x 64 in 0.18 (0.77: exponentials).  fp32: 8 x 8192^2 x 256 in
+// 4.2 ms (130 TFLOP/s).  One token of 16 x 16 (2) heads over 32768 keys: 4.6 TB/s.  Priorities (s_setprio)
+// around the products or the softmax changed nothing.
 template <typename T, int W, int DP, int BN, int MM, int kWaves, int OCC>
 __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args a) {
     using F = Forward<T, W, DP, BN, MM>;
@@ -346,7 +353,8 @@ struct PadArgs {
 };
 
 // Dense copies [batch, heads, rows, whole pieces] of operands, zeros past their width; one thread per
-// 16-byte piece.
+// 16-byte piece.  Staging such rows element by element inside the kernels took 200 to 300 us where the
+// copies of 4 x 3001 rows of 90 take 6 to 12.
 template <typename T>
 __global__ void pad_kernel(const PadArgs a) {
     constexpr int E = 16 / (int)sizeof(T);
@@ -405,7 +413,7 @@ struct BitArgs {
 
 // Bits of a boolean mask, one row of words for each of its distinct rows (a broadcast dimension
 // counts once): the kernels test a bit of a word where they would load a byte, and the heads that
-// share a mask read an eighth of it.  For the backward also by column: word (i / 32, j) holds rows
+// share a mask read an eighth of it (3001^2: 9 us, for 110 to 230 less in each kernel).  For the backward also by column: word (i / 32, j) holds rows
 // 32 (i / 32) .. + 31 of key j.  One wave per 64 keys x 32 rows; all of its loads are in flight at once.
 __global__ __launch_bounds__(256) void pack_mask_kernel(const BitArgs a) {
     const int64_t pairs = a.words / 2, steps = cdiv_dev(a.n, 32), id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);

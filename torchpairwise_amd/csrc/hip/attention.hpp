@@ -3,7 +3,8 @@
 //   s_ij = scale q_i . k_j (+ mask_ij),  p_ij = exp(s_ij - m_i) / l_i,  o_i = sum_j p_ij v_j
 //
 // with the row maximum m_i and sum l_i over the keys that the mask, the causal limit and the
-// lengths leave; a row that none is left to gives zeros.  No [n, m] matrix is written.
+// lengths leave; a row that none is left to gives zeros.  No [n, m] matrix is written (but for the score
+// gradients of wide fp32 rows, a bounded number of heads at a time).
 //
 // Products run on the matrix cores, transposed so that a lane owns one row: a block of W x W
 // scores is K (first operand, from LDS) times Q (second operand, in registers), and its
@@ -12,7 +13,7 @@
 // between its NG lanes.  The probabilities are the second operand of the next product as they
 // lie: in a step of KS = 8 NG keys a lane holds quads 2 t and 2 t + 1, and the order of keys
 // within a step is free as long as both operands agree, so V is read in that order (rows
-// 4 NG (2 t + u) + 4 g .. + 3: one transposing LDS read for bf16, four dwords for fp32).
+// 4 NG (2 t + u) + 4 g .. + 3: transposing LDS reads for bf16, plain ones for fp32).
 //
 //   bf16: v_mfma_f32_32x32x16_bf16, W = 32;  fp32: 8 x v_mfma_f32_16x16x4_f32 per step, W = 16.
 #pragma once
@@ -127,9 +128,10 @@ __device__ __forceinline__ void unpack8(const Frag<float> &f, float (&x)[8]) {
 
 // ---- LDS tiles -----------------------------------------------------------------------------
 // A tile of ROWS rows of DP features, with room for a power of two of them, lies as 16-byte pieces,
-// piece c of row r at position c ^ swz(r).  Every 16 consecutive rows put one piece into the 16 different 16-byte slots of the 64
-// banks (row fragments), and four consecutive rows put a run of four pieces into four different
-// quarters of them (transposing reads), so that either read moves 256 bytes a cycle.
+// piece c of row r at position c ^ swz(r).  Every 16 consecutive rows put one piece into the 16
+// different 16-byte slots of the 64 banks (row fragments), and four consecutive rows put a run of four
+// pieces into four different quarters of them (transposing reads), so that either read moves 256 bytes a
+// cycle (with eight slots in use, conflicts took 22 to 27 % of the bf16 kernels' cycles; now none).
 template <typename T, int DP>
 struct Tile {
     static constexpr int P = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;  // features a row has room for
@@ -409,11 +411,7 @@ __device__ __forceinline__ float over_groups_sum(float v) {
     return v;
 }
 
-// Row r of the n * group query rows that share a key head: its head and row, and the keys it
-// sees: j < lim.
-struct RowOf {
-    int64_t head, i;
-};
+// Keys of an entry that may be read.
 __device__ __forceinline__ int64_t key_end(const Args &a, int64_t b) {
     if (!a.lengths) return a.m;
     const int64_t l = a.lengths[b];
@@ -524,12 +522,13 @@ inline int mask_mode(const tpw_attention_desc *d) {
 }
 // Parts of a summed axis of `steps` tiles for `blocks` blocks, `per_cu` of which share a CU: the least
 // of the time that this model gives.
-//   - A tile takes a block step_us with its CU full and about half of that alone (fp32-masked bf16 at 128
-//     features: 3.3 us two by two, 2.4 alone).
+//   - A tile takes a block step_us with its CU full and less the fewer share it (bf16 at 128 features under a
+//     boolean mask: 3.3 us two by two, 2.4 alone).
 //   - Up to 256 per_cu blocks run at once, more as places come free: a started round costs a third of one.
 //     A square causal call's differ in length, the longest twice the mean; they start with the longest,
 //     which speeds up as it is left alone.
-//   - Parts cost the launch that joins them (6 us, host and device) and their bytes, written and read (part_us each).
+//   - Parts cost the launch that joins them (6 us, host and device) and their bytes, written and read
+//     (part_us each).
 // dk / dv of causal 2 x 4 key heads x 8192 keys x 128: 1.76 ms in 512 blocks, 1.23 + 0.035 in 1024;
 // forward of causal 8 x 4 (2) x 587 x 128: 28 + 24 us in seven parts.
 constexpr int kMaxParts = 64;  // the join gives each part a lane

@@ -33,6 +33,10 @@ __device__ __forceinline__ void stream_steps(Load load, Use use) {
 
 constexpr int kUnit = 32;  // rows (keys) of the streamed operand that are worked on at a time
 
+// dq: the forward's structure with a second product of scores (v, do) and one of keys.  It also leaves
+// base, 1 / sum and delta of every row for the kernel below.  bf16 2 x 16 (4) x 8192^2 x 128: 1.45 to 1.55
+// ms (1.06 to 1.14 PFLOP/s over three products); at 256 features one wave per SIMD holds q, do and dq, and
+// softmax and products alternate (8 x 8192^2: 0.98 to 1.15 ms, 720 to 840 TFLOP/s).
 template <typename T, int W, int DP, int BN, int MM, int kWaves, int OCC>
 __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Args a) {
     using M = Mma<T, W>;
@@ -247,6 +251,11 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
     CR::each(dq, lane, [&](int at, f32x4 v) { store4(p, at, (int)a.d, v * a.gscale); });
 }
 
+// dk, dv (or one of them, or dv with ds kept): a wave owns 32 keys (fp32: 16), streams q and do, and needs
+// 2 DP accumulators a lane beside its keys and values.  To stay at two waves per SIMD, 128 features read
+// the block's values from LDS (VLDS: 2.0 ms where spilled registers took 2.9), and bf16 at more takes dk and
+// dv in a launch each.  bf16 2 x 16 (4) x 8192^2 x 128: 2.04 to 2.3 ms (0.95 to 1.08 PFLOP/s over four
+// products); 8 x 8192^2 x 256: dv 0.53, dk 1.36 to 1.5 (one wave per SIMD).
 template <typename T, int W, int DP, int BM, int MM, int kWaves, int OCC, bool VLDS, int OUT>
 __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const Args a) {
     using M = Mma<T, W>;
@@ -509,6 +518,7 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
 }
 
 // base, 1 / sum and delta of every row, one wave per row (the dq kernel forms them where it runs).
+// Bound by memory: 8 x 8192 rows of 256 in 34 us (4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void attention_rows_kernel(const Args a) {
     const int64_t all = a.batch * a.heads * a.n, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -528,7 +538,8 @@ __global__ __launch_bounds__(256) void attention_rows_kernel(const Args a) {
 }
 
 // dk (KEYS) or dq from the kept ds: a wave owns 16 keys (query rows) and streams q (k) through LDS.
-// Only units that the kernel above wrote are read; what no row sees counts as zero.
+// Only units that the kernel above wrote are read; what no row sees counts as zero.  fp32 4 x 8192^2 x
+// 256: 1.19 and 1.24 ms (115 and 111 TFLOP/s beside reading 1 GiB).
 template <int DP, bool KEYS>
 __global__ __launch_bounds__(512, 2) void attention_ds_product_kernel(const Args a) {
     constexpr int W = 16, kWaves = 8;

