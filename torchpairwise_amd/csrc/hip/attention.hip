@@ -62,6 +62,10 @@ struct Forward {
         const int g = lane / W;
         const RowReader<T, DP, W> rr(lane);
         const CR cr(lane);
+        // added values: where registers allow, loaded ahead of the scores' products
+        constexpr bool kAhead = MM == kBias && DP <= 128;
+        f32x4 add[MM == kBias ? NQ : 1];
+        if constexpr (kAhead) mask_bias<NQ, 4 * M::NG>(a, mask_row(a, b, qh, qi < 0 ? 0 : qi), j0, 4 * g, BN, add);
         Acc s[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) s[i] = Acc{};
@@ -82,19 +86,13 @@ struct Forward {
         }
 
         if constexpr (MM == kBias) {
-            const void *mr = mask_row(a, b, qh, qi);
+            if constexpr (!kAhead) mask_bias<NQ, 4 * M::NG>(a, mask_row(a, b, qh, qi < 0 ? 0 : qi), j0, 4 * g, BN, add);
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+            for (int x = 0; x < NQ; ++x)
 #pragma unroll
-                for (int w = 0; w < M::Q; ++w) {
-                    const int j = j0 + W * i + 4 * M::NG * w + 4 * g;
-                    f32x4 add = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (j < lim) add = mask_bias4(a, mr, j);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = s[i][4 * w + e] * a.scale + add[e];
-                        s[i][4 * w + e] = add[e] == -INFINITY ? -INFINITY : x;
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const float y = s[x / M::Q][4 * (x % M::Q) + e] * a.scale + add[x][e];
+                    s[x / M::Q][4 * (x % M::Q) + e] = add[x][e] == -INFINITY ? -INFINITY : y;
                 }
         }
         if constexpr (MM == kKeep) {

@@ -424,40 +424,46 @@ __device__ __forceinline__ int64_t row_limit(const Args &a, int64_t len, int64_t
     return l < 0 ? 0 : l;
 }
 
-// kKeep: bits of keys 32 w .. 32 w + 31 of a row.  kBias: values of keys j .. j + 3 (any alignment;
-// keys past m are not read).
+// kKeep: bits of keys 32 w .. 32 w + 31 of a row.  kBias: values of a row (any alignment; keys past m are
+// not read).
 __device__ __forceinline__ const uint32_t *mask_words(const Args &a, int64_t b, int64_t h, int64_t i) {
     return reinterpret_cast<const uint32_t *>(a.mask) + b * a.mb + h * a.mh + i * a.mn;
 }
 __device__ __forceinline__ const void *mask_row(const Args &a, int64_t b, int64_t h, int64_t i) {
     return reinterpret_cast<const uint8_t *>(a.mask) + (b * a.mb + h * a.mh + i * a.mn) * (a.mask_bf16 ? 2 : 4);
 }
-__device__ __forceinline__ f32x4 mask_bias4(const Args &a, const void *row, int64_t j) {
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    const bool run = a.mm == 1 && j + 3 < a.m;
-    if (a.mask_bf16) {
-        const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
-        if (run) {
-            uint2 w;
-            __builtin_memcpy(&w, p + j, 8);
-            v = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                      __uint_as_float(w.y & 0xffff0000u)};
-        } else {
+__device__ __forceinline__ float mask_value(const Args &a, const void *row, int64_t at) {
+    return a.mask_bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(row)[at])
+                       : reinterpret_cast<const float *>(row)[at];
+}
+// Values of keys j0 + STEP x + off + e, x < N, of one row (STEP keys apart, `span` of them from j0 for the
+// wave).  Inside the row every load goes out at once, without a branch between them.
+template <int N, int STEP>
+__device__ __forceinline__ void mask_bias(const Args &a, const void *row, int j0, int off, int span, f32x4 (&v)[N]) {
+    if (a.mm == 1 && j0 + span <= a.m) {
+        if (a.mask_bf16) {
+            const uint16_t *p = reinterpret_cast<const uint16_t *>(row) + j0 + off;
+            uint2 w[N];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (j + e < a.m) v[e] = bf16_to_f32(p[(j + e) * a.mm]);
+            for (int x = 0; x < N; ++x) __builtin_memcpy(&w[x], p + STEP * x, 8);
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+                v[x] = f32x4{__uint_as_float(w[x].x << 16), __uint_as_float(w[x].x & 0xffff0000u),
+                             __uint_as_float(w[x].y << 16), __uint_as_float(w[x].y & 0xffff0000u)};
+        } else {
+            const float *p = reinterpret_cast<const float *>(row) + j0 + off;
+#pragma unroll
+            for (int x = 0; x < N; ++x) __builtin_memcpy(&v[x], p + STEP * x, 16);
         }
     } else {
-        const float *p = reinterpret_cast<const float *>(row);
-        if (run) {
-            __builtin_memcpy(&v, p + j, 16);
-        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (j + e < a.m) v[e] = p[(j + e) * a.mm];
-        }
+        for (int x = 0; x < N; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t j = (int64_t)j0 + STEP * x + off + e;
+                v[x][e] = j < a.m ? mask_value(a, row, j * a.mm) : 0.0f;
+            }
     }
-    return v;
 }
 
 __device__ __forceinline__ int64_t cdiv_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -175,20 +175,17 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
                     }
                 });
             if constexpr (MM == kBias) {
-                const void *mr = mask_row(a, b, qh, qi);
+                constexpr int N = NU * M::Q;
+                f32x4 add[N];
+                mask_bias<N, 4 * M::NG>(a, mask_row(a, b, qh, qi < 0 ? 0 : qi), j0, 4 * g, kUnit, add);
 #pragma unroll
-                for (int i = 0; i < NU; ++i)
+                for (int x = 0; x < N; ++x)
 #pragma unroll
-                    for (int w = 0; w < M::Q; ++w) {
-                        const int j = j0 + W * i + 4 * M::NG * w + 4 * g;
-                        f32x4 add = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if (j < lim) add = mask_bias4(a, mr, j);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool off = add[e] == -INFINITY;
-                            s[i][4 * w + e] = off ? -INFINITY : s[i][4 * w + e] * a.scale + add[e];
-                            if (off) dp[i][4 * w + e] = 0.0f;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const bool off = add[x][e] == -INFINITY;
+                        const float y = s[x / M::Q][4 * (x % M::Q) + e] * a.scale + add[x][e];
+                        s[x / M::Q][4 * (x % M::Q) + e] = off ? -INFINITY : y;
+                        if (off) dp[x / M::Q][4 * (x % M::Q) + e] = 0.0f;
                     }
             }
             if constexpr (MM == kKeep) {
@@ -411,22 +408,25 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
                         }
             }
             if constexpr (MM == kBias) {
-                const uint8_t *mr = reinterpret_cast<const uint8_t *>(mask_row(a, b, qh, 0));
+                // rows and keys past the end read the last ones, and are masked below
+                const void *mr = mask_row(a, b, qh, 0);
+                const int64_t at = (j < a.m ? j : a.m - 1) * a.mm;
 #pragma unroll
-                for (int i = 0; i < NU; ++i)
+                for (int x = 0; x < NU * M::Q; ++x) {
+                    float add[4];
 #pragma unroll
-                    for (int w = 0; w < M::Q; ++w)
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = u0 + 4 * M::NG * x + 4 * g + e;
+                        add[e] = mask_value(a, mr, (r < rows ? r : rows - 1) * a.mn + at);
+                    }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int r = u0 + W * i + 4 * M::NG * w + 4 * g + e;
-                            const int64_t at = r * a.mn + j * a.mm;
-                            const float add = !(live && r < rows) ? 0.0f
-                                              : a.mask_bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(mr)[at])
-                                                            : reinterpret_cast<const float *>(mr)[at];
-                            const bool off = add == -INFINITY;
-                            s[i][4 * w + e] = off ? -INFINITY : s[i][4 * w + e] * a.scale + add;
-                            if (off) dp[i][4 * w + e] = 0.0f;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const bool off = add[e] == -INFINITY;
+                        const float y = s[x / M::Q][4 * (x % M::Q) + e] * a.scale + add[e];
+                        s[x / M::Q][4 * (x % M::Q) + e] = off ? -INFINITY : y;
+                        if (off) dp[x / M::Q][4 * (x % M::Q) + e] = 0.0f;
+                    }
+                }
             }
             if (u0 < wlast || u0 + kUnit > rows) {
                 asm volatile("");  // a branch: most units skip this
