@@ -228,6 +228,14 @@ def test_two_and_three_dimensions(device):
                    (full[0], tp.attention(*on(device, q[0], k[0], v[0]), mask[0].to(device)))):
         assert got.shape == x.shape
         assert_close(got, x, rtol=1e-4, atol=1e-5)
+    for dtype in (F32, BF16):
+        x = [y.to(dtype) for y in (q, k, v, randn(2, 30, 20, seed=5))]
+        want = reference(*(y[:, None] for y in x[:3]), grad=x[3][:, None])
+        for pick in (slice(None), 0, slice(1)):  # 3-D, 2-D, one entry
+            leaves = [y[pick].detach().requires_grad_() for y in on(device, *x[:3])]
+            got = torch.autograd.grad(tp.attention(*leaves), leaves, x[3][pick].to(device))
+            for name, g in zip(("dq", "dk", "dv"), got):
+                assert_close(g, want[name][:, 0][pick], rtol=0.0, atol=want["tol_" + name][:, 0][pick] + TINY, what=name)
     shape = tp.attention(*on(device, rows(2, 4, 9, 16, 1, F32, True), rows(2, 2, 9, 16, 2), rows(2, 2, 9, 8, 3)))
     assert shape.transpose(1, 2).is_contiguous()  # rows before heads, as the queries have them
 

@@ -131,7 +131,7 @@ struct Forward {
         // a row with no key so far: exp2(-inf - 0) = 0 throughout
         const float base = top1 == -INFINITY ? 0.0f : top1;
         if (__any(top1 > top)) {
-            const float f = MM == kBias ? __builtin_amdgcn_exp2f((top - base) * kLog2e) : __builtin_amdgcn_exp2f(top - base);
+            const float f = __builtin_amdgcn_exp2f(MM == kBias ? (top - base) * kLog2e : top - base);
             sum *= f;
 #pragma unroll
             for (int i = 0; i < DB; ++i)
@@ -179,7 +179,8 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
     using F = Forward<T, W, DP, BN, MM>;
     using M = typename F::M;
     constexpr uint32_t kTileBytes = BN * Tile<T, DP>::kRowBytes;
-    __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];  // two buffers of a key tile and a value tile
+    // two buffers of a key tile and a value tile
+    __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     int64_t t = xcd_linear(blockIdx.x, gridDim.x);
     const int64_t part = t % a.splits;
@@ -268,7 +269,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
             const int s = s0 + G * u + (int)threadIdx.x / LANES;
             const bool in = s < a.splits;
             c[u] = __shfl(w, in ? s : 0, 64);
-            x[u] = in && f < a.dv ? *reinterpret_cast<const f32x4 *>(p + s * rows * pitch) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            x[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (in && f < a.dv) x[u] = *reinterpret_cast<const f32x4 *>(p + s * rows * pitch);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) o += x[u] * c[u];
@@ -335,11 +337,14 @@ namespace {
 int64_t round_up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 
 bool whole_pieces(const View &v, int64_t width, int64_t size) {
-    return aligned16(v.p) && width * size % 16 == 0 && v.b * size % 16 == 0 && v.h * size % 16 == 0 && v.n * size % 16 == 0;
+    const auto whole = [&](int64_t elements) { return elements * size % 16 == 0; };
+    return aligned16(v.p) && whole(width) && whole(v.b) && whole(v.h) && whole(v.n);
 }
 // Strides of dimensions of one entry reach nothing: whatever they are, they ask for no copy.
-View view_of(const void *p, const int64_t *strides, int64_t batch, int64_t heads, int64_t rows, int64_t width, int64_t size) {
-    return {p, batch == 1 ? 0 : strides[0], heads == 1 ? 0 : strides[1], rows == 1 ? cdiv(width * size, 16) * 16 / size : strides[2]};
+View view_of(const void *p, const int64_t *strides, int64_t batch, int64_t heads, int64_t rows, int64_t width,
+             int64_t size) {
+    return {p, batch == 1 ? 0 : strides[0], heads == 1 ? 0 : strides[1],
+            rows == 1 ? cdiv(width * size, 16) * 16 / size : strides[2]};
 }
 
 constexpr int kPadded = 6;  // q, k, v, do, o and its rest
@@ -411,7 +416,8 @@ struct BitArgs {
 
 // Bits of a boolean mask, one row of words for each of its distinct rows (a broadcast dimension
 // counts once): the kernels test a bit of a word where they would load a byte, and the heads that
-// share a mask read an eighth of it (3001^2: 9 us, for 110 to 230 less in each kernel).  For the backward also by column: word (i / 32, j) holds rows
+// share a mask read an eighth of it (3001^2: 9 us, for 110 to 230 less in each kernel).  For the
+// backward also by column: word (i / 32, j) holds rows
 // 32 (i / 32) .. + 31 of key j.  One wave per 64 keys x 32 rows; all of its loads are in flight at once.
 __global__ __launch_bounds__(256) void pack_mask_kernel(const BitArgs a) {
     const int64_t pairs = a.words / 2, steps = cdiv_dev(a.n, 32), id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -439,11 +445,13 @@ __global__ __launch_bounds__(256) void pack_mask_kernel(const BitArgs a) {
 // The bits' layout, its strides into the arguments; returns the bytes they take.
 int64_t plan_bits(Args &a, bool backward, uint8_t *at, BitArgs *p) {
     const int64_t words = round_up(cdiv(a.m, 32), 2);  // whole tiles of 64 keys
-    const int64_t n = a.mn ? a.n : 1, heads = a.mh ? a.heads : 1, lead = heads * (a.mb ? a.batch : 1), steps = cdiv(n, 32);
+    const int64_t n = a.mn ? a.n : 1, heads = a.mh ? a.heads : 1;
+    const int64_t lead = heads * (a.mb ? a.batch : 1), steps = cdiv(n, 32);
     const int64_t rows = round_up(lead * n * words * 4, 16);
     if (p)
         *p = {reinterpret_cast<const uint8_t *>(a.mask), reinterpret_cast<uint32_t *>(at),
-              backward ? reinterpret_cast<uint32_t *>(at + rows) : nullptr, a.mb, a.mh, a.mn, a.mm, heads, n, a.m, lead, words};
+              backward ? reinterpret_cast<uint32_t *>(at + rows) : nullptr,
+              a.mb, a.mh, a.mn, a.mm, heads, n, a.m, lead, words};
     a.mask = at;
     a.mask_cols = backward ? reinterpret_cast<uint32_t *>(at + rows) : nullptr;
     a.cn = a.mn ? a.m : 0;
@@ -471,7 +479,8 @@ void plan(Args &a) {
 
 size_t prepared_bytes(const Args &a, const tpw_attention_desc *d, bool backward) {
     Args b = a;
-    return plan_padding(b, d->dtype, backward, nullptr, nullptr) + (mask_mode(d) == kKeep ? (size_t)plan_bits(b, backward, nullptr, nullptr) : 0);
+    const size_t bits = mask_mode(d) == kKeep ? (size_t)plan_bits(b, backward, nullptr, nullptr) : 0;
+    return plan_padding(b, d->dtype, backward, nullptr, nullptr) + bits;
 }
 int prepare_operands(Args &a, const tpw_attention_desc *d, bool backward, void *at, hipStream_t s) {
     PadArgs p = {};
@@ -481,7 +490,7 @@ int prepare_operands(Args &a, const tpw_attention_desc *d, bool backward, void *
         TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: too many rows");
         bool pairs = d->dtype == TPW_BF16;  // bf16 rows of whole dwords: copied by dwords
         for (int t = 0; t < p.count; ++t)
-            pairs = pairs && p.width[t] % 2 == 0 && p.from[t].b % 2 == 0 && p.from[t].h % 2 == 0 && p.from[t].n % 2 == 0 &&
+            pairs = pairs && (p.width[t] | p.from[t].b | p.from[t].h | p.from[t].n) % 2 == 0 &&
                     reinterpret_cast<uintptr_t>(p.from[t].p) % 4 == 0;
         for (int t = 0; pairs && t < p.count; ++t) {
             p.width[t] /= 2;
@@ -613,10 +622,11 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
         if (const int rc = check_launch("attention_kernel")) return rc;
         if (a.splits > 1) {
             if (a.splits <= kFew)
-                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias>), dim3((unsigned)cdiv(rows * cdiv(a.dv, 4), 256)),
-                                   dim3(256), 0, s, a);
+                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias>),
+                                   dim3((unsigned)cdiv(rows * cdiv(a.dv, 4), 256)), dim3(256), 0, s, a);
             else
-                hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, Tile<T, DP>::P / 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
+                hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, Tile<T, DP>::P / 4>), dim3((unsigned)rows),
+                                   dim3(256), 0, s, a);
             return check_launch("attention_join_kernel");
         }
         return TPW_OK;

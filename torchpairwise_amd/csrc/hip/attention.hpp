@@ -227,7 +227,8 @@ struct RowReader {
         } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-                f.v[u] = __builtin_bit_cast(f32x4, lds_read16(L::piece(tile + at, 2 * S::NG * s + u, blk * W * L::kRowBytes)));
+                f.v[u] = __builtin_bit_cast(
+                    f32x4, lds_read16(L::piece(tile + at, 2 * S::NG * s + u, blk * W * L::kRowBytes)));
         }
         return f;
     }
@@ -316,7 +317,8 @@ struct ColReader<float, DP, 16> {
         for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int k = 0; k < (c / 2 < kWhole ? 4 : 2); ++k)
-                acc[4 * (c / 2) + k] = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e][k], p.v[c % 2][e], acc[4 * (c / 2) + k], 0, 0, 0);
+                acc[4 * (c / 2) + k] =
+                    __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e][k], p.v[c % 2][e], acc[4 * (c / 2) + k], 0, 0, 0);
     }
     template <typename F>
     static __device__ __forceinline__ void each(const M::Acc *acc, int lane, F &&f) {
@@ -563,7 +565,8 @@ inline int64_t parts_for(int64_t blocks, int64_t steps, int64_t per_cu, bool une
 // the kernels reach (0.9 PFLOP/s bf16, 120 TFLOP/s fp32).
 template <typename T, int DP>
 double step_us(int64_t own, int64_t streamed, int products, int64_t per_cu) {
-    return 2.0 * products * (double)own * (double)streamed * DP * (double)per_cu * 256.0 / (sizeof(T) == 2 ? 0.9e9 : 0.12e9);
+    const double flops = 2.0 * products * (double)own * (double)streamed * DP;
+    return flops * (double)per_cu * 256.0 / (sizeof(T) == 2 ? 0.9e9 : 0.12e9);
 }
 inline double part_us(int64_t rows, int64_t width) { return 2.0 * 4.0 * (double)rows * (double)width / 4.5e6; }
 

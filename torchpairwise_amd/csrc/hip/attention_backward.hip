@@ -455,15 +455,16 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const A
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float sv = s[i][4 * w + e];
-                        const float p = inv[e] * (MM == kBias ? __builtin_amdgcn_exp2f((sv - base[e]) * kLog2e)
-                                                              : __builtin_amdgcn_exp2f(__builtin_fmaf(sv, a.scale, -base[e])));
+                        const float p = inv[e] * __builtin_amdgcn_exp2f(MM == kBias ? (sv - base[e]) * kLog2e
+                                                                                    : __builtin_fmaf(sv, a.scale, -base[e]));
                         x[i * M::Q + w][e] = p;
                         s[i][4 * w + e] = p * (dp[i][4 * w + e] - delta[e]);
                     }
                 }
             if constexpr ((OUT & 4) != 0) {
                 if (live) {
-                    float *kept = a.ds + (((bk - a.first_bk) * a.group + (qh - kh * a.group)) * a.m + j) * a.ds_pitch + u0 + 4 * g;
+                    const int64_t head = (bk - a.first_bk) * a.group + qh - kh * a.group;
+                    float *kept = a.ds + (head * a.m + j) * a.ds_pitch + u0 + 4 * g;
 #pragma unroll
                     for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -691,7 +692,7 @@ int64_t ds_bytes(const Args &a) { return a.group * a.m * (cdiv(a.n, kUnit) * kUn
 template <typename T, int DP>
 int64_t keeps_ds(const Args &a) {
     if (sizeof(T) != 4 || DP == 64 || a.n == 0 || a.m == 0 || ds_bytes(a) > kKeptBytes) return 0;
-    const int64_t bk = a.batch * a.key_heads, most = kKeptBytes / ds_bytes(a), rounds = cdiv(bk, most), kept = cdiv(bk, rounds);
+    const int64_t bk = a.batch * a.key_heads, most = kKeptBytes / ds_bytes(a), kept = cdiv(bk, cdiv(bk, most));
     return kept * cdiv(a.m, kKeptKeys) >= 192 && kept * a.group * cdiv(a.n, kKeptKeys) >= 192 ? kept : 0;
 }
 template <typename T, int DP>
@@ -806,14 +807,19 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
             constexpr bool kApart = sizeof(T) == 2 && DP > 128;
             constexpr int kRows = Tiles<T, DP>::kRows, kWaves = Tiles<T, DP>::kRowWaves;
             if constexpr (kApart) {
-                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, 2, false, 2>), grid, block, 0, s, a);
-                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, DP == 256 ? 1 : 2, false, 1>), grid, block, 0, s, a);
+                constexpr int kOccK = DP == 256 ? 1 : 2;
+                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, 2, false, 2>), grid, block, 0, s,
+                                   a);
+                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, kOccK, false, 1>), grid, block, 0,
+                                   s, a);
             } else {
-                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, kOccKv, kValuesInLds, 3>), grid, block, 0, s, a);
+                hipLaunchKernelGGL((attention_dkv_kernel<T, W, DP, kRows, MM, kWaves, kOccKv, kValuesInLds, 3>), grid,
+                                   block, 0, s, a);
             }
             if (const int rc = check_launch("attention_dkv_kernel")) return rc;
             if (a.splits > 1)
-                return sum_parts<T>({a.part, {a.gk, a.gv}, {a.d, a.dv}, {a.gscale, 1.0f}, keys, a.key_heads, a.m, a.splits}, s);
+                return sum_parts<T>(
+                    {a.part, {a.gk, a.gv}, {a.d, a.dv}, {a.gscale, 1.0f}, keys, a.key_heads, a.m, a.splits}, s);
         }
         return TPW_OK;
     });

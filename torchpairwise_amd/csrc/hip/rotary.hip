@@ -34,7 +34,9 @@ __device__ __forceinline__ void angle(double position, double turns, float scale
 
 // P pairs at a time: P consecutive features of both halves, or 2 P consecutive ones (INTERLEAVED).
 template <typename T, int P, bool INTERLEAVED>
-__device__ __forceinline__ void turn(const T *x, T *o, int64_t p0, int64_t pairs, const float (&c)[P], const float (&s)[P]) {
+__device__ __forceinline__ void turn(const T *x, T *o, int64_t p0, int64_t pairs, const float (&c)[P],
+                                     const float (&s)[P]) {
+    constexpr int kAlign = 2 * P * sizeof(T) < 16 ? 2 * P * sizeof(T) : 16;
     T u[P], w[P];
     if constexpr (P == 1) {
         const int64_t i = INTERLEAVED ? 2 * p0 : p0, j = INTERLEAVED ? i + 1 : p0 + pairs;
@@ -45,14 +47,14 @@ __device__ __forceinline__ void turn(const T *x, T *o, int64_t p0, int64_t pairs
         from_f32(o + j, a * s[0] + b * c[0]);
     } else if constexpr (INTERLEAVED) {
         T v[2 * P], r[2 * P];
-        __builtin_memcpy(v, __builtin_assume_aligned(x + 2 * p0, 2 * P * sizeof(T) < 16 ? 2 * P * sizeof(T) : 16), sizeof(v));
+        __builtin_memcpy(v, __builtin_assume_aligned(x + 2 * p0, kAlign), sizeof(v));
 #pragma unroll
         for (int e = 0; e < P; ++e) {
             const float a = to_f32(v[2 * e]), b = to_f32(v[2 * e + 1]);
             from_f32(&r[2 * e], a * c[e] - b * s[e]);
             from_f32(&r[2 * e + 1], a * s[e] + b * c[e]);
         }
-        __builtin_memcpy(__builtin_assume_aligned(o + 2 * p0, 2 * P * sizeof(T) < 16 ? 2 * P * sizeof(T) : 16), r, sizeof(r));
+        __builtin_memcpy(__builtin_assume_aligned(o + 2 * p0, kAlign), r, sizeof(r));
     } else {
         T ru[P], rw[P];
         __builtin_memcpy(u, __builtin_assume_aligned(x + p0, P * sizeof(T)), sizeof(u));
@@ -156,7 +158,8 @@ extern "C" int tpw_rotary(const void *x, int dtype, int64_t batch, int64_t heads
         const int64_t rest = d - 2 * pairs, copy = 2 * p * size < 16 ? 2 * p * size : 16;
         return pairs % p == 0 && at(x, a.xb, a.xh, a.xn) && at(out, a.ob, a.oh, a.on) &&
                (rest == 0 || (rest % (2 * p) == 0 && 2 * pairs * size % copy == 0 &&
-                              reinterpret_cast<uintptr_t>(x) % copy == 0 && reinterpret_cast<uintptr_t>(out) % copy == 0 &&
+                              reinterpret_cast<uintptr_t>(x) % copy == 0 &&
+                              reinterpret_cast<uintptr_t>(out) % copy == 0 &&
                               a.xb * size % copy == 0 && a.xh * size % copy == 0 && a.xn * size % copy == 0 &&
                               a.ob * size % copy == 0 && a.oh * size % copy == 0 && a.on * size % copy == 0));
     };

@@ -87,7 +87,8 @@ Operands check_attention(const at::Tensor &query, const at::Tensor &key, const a
     if (lengths.has_value() && lengths->defined()) {
         const at::Tensor &l = *lengths;
         TORCH_CHECK(l.device() == query.device(), name, ": lengths are on another device");
-        TORCH_CHECK(l.dim() == 1 && l.size(0) == o.batch, name, ": lengths must have shape [batch_size], got ", l.sizes());
+        TORCH_CHECK(l.dim() == 1 && l.size(0) == o.batch, name, ": lengths must have shape [batch_size], got ",
+                    l.sizes());
         TORCH_CHECK(l.scalar_type() == at::kLong || l.scalar_type() == at::kInt, name,
                     ": lengths must be int64 or int32, got ", l.scalar_type());
         o.lengths = l.to(at::kLong).contiguous();
@@ -114,7 +115,8 @@ at::Tensor additive_mask(const Operands &o, bool causal, at::ScalarType t) {
     }
     const auto index = o.q.options().dtype(at::kLong);
     auto j = at::arange(o.m, index);
-    auto len = o.lengths.defined() ? o.lengths.clamp(0, o.m).view({o.batch, 1, 1, 1}) : at::full({1, 1, 1, 1}, o.m, index);
+    auto len = o.lengths.defined() ? o.lengths.clamp(0, o.m).view({o.batch, 1, 1, 1})
+                                   : at::full({1, 1, 1, 1}, o.m, index);
     if (o.lengths.defined()) exclude(j >= len);
     if (causal) exclude(j - at::arange(o.n, index).unsqueeze(1) > len - o.n);
     return add;
@@ -175,7 +177,8 @@ Results attention_backward_cpu(
     const at::Tensor &stats, const at::Tensor &rest, const OptTensor &mask, const OptTensor &lengths, bool causal,
     double scale) {
     const Operands o = check_attention(query, key, value, mask, lengths);
-    TORCH_CHECK(grad.sizes() == out.sizes(), "attention: gradient of shape ", grad.sizes(), " for an output of ", out.sizes());
+    TORCH_CHECK(grad.sizes() == out.sizes(), "attention: gradient of shape ", grad.sizes(), " for an output of ",
+                out.sizes());
     const auto t = compute_type(query);
     if (o.q.numel() == 0 || o.m == 0)
         return {at::zeros_like(query), at::zeros_like(key), at::zeros_like(value)};
@@ -215,9 +218,11 @@ void check_rotary(const at::Tensor &x, const at::Tensor &positions, const at::Te
                 ": positions must be int64 or int32, got ", positions.scalar_type());
     const int64_t n = x.size(-2), batch = x.dim() == 2 ? 1 : x.size(0);
     TORCH_CHECK((positions.dim() == 1 && positions.size(0) == n) ||
-                    (positions.dim() == 2 && positions.size(1) == n && (positions.size(0) == batch || positions.size(0) == 1)),
+                    (positions.dim() == 2 && positions.size(1) == n &&
+                     (positions.size(0) == batch || positions.size(0) == 1)),
                 name, ": positions must have shape [n] or [batch_size, n], got ", positions.sizes());
-    TORCH_CHECK(frequencies.dim() == 1 && (frequencies.scalar_type() == at::kDouble || frequencies.scalar_type() == at::kFloat),
+    const auto ft = frequencies.scalar_type();
+    TORCH_CHECK(frequencies.dim() == 1 && (ft == at::kDouble || ft == at::kFloat),
                 name, ": frequencies must be a float64 or float32 vector");
     TORCH_CHECK(2 * frequencies.size(0) <= x.size(-1), name, ": ", frequencies.size(0), " pairs do not fit rows of ",
                 x.size(-1), " features");
@@ -289,8 +294,9 @@ Results attention_cuda(const at::Tensor &query, const at::Tensor &key, const at:
     // what only the backward reads
     at::Tensor stats = train ? at::empty({2, o.batch, o.heads, o.n}, query.options().dtype(at::kFloat))
                              : at::empty({0}, query.options().dtype(at::kFloat));
-    at::Tensor rest = train && out.scalar_type() == at::kBFloat16 ? at::empty_strided(out.sizes(), out.strides(), out.options())
-                                                                  : at::empty({0}, out.options());
+    at::Tensor rest = train && out.scalar_type() == at::kBFloat16
+                          ? at::empty_strided(out.sizes(), out.strides(), out.options())
+                          : at::empty({0}, out.options());
     if (out.numel() > 0) {
         o.q = dense_rows(o.q, false);
         o.k = dense_rows(o.k, true);
@@ -313,7 +319,8 @@ Results attention_backward_cuda(
     const at::Tensor &stats, const at::Tensor &rest, const OptTensor &mask, const OptTensor &lengths, bool causal,
     double scale) {
     Operands o = check_attention(query, key, value, mask, lengths);
-    TORCH_CHECK(grad.sizes() == out.sizes(), "attention: gradient of shape ", grad.sizes(), " for an output of ", out.sizes());
+    TORCH_CHECK(grad.sizes() == out.sizes(), "attention: gradient of shape ", grad.sizes(), " for an output of ",
+                out.sizes());
     TORCH_CHECK(out.scalar_type() == query.scalar_type() && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
                     stats.numel() == 2 * o.batch * o.heads * o.n && out.device() == query.device() &&
                     stats.device() == query.device() && grad.device() == query.device(),
@@ -325,9 +332,12 @@ Results attention_backward_cuda(
         o.k = dense_rows(o.k, true);
         o.v = dense_rows(o.v, true);
         auto g4 = dense_rows(as4(grad.to(query.scalar_type())), true), o4 = as4(out);
-        TORCH_CHECK((rest.numel() == 0 || (rest.sizes() == o4.sizes() && rest.strides() == o4.strides() &&
-                                           rest.scalar_type() == out.scalar_type() && rest.device() == out.device())) &&
-                        (o4.size(3) == 1 || o4.stride(3) == 1),
+        const auto fits = [&](const at::Tensor &r) {
+            bool same = r.sizes() == o4.sizes() && r.scalar_type() == out.scalar_type() && r.device() == out.device();
+            for (int i = 0; same && i < 4; ++i) same = r.size(i) == 1 || r.stride(i) == o4.stride(i);
+            return same;
+        };
+        TORCH_CHECK((rest.numel() == 0 || fits(rest)) && (o4.size(3) == 1 || o4.stride(3) == 1),
                     "_attention_backward: out and rest must be what the forward returned");
         TORCH_CHECK(o4.size(0) == o.batch && o4.size(1) == o.heads && o4.size(2) == o.n && o4.size(3) == o.dv,
                     "_attention_backward: out must be what the forward returned");
@@ -403,7 +413,8 @@ at::Tensor attention(const at::Tensor &query, const at::Tensor &key, const at::T
                      : query.dim() > 0 && query.size(-1) > 0 ? 1.0 / std::sqrt((double)query.size(-1))
                                                              : 1.0;
     TORCH_CHECK(std::isfinite(s) && std::fabs(s) <= 1e30, "attention: scale must be finite, got ", s);
-    const bool train = at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad());
+    const bool train =
+        at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad());
     return std::get<0>(attention_op(query, key, value, mask, lengths, causal, s, train));
 }
 
@@ -444,7 +455,8 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
    public:
     static Variable forward(AutogradContext *ctx, const Variable &x, const Variable &positions, const Variable &frequencies,
                             bool interleaved, double scale, bool inverse) {
-        TORCH_CHECK(!frequencies.requires_grad(), "rotary_embedding: frequencies have no gradient; pass frequencies.detach()");
+        TORCH_CHECK(!frequencies.requires_grad(),
+                    "rotary_embedding: frequencies have no gradient; pass frequencies.detach()");
         at::AutoDispatchBelowADInplaceOrView g;
         ctx->save_for_backward({positions, frequencies});
         ctx->saved_data["interleaved"] = interleaved;
@@ -489,7 +501,8 @@ TORCH_LIBRARY_FRAGMENT(torchpairwise, m) {
           "float scale, bool train) -> (Tensor out, Tensor stats, Tensor rest)");
     m.def("_attention_backward(Tensor grad, Tensor query, Tensor key, Tensor value, Tensor out, Tensor stats, "
           "Tensor rest, Tensor? mask, Tensor? lengths, bool causal, float scale) -> (Tensor, Tensor, Tensor)");
-    m.def("_rotary(Tensor x, Tensor positions, Tensor frequencies, bool interleaved, float scale, bool inverse) -> Tensor");
+    m.def("_rotary(Tensor x, Tensor positions, Tensor frequencies, bool interleaved, float scale, "
+          "bool inverse) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(torchpairwise, CPU, m) {
