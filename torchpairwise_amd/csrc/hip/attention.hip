@@ -41,7 +41,7 @@ struct Forward {
         const T *row = live ? reinterpret_cast<const T *>(a.q.p) + b * a.q.b + qh * a.q.h + qi * a.q.n : nullptr;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
-            q[s] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d);
+            q[s] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d, a.dwords);
             if (a.qsign != 1.0f) {
                 float x[8];
                 unpack8(q[s], x);
@@ -200,9 +200,9 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
     const int t0 = (int)((int64_t)nt * part / a.splits), t1 = (int)((int64_t)nt * (part + 1) / a.splits);
 
     const uint32_t lds = tile::lds_addr(smem);
-    Stager<T, DP, BN, kWaves> sk, sv;
-    sk.init(a.k.n, (int)a.d, wave, lane);
-    sv.init(a.v.n, (int)a.dv, wave, lane);
+    Stager<T, DP, BN, kWaves, true> sk, sv;
+    sk.init(a.k.n, (int)a.d, wave, lane, a.dwords);
+    sv.init(a.v.n, (int)a.dv, wave, lane, a.dwords);
     const T *kb = reinterpret_cast<const T *>(a.k.p) + b * a.k.b + kh * a.k.h;
     const T *vb = reinterpret_cast<const T *>(a.v.p) + b * a.v.b + kh * a.v.h;
     const auto fetch = [&](int i) {
@@ -377,10 +377,28 @@ __global__ void pad_kernel(const PadArgs a) {
     reinterpret_cast<uint4 *>(a.to[t])[id] = w;
 }
 
+// Whether the forward's operands that are not whole pieces are whole dwords, to be read as they lie, and
+// the call is one where that takes less than copying them: each key is read by one tile of rows (one token of
+// 8 x 16 (4) heads over 16000 keys of 90 bf16: 52 us against 127 + 38), or there are few pairs (2^22: 4 x 8 x
+// 128 x 1000 x 50 fp32 23 against 13 + 18, 2 x 8 x 300 x 900 x 118 fp32 46 against 13 + 32; 2^25: 4 x 8 x
+// 1024^2 x 90 bf16 51 against 14 + 33).  The backward's kernels have no registers left for it.
+bool reads_dwords(const Args &a, int64_t size) {
+    bool pieces = true, dwords = true;
+    const auto look = [&](const View &v, int64_t width) {
+        pieces = pieces && whole_pieces(v, width, size);
+        dwords = dwords && reinterpret_cast<uintptr_t>(v.p) % 4 == 0 && (width | v.b | v.h | v.n) * size % 4 == 0;
+    };
+    look(a.q, a.d);
+    look(a.k, a.d);
+    look(a.v, a.dv);
+    return !pieces && dwords && (a.n * a.group <= 64 || a.batch * a.heads * a.n * a.m <= int64_t(1) << 22);
+}
+
 // The operands to copy, their addresses from `at` on; returns the bytes they take.
 size_t plan_padding(Args &a, int dtype, bool backward, uint8_t *at, PadArgs *p) {
     const int64_t size = dtype == TPW_F32 ? 4 : 2, e = 16 / size;
     size_t bytes = 0;
+    if (a.dwords) return 0;
     const auto take = [&](View &v, int64_t heads, int64_t rows, int64_t width, bool always = false) {
         if ((!always && whole_pieces(v, width, size)) || a.batch * heads * rows == 0) return;
         const int64_t pieces = cdiv(width, e), n = a.batch * heads * rows * pieces;
@@ -563,6 +581,7 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
         ok = ok && streamed(a.q, d->n, d->d) && streamed(a.go, d->n, d->dv);
     }
     TPW_REQUIRE(ok, "attention: rows of an operand overlap or lie more than 8 MiB apart");
+    a.dwords = !backward && reads_dwords(a, size);
     return TPW_OK;
 }
 

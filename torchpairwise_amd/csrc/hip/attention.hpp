@@ -28,8 +28,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 enum MaskMode { kNoMask = 0, kKeep = 1, kBias = 2 };
 
 // One operand: element strides of [batch, heads, rows, features] (features dense).  The kernels read
-// rows as 16-byte pieces at 16-byte aligned addresses, a last partial piece filled up with zeros:
-// operands that do not lie so are copied first (pad_kernel).
+// rows as 16-byte pieces at 16-byte aligned addresses, a last partial piece filled up with zeros.
+// Operands that do not lie so are copied first (pad_kernel), or read by dwords (Args::dwords).
 struct View {
     const void *p;
     int64_t b, h, n;
@@ -53,6 +53,7 @@ struct Args {
     float qsign;   // -1, 0 or 1: the sign of scale, folded into q as it is loaded
     float gscale;  // scale (backward)
     int causal;
+    int dwords;     // (forward) operands of whole dwords that are not whole pieces, read as they lie
     int64_t tiles;  // row tiles (dk / dv: key tiles) per (batch, key head)
     int splits;     // parts of the summed axis
     float *ds;      // kept score gradients (backward of wide fp32 rows): [key heads' heads, m, ds_pitch]
@@ -160,6 +161,10 @@ __device__ __forceinline__ void dma16(tpw_u32x4 rsrc, uint32_t voff, uint32_t ld
     asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds_base)
                  : "memory", "m0");
 }
+__device__ __forceinline__ void dma4(tpw_u32x4 rsrc, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds_base)
+                 : "memory", "m0");
+}
 __device__ __forceinline__ tpw_u32x4 resource(const void *base, int64_t bytes) {
     const uint64_t a = (uint64_t)(uintptr_t)base;
     const uint32_t num = bytes <= 0 ? 0u : bytes > (int64_t)kRange ? kRange : (uint32_t)bytes;
@@ -178,26 +183,39 @@ __device__ __forceinline__ const void *uniform(const void *p) {
 
 // Moves rows [0, ROWS) of a tile into LDS; rows at or past `rows` and features at or past `d`
 // become zeros and are not read.
-template <typename T, int DP, int ROWS, int WAVES>
+template <typename T, int DP, int ROWS, int WAVES, bool DWORDS = false>
 struct Stager {
     using L = Tile<T, DP>;
     static constexpr int kSlots = ROWS * L::C / (64 * WAVES);
     static_assert(ROWS * L::C % (64 * WAVES) == 0, "whole instructions");
     uint32_t off[kSlots];
     int64_t stride;  // bytes between rows
-    int wave;
+    int wave, width;  // width: bytes of a row where it is read by dwords, else 0
 
-    __device__ __forceinline__ void init(int64_t row_stride, int d, int wave_, int lane) {
+    __device__ __forceinline__ void init(int64_t row_stride, int d, int wave_, int lane, int dwords = 0) {
         stride = row_stride * (int64_t)sizeof(T);
         wave = wave_;
+        width = dwords ? d * (int)sizeof(T) : 0;
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
             const int s = (i * WAVES + wave) * 64 + lane, r = s / L::C, c = (s % L::C) ^ L::swz(r);
             off[i] = c * L::E < d ? (uint32_t)(r * stride + c * 16) : kBeyond;
         }
     }
-    __device__ __forceinline__ void load(const T *base, int64_t rows, uint32_t lds) const {
+    __device__ __forceinline__ void load(const T *base, int64_t rows, uint32_t to) const {
+        const uint32_t lds = DWORDS ? (uint32_t)__builtin_amdgcn_readfirstlane((int)to) : to;
         const tpw_u32x4 r = resource(base, rows * stride);
+        if (DWORDS && width) {  // four times the instructions, their offsets formed as they go
+            const int lane = threadIdx.x & 63;
+#pragma unroll 2
+            for (int i = 0; i < 4 * kSlots; ++i) {
+                const int s = (i * WAVES + wave) * 64 + lane, row = s / (4 * L::C);
+                const int byte = ((s / 4 % L::C) ^ L::swz(row)) * 16 + (s & 3) * 4;
+                dma4(r, byte < width ? (uint32_t)(row * stride + byte) : kBeyond,
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds + (uint32_t)((i * WAVES + wave) * 256))));
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) dma16(r, off[i], lds + (uint32_t)((i * WAVES + wave) * 1024));
     }
@@ -339,9 +357,20 @@ struct ColReader<float, DP, 16> {
 
 // Features f .. f + 7 of a row in global memory (null: zeros).
 template <typename T>
-__device__ __forceinline__ Frag<T> load_row8(const T *row, int f, int d) {
-    constexpr int E = 16 / (int)sizeof(T);
+__device__ __forceinline__ Frag<T> load_row8(const T *row, int f, int d, int dwords = 0) {
+    constexpr int E = 16 / (int)sizeof(T), D = 4 / (int)sizeof(T);
     T x[8];
+    if (dwords) {
+#pragma unroll
+        for (int u = 0; u < 8 / D; ++u) {
+            uint32_t w = 0;
+            if (row && f + u * D < d) w = *reinterpret_cast<const uint32_t *>(row + f + u * D);
+            __builtin_memcpy(x + u * D, &w, 4);
+        }
+        Frag<T> r;
+        __builtin_memcpy(&r, x, sizeof(r));
+        return r;
+    }
 #pragma unroll
     for (int u = 0; u < 8 / E; ++u) {
         uint4 w = make_uint4(0, 0, 0, 0);
