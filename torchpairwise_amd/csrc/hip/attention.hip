@@ -8,7 +8,7 @@ namespace tpw {
 namespace attn {
 
 // Per-row running softmax of one wave's W rows and the loop over one key tile.
-template <typename T, int W, int DP, int BN, int MM>
+template <typename T, int W, int DP, int BN, int MM, bool DWORDS>
 struct Forward {
     using M = Mma<T, W>;
     using Acc = typename M::Acc;
@@ -41,7 +41,7 @@ struct Forward {
         const T *row = live ? reinterpret_cast<const T *>(a.q.p) + b * a.q.b + qh * a.q.h + qi * a.q.n : nullptr;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
-            q[s] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d, a.dwords);
+            q[s] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d, DWORDS);
             if (a.qsign != 1.0f) {
                 float x[8];
                 unpack8(q[s], x);
@@ -174,9 +174,9 @@ struct Forward {
 // 8192^2 x 256 in 0.55 (0.99), 32 x 4096^2 x 64 in 0.18 (0.77: exponentials).  fp32: 8 x 8192^2 x 256 in
 // 4.2 ms (130 TFLOP/s).  One token of 16 x 16 (2) heads over 32768 keys: 4.6 TB/s.  Priorities (s_setprio)
 // around the products or the softmax changed nothing.
-template <typename T, int W, int DP, int BN, int MM, int kWaves, int OCC>
+template <typename T, int W, int DP, int BN, int MM, bool DWORDS, int kWaves, int OCC>
 __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args a) {
-    using F = Forward<T, W, DP, BN, MM>;
+    using F = Forward<T, W, DP, BN, MM, DWORDS>;
     using M = typename F::M;
     constexpr uint32_t kTileBytes = BN * Tile<T, DP>::kRowBytes;
     // two buffers of a key tile and a value tile
@@ -200,9 +200,9 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
     const int t0 = (int)((int64_t)nt * part / a.splits), t1 = (int)((int64_t)nt * (part + 1) / a.splits);
 
     const uint32_t lds = tile::lds_addr(smem);
-    Stager<T, DP, BN, kWaves, true> sk, sv;
-    sk.init(a.k.n, (int)a.d, wave, lane, a.dwords);
-    sv.init(a.v.n, (int)a.dv, wave, lane, a.dwords);
+    Stager<T, DP, BN, kWaves, DWORDS> sk, sv;
+    sk.init(a.k.n, (int)a.d, wave, lane);
+    sv.init(a.v.n, (int)a.dv, wave, lane);
     const T *kb = reinterpret_cast<const T *>(a.k.p) + b * a.k.b + kh * a.k.h;
     const T *vb = reinterpret_cast<const T *>(a.v.p) + b * a.v.b + kh * a.v.h;
     const auto fetch = [&](int i) {
@@ -636,8 +636,14 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
         }
         constexpr int kOcc = 2;
         constexpr int kWaves = Tiles<T, DP>::kWaves;
-        hipLaunchKernelGGL((attention_kernel<T, W, DP, Tiles<T, DP>::kKeys, MM, kWaves, kOcc>), dim3((unsigned)blocks),
-                           dim3(64 * kWaves), 0, s, a);
+        constexpr int kKeys = Tiles<T, DP>::kKeys;
+        // a kernel of its own: the branch alone would cost the others 2 %
+        if (a.dwords)
+            hipLaunchKernelGGL((attention_kernel<T, W, DP, kKeys, MM, true, kWaves, kOcc>), dim3((unsigned)blocks),
+                               dim3(64 * kWaves), 0, s, a);
+        else
+            hipLaunchKernelGGL((attention_kernel<T, W, DP, kKeys, MM, false, kWaves, kOcc>), dim3((unsigned)blocks),
+                               dim3(64 * kWaves), 0, s, a);
         if (const int rc = check_launch("attention_kernel")) return rc;
         if (a.splits > 1) {
             if (a.splits <= kFew)

@@ -190,12 +190,12 @@ struct Stager {
     static_assert(ROWS * L::C % (64 * WAVES) == 0, "whole instructions");
     uint32_t off[kSlots];
     int64_t stride;  // bytes between rows
-    int wave, width;  // width: bytes of a row where it is read by dwords, else 0
+    int wave, width;  // width: bytes of a row (DWORDS)
 
-    __device__ __forceinline__ void init(int64_t row_stride, int d, int wave_, int lane, int dwords = 0) {
+    __device__ __forceinline__ void init(int64_t row_stride, int d, int wave_, int lane) {
         stride = row_stride * (int64_t)sizeof(T);
         wave = wave_;
-        width = dwords ? d * (int)sizeof(T) : 0;
+        width = d * (int)sizeof(T);
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
             const int s = (i * WAVES + wave) * 64 + lane, r = s / L::C, c = (s % L::C) ^ L::swz(r);
@@ -205,7 +205,7 @@ struct Stager {
     __device__ __forceinline__ void load(const T *base, int64_t rows, uint32_t to) const {
         const uint32_t lds = DWORDS ? (uint32_t)__builtin_amdgcn_readfirstlane((int)to) : to;
         const tpw_u32x4 r = resource(base, rows * stride);
-        if (DWORDS && width) {  // four times the instructions, their offsets formed as they go
+        if constexpr (DWORDS) {  // four times the instructions, their offsets formed as they go
             const int lane = threadIdx.x & 63;
 #pragma unroll 2
             for (int i = 0; i < 4 * kSlots; ++i) {
@@ -214,10 +214,10 @@ struct Stager {
                 dma4(r, byte < width ? (uint32_t)(row * stride + byte) : kBeyond,
                      (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds + (uint32_t)((i * WAVES + wave) * 256))));
             }
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) dma16(r, off[i], lds + (uint32_t)((i * WAVES + wave) * 1024));
+            for (int i = 0; i < kSlots; ++i) dma16(r, off[i], lds + (uint32_t)((i * WAVES + wave) * 1024));
+        }
     }
 };
 
@@ -357,7 +357,7 @@ struct ColReader<float, DP, 16> {
 
 // Features f .. f + 7 of a row in global memory (null: zeros).
 template <typename T>
-__device__ __forceinline__ Frag<T> load_row8(const T *row, int f, int d, int dwords = 0) {
+__device__ __forceinline__ Frag<T> load_row8(const T *row, int f, int d, bool dwords = false) {
     constexpr int E = 16 / (int)sizeof(T), D = 4 / (int)sizeof(T);
     T x[8];
     if (dwords) {
