@@ -1,11 +1,13 @@
 """attention and rotary_embedding: forward, gradients, masks, lengths, layouts and refusals, against
 the plain 64-bit forms of tests/_attention.py with bounds derived there."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 import torchpairwise as tp
+from torchpairwise_amd import _capi as capi
 from tests._attention import reference, rotate
 from tests._util import assert_close, assert_equal, gen, randn
 
@@ -291,6 +293,62 @@ def test_refusals(device):
         tp.rotary_embedding(x, pos, f, scale=math.nan)
     with pytest.raises(RuntimeError, match="frequencies have no gradient"):
         tp.rotary_embedding(x, pos, f.clone().requires_grad_())
+
+
+def _desc(q, k, v, out, stats=None, **kw):
+    """tpw_attention_desc of dense 4-D rows (C entry)."""
+    a = capi.AttentionDesc(dtype=capi.TPW_F32 if q.dtype == F32 else capi.TPW_BF16, batch=q.shape[0], heads=q.shape[1],
+                           key_heads=k.shape[1], n=q.shape[2], m=k.shape[2], d=q.shape[3], dv=v.shape[3],
+                           scale=q.shape[3] ** -0.5, query=q.data_ptr(), key=k.data_ptr(), value=v.data_ptr(),
+                           out=out.data_ptr(), stats=None if stats is None else stats.data_ptr())
+    for name, x in (("query", q), ("key", k), ("value", v), ("out", out)):
+        getattr(a, name + "_strides")[:] = x.stride()[:3]
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def test_c_entries_refuse_on_the_host():
+    """Refusals and workspace sizes need no GPU: nothing is launched."""
+    lib = capi.lib()
+    q, k, v, out = (torch.zeros(1, 2, 3, 8) for _ in range(4))
+    for message, kw in ((b"1 to 256 features", {"d": 0}), (b"1 to 256 features", {"dv": 257}),
+                        (b"multiple of key_heads", {"key_heads": 3}), (b"unknown mask type", {"mask_type": 9}),
+                        (b"float32 or bfloat16", {"dtype": capi.TPW_F64}), (b"scale must be finite", {"scale": math.inf}),
+                        (b"negative size", {"n": -1}), (b"null operand", {"query": None}),
+                        (b"null mask", {"mask_type": 1}), (b"too many rows", {"m": 1 << 31})):
+        a = _desc(q, k, v, out, **kw)
+        assert lib.tpw_attention(C.byref(a), None, None) == 1 and message in lib.tpw_last_error(), message
+    a = _desc(q, k, v, out)
+    a.key_strides[2] = 4  # rows overlap
+    assert lib.tpw_attention(C.byref(a), None, None) == 1 and b"overlap" in lib.tpw_last_error()
+    a = _desc(q, k, v, out)
+    assert lib.tpw_attention_backward(C.byref(a), None, None) == 1  # gradients missing
+    for n, m in ((0, 3), (3, 0), (0, 0), (1, 1), (1, 100000), (5000, 5000)):
+        for dtype in (capi.TPW_F32, capi.TPW_BF16):
+            for d in (1, 50, 96, 130, 256):
+                a = _desc(q, k, v, out, dtype=dtype, n=n, m=m, d=d, dv=d)
+                for name in ("query", "key", "value", "out", "grad_out", "grad_query", "grad_key", "grad_value"):
+                    getattr(a, name + "_strides")[:] = [d * 5000 * 2, d * 5000, d]
+                assert lib.tpw_attention_workspace_size(C.byref(a)) >= 0
+                assert lib.tpw_attention_backward_workspace_size(C.byref(a)) >= 4 * 3 * 2 * n
+    s = (C.c_int64 * 3)(48, 24, 8)
+    assert lib.tpw_rotary(None, capi.TPW_F32, 1, 2, 3, 8, s, None, None, None, 5, 0, 0, 1.0, None, s, None) == 1
+    assert lib.tpw_rotary(None, capi.TPW_F64, 1, 2, 3, 8, s, None, None, None, 4, 0, 0, 1.0, None, s, None) == 1
+    assert lib.tpw_rotary(None, capi.TPW_F32, 1, 2, 3, 8, s, None, None, None, 4, 0, 0, 1.0, None, s, None) == 1
+    assert lib.tpw_rotary(None, capi.TPW_F32, 1, 2, 0, 8, s, None, None, None, 4, 0, 0, 1.0, None, s, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_c_entries_without_statistics(dtype):
+    """The C entry called directly, without statistics or rests, gives the operator's bits."""
+    q, k, v = on("cuda", rows(2, 4, 70, 64, 1, dtype), rows(2, 2, 300, 64, 2, dtype), rows(2, 2, 300, 64, 3, dtype))
+    out = torch.empty_like(q)
+    a = _desc(q, k, v, out)
+    ws = torch.empty(max(capi.lib().tpw_attention_workspace_size(C.byref(a)), 1), dtype=torch.uint8, device="cuda")
+    capi.call("tpw_attention", C.byref(a), ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert_equal(out, tp.attention(q, k, v))
 
 
 def test_gradients_against_differences():
