@@ -26,10 +26,12 @@ struct RotaryArgs {
 __device__ __forceinline__ void angle(double position, double turns, float scale, float sign, float &c, float &s) {
     double t = position * turns;
     t -= rint(t);
+    // what the angle loses in 32 bits turns the sine and cosine a little further
+    const float hi = (float)t, lo = (float)(t - (double)hi) * 6.28318530717958648f;
     float ss, cc;
-    sincospif(2.0f * (float)t, &ss, &cc);
-    c = cc * scale;
-    s = ss * scale * sign;
+    sincospif(2.0f * hi, &ss, &cc);
+    c = __builtin_fmaf(-lo, ss, cc) * scale;
+    s = __builtin_fmaf(lo, cc, ss) * scale * sign;
 }
 
 // P pairs at a time: P consecutive features of both halves, or 2 P consecutive ones (INTERLEAVED).
