@@ -168,6 +168,19 @@ def test_scales(device, dtype, scale):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("scale", [1e-46, -1e-300])
+@pytest.mark.parametrize("mask", [None, "keep", "bias"])
+def test_scales_below_the_range_of_32_bits(device, scale, mask):
+    """The same as a scale of zero: equal weights for the keys that are left, none for the others."""
+    if mask == "keep":
+        mask = torch.rand(33, 65, generator=gen(5)) < 0.5
+    elif mask == "bias":
+        mask = randn(33, 65, seed=5).masked_fill(torch.rand(33, 65, generator=gen(6)) < 0.5, -math.inf)
+    check(device, rows(1, 2, 33, 40, 1), rows(1, 2, 65, 40, 2), rows(1, 2, 65, 40, 3), mask, causal=True, scale=scale,
+          grad=rows(1, 2, 33, 40, 4))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_strides_and_alignment(device, dtype):
     """Sliced features (rows not dense), a column offset that breaks 16-byte alignment, transposed

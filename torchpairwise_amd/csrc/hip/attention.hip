@@ -565,8 +565,10 @@ int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
     a.mm = d->mask_strides[3];
     a.mask_bf16 = d->mask_type == TPW_MASK_ADD_BF16;
     const bool bias = mask_mode(d) == kBias;
-    a.qsign = d->scale > 0 ? 1.0f : d->scale < 0 ? -1.0f : 0.0f;
-    a.scale = d->scale == 0 ? 1.0f : (float)(fabs(d->scale) * (bias ? 1.0 : 1.4426950408889634));
+    // a scale that 32 bits hold as zero is zero: it would turn the -inf of a key that is left out to NaN
+    a.scale = (float)(fabs(d->scale) * (bias ? 1.0 : 1.4426950408889634));
+    a.qsign = a.scale == 0.0f ? 0.0f : d->scale > 0 ? 1.0f : -1.0f;
+    if (a.scale == 0.0f) a.scale = 1.0f;
     a.gscale = (float)d->scale;
     a.rest = d->dtype == TPW_BF16 ? d->out_rest : nullptr;
     const auto streamed = [&](const View &v, int64_t rows, int64_t width) {
