@@ -291,19 +291,22 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
     OutRow<T>(a, b, h, i).store(f, o * inv);
 }
 
-// The same for at most kFew parts: one thread per four features, every load in flight at once
-// (32 x 4096 rows of 64 features in two parts: 30 us, where a wave per row takes 80).
-constexpr int kFew = 8;
-template <typename T, bool BIAS>
+// The same for at most PARTS parts: one thread per four features, every load in flight at once
+// (32 x 4096 rows of 64 features in two parts: 30 us, where a wave per row takes 80).  Of 9 to 16 parts it
+// takes over where there are enough quads to fill the card (a call of 16 x 500 rows of 64, 128000 quads: 58.7
+// us, with a block per row 63.4; 8 x 200 of 128, 51200: 25.6, 27.0; 16 x 128 of 64, 32768: 23.9, 25.0; 16 x 32
+// of 64, 8192: 17.2 either way; 64 of 128, 2048: 12.2, 11.5).
+constexpr int64_t kManyQuads = 32768;
+template <typename T, bool BIAS, int PARTS>
 __global__ __launch_bounds__(256) void attention_join_few_kernel(const Args a) {
     const int64_t rows = a.batch * a.heads * a.n, quads = cdiv_dev(a.dv, 4);
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / quads;
     if (row >= rows) return;
     const int f = (int)(id % quads) * 4;
-    float top_s[kFew], sum_s[kFew];
-    f32x4 x[kFew];
+    float top_s[PARTS], sum_s[PARTS];
+    f32x4 x[PARTS];
 #pragma unroll
-    for (int s = 0; s < kFew; ++s) {
+    for (int s = 0; s < PARTS; ++s) {
         top_s[s] = -INFINITY;
         sum_s[s] = 0.0f;
         x[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -314,11 +317,11 @@ __global__ __launch_bounds__(256) void attention_join_few_kernel(const Args a) {
     }
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int s = 0; s < kFew; ++s) top = __builtin_fmaxf(top, top_s[s]);
+    for (int s = 0; s < PARTS; ++s) top = __builtin_fmaxf(top, top_s[s]);
     const float base = top == -INFINITY ? 0.0f : top;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int s = 0; s < kFew; ++s) {
+    for (int s = 0; s < PARTS; ++s) {
         const float w = __builtin_amdgcn_exp2f(BIAS ? (top_s[s] - base) * kLog2e : top_s[s] - base);
         sum += w * sum_s[s];
         o += x[s] * w;
@@ -648,9 +651,12 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
                                dim3(64 * kWaves), 0, s, a);
         if (const int rc = check_launch("attention_kernel")) return rc;
         if (a.splits > 1) {
-            if (a.splits <= kFew)
-                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias>),
-                                   dim3((unsigned)cdiv(rows * cdiv(a.dv, 4), 256)), dim3(256), 0, s, a);
+            const int64_t quads = rows * cdiv(a.dv, 4);
+            const dim3 few((unsigned)cdiv(quads, 256));
+            if (a.splits <= 8)
+                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias, 8>), few, dim3(256), 0, s, a);
+            else if (a.splits <= 16 && quads >= kManyQuads)
+                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias, 16>), few, dim3(256), 0, s, a);
             else
                 hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, Tile<T, DP>::P / 4>), dim3((unsigned)rows),
                                    dim3(256), 0, s, a);
