@@ -398,14 +398,15 @@ def test_few_rows_over_many_keys(dtype, n, h, hk, m, d, dv):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,h,hk,n,m,d,dv", [(BF16, 8, 8, 140, 2200, 128, 128), (BF16, 8, 4, 140, 3000, 128, 128),
-                                                 (F32, 16, 4, 130, 2500, 64, 64), (F32, 16, 4, 133, 2500, 64, 62)])
+                                                 (F32, 16, 4, 130, 2500, 64, 64), (F32, 16, 4, 133, 2500, 64, 62),
+                                                 (BF16, 16, 4, 130, 2500, 64, 64), (F32, 8, 4, 140, 3000, 128, 128)])
 def test_parts_of_many_rows(dtype, h, hk, n, m, d, dv):
-    """9 to 16 parts of enough rows that a thread joins four features of all of them; parts without keys."""
+    """9 to 32 parts of enough rows that a thread joins four features of all of them; parts without keys."""
     q, k, v = rows(1, h, n, d, 1, dtype), rows(1, hk, m, d, 2, dtype), rows(1, hk, m, dv, 3, dtype)
     if dv == d:
         a = _desc(q, k, v, torch.zeros(1, h, n, dv, dtype=dtype))
         parts = capi.lib().tpw_attention_workspace_size(C.byref(a)) / (4 * h * n * (dv + 2))
-        assert 8 < parts <= 16 and parts == int(parts) and h * n * dv // 4 >= 32768
+        assert 8 < parts <= 32 and parts == int(parts) and h * n * dv // 4 >= 32768
     check("cuda", q, k, v, causal=True, grad=rows(1, h, n, dv, 4, dtype))
     check("cuda", q, k, v, lengths=torch.tensor([100]))
     bias = randn(h, n, m, seed=5)

@@ -292,10 +292,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
 }
 
 // The same for at most PARTS parts: one thread per four features, every load in flight at once
-// (32 x 4096 rows of 64 features in two parts: 30 us, where a wave per row takes 80).  Of 9 to 16 parts it
-// takes over where there are enough quads to fill the card (a call of 16 x 500 rows of 64, 128000 quads: 58.7
-// us, with a block per row 63.4; 8 x 200 of 128, 51200: 25.6, 27.0; 16 x 128 of 64, 32768: 23.9, 25.0; 16 x 32
-// of 64, 8192: 17.2 either way; 64 of 128, 2048: 12.2, 11.5).
+// (32 x 4096 rows of 64 features in two parts: 30 us, where a wave per row takes 80).  Of 9 to 32 parts it
+// takes over where there are enough quads to fill the card (whole calls; 16 parts: 16 x 500 rows of 64, 128000
+// quads, 58.7 us, with a block per row 63.4; 8 x 200 of 128, 51200 quads, 25.6, 27.0; 256 of 128, 8192 quads,
+// equal; 32 parts: 16 x 128 of 64, 32768 quads, 23.9, 25.0; 26 parts: 64 of 128, 2048 quads, 12.2, 11.5).
 constexpr int64_t kManyQuads = 32768;
 template <typename T, bool BIAS, int PARTS>
 __global__ __launch_bounds__(256) void attention_join_few_kernel(const Args a) {
@@ -657,6 +657,8 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
                 hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias, 8>), few, dim3(256), 0, s, a);
             else if (a.splits <= 16 && quads >= kManyQuads)
                 hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias, 16>), few, dim3(256), 0, s, a);
+            else if (a.splits <= 32 && quads >= kManyQuads)
+                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias, 32>), few, dim3(256), 0, s, a);
             else
                 hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, Tile<T, DP>::P / 4>), dim3((unsigned)rows),
                                    dim3(256), 0, s, a);
