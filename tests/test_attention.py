@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import torchpairwise as tp
 from torchpairwise_amd import _capi as capi
@@ -377,6 +378,24 @@ def test_gradients_against_differences():
     for inter in (False, True):
         assert torch.autograd.gradcheck(
             lambda x: tp.rotary_embedding(x, torch.arange(6) * 11, f, interleaved=inter, scale=s), (q,))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_is_refused(device):
+    """A tangent on any operand raises, with and without gradients enabled: none is dropped."""
+    ops = dict(zip("qkv", on(device, rows(1, 2, 3, 8, 1), rows(1, 2, 5, 8, 2), rows(1, 2, 5, 4, 3))))
+    ops["mask"] = torch.zeros(3, 5, device=device)
+    for name, x in ops.items():
+        for enabled in (True, False):
+            with forward_ad.dual_level(), torch.set_grad_enabled(enabled):
+                args = dict(ops, **{name: forward_ad.make_dual(x, torch.ones_like(x))})
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    tp.attention(*args.values())
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(lambda y: tp.attention(*dict(ops, **{name: y}).values()), (x,), (torch.ones_like(x),))
+    # a dual level without tangents changes nothing
+    with forward_ad.dual_level():
+        assert_equal(tp.attention(*ops.values()), tp.attention(*ops.values()))
 
 
 # ---------------------------------------------------------------- single tokens, long rows of keys

@@ -472,8 +472,17 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     }
 };
 
+// Below autograd a tangent would be lost without a word.
+void refuse_tangent(const at::Tensor &x) {
+    TORCH_CHECK(!x.defined() || !x._fw_grad(0).defined(), "attention: forward-mode derivatives are not implemented");
+}
+
 Results attention_autograd(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value, const OptTensor &mask,
                            const OptTensor &lengths, bool causal, double scale, bool train) {
+    refuse_tangent(query);
+    refuse_tangent(key);
+    refuse_tangent(value);
+    if (mask.has_value()) refuse_tangent(*mask);
     if (!train) {
         TORCH_CHECK(!(at::GradMode::is_enabled() && mask.has_value() && mask->defined() && mask->requires_grad()),
                     "attention: the mask has no gradient; pass mask.detach()");
