@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import torchpairwise as tp
 from torchpairwise_amd import _capi as capi
@@ -396,6 +397,27 @@ def test_forward_mode_is_refused(device):
     # a dual level without tangents changes nothing
     with forward_ad.dual_level():
         assert_equal(tp.attention(*ops.values()), tp.attention(*ops.values()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_graph_traced_without_gradients_gives_them(device):
+    """A call recorded on operands without gradients, run on operands that require them."""
+    q, k, v, grad = rows(1, 4, 9, 16, 1), rows(1, 2, 21, 16, 2), rows(1, 2, 21, 8, 3), rows(1, 4, 9, 8, 4)
+    bias = randn(9, 21, seed=5)
+    dq, dk, dv, dg, db = on(device, q, k, v, grad, bias)
+    graph = make_fx(lambda a, b, c, m: tp.attention(a, b, c, m, causal=True))(dq, dk, dv, db)
+    want = reference(q, k, v, bias, True, grad=grad)
+    for which in range(3):  # each operand alone
+        leaves = [x.detach().clone().requires_grad_(i == which) for i, x in enumerate((dq, dk, dv))]
+        out = graph(*leaves, db)
+        assert_close(out, want["out"], rtol=0.0, atol=want["tol_out"] + TINY)
+        name = ("dq", "dk", "dv")[which]
+        (got,) = torch.autograd.grad(out, leaves[which], dg)
+        assert_close(got, want[name], rtol=0.0, atol=want["tol_" + name] + TINY, what=name)
+        with torch.no_grad():
+            assert not graph(*leaves, db).requires_grad
+    with pytest.raises(RuntimeError, match="mask has no gradient"):
+        graph(dq, dk, dv, db.clone().requires_grad_())
 
 
 # ---------------------------------------------------------------- single tokens, long rows of keys

@@ -413,9 +413,7 @@ at::Tensor attention(const at::Tensor &query, const at::Tensor &key, const at::T
                      : query.dim() > 0 && query.size(-1) > 0 ? 1.0 / std::sqrt((double)query.size(-1))
                                                              : 1.0;
     TORCH_CHECK(std::isfinite(s) && std::fabs(s) <= 1e30, "attention: scale must be finite, got ", s);
-    const bool train =
-        at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad());
-    return std::get<0>(attention_op(query, key, value, mask, lengths, causal, s, train));
+    return std::get<0>(attention_op(query, key, value, mask, lengths, causal, s, false));
 }
 
 at::Tensor rotary_embedding(const at::Tensor &x, const at::Tensor &positions, const at::Tensor &frequencies,
@@ -428,8 +426,6 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
    public:
     static variable_list forward(AutogradContext *ctx, const Variable &query, const Variable &key, const Variable &value,
                                  const OptTensor &mask, const OptTensor &lengths, bool causal, double scale) {
-        TORCH_CHECK(!(mask.has_value() && mask->defined() && mask->requires_grad()),
-                    "attention: the mask has no gradient; pass mask.detach()");
         at::AutoDispatchBelowADInplaceOrView g;
         auto r = attention_op(query, key, value, mask, lengths, causal, scale, true);
         auto out = std::get<0>(r), stats = std::get<1>(r), rest = std::get<2>(r);
@@ -483,9 +479,11 @@ Results attention_autograd(const at::Tensor &query, const at::Tensor &key, const
     refuse_tangent(key);
     refuse_tangent(value);
     if (mask.has_value()) refuse_tangent(*mask);
-    if (!train) {
-        TORCH_CHECK(!(at::GradMode::is_enabled() && mask.has_value() && mask->defined() && mask->requires_grad()),
-                    "attention: the mask has no gradient; pass mask.detach()");
+    const bool grad = at::GradMode::is_enabled();
+    TORCH_CHECK(!(grad && mask.has_value() && mask->defined() && mask->requires_grad()),
+                "attention: the mask has no gradient; pass mask.detach()");
+    // The operands decide, whatever a recorded call was made on.
+    if (!train && !(grad && (query.requires_grad() || key.requires_grad() || value.requires_grad()))) {
         at::AutoDispatchBelowADInplaceOrView g;
         return attention_op(query, key, value, mask, lengths, causal, scale, false);
     }
