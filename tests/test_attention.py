@@ -2,6 +2,9 @@
 the plain 64-bit forms of tests/_attention.py with bounds derived there."""
 import ctypes as C
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -270,6 +273,19 @@ def test_empty_sizes(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [8, 128, 256])
+@pytest.mark.parametrize("b,h,n,m", [(0, 2, 3, 4), (2, 0, 3, 4), (2, 2, 0, 4), (2, 2, 3, 0)])
+def test_empty_sizes_by_width(device, dtype, d, b, h, n, m):
+    q, k, v = (torch.ones(*s, dtype=dtype, device=device, requires_grad=True)
+               for s in ((b, h, n, d), (b, 2, m, d), (b, 2, m, d)))
+    out = tp.attention(q, k, v)
+    assert out.shape == (b, h, n, d) and not out.any()
+    for g, x in zip(torch.autograd.grad(out.sum(), (q, k, v)), (q, k, v)):
+        assert g.shape == x.shape and not g.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_refusals(device):
     q, k, v = (x.to(device) for x in (randn(2, 4, 5, 8, seed=1), randn(2, 2, 6, 8, seed=2), randn(2, 2, 6, 3, seed=3)))
     at = tp.attention
@@ -352,6 +368,35 @@ def test_c_entries_refuse_on_the_host():
     assert lib.tpw_rotary(None, capi.TPW_F64, 1, 2, 3, 8, s, None, None, None, 4, 0, 0, 1.0, None, s, None) == 1
     assert lib.tpw_rotary(None, capi.TPW_F32, 1, 2, 3, 8, s, None, None, None, 4, 0, 0, 1.0, None, s, None) == 1
     assert lib.tpw_rotary(None, capi.TPW_F32, 1, 2, 0, 8, s, None, None, None, 4, 0, 0, 1.0, None, s, None) == 0
+
+
+def test_workspaces_of_empty_and_of_huge_calls():
+    """Sizes that divide nothing: no heads, no batch, no rows, and counts whose product passes 64 bits.
+    In a process of its own, as a trapped division would end the test run."""
+    code = """
+import ctypes as C
+from torchpairwise_amd import _capi as capi
+lib = capi.lib()
+def sizes(dtype, b, h, hk, n, m, d):
+    a = capi.AttentionDesc(dtype=dtype, batch=b, heads=h, key_heads=hk, n=n, m=m, d=d, dv=d, scale=1.0)
+    for name, _ in a._fields_:
+        if name.endswith("_strides"):
+            getattr(a, name)[2] = d
+    return lib.tpw_attention_workspace_size(C.byref(a)), lib.tpw_attention_backward_workspace_size(C.byref(a))
+for dtype in (capi.TPW_F32, capi.TPW_BF16):
+    for d in (64, 96, 128, 192, 256):
+        for b, h, hk, n, m in ((1, 0, 1, 8, 8), (0, 1, 1, 8, 8), (0, 0, 2, 8, 8), (2, 0, 2, 0, 8), (2, 4, 2, 8, 0),
+                               (2, 4, 2, 0, 8), (0, 4, 2, 5000, 5000)):
+            forward, backward = sizes(dtype, b, h, hk, n, m, d)
+            rows = b * h * n
+            assert forward >= 0 and backward >= 12 * rows and (rows or forward == 0), (b, h, hk, n, m, d)
+            if rows * m == 0:  # nothing to split, keep or copy
+                assert backward <= 12 * rows + 12, (b, h, hk, n, m, d, backward)
+        sizes(dtype, 1, 16, 1, 1 << 30, 1 << 30, d)
+print("done")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parent.parent, capture_output=True, text=True)
+    assert r.returncode == 0 and "done" in r.stdout, (r.returncode, r.stdout, r.stderr[-2000:])
 
 
 @pytest.mark.gpu

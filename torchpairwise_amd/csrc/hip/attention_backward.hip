@@ -691,8 +691,12 @@ constexpr int64_t kKeptBytes = int64_t(1) << 30, kKeptKeys = 128;
 int64_t ds_bytes(const Args &a) { return a.group * a.m * (cdiv(a.n, kUnit) * kUnit) * 4; }  // of one key head
 template <typename T, int DP>
 int64_t keeps_ds(const Args &a) {
-    if (sizeof(T) != 4 || DP == 64 || a.n == 0 || a.m == 0 || ds_bytes(a) > kKeptBytes) return 0;
-    const int64_t bk = a.batch * a.key_heads, most = kKeptBytes / ds_bytes(a), kept = cdiv(bk, cdiv(bk, most));
+    const int64_t bk = a.batch * a.key_heads;
+    // nothing to keep of empty calls; the bytes of a key head are compared without their product
+    if (sizeof(T) != 4 || DP == 64 || bk * a.group == 0 || a.n == 0 || a.m == 0 ||
+        a.group > kKeptBytes / 4 / (cdiv(a.n, kUnit) * kUnit) / a.m)
+        return 0;
+    const int64_t most = kKeptBytes / ds_bytes(a), kept = cdiv(bk, cdiv(bk, most));
     return kept * cdiv(a.m, kKeptKeys) >= 192 && kept * a.group * cdiv(a.n, kKeptKeys) >= 192 ? kept : 0;
 }
 template <typename T, int DP>
