@@ -286,6 +286,38 @@ def test_empty_sizes_by_width(device, dtype, d, b, h, n, m):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [50, 128])
+@pytest.mark.parametrize("b,h,n,m", [(0, 2, 3, 4), (2, 0, 3, 4), (2, 2, 0, 4), (2, 2, 3, 0)])
+@pytest.mark.parametrize("kind", ["keep", "bias", "bias_heads"])
+def test_empty_sizes_with_masks(device, dtype, d, b, h, n, m, kind):
+    mask = {"keep": lambda: torch.ones(n, m, dtype=torch.bool), "bias": lambda: torch.zeros(n, m),
+            "bias_heads": lambda: torch.zeros(b, h, n, m)}[kind]().to(device)
+    q, k, v = (torch.ones(*s, dtype=dtype, device=device, requires_grad=True)
+               for s in ((b, h, n, d), (b, 2, m, d), (b, 2, m, d)))
+    out = tp.attention(q, k, v, mask)
+    assert out.shape == (b, h, n, d) and not out.any()
+    for g, x in zip(torch.autograd.grad(out.sum(), (q, k, v)), (q, k, v)):
+        assert g.shape == x.shape and not g.any()
+
+
+def test_c_entries_ask_for_no_mask_without_queries():
+    """A mask over no queries has no address: the entry asks for what comes after the mask.  Nothing is
+    launched."""
+    lib = capi.lib()
+    q, k, v, out = (torch.zeros(1, 2, n, 8) for n in (0, 3, 3, 0))
+    for mask_type in (1, 2):
+        a = _desc(q, k, v, out, mask_type=mask_type, grad_key=None, grad_value=None)
+        # stops at the gradients' addresses, which come after the operands' and before any launch
+        assert lib.tpw_attention_backward(C.byref(a), None, None) == 1 and b"null operand" in lib.tpw_last_error()
+        gk, gv = torch.zeros_like(k), torch.zeros_like(v)
+        a = _desc(q, k, v, out, mask_type=mask_type, grad_key=gk.data_ptr(), grad_value=gv.data_ptr())
+        a.grad_key_strides[:] = a.grad_value_strides[:] = k.stride()[:3]
+        # the workspace is asked for after the mask
+        assert lib.tpw_attention_backward(C.byref(a), None, None) == 1 and b"workspace" in lib.tpw_last_error()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_refusals(device):
     q, k, v = (x.to(device) for x in (randn(2, 4, 5, 8, seed=1), randn(2, 2, 6, 8, seed=2), randn(2, 2, 6, 3, seed=3)))
     at = tp.attention

@@ -527,7 +527,6 @@ int prepare_operands(Args &a, const tpw_attention_desc *d, bool backward, void *
     if (mask_mode(d) == kKeep) {
         BitArgs m = {};
         plan_bits(a, backward, next, &m);
-        if (m.lead * m.n * m.words == 0) return TPW_OK;
         const int64_t blocks = cdiv(m.lead * cdiv(m.n, 32) * (m.words / 2), 4);
         TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: mask too large");
         hipLaunchKernelGGL(pack_mask_kernel, dim3((unsigned)blocks), dim3(256), 0, s, m);
@@ -621,7 +620,7 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
     if (const int rc = read_args(d, false, a)) return rc;
     if (a.batch * a.heads * a.n == 0) return TPW_OK;
     TPW_REQUIRE(a.q.p && a.o.p && (a.m == 0 || (a.k.p && a.v.p)), "attention: null operand");
-    TPW_REQUIRE(d->mask_type == TPW_MASK_NONE || a.mask || a.m == 0, "attention: null mask");
+    TPW_REQUIRE(mask_mode(d) == kNoMask || a.mask, "attention: null mask");
     hipStream_t s = as_stream(stream);
     const size_t prepared = prepared_bytes(a, d, false);
     if (prepared) {

@@ -554,7 +554,9 @@ template <typename F>
 int by_type(const Args &a, int dtype, int mode, F &&f) {
     return dtype == TPW_BF16 ? by_width<uint16_t>(a, mode, f) : by_width<float>(a, mode, f);
 }
+// A mask over no pairs is none: it may have no address.
 inline int mask_mode(const tpw_attention_desc *d) {
+    if (d->batch == 0 || d->heads == 0 || d->n == 0 || d->m == 0) return kNoMask;
     return d->mask_type == TPW_MASK_NONE ? kNoMask : d->mask_type == TPW_MASK_KEEP ? kKeep : kBias;
 }
 // Parts of a summed axis of `steps` tiles for `blocks` blocks, `per_cu` of which share a CU: the least

@@ -770,7 +770,7 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
     if (rows + keys == 0) return TPW_OK;
     TPW_REQUIRE(rows == 0 || (a.q.p && a.o.p && a.go.p && a.gq.p && a.stats), "attention backward: null operand");
     TPW_REQUIRE(keys == 0 || (a.k.p && a.v.p && a.gk.p && a.gv.p), "attention backward: null operand");
-    TPW_REQUIRE(d->mask_type == TPW_MASK_NONE || a.mask || a.m == 0, "attention: null mask");
+    TPW_REQUIRE(mask_mode(d) == kNoMask || a.mask, "attention: null mask");
     TPW_REQUIRE(workspace && aligned16(workspace), "attention backward: null or unaligned workspace");
     hipStream_t s = as_stream(stream);
     const size_t prepared = prepared_bytes(a, d, true);
