@@ -763,3 +763,22 @@ def test_rotary_frequencies():
                 {"width": 8, "scaling": "parts", "factor": 2.0, "original_length": 64, "fast": 1.0}):
         with pytest.raises(ValueError):
             tp.rotary_frequencies(**bad)
+
+
+@pytest.mark.parametrize("width,base,length,factor", [(128, 1e4, 131072, 4.0), (64, 1e4, 1 << 20, 4.0), (128, 1e4, 65536, 8.0),
+                                                      (64, 1e4, 4096, 2.0), (32, 500.0, 100, 4.0), (16, 1e4, 4, 4.0),
+                                                      (2, 1e4, 100, 4.0)])
+def test_parts_of_the_frequencies_by_their_turns(width, base, length, factor):
+    """Kept where a pair makes 32 turns or more over the original length, divided by the factor where it makes
+    one or fewer, a line over the pairs between, also where its ends lie outside the pairs there are."""
+    f = tp.rotary_frequencies(width, base)[0]
+    got = tp.rotary_frequencies(width, base, scaling="parts", factor=factor, original_length=length)[0] / f
+    turns = length * f / (2 * math.pi)
+    assert_close(got[turns >= 32.0], torch.ones_like(got[turns >= 32.0]), rtol=1e-12, atol=0.0)
+    assert_close(got[turns <= 1.0], torch.full_like(got[turns <= 1.0], 1 / factor), rtol=1e-12, atol=0.0)
+    # turns fall by `step` in their logarithm from pair to pair: where they reach 32 and 1
+    step = 2 * math.log(base) / width
+    ends = [math.log(length / (2 * math.pi * t)) / step for t in (32.0, 1.0)]
+    first, last = math.floor(ends[0]), math.ceil(ends[1])
+    share = ((torch.arange(width // 2, dtype=torch.float64) - first) / (last - first)).clamp(0.0, 1.0)
+    assert_close(got, 1.0 - share * (1.0 - 1 / factor), rtol=1e-12, atol=0.0)

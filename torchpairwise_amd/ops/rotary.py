@@ -24,8 +24,9 @@ def rotary_frequencies(width: int, base: float = 10000.0, *, scaling: str = "non
     * ``"base"``: the base raised to ``base * factor ** (width / (width - 2))``, which leaves the
       fastest pair and divides the slowest one's frequency by ``factor``;
     * ``"parts"``: pairs that make ``fast`` turns or more over ``original_length`` positions stay, those
-      that make ``slow`` or fewer are divided by ``factor``, with a linear ramp over the pairs between;
-      the result is scaled by ``0.1 ln(factor) + 1``.
+      that make ``slow`` or fewer are divided by ``factor``, with a linear ramp over the pairs between
+      (from the last whole pair of the first to the first of the second, whether or not the width reaches
+      them); the result is scaled by ``0.1 ln(factor) + 1``.
     """
     if width < 2 or width % 2:
         raise ValueError(f"rotary_frequencies: width must be even and at least 2, got {width}")
@@ -52,8 +53,9 @@ def rotary_frequencies(width: int, base: float = 10000.0, *, scaling: str = "non
         def pair_of(turns: float) -> float:
             return half * math.log(original_length / (2 * math.pi * turns)) / math.log(base)
 
-        first, last = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), half - 1)
-        ramp = ((pair - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
+        # not held to the pairs there are: an end moved inwards would change the slope
+        first, last = math.floor(pair_of(fast)), math.ceil(pair_of(slow))
+        ramp = ((pair - first) / max(last - first, 1)).clamp(0.0, 1.0)
         frequencies = frequencies * (1.0 - ramp) + frequencies / factor * ramp
         scale = 0.1 * math.log(factor) + 1.0
     return frequencies.to(device), scale
