@@ -782,3 +782,20 @@ def test_parts_of_the_frequencies_by_their_turns(width, base, length, factor):
     first, last = math.floor(ends[0]), math.ceil(ends[1])
     share = ((torch.arange(width // 2, dtype=torch.float64) - first) / (last - first)).clamp(0.0, 1.0)
     assert_close(got, 1.0 - share * (1.0 - 1 / factor), rtol=1e-12, atol=0.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_frequencies_held_as_a_parameter(device):
+    """They have no gradient, so they are refused only where one would be lost."""
+    x, pos = randn(2, 3, 5, 16, seed=1).to(device), torch.arange(5, device=device)
+    f = torch.rand(8, dtype=torch.float64, generator=gen(2)).to(device)
+    held = torch.nn.Parameter(f)
+    with torch.no_grad():
+        assert_equal(tp.rotary_embedding(x, pos, held), tp.rotary_embedding(x, pos, f))
+    with torch.inference_mode():
+        assert_equal(tp.rotary_embedding(x, pos, held), tp.rotary_embedding(x, pos, f))
+    leaf = x.clone().requires_grad_()
+    assert tp.rotary_embedding(leaf, pos, held.detach()).requires_grad
+    for y in (x, leaf):
+        with pytest.raises(RuntimeError, match="frequencies have no gradient"):
+            tp.rotary_embedding(y, pos, held)

@@ -451,8 +451,6 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
    public:
     static Variable forward(AutogradContext *ctx, const Variable &x, const Variable &positions, const Variable &frequencies,
                             bool interleaved, double scale, bool inverse) {
-        TORCH_CHECK(!frequencies.requires_grad(),
-                    "rotary_embedding: frequencies have no gradient; pass frequencies.detach()");
         at::AutoDispatchBelowADInplaceOrView g;
         ctx->save_for_backward({positions, frequencies});
         ctx->saved_data["interleaved"] = interleaved;
@@ -492,6 +490,8 @@ Results attention_autograd(const at::Tensor &query, const at::Tensor &key, const
 }
 at::Tensor rotary_autograd(const at::Tensor &x, const at::Tensor &positions, const at::Tensor &frequencies,
                            bool interleaved, double scale, bool inverse) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && frequencies.requires_grad()),
+                "rotary_embedding: frequencies have no gradient; pass frequencies.detach()");
     return RotaryFunction::apply(x, positions, frequencies, interleaved, scale, inverse);
 }
 
