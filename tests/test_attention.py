@@ -514,6 +514,62 @@ def test_few_rows_over_many_keys(dtype, n, h, hk, m, d, dv):
     check("cuda", rows(3, h, n, d, 1, dtype), rows(3, hk, m, d, 2, dtype), rows(3, hk, m, dv, 3, dtype), bias)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,h,hk,m,d", [(1, 1, 1, 5000, 64), (1, 16, 2, 4097, 128), (1, 8, 1, 3001, 256), (4, 8, 2, 2050, 96),
+                                        (3, 40, 1, 1030, 128), (1, 3, 3, 700, 50), (2, 16, 1, 9000, 128), (130, 16, 4, 2500, 64),
+                                        (140, 8, 8, 2200, 128), (70, 4, 4, 300, 192)])
+def test_every_key_counts_once(device, dtype, n, h, hk, m, d):
+    """Equal weights and one-hot values: feature f of a row that sees L keys is the number of keys j < L with
+    j % d == f over L, so that one key lost or read twice shows at any length and in any type."""
+    q, k = rows(3, h, n, d, 1, dtype), rows(3, hk, m, d, 2, dtype)
+    v = torch.eye(d, dtype=dtype)[torch.arange(m) % d].expand(3, hk, m, d)
+    lengths = torch.tensor([m, m // 2 + 1, 65])
+    seen = (lengths[:, None] - n + 1 + torch.arange(n)).clamp(min=0)[:, None, :, None]  # causal: of row i
+    count = (seen - torch.arange(d) + d - 1) // d
+    # the numerators, their sum and the weights of parts are whole numbers: 1 / sum, the product and the
+    # result's rounding are left
+    rtol = torch.finfo(dtype).eps / 2 + 8 * 2.0 ** -24
+    assert count.max() * rtol < 0.5  # a key more or less is at least twice the bound
+    out = tp.attention(*on(device, q, k), v.to(device), causal=True, lengths=lengths.to(device), scale=0.0)
+    want = (count / seen.clamp(min=1).double()).expand(3, h, n, d)
+    assert_close(out, want, rtol=rtol, atol=0.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,h,hk,m,d", [(1, 1, 1, 5000, 64), (1, 16, 2, 4098, 128), (1, 8, 1, 3002, 256), (4, 8, 2, 2050, 96),
+                                        (2, 16, 1, 9000, 128), (140, 8, 8, 2200, 128), (70, 4, 4, 300, 192),
+                                        (200, 64, 64, 400, 128)])
+def test_every_key_counts_once_in_the_gradients(device, dtype, n, h, hk, m, d):
+    """Equal weights, one-hot keys and values of 1 and -1 in turn: the scores' gradients are 1 / m and -1 / m, so
+    that feature f of dq is the number of keys j with j % d == f over m, with the sign of f.  dv of every key is
+    the number of rows that see it over m."""
+    q = torch.zeros(1, h, n, d, dtype=dtype)
+    k = torch.eye(d, dtype=dtype)[torch.arange(m) % d].expand(1, hk, m, d).contiguous()
+    sign = 1.0 - 2.0 * (torch.arange(m) % 2)
+    v, grad = torch.zeros(1, hk, m, 8, dtype=dtype), torch.zeros(1, h, n, 8, dtype=dtype)
+    v[..., 0], grad[..., 0] = sign.to(dtype), 1.0
+    leaves = [x.requires_grad_() for x in on(device, q, k, v)]
+    out = tp.attention(*leaves, scale=1.0)
+    assert not out.any()
+    dq, dk, dv = torch.autograd.grad(out, leaves, *on(device, grad))
+    count = (m - torch.arange(d) + d - 1) // d
+    # 1 / m, its rounding for the products (the gradients' type), sums of equal terms, the result's rounding
+    eps = torch.finfo(dtype).eps / 2
+    rtol = 2 * eps + (int(count.max()) + 8) * 2.0 ** -24
+    assert count.max() * rtol < 1  # a key more or less is beyond the bound
+    assert_close(dq, (count * sign[:d] / m).expand(1, h, n, d), rtol=rtol, atol=0.0, what="dq")
+    assert not dk.any()
+    rows_of_key = h // hk * n
+    rtol = 2 * eps + (rows_of_key + 8) * 2.0 ** -24
+    want = torch.zeros(1, hk, m, 8, dtype=torch.float64)
+    want[..., 0] = rows_of_key / m
+    assert_close(dv, want, rtol=rtol, atol=0.0, what="dv")
+    if dtype == F32 or rows_of_key <= 100:
+        assert rows_of_key * rtol < 1  # a row more or less is beyond the bound
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,h,hk,n,m,d,dv", [(BF16, 8, 8, 140, 2200, 128, 128), (BF16, 8, 4, 140, 3000, 128, 128),
                                                  (F32, 16, 4, 130, 2500, 64, 64), (F32, 16, 4, 133, 2500, 64, 62),
