@@ -781,8 +781,11 @@ int tpw_knn_mask_euclidean(const void *x1, const void *x2, int dtype, int64_t n,
  *   - j < lengths[b] (clamped to 0 .. m; null: m); later keys and values are not read,
  *   - causal: j - i <= length - n (the last query sees every key),
  *   - TPW_MASK_KEEP: whose mask byte is not 0; TPW_MASK_ADD_*: whose added value is not -inf.
- * A key that a mask leaves out has no weight in the row, whatever its score; its value row must be
- * finite all the same (0 * inf is NaN in the products).
+ * In the forward a key that a mask or the causal limit leaves out has no weight in the row, whatever its
+ * score (NaN too); its value row must be finite all the same (0 * inf is NaN in the products).  In the
+ * backward every row before the lengths must be finite, keys and values that are left out and queries (and
+ * grad_out) that see nothing among them: their score gradient of 0 is multiplied with them.  Rows at or
+ * past a length are not read in either.
  * Element strides are of [batch, heads, rows], features dense; the mask's are of [batch, heads,
  * n, m] (0 where it is broadcast).  key and value (in the backward query and grad_out too) need a
  * row stride of at least their width and at most 8 MiB.  stats [2, batch, heads, n] (fp32) carries

@@ -154,6 +154,19 @@ def test_keys_that_a_mask_leaves_out_may_score_nan(device, dtype, additive):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_keys_behind_the_causal_limit_may_score_nan(device, dtype):
+    n, d = 150, 64
+    q, k, v = rows(1, 2, n, d, 1, dtype), rows(1, 2, n, d, 2, dtype), rows(1, 2, n, d, 3, dtype)
+    want = reference(q, k, v, causal=True)
+    k = k.clone()
+    k[:, :, 70], k[:, :, 140] = math.inf, math.nan
+    out = tp.attention(*on(device, q, k, v), causal=True).cpu()
+    assert_close(out[:, :, :70], want["out"][:, :, :70], rtol=0.0, atol=want["tol_out"][:, :, :70])
+    assert out[:, :, 140:].isnan().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_nan_and_infinite_scores_stay_in_their_row(device):
     q, k, v = rows(1, 1, 40, 64, 1), rows(1, 1, 70, 64, 2), rows(1, 1, 70, 64, 3)
     want = reference(q, k, v)

@@ -516,7 +516,9 @@ struct Tiles {
     static constexpr int kWaves = kRowBytes == 1024 ? 8 : 4;
     static constexpr int kKeys = kRowBytes <= 256 ? 64 : 32;
     static constexpr int kRowWaves = 4, kRows = 32;          // dk / dv kernel
-    // blocks that share a CU (waves per SIMD, for the compiler): forward, dq, dk / dv
+    // blocks that share a CU, as parts_for takes them: forward, dq, dk / dv.  What the registers and the LDS
+    // of the kernels without added values leave (dk / dv of fp32 up to 64 features: three; of the two launches
+    // for bf16 at 256 features: dk's one).
     static constexpr bool kNarrow = kRowBytes == 128;  // bf16 up to 64 features
     static constexpr int kPerCu = kNarrow ? 4 : kWaves == 8 ? 1 : 2;
     static constexpr int kPerCuQ = kNarrow ? 3 : kWaves == 8 || DP == 256 ? 1 : 2;

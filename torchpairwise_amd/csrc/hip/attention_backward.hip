@@ -6,9 +6,11 @@
 //   dq_i = scale sum_j ds_ij k_j                    attention_dq_kernel: a wave owns query rows
 //   dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij do_i   attention_dkv_kernel: a wave owns keys
 // Seven products where five would do with dq summed in memory: the two scores' products are formed
-// in both kernels.  On the fp32 matrix cores two products of wide rows cost more than writing and
-// reading ds: there (see keeps_ds) the kernel that owns keys keeps ds in the workspace, for as many heads
-// at a time as 1 GiB holds, and dk and dq are one product each (attention_ds_product_kernel).
+// in both kernels (eight for bf16 rows of more than 128 features, whose dk and dv are a launch each: the
+// scores of q and k once more).  On the fp32 matrix cores two products of wide rows cost more than writing
+// and reading ds: there (see keeps_ds) the kernel that owns keys keeps ds in the workspace, for as many
+// heads at a time as 1 GiB holds, and dk and dq are one product each (attention_ds_product_kernel), five
+// in all.
 #include <math.h>
 
 #include "attention.hpp"
@@ -36,7 +38,10 @@ constexpr int kUnit = 32;  // rows (keys) of the streamed operand that are worke
 // dq: the forward's structure with a second product of scores (v, do) and one of keys.  It also leaves
 // base, 1 / sum and delta of every row for the kernel below.  bf16 2 x 16 (4) x 8192^2 x 128: 1.45 to 1.55
 // ms (1.06 to 1.14 PFLOP/s over three products); at 256 features one wave per SIMD holds q, do and dq, and
-// softmax and products alternate (8 x 8192^2: 0.98 to 1.15 ms, 720 to 840 TFLOP/s).
+// softmax and products alternate (8 x 8192^2: 0.98 to 1.15 ms, 720 to 840 TFLOP/s); at 192 two waves hold
+// them but for 54 to 74 spilled registers (8 x 8192^2: 0.78 ms, 790 TFLOP/s).  fp32 forms it at 8 x 4096^2 x
+// 64 in 0.43 ms (120 TFLOP/s).  Added values are loaded behind the scores' products (16 x 4096^2 x 128 bf16
+// with values per head: 0.37 ms, 1 GiB of them).
 template <typename T, int W, int DP, int BN, int MM, int kWaves, int OCC>
 __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Args a) {
     using M = Mma<T, W>;
@@ -249,10 +254,14 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dq_kernel(const Ar
 }
 
 // dk, dv (or one of them, or dv with ds kept): a wave owns 32 keys (fp32: 16), streams q and do, and needs
-// 2 DP accumulators a lane beside its keys and values.  To stay at two waves per SIMD, 128 features read
-// the block's values from LDS (VLDS: 2.0 ms where spilled registers took 2.9), and bf16 at more takes dk and
-// dv in a launch each.  bf16 2 x 16 (4) x 8192^2 x 128: 2.04 to 2.3 ms (0.95 to 1.08 PFLOP/s over four
-// products); 8 x 8192^2 x 256: dv 0.53, dk 1.36 to 1.5 (one wave per SIMD).
+// 2 DP accumulators a lane beside its keys and values.  To stay at two waves per SIMD, bf16 at 65 to 128
+// features reads the block's values from LDS (VLDS: 2.0 ms where spilled registers took 2.9), and at more
+// takes dk and dv in a launch each; dk at 192 spills 38 to 59 registers all the same, and with added values
+// 128 features spill 14 and dv at 256 24.  fp32 at 96 and 128 reads its values from LDS too, at one wave per
+// SIMD.  bf16 2 x 16 (4) x 8192^2 x 128: 2.04 to 2.3 ms (0.95 to 1.08 PFLOP/s over four products); 8 x 8192^2
+// x 192: dv 0.46, dk 0.88; x 256: dv 0.53, dk 1.36 to 1.5 (one wave per SIMD).  fp32 8 x 4096^2 x 64: 0.59 ms
+// (117 TFLOP/s over four), 2 x 4096^2 x 128 0.34 (102).  Added values come one by one behind the scores'
+// products: 16 x 4096^2 x 128 bf16 with values per head 0.64 ms.
 template <typename T, int W, int DP, int BM, int MM, int kWaves, int OCC, bool VLDS, int OUT>
 __global__ __launch_bounds__(64 * kWaves, OCC) void attention_dkv_kernel(const Args a) {
     using M = Mma<T, W>;
@@ -709,6 +718,8 @@ BackwardPlan backward_plan(const Args &a) {
     p.q_splits = (int)parts_for(bk * p.q_tiles, cdiv(a.m, L::kKeys), L::kPerCuQ, uneven(a),
                                 step_us<T, DP>((int64_t)L::kWaves * L::kWidth, L::kKeys, 3, L::kPerCuQ),
                                 part_us(a.batch * a.heads * a.n, quads4(a.d)));
+    // four products: what one launch for dk and dv has.  Of a launch each (wide bf16 rows) dk has three and
+    // dv two; the parts were not measured with those.
     p.k_splits = (int)parts_for(bk * p.k_tiles, a.group * cdiv(a.n, L::kRows), L::kPerCuK, uneven(a),
                                 step_us<T, DP>((int64_t)L::kRowWaves * L::kWidth, L::kRows, 4, L::kPerCuK),
                                 part_us(bk * a.m, quads4(a.d) + quads4(a.dv)));
@@ -806,8 +817,8 @@ extern "C" int tpw_attention_backward(const tpw_attention_desc *d, void *workspa
             a.tiles = p.k_tiles;
             a.splits = p.k_splits;
             const dim3 grid((unsigned)(bk * a.tiles * a.splits)), block(64 * Tiles<T, DP>::kRowWaves);
-            // bf16 at 256 features: dk and dv would take all 256 accumulation registers and leave none for
-            // the scores, so each is a launch of its own
+            // bf16 at more than 128 features: dk and dv together would take 192 or all 256 accumulation
+            // registers and leave too few for the scores, so each is a launch of its own
             constexpr bool kApart = sizeof(T) == 2 && DP > 128;
             constexpr int kRows = Tiles<T, DP>::kRows, kWaves = Tiles<T, DP>::kRowWaves;
             if constexpr (kApart) {

@@ -122,11 +122,6 @@ at::Tensor additive_mask(const Operands &o, bool causal, at::ScalarType t) {
     return add;
 }
 
-struct Scores {
-    at::Tensor p, q, k, v;  // probabilities' numerators or probabilities; operands, grouped by key head
-    at::Tensor top, sum;    // [batch, heads, n]
-};
-
 // Rows of the heads that share a key head are rows of one product.
 at::Tensor grouped(const at::Tensor &x, const Operands &o, at::ScalarType t) {
     return x.to(t).reshape({o.batch, o.key_heads, o.heads / o.key_heads * o.n, x.size(3)});
