@@ -553,7 +553,7 @@ def test_every_key_counts_once(device, dtype, n, h, hk, m, d):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n,h,hk,m,d", [(1, 1, 1, 5000, 64), (1, 16, 2, 4098, 128), (1, 8, 1, 3002, 256), (4, 8, 2, 2050, 96),
                                         (2, 16, 1, 9000, 128), (140, 8, 8, 2200, 128), (70, 4, 4, 300, 192),
-                                        (200, 64, 64, 400, 128)])
+                                        (300, 64, 64, 400, 128)])
 def test_every_key_counts_once_in_the_gradients(device, dtype, n, h, hk, m, d):
     """Equal weights, one-hot keys and values of 1 and -1 in turn: the scores' gradients are 1 / m and -1 / m, so
     that feature f of dq is the number of keys j with j % d == f over m, with the sign of f.  dv of every key is
@@ -868,3 +868,14 @@ def test_frequencies_held_as_a_parameter(device):
     for y in (x, leaf):
         with pytest.raises(RuntimeError, match="frequencies have no gradient"):
             tp.rotary_embedding(y, pos, held)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("enabled", [True, False])
+def test_rotary_refuses_tangents(device, enabled):
+    x, f = randn(2, 3, 5, 16, seed=1).to(device), torch.rand(8, dtype=torch.float64, generator=gen(2)).to(device)
+    pos = torch.arange(5, device=device)
+    with forward_ad.dual_level(), torch.set_grad_enabled(enabled):
+        for args in ((forward_ad.make_dual(x, x), pos, f), (x, pos, forward_ad.make_dual(f, f))):
+            with pytest.raises(RuntimeError):
+                tp.rotary_embedding(*args)
