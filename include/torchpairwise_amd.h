@@ -822,6 +822,45 @@ int tpw_attention(const tpw_attention_desc *desc, void *workspace, void *stream)
 size_t tpw_attention_backward_workspace_size(const tpw_attention_desc *desc);
 int tpw_attention_backward(const tpw_attention_desc *desc, void *workspace, void *stream);
 
+/* ---- a cache of keys and values in 4 or 8 bits ------------------------------------------
+ * Blocks of 32 features of a row share a power of two 2^e, kept as the byte e + 127 (255: the block is
+ * NaN), and hold codes v: x = v 2^e.  4 bits: sign, two exponent bits, one mantissa bit (0 .5 1 1.5 2 3 4 6),
+ * two features a byte, the even one in the low half; 8 bits: sign, 4, 3 (float8 e4m3, largest 448).  Writing
+ * takes the first e >= -127 with max |x| < 7 2^e (464 2^e), then rounds x / 2^e to nearest, ties to even;
+ * a block that holds NaN or an infinity becomes NaN.
+ * codes [first, heads, rows, blocks] of 16 (32) bytes, the bytes of a row dense; scales [first, heads, blocks,
+ * rows], rows dense.  Strides are in bytes, of [first, heads, rows] and [first, heads, blocks]; they and the
+ * addresses are multiples of 16, and so is rows.  Without a table of pages first is the batch and rows what
+ * each sequence has room for; with one (int32, or int64 where pages_wide), row j of sequence b is row j % rows
+ * of page pages[b * page_pitch + j / rows], rows being a power of two.  Entries outside [0, first) stand for no
+ * page: their rows are not written, read as zeros, and are no keys. */
+typedef struct tpw_cache_desc {
+    int32_t bits; /* 4 or 8 */
+    int32_t pages_wide;
+    int64_t first, heads, rows;
+    int64_t key_blocks, value_blocks; /* 1 to 8 */
+    void *key_codes, *key_scales, *value_codes, *value_scales;
+    int64_t key_code_strides[3], key_scale_strides[3], value_code_strides[3], value_scale_strides[3];
+    const void *pages; /* [batch, page_count], or null */
+    int64_t page_pitch, page_count;
+} tpw_cache_desc;
+
+/* Rows i < counts[b] (null: n) of key [batch, heads, n, width] and value [.., value_width] (float32 or
+ * bfloat16, element strides of [batch, heads, n], features dense) to rows starts[b] + i (null: i) of sequence
+ * b; rows outside the cache are dropped.  The other rows stay as they are. */
+int tpw_cache_write(const tpw_cache_desc *desc, int dtype, int64_t batch, int64_t n, const void *key, int64_t width,
+                    const int64_t *key_strides, const void *value, int64_t value_width, const int64_t *value_strides,
+                    const int64_t *starts, const int64_t *counts, void *stream);
+/* The same rows out of the cache; those past the counts or outside the cache are zeros. */
+int tpw_cache_read(const tpw_cache_desc *desc, int dtype, int64_t batch, int64_t n, void *key, int64_t width,
+                   const int64_t *key_strides, void *value, int64_t value_width, const int64_t *value_strides,
+                   const int64_t *starts, const int64_t *counts, void *stream);
+/* tpw_attention's forward with the cache in the place of key and value (their pointers and strides are not
+ * read): key_heads is the cache's heads, m the rows that a sequence has room for, d at most 32 key_blocks, dv
+ * at most 32 value_blocks.  out_rest and stats must be null. */
+size_t tpw_cache_attention_workspace_size(const tpw_attention_desc *desc, const tpw_cache_desc *cache);
+int tpw_cache_attention(const tpw_attention_desc *desc, const tpw_cache_desc *cache, void *workspace, void *stream);
+
 /* ---- rotary positions -----------------------------------------------------------------
  * Turns the first 2 * pairs features of every row of x [batch, heads, n, d] (float32 or bfloat16)
  * by the angles t = position * frequencies[pair] (positions [batch, n] int64 with strides in

@@ -37,7 +37,20 @@ class AttentionDesc(C.Structure):
                 ("mask_strides", _i64 * 4)]
 
 
+class CacheDesc(C.Structure):
+    """``tpw_cache_desc``."""
+    _fields_ = [("bits", C.c_int32), ("pages_wide", C.c_int32),
+                *[(f, _i64) for f in ("first", "heads", "rows", "key_blocks", "value_blocks")],
+                *[(f, _p) for f in ("key_codes", "key_scales", "value_codes", "value_scales")],
+                *[(f + "_strides", _i64 * 3) for f in ("key_code", "key_scale", "value_code", "value_scale")],
+                ("pages", _p), ("page_pitch", _i64), ("page_count", _i64)]
+
+
 _SIGNATURES = {
+    "tpw_cache_write": (_i, [_p, _i, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _p]),
+    "tpw_cache_read": (_i, [_p, _i, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _p]),
+    "tpw_cache_attention_workspace_size": (_sz, [_p, _p]),
+    "tpw_cache_attention": (_i, [_p, _p, _p, _p]),
     "tpw_attention_workspace_size": (_sz, [_p]),
     "tpw_attention": (_i, [_p, _p, _p]),
     "tpw_attention_backward_workspace_size": (_sz, [_p]),

@@ -2,169 +2,10 @@
 // with the running maximum and sum of every row (layouts: attention.hpp).
 #include <math.h>
 
-#include "attention.hpp"
+#include "attention_forward.hpp"
 
 namespace tpw {
 namespace attn {
-
-// Per-row running softmax of one wave's W rows and the loop over one key tile.
-template <typename T, int W, int DP, int BN, int MM, bool DWORDS>
-struct Forward {
-    using M = Mma<T, W>;
-    using Acc = typename M::Acc;
-    using CR = ColReader<T, DP, W>;
-    static constexpr int NB = BN / W, NQ = NB * M::Q, DB = DP / W, QS = DP / M::KS;
-
-    Frag<T> q[QS];
-    Acc o[DB];
-    float top, sum;  // running maximum (in units of log2 e; kBias: natural) and the lane's part of the sum
-    int lim, wlim_min, wlim_max;  // keys seen: this lane's row, over the wave's rows
-    int64_t qh, qi;               // head and row (row -1: none)
-
-    __device__ __forceinline__ void init(const Args &a, int64_t b, int64_t kh, int64_t row0, int64_t len, int lane) {
-        const int64_t r = row0 + lane % W, rows = a.n * a.group;
-        const bool live = r < rows;
-        qh = kh * a.group + (live ? r / a.n : 0);
-        qi = live ? r % a.n : -1;
-        const int64_t l = live ? row_limit(a, len, qi) : 0;
-        lim = (int)l;
-        wlim_max = lim;
-        wlim_min = live ? lim : 0x7fffffff;
-#pragma unroll
-        for (int s = 1; s < W; s <<= 1) {
-            const int x = __shfl_xor(wlim_max, s, 64), y = __shfl_xor(wlim_min, s, 64);
-            wlim_max = wlim_max > x ? wlim_max : x;
-            wlim_min = wlim_min < y ? wlim_min : y;
-        }
-        wlim_max = __builtin_amdgcn_readfirstlane(wlim_max);
-        wlim_min = __builtin_amdgcn_readfirstlane(wlim_min);
-        const T *row = live ? reinterpret_cast<const T *>(a.q.p) + b * a.q.b + qh * a.q.h + qi * a.q.n : nullptr;
-#pragma unroll
-        for (int s = 0; s < QS; ++s) {
-            q[s] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d, DWORDS);
-            if (a.qsign != 1.0f) {
-                float x[8];
-                unpack8(q[s], x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] *= a.qsign;
-                q[s] = pack8(x, T{});
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < DB; ++i) o[i] = Acc{};
-        top = -INFINITY;
-        sum = 0.0f;
-    }
-
-    // keys j0 .. j0 + BN - 1 in LDS at kt (keys) and vt (values)
-    __device__ __forceinline__ void tile(const Args &a, int64_t b, uint32_t kt, uint32_t vt, int j0, int lane) {
-        if (j0 >= wlim_max) return;
-        const int g = lane / W;
-        const RowReader<T, DP, W> rr(lane);
-        const CR cr(lane);
-        // added values: where registers allow, loaded ahead of the scores' products
-        constexpr bool kAhead = MM == kBias && DP <= 128;
-        f32x4 add[MM == kBias ? NQ : 1];
-        if constexpr (kAhead) mask_bias<NQ, 4 * M::NG>(a, mask_row(a, b, qh, qi < 0 ? 0 : qi), j0, 4 * g, BN, add);
-        Acc s[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) s[i] = Acc{};
-#pragma unroll
-        for (int k = 0; k < QS; ++k) {
-            if constexpr (sizeof(T) == 4) {  // independent products side by side
-                Frag<T> f[NB];
-#pragma unroll
-                for (int i = 0; i < NB; ++i) f[i] = rr.read(kt, i, k);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) M::mma1(s[i], f[i], q[k], e);
-            } else {
-#pragma unroll
-                for (int i = 0; i < NB; ++i) M::mma(s[i], rr.read(kt, i, k), q[k]);
-            }
-        }
-
-        if constexpr (MM == kBias) {
-            if constexpr (!kAhead) mask_bias<NQ, 4 * M::NG>(a, mask_row(a, b, qh, qi < 0 ? 0 : qi), j0, 4 * g, BN, add);
-#pragma unroll
-            for (int x = 0; x < NQ; ++x)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float y = s[x / M::Q][4 * (x % M::Q) + e] * a.scale + add[x][e];
-                    s[x / M::Q][4 * (x % M::Q) + e] = add[x][e] == -INFINITY ? -INFINITY : y;
-                }
-        }
-        if constexpr (MM == kKeep) {
-            const uint32_t *mr = mask_words(a, b, qh, qi) + j0 / 32;
-#pragma unroll
-            for (int u = 0; u < BN / 32; ++u) {
-                const uint32_t keep = j0 + 32 * u < lim ? mr[u] >> (4 * g) : 0;
-#pragma unroll
-                for (int x = 0; x < 32 / (4 * M::NG); ++x)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int at = 32 * u + 4 * M::NG * x;  // of the tile's keys
-                        if (!(keep & (1u << (4 * M::NG * x + e)))) s[at / W][4 * (at % W / (4 * M::NG)) + e] = -INFINITY;
-                    }
-            }
-        }
-        if (j0 + BN > wlim_min) {
-            asm volatile("");  // a branch: most tiles skip this
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int w = 0; w < M::Q; ++w)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j0 + W * i + 4 * M::NG * w + 4 * g + e >= lim) s[i][4 * w + e] = -INFINITY;
-        }
-
-        float mx = s[0][0];
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int e = 0; e < 4 * M::Q; ++e) mx = __builtin_fmaxf(mx, s[i][e]);
-        mx = over_groups_max<W>(mx);
-        if constexpr (MM != kBias) mx *= a.scale;
-        const float top1 = __builtin_fmaxf(top, mx);
-        // a row with no key so far: exp2(-inf - 0) = 0 throughout
-        const float base = top1 == -INFINITY ? 0.0f : top1;
-        if (__any(top1 > top)) {
-            const float f = __builtin_amdgcn_exp2f(MM == kBias ? (top - base) * kLog2e : top - base);
-            sum *= f;
-#pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int e = 0; e < 4 * M::Q; ++e) o[i][e] *= f;
-        }
-        top = top1;
-        float part = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int e = 0; e < 4 * M::Q; ++e) {
-                const float x = MM == kBias ? __builtin_amdgcn_exp2f((s[i][e] - base) * kLog2e)
-                                            : __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], a.scale, -base));
-                s[i][e] = x;
-                part += x;
-            }
-        sum += part;
-        // The probabilities of bf16 inputs are rounded to bf16 for the matrix cores (within 2^-8 of
-        // each, as the values are); their sum is not.
-#pragma unroll
-        for (int t = 0; t < BN / M::KS; ++t) {
-            float x[8];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * u + e] = s[(2 * t + u) / M::Q][4 * ((2 * t + u) % M::Q) + e];
-            const Frag<T> p = pack8(x, T{});
-#pragma unroll
-            for (int c = 0; c < CR::kPieces; ++c) CR::use(o, c, cr.read(vt, t, c), p);
-        }
-    }
-};
 
 // One block: kWaves * W query rows of the rows that share a key head, over the keys of one part.  The
 // next tile of keys and values travels by DMA while this one is worked on, one barrier a tile.
@@ -403,7 +244,7 @@ size_t plan_padding(Args &a, int dtype, bool backward, uint8_t *at, PadArgs *p) 
     size_t bytes = 0;
     if (a.dwords) return 0;
     const auto take = [&](View &v, int64_t heads, int64_t rows, int64_t width, bool always = false) {
-        if ((!always && whole_pieces(v, width, size)) || a.batch * heads * rows == 0) return;
+        if (!v.p || (!always && whole_pieces(v, width, size)) || a.batch * heads * rows == 0) return;
         const int64_t pieces = cdiv(width, e), n = a.batch * heads * rows * pieces;
         if (p) {
             const int t = p->count++;
@@ -485,17 +326,6 @@ int64_t plan_bits(Args &a, bool backward, uint8_t *at, BitArgs *p) {
     return rows + (backward ? round_up(lead * steps * a.m * 4, 16) : 0);
 }
 
-// Sets tiles and splits for the element type and width.
-template <typename T, int DP>
-void plan(Args &a) {
-    using L = Tiles<T, DP>;
-    constexpr int64_t kOwn = L::kWaves * L::kWidth;
-    a.tiles = cdiv(a.n * a.group, kOwn);
-    a.splits = (int)parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, L::kKeys), L::kPerCu, uneven(a),
-                              step_us<T, DP>(kOwn, L::kKeys, 2, L::kPerCu),
-                              part_us(a.batch * a.heads * a.n, quads4(a.dv)));
-}
-
 }  // namespace
 
 size_t prepared_bytes(const Args &a, const tpw_attention_desc *d, bool backward) {
@@ -533,6 +363,31 @@ int prepare_operands(Args &a, const tpw_attention_desc *d, bool backward, void *
         return check_launch("pack_mask_kernel");
     }
     return TPW_OK;
+}
+
+int join_parts(const Args &a, int dtype, bool bias, hipStream_t s) {
+    const int64_t rows = a.batch * a.heads * a.n, quads = rows * cdiv(a.dv, 4), width = a.d > a.dv ? a.d : a.dv;
+    const dim3 few((unsigned)cdiv(quads, 256)), one((unsigned)rows);
+    const auto by_lanes = [&](auto t, auto biased, auto lanes) {
+        using T = decltype(t);
+        constexpr bool BIAS = decltype(biased)::value;
+        if (a.splits <= 8)
+            hipLaunchKernelGGL((attention_join_few_kernel<T, BIAS, 8>), few, dim3(256), 0, s, a);
+        else if (a.splits <= 16 && quads >= kManyQuads)
+            hipLaunchKernelGGL((attention_join_few_kernel<T, BIAS, 16>), few, dim3(256), 0, s, a);
+        else if (a.splits <= 32 && quads >= kManyQuads)
+            hipLaunchKernelGGL((attention_join_few_kernel<T, BIAS, 32>), few, dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL((attention_join_kernel<T, BIAS, decltype(lanes)::value>), one, dim3(256), 0, s, a);
+        return check_launch("attention_join_kernel");
+    };
+    const auto by_bias = [&](auto t, auto biased) {
+        if (width <= 64) return by_lanes(t, biased, Const<16>{});
+        if (width <= 128) return by_lanes(t, biased, Const<32>{});
+        return by_lanes(t, biased, Const<64>{});
+    };
+    const auto by_rows = [&](auto t) { return bias ? by_bias(t, Const<1>{}) : by_bias(t, Const<0>{}); };
+    return dtype == TPW_BF16 ? by_rows(uint16_t{}) : by_rows(float{});
 }
 
 int read_args(const tpw_attention_desc *d, bool backward, Args &a) {
@@ -649,20 +504,7 @@ extern "C" int tpw_attention(const tpw_attention_desc *d, void *workspace, void 
             hipLaunchKernelGGL((attention_kernel<T, W, DP, kKeys, MM, false, kWaves, kOcc>), dim3((unsigned)blocks),
                                dim3(64 * kWaves), 0, s, a);
         if (const int rc = check_launch("attention_kernel")) return rc;
-        if (a.splits > 1) {
-            const int64_t quads = rows * cdiv(a.dv, 4);
-            const dim3 few((unsigned)cdiv(quads, 256));
-            if (a.splits <= 8)
-                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias, 8>), few, dim3(256), 0, s, a);
-            else if (a.splits <= 16 && quads >= kManyQuads)
-                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias, 16>), few, dim3(256), 0, s, a);
-            else if (a.splits <= 32 && quads >= kManyQuads)
-                hipLaunchKernelGGL((attention_join_few_kernel<T, MM == kBias, 32>), few, dim3(256), 0, s, a);
-            else
-                hipLaunchKernelGGL((attention_join_kernel<T, MM == kBias, Tile<T, DP>::P / 4>), dim3((unsigned)rows),
-                                   dim3(256), 0, s, a);
-            return check_launch("attention_join_kernel");
-        }
+        if (a.splits > 1) return join_parts(a, d->dtype, MM == kBias, s);
         return TPW_OK;
     });
 }

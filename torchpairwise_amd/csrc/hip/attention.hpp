@@ -53,6 +53,7 @@ struct Args {
     float qsign;   // -1, 0 or 1: the sign of scale, folded into q as it is loaded
     float gscale;  // scale (backward)
     int causal;
+    int whole_q;    // (few rows over a cache) queries are whole pieces of 8 features
     int dwords;     // (forward) operands of whole dwords that are not whole pieces, read as they lie
     int64_t tiles;  // row tiles (dk / dv: key tiles) per (batch, key head)
     int splits;     // parts of the summed axis
@@ -531,6 +532,8 @@ struct Tiles {
 int read_args(const tpw_attention_desc *d, bool backward, Args &a);
 size_t prepared_bytes(const Args &a, const tpw_attention_desc *d, bool backward);
 int prepare_operands(Args &a, const tpw_attention_desc *d, bool backward, void *at, hipStream_t s);
+// Joins a.splits parts of every row into a.o (and a.stats).
+int join_parts(const Args &a, int dtype, bool bias, hipStream_t s);
 
 // Runs f(type tag, DP, mask mode) for the arguments' types and widths.
 template <int V>

@@ -1,0 +1,105 @@
+// Shared pieces of the kernels over a cache of keys and values in 4 or 8 bits (cache.hip, cache_rows.hpp,
+// cache_tiles.hpp).
+//
+// A block of 32 features of a row shares a power of two, the first with which the block's largest
+// magnitude a does not round past the last code:
+//   4 bits: sign, 2 exponent and 1 mantissa bit, 0 .5 1 1.5 2 3 4 6;  a < 7 2^e  (7 would round to 8)
+//   8 bits: sign, 4 and 3, largest 448;  a < 464 2^e
+// so every value is off by at most half a step of its own binade.  x / 2^e is exact, its rounding (to
+// nearest, ties to even) the only one: the codes are the same on every machine.  The scale is kept as the
+// byte e + 127, whose place in a float's bits is its exponent: gfx950's conversions (v_cvt_scalef32_*) take
+// that float, read 0 as 2^-127 and 255 as NaN, whatever the code.  A block that holds NaN or an infinity
+// has scale 255 and codes of zero.
+// Every value is exact in bfloat16 (2 or 4 significant bits).
+//
+// Codes: [batch | pages, heads, rows, blocks] of 16 bytes (two features a byte, the even one low) or 32.
+// Scales: [batch | pages, heads, blocks, rows], rows dense: eight bytes are eight keys' scales of a block.
+// Rows come in multiples of 16, so that no read of 8 whole rows leaves the cache.
+#pragma once
+
+#include "common.hpp"
+
+namespace tpw {
+namespace cache {
+
+struct Side {  // the keys or the values; strides in bytes
+    uint8_t *codes, *scales;
+    int64_t cf, ch, cr;  // codes: first dimension, heads, rows
+    int64_t sf, sh, sb;  // scales: first dimension, heads, blocks
+    int blocks;
+};
+
+struct Cache {
+    Side k, v;
+    const void *pages;  // table [batch, pages of a sequence] (dense in the second), or null
+    int64_t pitch;      // its entries between sequences
+    int64_t first;      // pages there are (without a table: sequences)
+    int wide;           // its entries are 64-bit
+    int shift, mask;    // rows of a page: 1 << shift, and less one (without a table: 31, all ones)
+};
+
+// Where row j of sequence b lies: entry of the first dimension (-1: nowhere) and row.
+struct Place {
+    int64_t first;
+    int row;
+};
+__device__ __forceinline__ Place place(const Cache &c, int64_t b, int j) {
+    if (!c.pages) return {b, j};
+    const int64_t at = b * c.pitch + (j >> c.shift);
+    const int64_t p = c.wide ? reinterpret_cast<const int64_t *>(c.pages)[at]
+                             : (int64_t) reinterpret_cast<const int32_t *>(c.pages)[at];
+    return {p >= 0 && p < c.first ? p : -1, j & c.mask};
+}
+
+// The float that the conversions take for scale byte `b`.
+__device__ __forceinline__ float scale_of(uint32_t b) { return __uint_as_float(b << 23); }
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef short s2 __attribute__((ext_vector_type(2)));
+
+// Two values of four codes' word: 4 bits: features 2 C, 2 C + 1 of eight; 8 bits: of four.
+template <int BITS, int C>
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t w, float scale) {
+    if constexpr (BITS == 4)
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, C));
+    else
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, C != 0));
+}
+template <int BITS, int C>
+__device__ __forceinline__ f2 f32_pair(uint32_t w, float scale) {
+    if constexpr (BITS == 4)
+        return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, C);
+    else
+        return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, C != 0);
+}
+// Eight consecutive features: one word of 4-bit codes, two of 8-bit ones.
+template <int BITS>
+struct Eight {
+    uint32_t w[BITS / 4];
+    __device__ __forceinline__ uint4 bf16(float s) const {
+        if constexpr (BITS == 4)
+            return make_uint4(bf16_pair<4, 0>(w[0], s), bf16_pair<4, 1>(w[0], s), bf16_pair<4, 2>(w[0], s),
+                              bf16_pair<4, 3>(w[0], s));
+        else
+            return make_uint4(bf16_pair<8, 0>(w[0], s), bf16_pair<8, 1>(w[0], s), bf16_pair<8, 0>(w[1], s),
+                              bf16_pair<8, 1>(w[1], s));
+    }
+    __device__ __forceinline__ void f32(float s, float (&x)[8]) const {
+        f2 y[4];
+        if constexpr (BITS == 4) {
+            y[0] = f32_pair<4, 0>(w[0], s), y[1] = f32_pair<4, 1>(w[0], s);
+            y[2] = f32_pair<4, 2>(w[0], s), y[3] = f32_pair<4, 3>(w[0], s);
+        } else {
+            y[0] = f32_pair<8, 0>(w[0], s), y[1] = f32_pair<8, 1>(w[0], s);
+            y[2] = f32_pair<8, 0>(w[1], s), y[3] = f32_pair<8, 1>(w[1], s);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = y[i / 2][i % 2];
+    }
+};
+
+// Host side (cache.hip): checks a cache against its batch and reads it into the kernels' form.
+int read_cache(const tpw_cache_desc *d, int64_t batch, Cache &c);
+
+}  // namespace cache
+}  // namespace tpw

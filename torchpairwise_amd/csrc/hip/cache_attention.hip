@@ -1,0 +1,99 @@
+// Attention over a cache in 4 or 8 bits: entry points and the choice of the form.
+#include "attention_forward.hpp"
+#include "cache_attention.hpp"
+
+namespace tpw {
+namespace attn {
+namespace {
+
+// Reads both descriptors.  The arguments' keys and values have no address: the cache has them.
+int read_call(const tpw_attention_desc *d, const tpw_cache_desc *cd, tpw_attention_desc &own, Args &a, cache::Cache &c) {
+    TPW_REQUIRE(d && cd, "null descriptor");
+    own = *d;
+    TPW_REQUIRE(!d->stats && !d->out_rest, "attention over a cache has no backward: stats and out_rest must be null");
+    own.key = own.value = nullptr;
+    const int64_t none[3] = {0, 0, 256};
+    for (int i = 0; i < 3; ++i) own.key_strides[i] = own.value_strides[i] = none[i];
+    if (const int rc = read_args(&own, false, a)) return rc;
+    if (const int rc = cache::read_cache(cd, d->batch, c)) return rc;
+    TPW_REQUIRE(d->key_heads == cd->heads, "attention: key_heads differ from the cache's heads");
+    TPW_REQUIRE(d->m == (cd->pages ? cd->page_count * cd->rows : cd->rows), "attention: m differs from the cache's rows");
+    TPW_REQUIRE(d->d <= 32 * cd->key_blocks && d->dv <= 32 * cd->value_blocks, "attention: rows are wider than the cache's");
+    a.dwords = 0;
+    const int64_t size = d->dtype == TPW_F32 ? 4 : 2;
+    a.whole_q = a.d % 8 == 0 && aligned16(a.q.p) && (a.q.b | a.q.h | a.q.n) * size % 16 == 0;
+    if (cd->first == 0) a.m = 0;  // a table without pages
+    return TPW_OK;
+}
+
+// float32 rows of more than 128 features have no registers left for a second 16.
+bool few_rows(const Args &a, int dtype) {
+    return a.n * a.group <= (dtype == TPW_F32 && (a.d > 128 || a.dv > 128) ? 16 : kFewRows);
+}
+
+size_t parts_bytes(const Args &a) {
+    return a.splits > 1 ? (size_t)a.splits * a.batch * a.heads * a.n * (quads4(a.dv) + 2) * 4 : 0;
+}
+
+}  // namespace
+
+void plan_tiles(Args &a, int dtype) {
+    by_type(a, dtype, kNoMask, [&](auto t, auto dp, auto) {
+        plan<decltype(t), decltype(dp)::value>(a);
+        return TPW_OK;
+    });
+}
+
+}  // namespace attn
+}  // namespace tpw
+
+using namespace tpw;
+using namespace tpw::attn;
+
+extern "C" size_t tpw_cache_attention_workspace_size(const tpw_attention_desc *d, const tpw_cache_desc *cd) {
+    Args a = {};
+    cache::Cache c = {};
+    tpw_attention_desc own;
+    if (read_call(d, cd, own, a, c) != TPW_OK || a.batch * a.heads * a.n == 0) return 0;
+    if (few_rows(a, d->dtype)) {
+        plan_rows(a);
+        return parts_bytes(a);
+    }
+    plan_tiles(a, d->dtype);
+    return prepared_bytes(a, &own, false) + parts_bytes(a);
+}
+
+extern "C" int tpw_cache_attention(const tpw_attention_desc *d, const tpw_cache_desc *cd, void *workspace,
+                                   void *stream) {
+    Args a = {};
+    cache::Cache c = {};
+    tpw_attention_desc own;
+    if (const int rc = read_call(d, cd, own, a, c)) return rc;
+    if (a.batch * a.heads * a.n == 0) return TPW_OK;
+    TPW_REQUIRE(a.q.p && a.o.p, "attention: null operand");
+    const int mode = mask_mode(d);
+    TPW_REQUIRE(mode == kNoMask || a.mask, "attention: null mask");
+    hipStream_t s = as_stream(stream);
+    size_t prepared = 0;
+    const bool few = few_rows(a, d->dtype);
+    if (few) {
+        if (mode == kNoMask) a.mask = nullptr;
+        plan_rows(a);
+    } else {
+        plan_tiles(a, d->dtype);
+        prepared = prepared_bytes(a, &own, false);
+    }
+    TPW_REQUIRE(prepared + parts_bytes(a) == 0 || (workspace && aligned16(workspace)),
+                "attention: null or unaligned workspace");
+    if (prepared)
+        if (const int rc = prepare_operands(a, &own, false, workspace, s)) return rc;
+    if (a.splits > 1) {
+        a.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + prepared);
+        a.part_stats = a.part + a.splits * a.batch * a.heads * a.n * quads4(a.dv);
+    }
+    const int rc = few            ? cache_rows(a, c, cd->bits, d->dtype, mode == kBias, s)
+                   : cd->bits == 4 ? cache_tiles4(a, c, d->dtype, mode, s)
+                                   : cache_tiles8(a, c, d->dtype, mode, s);
+    if (rc || a.splits == 1) return rc;
+    return join_parts(a, d->dtype, mode == kBias, s);
+}

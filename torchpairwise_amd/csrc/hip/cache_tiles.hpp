@@ -1,0 +1,167 @@
+// Attention of many query rows a key head over a cache in 4 or 8 bits: the tiles of attention.hip's forward,
+// formed from the codes on their way into LDS.
+#pragma once
+
+#include "attention_forward.hpp"
+#include "cache_attention.hpp"
+
+namespace tpw {
+namespace attn {
+
+using cache::Cache;
+using cache::Eight;
+using cache::Side;
+
+// Brings tiles of BN keys and their values into LDS as the element type T.  A slot is a block of 32 features
+// of one row: threads of 64 (32) consecutive rows share a block, so that the 16-byte stores of 16 of them
+// fall on 16 different slots of the banks.  Codes wait in registers while the tile before is worked on.
+template <typename T, int DP, int BN, int WAVES, int BITS>
+struct Decoder {
+    using L = Tile<T, DP>;
+    static constexpr int kThreads = 64 * WAVES, kBlocks = L::P / 32, kSlots = 2 * BN * kBlocks / kThreads;
+    static_assert(2 * BN * kBlocks % kThreads == 0 && BN * kBlocks % 64 == 0, "whole waves of slots");
+    uint4 codes[kSlots][BITS / 4];
+    uint32_t scale[kSlots];
+    uint64_t present;  // keys of the tile that have a place (bits past the length are set too)
+
+    // Keys j0 .. j0 + BN - 1 of sequence b.  Rows at or past len, blocks past the row's and rows without a
+    // place become zeros and are not read.
+    __device__ __forceinline__ void load(const Cache &c, int64_t b, int64_t kh, int j0, int len, int tid) {
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+            const int id = i * kThreads + tid, r = id % BN, block = id / BN % kBlocks;
+            const bool values = id / (BN * kBlocks) != 0;
+            const Side &s = values ? c.v : c.k;
+            const int j = j0 + r;
+            const bool in = j < len && block < s.blocks;
+            cache::Place p = {-1, 0};
+            if (in) p = cache::place(c, b, j);
+            scale[i] = 0;
+#pragma unroll
+            for (int x = 0; x < BITS / 4; ++x) codes[i][x] = make_uint4(0, 0, 0, 0);
+            if (p.first >= 0) {
+                const uint4 *at = reinterpret_cast<const uint4 *>(s.codes + p.first * s.cf + kh * s.ch + p.row * s.cr +
+                                                                  block * (4 * BITS));
+#pragma unroll
+                for (int x = 0; x < BITS / 4; ++x) codes[i][x] = at[x];
+                scale[i] = s.scales[p.first * s.sf + kh * s.sh + block * s.sb + p.row];
+            }
+        }
+        present = ~uint64_t(0);
+        if (c.pages) {  // every wave for itself
+            const int j = j0 + (tid & 63);
+            present = __ballot(j >= len || cache::place(c, b, j).first >= 0);
+        }
+    }
+
+    // The tile into LDS, keys at `to`, values behind them.
+    __device__ __forceinline__ void store(uint32_t to, int tid) const {
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+            const int id = i * kThreads + tid, r = id % BN, block = id / BN;  // blocks of the keys, then the values
+            const int piece = block % kBlocks * (32 / L::E);
+            if (DP < L::P && block % kBlocks * 32 >= DP) continue;
+            const uint32_t row = to + (uint32_t)(block / kBlocks * BN * L::kRowBytes + r * L::kRowBytes);
+            const float f = cache::scale_of(scale[i]);
+            const uint32_t w[8] = {codes[i][0].x, codes[i][0].y, codes[i][0].z, codes[i][0].w,
+                                   codes[i][BITS / 8].x, codes[i][BITS / 8].y, codes[i][BITS / 8].z,
+                                   codes[i][BITS / 8].w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {  // eight features at a time
+                Eight<BITS> e;
+#pragma unroll
+                for (int y = 0; y < BITS / 4; ++y) e.w[y] = w[x * (BITS / 4) + y];
+                if constexpr (sizeof(T) == 2) {
+                    put(row, r, piece + x, e.bf16(f));
+                } else {
+                    float v[8];
+                    e.f32(f, v);
+                    put(row, r, piece + 2 * x, *reinterpret_cast<uint4 *>(v));
+                    put(row, r, piece + 2 * x + 1, *reinterpret_cast<uint4 *>(v + 4));
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ void put(uint32_t row, int r, int c, uint4 v) {
+        *reinterpret_cast<__attribute__((address_space(3))) tpw_u32x4 *>((uintptr_t)(row + (uint32_t)((c ^ L::swz(r)) * 16))) =
+            __builtin_bit_cast(tpw_u32x4, v);
+    }
+};
+
+// One block: kWaves * W query rows of the rows that share a key head, over the keys of one part.
+template <typename T, int W, int DP, int BN, int MM, int BITS, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void cache_tiles_kernel(const Args a, const Cache c) {
+    using F = Forward<T, W, DP, BN, MM, false, true>;
+    constexpr uint32_t kTileBytes = BN * Tile<T, DP>::kRowBytes;
+    // two buffers of a key tile and a value tile
+    __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int64_t t = xcd_linear(blockIdx.x, gridDim.x);
+    const int64_t part = t % a.splits;
+    t /= a.splits;
+    const int64_t tile = a.tiles - 1 - t % a.tiles;  // longest rows of a causal call first
+    const int64_t bk = t / a.tiles, b = bk / a.key_heads, kh = bk % a.key_heads;
+    const int64_t len = key_end(a, b), rows = a.n * a.group;
+    const int64_t row0 = tile * (kWaves * W), row1 = row0 + kWaves * W < rows ? row0 + kWaves * W : rows;
+
+    F f;
+    f.init(a, b, kh, row0 + wave * W, len, lane);
+
+    // keys that some row of the block sees
+    int64_t end = len;
+    if (a.causal && row0 / a.n == (row1 - 1) / a.n) end = row_limit(a, len, (row1 - 1) % a.n);
+    const int nt = (int)cdiv_dev(end, BN);
+    const int t0 = (int)((int64_t)nt * part / a.splits), t1 = (int)((int64_t)nt * (part + 1) / a.splits);
+
+    const uint32_t lds = tile::lds_addr(smem);
+    Decoder<T, DP, BN, kWaves, BITS> d;
+    if (t0 < t1) {
+        d.load(c, b, kh, t0 * BN, (int)len, threadIdx.x);
+        d.store(lds, threadIdx.x);
+    }
+    for (int i = t0; i < t1; ++i) {
+        const uint64_t present = d.present;
+        if (i + 1 < t1) d.load(c, b, kh, (i + 1) * BN, (int)len, threadIdx.x);
+        tile::barrier_lds();  // tile i is there, and nobody reads the other buffer any more
+        const uint32_t buf = lds + (uint32_t)((i - t0) & 1) * 2 * kTileBytes;
+        f.tile(a, b, buf, buf + kTileBytes, i * BN, lane, present);
+        if (i + 1 < t1) d.store(lds + (uint32_t)((i + 1 - t0) & 1) * 2 * kTileBytes, threadIdx.x);
+    }
+
+    const float sum = over_groups_sum<W>(f.sum);
+    if (f.qi < 0) return;
+    const int g = lane / W;
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const int64_t row = (b * a.heads + f.qh) * a.n + f.qi;
+    if (a.splits > 1) {
+        const int64_t all = a.batch * a.heads * a.n;
+        float *st = a.part_stats + part * 2 * all;
+        if (g == 0) {
+            st[row] = f.top;
+            st[all + row] = sum;
+        }
+        const int width = (int)quads4(a.dv);
+        float *p = a.part + (part * all + row) * width;
+        F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, width, v); });
+        return;
+    }
+    const OutRow<T> out(a, b, f.qh, f.qi);
+    F::CR::each(f.o, lane, [&](int at, f32x4 v) { out.store(at, v * inv); });
+}
+
+template <int BITS>
+int launch_tiles(const Args &a, const Cache &c, int dtype, int mode, hipStream_t s) {
+    return by_type(a, dtype, mode, [&](auto t, auto dp, auto mm) {
+        using T = decltype(t);
+        constexpr int DP = decltype(dp)::value, MM = decltype(mm)::value, W = Tiles<T, DP>::kWidth;
+        constexpr int kWaves = Tiles<T, DP>::kWaves, kKeys = Tiles<T, DP>::kKeys;
+        const int64_t blocks = a.batch * a.key_heads * a.tiles * a.splits;
+        TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: too many rows");
+        hipLaunchKernelGGL((cache_tiles_kernel<T, W, DP, kKeys, MM, BITS, kWaves>), dim3((unsigned)blocks),
+                           dim3(64 * kWaves), 0, s, a, c);
+        return check_launch("cache_tiles_kernel");
+    });
+}
+
+}  // namespace attn
+}  // namespace tpw

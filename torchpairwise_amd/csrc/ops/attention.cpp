@@ -7,7 +7,7 @@
 #include <cmath>
 #include <limits>
 
-#include "tpw_common.h"
+#include "tpw_attention.h"
 
 namespace tpw_ext {
 namespace {
@@ -15,32 +15,14 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
-using OptTensor = c10::optional<at::Tensor>;
+
+using Results = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
 
 constexpr int64_t kMaxFeatures = 256;
 
-// Rows as [batch, heads, n, features]: 2-D is one batch entry of one head, 3-D one head.
-at::Tensor as4(const at::Tensor &x) {
-    return x.dim() == 2 ? x.unsqueeze(0).unsqueeze(0) : x.dim() == 3 ? x.unsqueeze(1) : x;
-}
 at::Tensor like_dims(const at::Tensor &x4, const at::Tensor &ref) {
     return ref.dim() == 2 ? x4.squeeze(0).squeeze(0) : ref.dim() == 3 ? x4.squeeze(1) : x4;
 }
-
-// New rows in the order of `ref` (both [batch, heads, rows, features]): rows before heads where ref
-// has them so, as a transposed view of a dense tensor.
-at::Tensor empty_rows(at::IntArrayRef sizes, const at::Tensor &ref) {
-    if (ref.size(1) > 1 && ref.size(2) > 1 && ref.stride(1) < ref.stride(2))
-        return at::empty({sizes[0], sizes[2], sizes[1], sizes[3]}, ref.options()).transpose(1, 2);
-    return at::empty(sizes, ref.options());
-}
-
-struct Operands {
-    at::Tensor q, k, v;          // 4-D
-    at::Tensor mask;             // [batch, heads, n, m] (expanded) or undefined
-    at::Tensor lengths;          // int64 [batch] or undefined
-    int64_t batch, heads, key_heads, n, m, d, dv;
-};
 
 Operands check_attention(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value,
                          const OptTensor &mask, const OptTensor &lengths) {
@@ -72,27 +54,7 @@ Operands check_attention(const at::Tensor &query, const at::Tensor &key, const a
                 o.key_heads);
     TORCH_CHECK(o.d >= 1 && o.d <= kMaxFeatures && o.dv >= 1 && o.dv <= kMaxFeatures, name,
                 ": rows must have 1 to ", kMaxFeatures, " features, got ", o.d, " and ", o.dv);
-    if (mask.has_value() && mask->defined()) {
-        const at::Tensor &w = *mask;
-        TORCH_CHECK(w.device() == query.device(), name, ": mask is on another device");
-        TORCH_CHECK(w.scalar_type() == at::kBool || w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16 ||
-                        (w.is_cpu() && w.scalar_type() == at::kDouble),
-                    name, ": mask must be bool (true: kept), or float32 or bfloat16 (added), got ", w.scalar_type());
-        auto want = query.sizes().vec();
-        want.back() = o.m;
-        TORCH_CHECK(w.dim() <= query.dim() && at::is_expandable_to(w.sizes(), want), name,
-                    ": mask of shape ", w.sizes(), " does not broadcast to ", at::IntArrayRef(want));
-        o.mask = as4(w.expand(want));
-    }
-    if (lengths.has_value() && lengths->defined()) {
-        const at::Tensor &l = *lengths;
-        TORCH_CHECK(l.device() == query.device(), name, ": lengths are on another device");
-        TORCH_CHECK(l.dim() == 1 && l.size(0) == o.batch, name, ": lengths must have shape [batch_size], got ",
-                    l.sizes());
-        TORCH_CHECK(l.scalar_type() == at::kLong || l.scalar_type() == at::kInt, name,
-                    ": lengths must be int64 or int32, got ", l.scalar_type());
-        o.lengths = l.to(at::kLong).contiguous();
-    }
+    check_mask_and_lengths(name, o, query, mask, lengths);
     return o;
 }
 
@@ -141,8 +103,6 @@ at::Tensor masked_scores(const at::Tensor &q, const at::Tensor &k, const Operand
     return at::where(add == -std::numeric_limits<double>::infinity(), add, s + add);
 }
 at::ScalarType compute_type(const at::Tensor &x) { return x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
-
-using Results = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
 
 Results attention_cpu(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value, const OptTensor &mask,
                       const OptTensor &lengths, bool causal, double scale, bool train) {
@@ -249,17 +209,6 @@ at::Tensor rotary_cpu(const at::Tensor &x, const at::Tensor &positions, const at
 }
 
 // ------------------------------------------------------------------ GPU
-// Features dense; with `streamed`, rows neither overlap nor lie more than the kernels' reach apart.
-at::Tensor dense_rows(const at::Tensor &x, bool streamed) {
-    const bool dense = x.size(3) == 1 || x.stride(3) == 1;
-    const bool apart = !streamed || x.size(2) <= 1 ||
-                       (x.stride(2) >= x.size(3) && x.stride(2) * x.element_size() <= (int64_t(1) << 23));
-    return dense && apart ? x : x.contiguous();
-}
-void set_strides(int64_t (&s)[3], const at::Tensor &x) {
-    for (int i = 0; i < 3; ++i) s[i] = x.stride(i);
-}
-
 tpw_attention_desc describe(const Operands &o, bool causal, double scale) {
     tpw_attention_desc a = {};
     a.dtype = o.q.scalar_type() == at::kFloat ? TPW_F32 : TPW_BF16;
@@ -271,13 +220,7 @@ tpw_attention_desc describe(const Operands &o, bool causal, double scale) {
     set_strides(a.query_strides, o.q);
     set_strides(a.key_strides, o.k);
     set_strides(a.value_strides, o.v);
-    if (o.mask.defined()) {
-        const auto t = o.mask.scalar_type();
-        a.mask_type = t == at::kBool ? TPW_MASK_KEEP : t == at::kFloat ? TPW_MASK_ADD_F32 : TPW_MASK_ADD_BF16;
-        a.mask = o.mask.data_ptr();
-        for (int i = 0; i < 4; ++i) a.mask_strides[i] = o.mask.stride(i);
-    }
-    if (o.lengths.defined()) a.lengths = o.lengths.data_ptr<int64_t>();
+    describe_mask(a, o);
     return a;
 }
 
@@ -375,6 +318,8 @@ at::Tensor rotary_cuda(const at::Tensor &x, const at::Tensor &positions, const a
     return like_dims(out, x);
 }
 
+}  // namespace
+
 // ------------------------------------------------------------------ dispatch
 Results attention_op(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const OptTensor &mask,
                      const OptTensor &lengths, bool causal, double scale, bool train) {
@@ -384,6 +329,9 @@ Results attention_op(const at::Tensor &q, const at::Tensor &k, const at::Tensor 
                                         const OptTensor &, bool, double, bool)>();
     return op.call(q, k, v, mask, lengths, causal, scale, train);
 }
+
+namespace {
+
 Results attention_backward_op(const at::Tensor &grad, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
                               const at::Tensor &out, const at::Tensor &stats, const at::Tensor &rest, const OptTensor &mask,
                               const OptTensor &lengths, bool causal, double scale) {
@@ -404,10 +352,7 @@ at::Tensor rotary_op(const at::Tensor &x, const at::Tensor &positions, const at:
 
 at::Tensor attention(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value, const OptTensor &mask,
                      bool causal, c10::optional<double> scale, const OptTensor &lengths) {
-    const double s = scale.has_value() ? *scale
-                     : query.dim() > 0 && query.size(-1) > 0 ? 1.0 / std::sqrt((double)query.size(-1))
-                                                             : 1.0;
-    TORCH_CHECK(std::isfinite(s) && std::fabs(s) <= 1e30, "attention: scale must be finite, got ", s);
+    const double s = attention_scale("attention", query, scale);
     return std::get<0>(attention_op(query, key, value, mask, lengths, causal, s, false));
 }
 

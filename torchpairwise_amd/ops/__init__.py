@@ -27,11 +27,12 @@ _INTERNALS = [
     "pwand_sum", "pwor_sum", "pwxor_sum", "pweq_sum", "pwne_sum", "pweq_mean", "pwne_mean",
     "prf_div", "prf_ldiv", "prf_div_", "prf_ldiv_",
 ]
-_ATTENTION = ["attention", "rotary_embedding"]
+_ATTENTION = ["attention", "rotary_embedding", "cache_attention", "cache_read", "cache_write_"]
 
 for _name in _METRICS + _CPDIST + _INTERNALS + _ATTENTION:
     globals()[_name] = getattr(torch.ops.torchpairwise, _name)
 
+from .cache import quantized_cache  # noqa: E402
 from .rotary import rotary_frequencies  # noqa: E402
 
-__all__ = list(_METRICS) + list(_CPDIST) + list(_INTERNALS) + list(_ATTENTION) + ["rotary_frequencies"]
+__all__ = list(_METRICS) + list(_CPDIST) + list(_INTERNALS) + list(_ATTENTION) + ["quantized_cache", "rotary_frequencies"]
