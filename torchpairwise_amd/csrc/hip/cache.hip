@@ -66,34 +66,16 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const RowsArgs a) {
         const uint32_t m = __float_as_uint(x[e]) & 0x7fffffffu;
         top = m > top ? m : top;
     }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        const uint32_t m = (uint32_t)__shfl_xor((int)top, o, 64);
-        top = m > top ? m : top;
-    }
-    // exponent of the first power of two: one more from 7/4 (29/16) of a binade on
-    const int e = BITS == 4 ? (int)((top + 0x200000u) >> 23) - 2 : (int)((top + 0x180000u) >> 23) - 8;
-    const bool finite = top < 0x7f800000u;
-    const uint32_t byte = !finite ? 255u : e < 0 ? 0u : (uint32_t)e;
+    const uint32_t byte = cache::scale_byte<BITS>(cache::over_block(top));
     const float scale = scale_of(byte);
+    const bool finite = byte != 255;
     const Side &s = side ? a.c.v : a.c.k;
     uint8_t *codes = s.codes + p.at.first * s.cf + p.h * s.ch + p.at.row * s.cr;
     if constexpr (BITS == 4) {
-        uint32_t w = 0;
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
-        reinterpret_cast<uint32_t *>(codes)[p.piece] = finite ? w : 0u;
+        reinterpret_cast<uint32_t *>(codes)[p.piece] = finite ? to_fp4(x, scale) : 0u;
     } else {
-        s2 lo = {0, 0}, hi = {0, 0};
-        lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[0], x[1], scale, false);
-        lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[2], x[3], scale, true);
-        hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x[4], x[5], scale, false);
-        hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x[6], x[7], scale, true);
-        reinterpret_cast<uint2 *>(codes)[p.piece] = finite ? make_uint2(__builtin_bit_cast(uint32_t, lo),
-                                                                        __builtin_bit_cast(uint32_t, hi))
-                                                           : make_uint2(0u, 0u);
+        const uint2 w = to_fp8(x, scale);
+        reinterpret_cast<uint2 *>(codes)[p.piece] = finite ? w : make_uint2(0u, 0u);
     }
     if (p.piece % 4 == 0)
         s.scales[p.at.first * s.sf + p.h * s.sh + p.piece / 4 * s.sb + p.at.row] = (uint8_t)byte;

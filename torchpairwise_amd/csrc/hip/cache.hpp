@@ -51,8 +51,23 @@ __device__ __forceinline__ Place place(const Cache &c, int64_t b, int j) {
     return {p >= 0 && p < c.first ? p : -1, j & c.mask};
 }
 
+// The same for a row that a wave's lanes agree on, in scalar registers.
+__device__ __forceinline__ Place uniform_place(const Cache &c, int64_t b, int j) {
+    if (!c.pages) return {b, j};
+    const int64_t at = b * c.pitch + (j >> c.shift);
+    typedef __attribute__((address_space(4))) const int64_t *Wide;
+    typedef __attribute__((address_space(4))) const int32_t *Narrow;
+    const int64_t p = c.wide ? reinterpret_cast<Wide>(reinterpret_cast<uintptr_t>(c.pages))[at]
+                             : (int64_t) reinterpret_cast<Narrow>(reinterpret_cast<uintptr_t>(c.pages))[at];
+    return {p >= 0 && p < c.first ? p : -1, j & c.mask};
+}
+
 // The float that the conversions take for scale byte `b`.
 __device__ __forceinline__ float scale_of(uint32_t b) { return __uint_as_float(b << 23); }
+// The same for byte k of a word, by one shift: only the exponent's bits are read.
+__device__ __forceinline__ float scale_in(uint32_t w, int k) {
+    return __uint_as_float(k < 3 ? w << (23 - 8 * k) : w >> 1);
+}
 
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef short s2 __attribute__((ext_vector_type(2)));
@@ -97,6 +112,37 @@ struct Eight {
         for (int i = 0; i < 8; ++i) x[i] = y[i / 2][i % 2];
     }
 };
+
+// The largest of a block's magnitudes (as bits: NaN above infinity above all numbers) out of its 4 lanes'.
+__device__ __forceinline__ uint32_t over_block(uint32_t top) {
+    const uint32_t a = (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true);  // lanes 1 0 3 2
+    top = a > top ? a : top;
+    const uint32_t b = (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true);  // lanes 2 3 0 1
+    top = b > top ? b : top;
+    return top;
+}
+// The scale byte of a block with that largest magnitude: one more from 7/4 (29/16) of a binade on.
+template <int BITS>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+    const int e = BITS == 4 ? (int)((top + 0x200000u) >> 23) - 2 : (int)((top + 0x180000u) >> 23) - 8;
+    return top >= 0x7f800000u ? 255u : e < 0 ? 0u : (uint32_t)e;
+}
+// Eight features to codes.
+__device__ __forceinline__ uint32_t to_fp4(const float (&x)[8], float scale) {
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
+}
+__device__ __forceinline__ uint2 to_fp8(const float (&x)[8], float scale) {
+    s2 lo = {0, 0}, hi = {0, 0};
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[0], x[1], scale, false);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[2], x[3], scale, true);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x[4], x[5], scale, false);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, x[6], x[7], scale, true);
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
 
 // Host side (cache.hip): checks a cache against its batch and reads it into the kernels' form.
 int read_cache(const tpw_cache_desc *d, int64_t batch, Cache &c);

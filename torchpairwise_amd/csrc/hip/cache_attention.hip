@@ -26,16 +26,28 @@ int read_call(const tpw_attention_desc *d, const tpw_cache_desc *cd, tpw_attenti
     return TPW_OK;
 }
 
-// float32 rows of more than 128 features have no registers left for a second 16.
-bool few_rows(const Args &a, int dtype) {
-    return a.n * a.group <= (dtype == TPW_F32 && (a.d > 128 || a.dv > 128) ? 16 : kFewRows);
+// The form for few rows reads a mask's keys side by side, and has no registers left for a second 16 rows of
+// float32 with more than 128 features.
+bool few_rows(const Args &a, int dtype, int mode) {
+    return a.n * a.group <= (dtype == TPW_F32 && (a.d > 128 || a.dv > 128) ? 16 : kFewRows) &&
+           (mode == kNoMask || a.mm == 1);
 }
 
 size_t parts_bytes(const Args &a) {
     return a.splits > 1 ? (size_t)a.splits * a.batch * a.heads * a.n * (quads4(a.dv) + 2) * 4 : 0;
 }
 
-}  // namespace
+// As many parts as fill the card's places once: a block's own time (queries, first loads, joining) is that of
+// 16 chunks of 32 keys, so a second round costs more than long parts do.
+void plan_rows(Args &a, const cache::Cache &c, int bits, int dtype) {
+    const int nb = row_blocks(c.k.blocks > c.v.blocks ? c.k.blocks : c.v.blocks);
+    const int64_t per_cu = rows_per_cu(bits, nb, dtype == TPW_F32 ? 3 : 1, a.n * a.group <= 16 ? 1 : 2);
+    const int64_t bk = a.batch * a.key_heads, most = cdiv(cdiv(a.m, 32), kRowWaves);
+    int64_t splits = bk > 0 ? 256 * per_cu / bk : 1;
+    splits = splits > most ? most : splits;
+    a.splits = (int)(splits < 1 ? 1 : splits > kMaxParts ? kMaxParts : splits);
+    a.tiles = 1;
+}
 
 void plan_tiles(Args &a, int dtype) {
     by_type(a, dtype, kNoMask, [&](auto t, auto dp, auto) {
@@ -44,6 +56,7 @@ void plan_tiles(Args &a, int dtype) {
     });
 }
 
+}  // namespace
 }  // namespace attn
 }  // namespace tpw
 
@@ -55,8 +68,8 @@ extern "C" size_t tpw_cache_attention_workspace_size(const tpw_attention_desc *d
     cache::Cache c = {};
     tpw_attention_desc own;
     if (read_call(d, cd, own, a, c) != TPW_OK || a.batch * a.heads * a.n == 0) return 0;
-    if (few_rows(a, d->dtype)) {
-        plan_rows(a);
+    if (few_rows(a, d->dtype, mask_mode(d))) {
+        plan_rows(a, c, cd->bits, d->dtype);
         return parts_bytes(a);
     }
     plan_tiles(a, d->dtype);
@@ -75,10 +88,10 @@ extern "C" int tpw_cache_attention(const tpw_attention_desc *d, const tpw_cache_
     TPW_REQUIRE(mode == kNoMask || a.mask, "attention: null mask");
     hipStream_t s = as_stream(stream);
     size_t prepared = 0;
-    const bool few = few_rows(a, d->dtype);
+    const bool few = few_rows(a, d->dtype, mode);
     if (few) {
         if (mode == kNoMask) a.mask = nullptr;
-        plan_rows(a);
+        plan_rows(a, c, cd->bits, d->dtype);
     } else {
         plan_tiles(a, d->dtype);
         prepared = prepared_bytes(a, &own, false);
@@ -91,9 +104,8 @@ extern "C" int tpw_cache_attention(const tpw_attention_desc *d, const tpw_cache_
         a.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + prepared);
         a.part_stats = a.part + a.splits * a.batch * a.heads * a.n * quads4(a.dv);
     }
-    const int rc = few            ? cache_rows(a, c, cd->bits, d->dtype, mode == kBias, s)
-                   : cd->bits == 4 ? cache_tiles4(a, c, d->dtype, mode, s)
-                                   : cache_tiles8(a, c, d->dtype, mode, s);
+    const int rc = few ? (cd->bits == 4 ? cache_rows4 : cache_rows8)(a, c, d->dtype, mode, s)
+                       : (cd->bits == 4 ? cache_tiles4 : cache_tiles8)(a, c, d->dtype, mode, s);
     if (rc || a.splits == 1) return rc;
     return join_parts(a, d->dtype, mode == kBias, s);
 }

@@ -9,13 +9,20 @@
 namespace tpw {
 namespace attn {
 
-// Rows of a key head up to which the form for few rows is taken (cache_rows.hip).
+// The form for few rows, up to kFewRows a key head (cache_rows.hpp).
 constexpr int64_t kFewRows = 32;
-void plan_rows(Args &a);
-int cache_rows(const Args &a, const cache::Cache &c, int bits, int dtype, bool bias, hipStream_t s);
+constexpr int kRowWaves = 4;  // waves of a block
+// Blocks that share a CU, as their registers leave (NP: summands of a probability, RT: 16 rows each): three up
+// to 128 features in 4 bits, one where two rows of sums, wide rows in 8 bits or float32's summands fill them.
+constexpr int rows_per_cu(int bits, int nb, int np, int rt) {
+    return (nb == 8 && (bits == 8 || np > 1 || rt > 1)) || (np > 1 && rt > 1) ? 1 : bits == 4 && np == 1 && rt == 1 ? 3 : 2;
+}
+// 64, 128 or 256 features.
+constexpr int row_blocks(int most) { return most <= 2 ? 2 : most <= 4 ? 4 : 8; }
+int cache_rows4(const Args &a, const cache::Cache &c, int dtype, int mode, hipStream_t s);
+int cache_rows8(const Args &a, const cache::Cache &c, int dtype, int mode, hipStream_t s);
 
-// The form for many rows (cache_tiles4.hip, cache_tiles8.hip).
-void plan_tiles(Args &a, int dtype);
+// The form for many rows (cache_tiles.hpp).
 int cache_tiles4(const Args &a, const cache::Cache &c, int dtype, int mode, hipStream_t s);
 int cache_tiles8(const Args &a, const cache::Cache &c, int dtype, int mode, hipStream_t s);
 
