@@ -1,4 +1,6 @@
 // Rows into a cache of keys and values in 4 or 8 bits, and out of it (format and layouts: cache.hpp).
+#include <type_traits>
+
 #include "cache.hpp"
 
 namespace tpw {
@@ -14,111 +16,214 @@ struct RowsArgs {
     int whole[2];            // rows are whole pieces of 8 features at 16-byte aligned addresses
     const int64_t *starts;   // [batch] or null (0)
     const int64_t *counts;   // [batch] or null (n)
-    int64_t heads, n, m;     // rows of a call; rows that a sequence has room for
-    int64_t tiles;           // blocks of 256 threads per (sequence, head), those of the wider side
+    int64_t n, m;            // rows of a call; rows that a sequence has room for
+    uint32_t heads, tiles;   // blocks of 256 threads per (sequence, head), those of the wider side
 };
 
-// What one thread works on: 8 features (a piece) of row i; 4 consecutive lanes share a block of 32.
-struct Piece {
-    int64_t b, h, i;
-    int piece;
-    bool live;  // row i is one of the call's
-    Place at;   // first < 0: no place in the cache
+// A block's share: a thread works on 8 features (a piece) of ROWS consecutive rows (whose scales lie side by
+// side: one word); 4 consecutive lanes share a block of 32 features.  What the call does not have is read from somewhere that exists and dropped: without
+// branches between them all of a thread's loads are in flight at once.
+template <int ROWS, bool PAGED>
+struct Share {
+    int64_t b, h, first;  // first row of the block's
+    int piece, r, per;    // the thread's piece and its place among the `per` threads of that
+    int rows;             // of the call's
+    int64_t entry[ROWS];  // where the thread's rows lie: entry of the cache's first dimension
+    int row[ROWS];
+    bool live[ROWS];      // the call has the row, and it has a place
+    __device__ __forceinline__ Share(const RowsArgs &a, const Side &s) {
+        // 32 bits: divisions in 64 would be most of a block's instructions
+        const uint32_t pieces = 4 * s.blocks, t = threadIdx.x;
+        per = (int)(256 / pieces);
+        r = (int)(t / pieces);
+        piece = (int)(t % pieces);
+        const uint32_t id = xcd_range(blockIdx.x, gridDim.x), bh = id / a.tiles;
+        b = bh / a.heads;
+        h = bh % a.heads;
+        first = (int64_t)(id % a.tiles) * (ROWS * per);
+        const int64_t left = a.n - first;
+        rows = left < ROWS * per ? (int)left : ROWS * per;
+        const int64_t start = (a.starts ? a.starts[b] : 0) + first, counted = a.counts ? a.counts[b] - first : rows;
+        const int count = counted < 0 ? 0 : counted < rows ? (int)counted : rows;
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            const int64_t q = start + own(k);
+            live[k] = r < per && own(k) < count && q >= 0 && q < a.m;
+            row[k] = live[k] ? (int)q : 0;
+            entry[k] = b;
+        }
+        if constexpr (PAGED) {
+            if (a.m == 0) return;  // no table
+            if (a.c.wide)
+                look<int64_t>(a);
+            else
+                look<int32_t>(a);
+        }
+    }
+    template <typename I>
+    __device__ __forceinline__ void look(const RowsArgs &a) {
+        const I *table = reinterpret_cast<const I *>(a.c.pages) + b * a.c.pitch;
+        I page[ROWS];
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) page[k] = table[row[k] >> a.c.shift];
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            live[k] = live[k] && page[k] >= 0 && (int64_t)page[k] < a.c.first;
+            entry[k] = live[k] ? (int64_t)page[k] : 0;
+            row[k] = live[k] ? row[k] & a.c.mask : 0;
+        }
+    }
+    __device__ __forceinline__ uint8_t *codes(const Side &s, int k) const {
+        return s.codes + entry[k] * s.cf + h * s.ch + (int64_t)row[k] * s.cr;
+    }
+    __device__ __forceinline__ uint8_t *scale(const Side &s, int k) const {
+        return s.scales + entry[k] * s.sf + h * s.sh + piece / 4 * s.sb + row[k];
+    }
+    // Row k of the thread's among the call's, and whether it is there.
+    __device__ __forceinline__ int own(int k) const { return r * ROWS + k; }
+    __device__ __forceinline__ bool has(int k) const { return r < per && own(k) < rows; }
+    // Ids go round-robin over the 8 XCDs: where they divide, each XCD gets a contiguous range, so that the
+    // scales of neighbouring rows, a byte each, meet in one L2.
+    static __device__ __forceinline__ uint32_t xcd_range(uint32_t id, uint32_t all) {
+        return (all & 7) == 0 ? (id & 7) * (all >> 3) + (id >> 3) : id;
+    }
 };
-__device__ __forceinline__ bool piece_of(const RowsArgs &a, int side, Piece &p) {
-    const Side &s = side ? a.c.v : a.c.k;
-    const int pieces = 4 * s.blocks, per = 256 / pieces, t = (int)threadIdx.x, r = t / pieces;
-    const int64_t id = blockIdx.x, bh = id / a.tiles;
-    p.piece = t - r * pieces;
-    p.b = bh / a.heads;
-    p.h = bh - p.b * a.heads;
-    p.i = (id - bh * a.tiles) * per + r;
-    if (r >= per || p.i >= a.n) return false;
-    p.live = !a.counts || p.i < a.counts[p.b];
-    const int64_t j = (a.starts ? a.starts[p.b] : 0) + p.i;
-    p.at = {-1, 0};
-    if (p.live && j >= 0 && j < a.m) p.at = place(a.c, p.b, (int)j);
-    return true;
-}
 
-// One thread per 8 features.  The largest magnitude is taken over the bits (NaN above infinity above all
-// numbers) within the thread and over 4 lanes.  Bound by memory: 2 x 4 x 16 x 8192 x 128 bf16 (268 MB read,
-// 71 MB written).
-template <typename T, int BITS>
+// WHOLE: rows are whole pieces of 8 features at 16-byte aligned addresses.  Bound by memory: 2 x 4 x 16 x 8192 x
+// 128 bf16 in 72 to 75 us back to back (4.6 TB/s read and written), behind a read of as much in 93.
+template <typename T, int BITS, int ROWS, bool WHOLE, bool PAGED>
 __global__ __launch_bounds__(256) void cache_write_kernel(const RowsArgs a) {
     const int side = blockIdx.y;
-    Piece p;
-    if (!piece_of(a, side, p) || p.at.first < 0) return;  // the four lanes of a block alike
-    const T *row = reinterpret_cast<const T *>(a.x[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.i * a.xn[side];
-    const int f = 8 * p.piece, d = a.width[side];
-    T raw[8];
-    if (a.whole[side] && f < d) {
-        __builtin_memcpy(raw, __builtin_assume_aligned(row + f, 16), sizeof(raw));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) raw[e] = f + e < d ? row[f + e] : T(0);
-    }
-    float x[8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        x[e] = to_f32(raw[e]);
-        const uint32_t m = __float_as_uint(x[e]) & 0x7fffffffu;
-        top = m > top ? m : top;
-    }
-    const uint32_t byte = cache::scale_byte<BITS>(cache::over_block(top));
-    const float scale = scale_of(byte);
-    const bool finite = byte != 255;
     const Side &s = side ? a.c.v : a.c.k;
-    uint8_t *codes = s.codes + p.at.first * s.cf + p.h * s.ch + p.at.row * s.cr;
-    if constexpr (BITS == 4) {
-        reinterpret_cast<uint32_t *>(codes)[p.piece] = finite ? to_fp4(x, scale) : 0u;
-    } else {
-        const uint2 w = to_fp8(x, scale);
-        reinterpret_cast<uint2 *>(codes)[p.piece] = finite ? w : make_uint2(0u, 0u);
+    const Share<ROWS, PAGED> p(a, s);
+    const T *base = reinterpret_cast<const T *>(a.x[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.first * a.xn[side];
+    const int f = 8 * p.piece, d = a.width[side];
+    T raw[ROWS][8] = {};
+    uint32_t bytes[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        const T *row = base + (p.has(k) ? p.own(k) : 0) * a.xn[side];
+        if constexpr (WHOLE) {
+            __builtin_memcpy(raw[k], __builtin_assume_aligned(row + (f < d ? f : 0), 16), sizeof(raw[k]));
+        } else if (d >= 8) {  // any alignment
+            __builtin_memcpy(raw[k], row + (f + 8 <= d ? f : 0), sizeof(raw[k]));
+        }
     }
-    if (p.piece % 4 == 0)
-        s.scales[p.at.first * s.sf + p.h * s.sh + p.piece / 4 * s.sb + p.at.row] = (uint8_t)byte;
+    if (!WHOLE && f < d && f + 8 > d) {  // a row's last piece
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                raw[k][e] = base[(p.has(k) ? p.own(k) : 0) * a.xn[side] + (f + e < d ? f + e : d - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        float x[8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = (WHOLE ? f : f + e) < d ? to_f32(raw[k][e]) : 0.0f;
+            const uint32_t m = __float_as_uint(x[e]) & 0x7fffffffu;
+            top = m > top ? m : top;
+        }
+        const uint32_t byte = scale_byte<BITS>(over_block(top));
+        const float scale = scale_of(byte);
+        const bool finite = byte != 255;
+        bytes[k] = byte;
+        if (!p.live[k]) continue;  // the four lanes of a block alike
+        if constexpr (BITS == 4) {
+            reinterpret_cast<uint32_t *>(p.codes(s, k))[p.piece] = finite ? to_fp4(x, scale) : 0u;
+        } else {
+            const uint2 w = to_fp8(x, scale);
+            reinterpret_cast<uint2 *>(p.codes(s, k))[p.piece] = finite ? w : make_uint2(0u, 0u);
+        }
+    }
+    if (p.piece % 4 != 0) return;
+    if constexpr (ROWS == 4) {  // four rows' scales of a block lie side by side: one store where they all go there
+        if (p.live[0] && p.live[1] && p.live[2] && p.live[3] && p.row[0] % 4 == 0) {  // (pages: in one of them)
+            *reinterpret_cast<uint32_t *>(p.scale(s, 0)) = bytes[0] | bytes[1] << 8 | bytes[2] << 16 | bytes[3] << 24;
+            return;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+        if (p.live[k]) *p.scale(s, k) = (uint8_t)bytes[k];
 }
 
-// One thread per 8 features; rows that are not the call's, or that lie nowhere, are zeros.
-template <typename T, int BITS>
+// Rows that are not the call's, or that lie nowhere, are zeros.  Bound by memory: 2 x 16 x 2 x 32768 x 128 in 122
+// to 132 us (5 TB/s); one row a thread, with branches around its loads, took 205.
+template <typename T, int BITS, int ROWS, bool WHOLE, bool PAGED>
 __global__ __launch_bounds__(256) void cache_read_kernel(const RowsArgs a) {
     const int side = blockIdx.y;
-    Piece p;
-    if (!piece_of(a, side, p)) return;
-    T *row = reinterpret_cast<T *>(a.y[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.i * a.xn[side];
+    const Side &s = side ? a.c.v : a.c.k;
+    const Share<ROWS, PAGED> p(a, s);
+    T *base = reinterpret_cast<T *>(a.y[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.first * a.xn[side];
     const int f = 8 * p.piece, d = a.width[side];
-    if (f >= d) return;
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (p.at.first >= 0) {
-        const Side &s = side ? a.c.v : a.c.k;
-        const uint8_t *codes = s.codes + p.at.first * s.cf + p.h * s.ch + p.at.row * s.cr;
-        Eight<BITS> w;
-        __builtin_memcpy(&w, __builtin_assume_aligned(codes + BITS * p.piece, BITS), sizeof(w));
-        w.f32(scale_of(s.scales[p.at.first * s.sf + p.h * s.sh + p.piece / 4 * s.sb + p.at.row]), x);
+    if (f >= d || p.r >= p.per) return;
+    Eight<BITS> w[ROWS] = {};
+    uint32_t byte[ROWS] = {};
+    if (a.m > 0 && a.c.first > 0) {
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            __builtin_memcpy(&w[k], __builtin_assume_aligned(p.codes(s, k) + BITS * p.piece, BITS), sizeof(w[k]));
+            byte[k] = *p.scale(s, k);
+        }
     }
-    T out[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) from_f32(&out[e], x[e]);
-    if (a.whole[side]) {
-        __builtin_memcpy(__builtin_assume_aligned(row + f, 16), out, sizeof(out));
-    } else {
+    for (int k = 0; k < ROWS; ++k) {
+        T out[8];
+        const float scale = scale_of(byte[k]);
+        if (sizeof(T) == 2 && __all(byte[k] >= 32)) {  // exact
+            const uint4 y = w[k].bf16(scale);
+            __builtin_memcpy(out, &y, 16);
+        } else {  // (bfloat16 below its normal range: rounded)
+            float x[8];
+            w[k].f32(scale, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (f + e < d) row[f + e] = out[e];
+            for (int e = 0; e < 8; ++e) from_f32(&out[e], x[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = p.live[k] ? out[e] : T(0);
+        if (!p.has(k)) continue;
+        T *row = base + p.own(k) * a.xn[side] + f;
+        if constexpr (WHOLE) {
+            __builtin_memcpy(__builtin_assume_aligned(row, 16), out, sizeof(out));
+        } else if (f + 8 <= d) {  // any alignment
+            __builtin_memcpy(row, out, sizeof(out));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (f + e < d) row[e] = out[e];
+        }
     }
 }
 
+// Rows of a thread: several where there are blocks enough to fill the card's places all the same.
+constexpr int kManyRows = 4;
 template <typename T, int BITS>
-int launch(const RowsArgs &a, bool write, int64_t blocks, hipStream_t s) {
-    const dim3 grid((unsigned)blocks, 2);
-    if (write) {
-        hipLaunchKernelGGL((cache_write_kernel<T, BITS>), grid, dim3(256), 0, s, a);
-        return check_launch("cache_write_kernel");
-    }
-    hipLaunchKernelGGL((cache_read_kernel<T, BITS>), grid, dim3(256), 0, s, a);
-    return check_launch("cache_read_kernel");
+int launch(RowsArgs &a, bool write, int64_t batch, int64_t blocks, hipStream_t s) {
+    const auto go = [&](auto rows, auto whole, auto paged) {
+        constexpr int ROWS = decltype(rows)::value;
+        constexpr bool WHOLE = decltype(whole)::value, PAGED = decltype(paged)::value;
+        const int64_t tiles = cdiv(a.n, ROWS * (256 / (4 * blocks))), all = tiles * batch * a.heads;
+        TPW_REQUIRE(all < (int64_t(1) << 31), "cache: too many rows");
+        a.tiles = (uint32_t)tiles;
+        const dim3 grid((unsigned)all, 2);
+        if (write) {
+            hipLaunchKernelGGL((cache_write_kernel<T, BITS, ROWS, WHOLE, PAGED>), grid, dim3(256), 0, s, a);
+            return check_launch("cache_write_kernel");
+        }
+        hipLaunchKernelGGL((cache_read_kernel<T, BITS, ROWS, WHOLE, PAGED>), grid, dim3(256), 0, s, a);
+        return check_launch("cache_read_kernel");
+    };
+    const auto by_page = [&](auto rows, auto whole) {
+        return a.c.pages ? go(rows, whole, std::true_type{}) : go(rows, whole, std::false_type{});
+    };
+    const auto by_row = [&](auto rows) {
+        return a.whole[0] && a.whole[1] ? by_page(rows, std::true_type{}) : by_page(rows, std::false_type{});
+    };
+    const int64_t all = cdiv(a.n, kManyRows * (256 / (4 * blocks))) * batch * a.heads * 2;
+    return all >= 256 * 8 ? by_row(std::integral_constant<int, kManyRows>{}) : by_row(std::integral_constant<int, 1>{});
 }
 
 int move_rows(const tpw_cache_desc *d, bool write, int dtype, int64_t batch, int64_t n, const void *key, int64_t width,
@@ -147,16 +252,14 @@ int move_rows(const tpw_cache_desc *d, bool write, int dtype, int64_t batch, int
     }
     a.starts = starts;
     a.counts = counts;
-    a.heads = d->heads;
+    a.heads = (uint32_t)d->heads;
     a.n = n;
     a.m = d->pages ? d->page_count * d->rows : d->rows;
-    a.tiles = cdiv(n, 256 / (4 * blocks));
-    const int64_t grid = a.tiles * batch * d->heads;
-    TPW_REQUIRE(grid < (int64_t(1) << 31), "cache: too many rows");
+    if (write && (a.m == 0 || a.c.first == 0)) return TPW_OK;  // nowhere to go
     hipStream_t s = as_stream(stream);
     if (dtype == TPW_F32)
-        return d->bits == 4 ? launch<float, 4>(a, write, grid, s) : launch<float, 8>(a, write, grid, s);
-    return d->bits == 4 ? launch<uint16_t, 4>(a, write, grid, s) : launch<uint16_t, 8>(a, write, grid, s);
+        return d->bits == 4 ? launch<float, 4>(a, write, batch, blocks, s) : launch<float, 8>(a, write, batch, blocks, s);
+    return d->bits == 4 ? launch<uint16_t, 4>(a, write, batch, blocks, s) : launch<uint16_t, 8>(a, write, batch, blocks, s);
 }
 
 }  // namespace
@@ -197,13 +300,16 @@ int read_cache(const tpw_cache_desc *d, int64_t batch, Cache &c) {
         s.sf = d->first == 1 ? 0 : ss[0];
         s.sh = d->heads == 1 ? 0 : ss[1];
         s.sb = blocks == 1 ? 0 : ss[2];
+        // rows and scales within the kernels' 32-bit reach
+        if (s.cr < 0 || s.cr > (int64_t(1) << 23) || s.sb < 0 || s.sb > (int64_t(1) << 28)) return false;
         return aligned16(codes) && aligned16(scales) && (s.cf | s.ch | s.cr | s.sf | s.sh | s.sb) % 16 == 0 &&
                (m * d->first == 0 || (codes && scales));
     };
     TPW_REQUIRE(side(c.k, d->key_codes, d->key_scales, d->key_code_strides, d->key_scale_strides, d->key_blocks) &&
                     side(c.v, d->value_codes, d->value_scales, d->value_code_strides, d->value_scale_strides,
                          d->value_blocks),
-                "cache: codes and scales must lie at 16-byte aligned addresses and strides");
+                "cache: codes and scales must lie at 16-byte aligned addresses and strides, rows at most 8 MiB and scales of "
+                "a block at most 256 MiB apart");
     return TPW_OK;
 }
 

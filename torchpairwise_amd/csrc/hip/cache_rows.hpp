@@ -44,7 +44,6 @@ struct Rows {
     f32x4 o[RT][V];
     float base[RT], sum[RT];  // the row's running base, at most kSlack below its maximum; the lane's sum
     int lim[RT];              // keys that the row sees
-    int64_t qh[RT], qi[RT];   // head and row (row -1: none)
     int64_t mrow[RT];         // bytes to its row of the mask
     int msize;                // bytes of one of its values
     uint32_t kat[KS], ksat[KS], vat, vsat;  // bytes of the lane's part: codes and scales of its key, its values
@@ -64,15 +63,15 @@ struct Rows {
         vsat = (uint32_t)(block * c.v.sb + 8 * g);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int64_t r = 16 * t + i, rows = a.n * a.group;
-            const bool in = r < rows;
-            qh[t] = kh * a.group + (in ? r / a.n : 0);
-            qi[t] = in ? r % a.n : -1;
-            const int64_t l = in ? row_limit(a, len, qi[t]) : 0;
+            const int r = 16 * t + i, n = (int)a.n;
+            const bool in = r < n * (int)a.group;
+            const int h = in ? n == 1 ? r : r / n : 0;
+            const int64_t qh = kh * a.group + h, qi = in ? r - h * n : 0;
+            const int64_t l = in ? row_limit(a, len, qi) : 0;
             lim[t] = (int)(l < len ? l : len);
             if constexpr (MM != kNoMask) {
                 msize = MM == kKeep ? 1 : a.mask_bf16 ? 2 : 4;
-                mrow[t] = (b * a.mb + qh[t] * a.mh + (in ? qi[t] : 0) * a.mn) * msize;
+                mrow[t] = (b * a.mb + qh * a.mh + qi * a.mn) * msize;
             }
 #pragma unroll
             for (int k = 0; k < V; ++k) o[t][k] = f32x4{0, 0, 0, 0};
@@ -412,14 +411,15 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args 
     float *const mine = reinterpret_cast<float *>(smem);
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
-    int64_t t = xcd_linear(blockIdx.x, gridDim.x);
-    const int64_t part = t % a.splits;
-    t /= a.splits;
-    const int64_t b = t / a.key_heads, kh = t % a.key_heads;
+    // 32 bits: divisions in 64 would take as long as several chunks
+    const uint32_t all = gridDim.x, id = (all & 7) == 0 ? (blockIdx.x & 7) * (all >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    const uint32_t part = id % (uint32_t)a.splits, bk = id / (uint32_t)a.splits;
+    const int64_t b = bk / (uint32_t)a.key_heads, kh = bk % (uint32_t)a.key_heads;
     typename R::Piece y[R::kOwn];
     R::load_queries(a, b, kh, y);
-    const int len = (int)key_end(a, b), chunks = (int)cdiv_dev(len, 32);
-    const int c0 = (int)((int64_t)chunks * part / a.splits), c1 = (int)((int64_t)chunks * (part + 1) / a.splits);
+    const int len = (int)key_end(a, b);
+    const uint32_t chunks = (uint32_t)(len + 31) / 32;  // below 2^26, parts at most 64
+    const int c0 = (int)(chunks * part / (uint32_t)a.splits), c1 = (int)(chunks * (part + 1) / (uint32_t)a.splits);
 
     R r;
     r.init(a, c, b, kh, len, lane);
@@ -491,12 +491,12 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args 
         const int n = (int)a.n, hi = n == 1 ? q : q / n;
         const int64_t h = kh * a.group + hi, qi = q - hi * n, row = (b * a.heads + h) * n + qi;
         if (a.splits > 1) {
-            const int64_t all = a.batch * a.heads * n;
+            const int64_t all = a.batch * a.heads * n, at = part;
             if (f == 0) {
-                a.part_stats[part * 2 * all + row] = top;
-                a.part_stats[(part * 2 + 1) * all + row] = sum;
+                a.part_stats[at * 2 * all + row] = top;
+                a.part_stats[(at * 2 + 1) * all + row] = sum;
             }
-            store4(a.part + (part * all + row) * width, 4 * f, width, o);
+            store4(a.part + (at * all + row) * width, 4 * f, width, o);
         } else {
             const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
             store4(reinterpret_cast<typename R::T *>(const_cast<void *>(a.o.p)) + b * a.o.b + h * a.o.h + qi * a.o.n, 4 * f,
