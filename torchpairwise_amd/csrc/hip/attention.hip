@@ -88,6 +88,12 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
 // Joins the parts of every row: m = max m_s, l = sum l_s 2^(m_s - m), o = sum o_s 2^(m_s - m) / l.
 // One block per row: lane s of every wave holds part s's weight; then LANES lanes of four features
 // each, 256 / LANES parts at a time, in an order that the sizes fix.
+// Row r's entry, head and row.  Rows are below 2^31: divisions in 64 bits would be a third of the kernel's time.
+template <typename T>
+__device__ __forceinline__ OutRow<T> joined_row(const Args &a, uint32_t r) {
+    const uint32_t n = (uint32_t)a.n, i = r % n, bh = r / n;
+    return OutRow<T>(a, bh / (uint32_t)a.heads, bh % (uint32_t)a.heads, i);
+}
 template <typename T, bool BIAS, int LANES>
 __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
     constexpr int G = 256 / LANES, U = kMaxParts / G < 8 ? kMaxParts / G : 8;
@@ -128,8 +134,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
         a.stats[row] = top;
         a.stats[rows + row] = sum;
     }
-    const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
-    OutRow<T>(a, b, h, i).store(f, o * inv);
+    joined_row<T>(a, (uint32_t)row).store(f, o * inv);
 }
 
 // The same for at most PARTS parts: one thread per four features, every load in flight at once
@@ -140,10 +145,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
 constexpr int64_t kManyQuads = 32768;
 template <typename T, bool BIAS, int PARTS>
 __global__ __launch_bounds__(256) void attention_join_few_kernel(const Args a) {
-    const int64_t rows = a.batch * a.heads * a.n, quads = cdiv_dev(a.dv, 4);
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / quads;
+    const int64_t rows = a.batch * a.heads * a.n, quads = quads4(a.dv) / 4, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = rows * quads < (int64_t(1) << 32) ? (uint32_t)id / (uint32_t)quads : id / quads;
     if (row >= rows) return;
-    const int f = (int)(id % quads) * 4;
+    const int f = (int)(id - row * quads) * 4;
     float top_s[PARTS], sum_s[PARTS];
     f32x4 x[PARTS];
 #pragma unroll
@@ -172,8 +177,7 @@ __global__ __launch_bounds__(256) void attention_join_few_kernel(const Args a) {
         a.stats[row] = top;
         a.stats[rows + row] = sum;
     }
-    const int64_t i = row % a.n, h = row / a.n % a.heads, b = row / a.n / a.heads;
-    OutRow<T>(a, b, h, i).store(f, o * inv);
+    joined_row<T>(a, (uint32_t)row).store(f, o * inv);
 }
 
 namespace {
