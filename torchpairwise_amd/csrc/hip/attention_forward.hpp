@@ -142,12 +142,21 @@ struct Forward {
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int e = 0; e < 4 * M::Q; ++e) mx = __builtin_fmaxf(mx, s[i][e]);
-        mx = over_groups_max<W>(mx);
-        if constexpr (MM != kBias) mx *= a.scale;
-        const float top1 = __builtin_fmaxf(top, mx);
+        float top1 = top;
+        bool move = true;
+        if constexpr (GAPS) {  // the base follows once the maximum is 2^8 ahead: few tiles exchange and rescale
+            if constexpr (MM != kBias) mx *= a.scale;
+            move = __any(mx > top + (MM == kBias ? 5.0f : 8.0f));
+            if (move) top1 = __builtin_fmaxf(top, over_groups_max<W>(mx));
+        } else {
+            mx = over_groups_max<W>(mx);
+            if constexpr (MM != kBias) mx *= a.scale;
+            top1 = __builtin_fmaxf(top, mx);
+            move = __any(top1 > top);
+        }
         // a row with no key so far: exp2(-inf - 0) = 0 throughout
         const float base = top1 == -INFINITY ? 0.0f : top1;
-        if (__any(top1 > top)) {
+        if (move) {
             const float f = __builtin_amdgcn_exp2f(MM == kBias ? (top - base) * kLog2e : top - base);
             sum *= f;
 #pragma unroll

@@ -96,11 +96,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_tiles_kernel(const Args 
     // two buffers of a key tile and a value tile
     __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
-    int64_t t = xcd_linear(blockIdx.x, gridDim.x);
-    const int64_t part = t % a.splits;
-    t /= a.splits;
-    const int64_t tile = a.tiles - 1 - t % a.tiles;  // longest rows of a causal call first
-    const int64_t bk = t / a.tiles, b = bk / a.key_heads, kh = bk % a.key_heads;
+    const uint32_t all = gridDim.x, id = (all & 7) == 0 ? (blockIdx.x & 7) * (all >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    const uint32_t part = id % (uint32_t)a.splits, t = id / (uint32_t)a.splits;
+    const int64_t tile = a.tiles - 1 - t % (uint32_t)a.tiles;  // longest rows of a causal call first
+    const uint32_t bk = t / (uint32_t)a.tiles;
+    const int64_t b = bk / (uint32_t)a.key_heads, kh = bk % (uint32_t)a.key_heads;
     const int64_t len = key_end(a, b), rows = a.n * a.group;
     const int64_t row0 = tile * (kWaves * W), row1 = row0 + kWaves * W < rows ? row0 + kWaves * W : rows;
 
@@ -134,14 +134,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_tiles_kernel(const Args 
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     const int64_t row = (b * a.heads + f.qh) * a.n + f.qi;
     if (a.splits > 1) {
-        const int64_t all = a.batch * a.heads * a.n;
-        float *st = a.part_stats + part * 2 * all;
+        const int64_t lines = a.batch * a.heads * a.n, at = part;
+        float *st = a.part_stats + at * 2 * lines;
         if (g == 0) {
             st[row] = f.top;
-            st[all + row] = sum;
+            st[lines + row] = sum;
         }
         const int width = (int)quads4(a.dv);
-        float *p = a.part + (part * all + row) * width;
+        float *p = a.part + (at * lines + row) * width;
         F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, width, v); });
         return;
     }
