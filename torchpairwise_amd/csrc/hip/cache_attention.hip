@@ -41,7 +41,8 @@ size_t parts_bytes(const Args &a) {
 // 16 chunks of 32 keys, so a second round costs more than long parts do.
 void plan_rows(Args &a, const cache::Cache &c, int bits, int dtype) {
     const int nb = row_blocks(c.k.blocks > c.v.blocks ? c.k.blocks : c.v.blocks);
-    const int64_t per_cu = rows_per_cu(bits, nb, dtype == TPW_F32 ? 3 : 1, a.n * a.group <= 16 ? 1 : 2);
+    const int64_t rows = a.n * a.group;
+    const int64_t per_cu = rows_per_cu(bits, nb, dtype == TPW_F32 && rows > kPackedRows ? 3 : 1, rows <= 16 ? 1 : 2);
     const int64_t bk = a.batch * a.key_heads, most = cdiv(cdiv(a.m, 32), kRowWaves);
     int64_t splits = bk > 0 ? 256 * per_cu / bk : 1;
     splits = splits > most ? most : splits;

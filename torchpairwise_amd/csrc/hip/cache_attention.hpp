@@ -11,6 +11,7 @@ namespace attn {
 
 // The form for few rows, up to kFewRows a key head (cache_rows.hpp).
 constexpr int64_t kFewRows = 32;
+constexpr int64_t kPackedRows = 4;  // of float32 whose summands share a product
 constexpr int kRowWaves = 4;  // waves of a block
 // Blocks that share a CU, as their registers leave (NP: summands of a probability, RT: 16 rows each): three up
 // to 128 features in 4 bits, one where two rows of sums, wide rows in 8 bits or float32's summands fill them.

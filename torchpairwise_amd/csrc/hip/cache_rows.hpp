@@ -33,14 +33,19 @@ struct Codes {
     uint32_t m[RT][MM == kBias ? 8 : MM == kKeep ? 2 : 1];  // the mask's values for the lane's eight keys
 };
 
-template <int BITS, int NB, int NP, int RT, int MM, bool HALVES, int WAVES>
+// NP: summands in bfloat16 of a query and a probability (float32: three).  PACK: at most 4 rows, whose summands
+// take 4 columns of a product each: one product for all three, where 16 rows take three (float32, 8 x 16 (4) heads
+// over 16000 of 90: 19.3 -> 16.9 us).
+template <int BITS, int NB, int NP, int RT, int MM, bool HALVES, bool PACK, int WAVES>
 struct Rows {
+    static_assert(!PACK || (NP == 3 && RT == 1), "three summands of 4 rows");
+    static constexpr int NM = PACK ? 1 : NP;  // products for a tile of 16 rows
     using C = Codes<BITS, NB, RT, MM>;
     static constexpr bool BIAS = MM == kBias;
     using T = std::conditional_t<NP == 1, uint16_t, float>;
     static constexpr int KS = C::KS, F = 8 * NB, V = 2 * NB;
 
-    Frag<uint16_t> q[RT][NB][NP];
+    Frag<uint16_t> q[RT][NB][NM];
     f32x4 o[RT][V];
     float base[RT], sum[RT];  // the row's running base, at most kSlack below its maximum; the lane's sum
     int lim[RT];              // keys that the row sees
@@ -63,7 +68,7 @@ struct Rows {
         vsat = (uint32_t)(block * c.v.sb + 8 * g);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int r = 16 * t + i, n = (int)a.n;
+            const int r = PACK ? i & 3 : 16 * t + i, n = (int)a.n;
             const bool in = r < n * (int)a.group;
             const int h = in ? n == 1 ? r : r / n : 0;
             const int64_t qh = kh * a.group + h, qi = in ? r - h * n : 0;
@@ -143,9 +148,12 @@ struct Rows {
 #pragma unroll
             for (int s = 0; s < NB; ++s)
 #pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    q[t][s][p].v = *reinterpret_cast<const uint4 *>(from + p * kPlane + (16 * t + i) * kRow +
-                                                                    2 * (F * g + 8 * s));
+                for (int p = 0; p < NM; ++p) {
+                    // PACK: columns 12 to 15 repeat the last summand's place and are made zeros
+                    const int plane = PACK ? (i >> 2 < NP ? i >> 2 : NP - 1) : p, row = PACK ? i & 3 : 16 * t + i;
+                    q[t][s][p].v = *reinterpret_cast<const uint4 *>(from + plane * kPlane + row * kRow + 2 * (F * g + 8 * s));
+                    if (PACK && i >= 12) q[t][s][p].v = make_uint4(0, 0, 0, 0);
+                }
     }
 
     // One summand in bfloat16, rounded (queries: exact); or three that hold all 24 bits, each what is left cut
@@ -165,6 +173,27 @@ struct Rows {
                 f[p].v = make_uint4(high(w[0], w[1]), high(w[2], w[3]), high(w[4], w[5]), high(w[6], w[7]));
             }
         }
+    }
+    // The lane's own summand of its row's eight probabilities (the fourth: nothing is left for it).
+    static __device__ __forceinline__ void split_own(float (&x)[8], int i, Frag<uint16_t> &f) {
+        uint32_t w[8];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const float on = p < i >> 2 ? 1.0f : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] = __builtin_fmaf(-on, __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u), x[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(x[e]);
+        f.v = make_uint4(high(w[0], w[1]), high(w[2], w[3]), high(w[4], w[5]), high(w[6], w[7]));
+    }
+    // The sum over a row's four columns (lanes i, i + 4, .. of 16), the same bits in every one of them: 8 apart
+    // first, then 4 (the other way round the orders would differ, and with them, now and then, the columns' ideas
+    // of what a probability's first summand is).
+    static __device__ __forceinline__ float over_columns(float x) {
+        x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));  // row_ror:8
+        return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x124, 0xf, 0xf, true));  // row_ror:4
     }
     static __device__ __forceinline__ uint32_t high(uint32_t lo, uint32_t hi) {
         return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
@@ -315,19 +344,19 @@ struct Rows {
                 for (int x = 0; x < BITS / 4; ++x) e.w[x] = w.k[t][k / kSteps][k % kSteps * (BITS / 4) + x];
                 const bf16x8 f = __builtin_bit_cast(bf16x8, e.bf16(scale));
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p)
+                for (int p = NM - 1; p >= 0; --p)
 #pragma unroll
                     for (int r = 0; r < RT; ++r)
                         s[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, q[r][k][p].v),
                                                                           s[t][r], 0, 0, 0);
             }
         }
-        Frag<uint16_t> pr[RT][NP];
+        Frag<uint16_t> pr[RT][NM];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[e / 4][r][e % 4];
+            for (int e = 0; e < 8; ++e) x[e] = PACK ? over_columns(s[e / 4][r][e % 4]) : s[e / 4][r][e % 4];
             masked(a, w, r, x);
             // of the lane's eight keys, those the row sees
             const int end = lim[r] - j < live ? lim[r] - j : live;
@@ -357,7 +386,10 @@ struct Rows {
                 sum[r] += x[e];
             }
             // bfloat16 queries: probabilities rounded to bfloat16 (within 2^-9 of each), their sum is not
-            split(x, pr[r]);
+            if constexpr (PACK)
+                split_own(x, i, pr[r][0]);
+            else
+                split(x, pr[r]);
         }
         float vscale[8];
 #pragma unroll
@@ -369,13 +401,13 @@ struct Rows {
     static constexpr float kSlack = BIAS ? 5.0f : 8.0f;
 
     template <int... P>
-    __device__ __forceinline__ void values(const C &w, const float (&scale)[8], const Frag<uint16_t> (&pr)[RT][NP],
+    __device__ __forceinline__ void values(const C &w, const float (&scale)[8], const Frag<uint16_t> (&pr)[RT][NM],
                                            std::integer_sequence<int, P...>) {
         (pair<P>(w, scale, pr), ...);
     }
     // Features 2 P and 2 P + 1 of the lane's.
     template <int P>
-    __device__ __forceinline__ void pair(const C &w, const float (&scale)[8], const Frag<uint16_t> (&pr)[RT][NP]) {
+    __device__ __forceinline__ void pair(const C &w, const float (&scale)[8], const Frag<uint16_t> (&pr)[RT][NM]) {
         constexpr int kWord = BITS == 4 ? P / 4 : P / 2, kPart = BITS == 4 ? P % 4 : P % 2;
         uint32_t x[8];
 #pragma unroll
@@ -389,7 +421,7 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p) {
+            for (int p = NM - 1; p >= 0; --p) {
                 const bf16x8 f = __builtin_bit_cast(bf16x8, pr[r][p].v);
                 o[r][2 * P] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                     __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3])), f, o[r][2 * P], 0, 0, 0);
@@ -401,9 +433,9 @@ struct Rows {
 
 // One block: the rows of a (sequence, key head), over the keys of one part; its waves take 32 keys in turn and
 // are joined at the end, in an order that the sizes fix.
-template <int BITS, int NB, int NP, int RT, int MM, bool HALVES, int WAVES, int DEPTH, int OCC>
+template <int BITS, int NB, int NP, int RT, int MM, bool HALVES, bool PACK, int WAVES, int DEPTH, int OCC>
 __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args a, const Cache c) {
-    using R = Rows<BITS, NB, NP, RT, MM, HALVES, WAVES>;
+    using R = Rows<BITS, NB, NP, RT, MM, HALVES, PACK, WAVES>;
     constexpr int V = R::V, kRows = 16 * RT, kWide = 32 * NB + 4;  // floats of a row: 16 rows fill the banks
     constexpr int kParts = WAVES * kRows * kWide * 4;
     __shared__ __attribute__((aligned(16))) uint8_t smem[kParts > R::kQueryBytes ? kParts : R::kQueryBytes];
@@ -459,6 +491,12 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args 
 
     // The waves' parts side by side in LDS; then each thread joins quads of features.
     __syncthreads();
+    if constexpr (PACK) {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.o[0][k][e] = R::over_columns(r.o[0][k][e]);
+    }
 #pragma unroll
     for (int q = 0; q < RT; ++q) {
         const float s = over_groups_sum<16>(r.sum[q]);
@@ -505,38 +543,39 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args 
     }
 }
 
-template <int BITS, int NB, int NP, int RT>
+template <int BITS, int NB, int NP, int RT, bool PACK>
 int launch_rows(const Args &a, const Cache &c, int mode, unsigned blocks, hipStream_t s) {
     const auto go = [&](auto mm, auto halves) {
-        hipLaunchKernelGGL((cache_rows_kernel<BITS, NB, NP, RT, decltype(mm)::value, decltype(halves)::value != 0, kRowWaves,
-                                              2, rows_per_cu(BITS, NB, NP, RT)>),
-                           dim3(blocks), dim3(64 * kRowWaves), 0, s, a, c);
+        constexpr int MM = decltype(mm)::value, kOcc = rows_per_cu(BITS, NB, PACK ? 1 : NP, RT);
+        constexpr bool HALVES = decltype(halves)::value != 0;
+        hipLaunchKernelGGL((cache_rows_kernel<BITS, NB, NP, RT, MM, HALVES, PACK, kRowWaves, 2, kOcc>), dim3(blocks),
+                           dim3(64 * kRowWaves), 0, s, a, c);
         return check_launch("cache_rows_kernel");
     };
     const auto by_page = [&](auto mm) { return c.shift == 4 ? go(mm, Const<1>{}) : go(mm, Const<0>{}); };
     return mode == kNoMask ? by_page(Const<kNoMask>{}) : mode == kKeep ? by_page(Const<kKeep>{}) : by_page(Const<kBias>{});
 }
-template <int BITS, int NP, int RT>
+template <int BITS, int NP, int RT, bool PACK = false>
 int rows_by_blocks(const Args &a, const Cache &c, int mode, unsigned blocks, hipStream_t s) {
     const int nb = row_blocks(c.k.blocks > c.v.blocks ? c.k.blocks : c.v.blocks);
-    if (nb == 2) return launch_rows<BITS, 2, NP, RT>(a, c, mode, blocks, s);
+    if (nb == 2) return launch_rows<BITS, 2, NP, RT, PACK>(a, c, mode, blocks, s);
     // wider float32 rows come 16 at most
     if constexpr (NP > 1 && RT > 1)
-        return launch_rows<BITS, 4, NP, RT>(a, c, mode, blocks, s);
+        return launch_rows<BITS, 4, NP, RT, PACK>(a, c, mode, blocks, s);
     else
-        return nb == 4 ? launch_rows<BITS, 4, NP, RT>(a, c, mode, blocks, s)
-                         : launch_rows<BITS, 8, NP, RT>(a, c, mode, blocks, s);
+        return nb == 4 ? launch_rows<BITS, 4, NP, RT, PACK>(a, c, mode, blocks, s)
+                       : launch_rows<BITS, 8, NP, RT, PACK>(a, c, mode, blocks, s);
 }
 template <int BITS>
 int rows_by_type(const Args &a, const Cache &c, int dtype, int mode, hipStream_t s) {
-    const int64_t blocks = a.batch * a.key_heads * a.splits;
+    const int64_t blocks = a.batch * a.key_heads * a.splits, rows = a.n * a.group;
     TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: too many rows");
-    const bool one = a.n * a.group <= 16;
     if (dtype == TPW_BF16)
-        return one ? rows_by_blocks<BITS, 1, 1>(a, c, mode, (unsigned)blocks, s)
-                   : rows_by_blocks<BITS, 1, 2>(a, c, mode, (unsigned)blocks, s);
-    return one ? rows_by_blocks<BITS, 3, 1>(a, c, mode, (unsigned)blocks, s)
-               : rows_by_blocks<BITS, 3, 2>(a, c, mode, (unsigned)blocks, s);
+        return rows <= 16 ? rows_by_blocks<BITS, 1, 1>(a, c, mode, (unsigned)blocks, s)
+                          : rows_by_blocks<BITS, 1, 2>(a, c, mode, (unsigned)blocks, s);
+    return rows <= kPackedRows ? rows_by_blocks<BITS, 3, 1, true>(a, c, mode, (unsigned)blocks, s)
+           : rows <= 16        ? rows_by_blocks<BITS, 3, 1>(a, c, mode, (unsigned)blocks, s)
+                               : rows_by_blocks<BITS, 3, 2>(a, c, mode, (unsigned)blocks, s);
 }
 
 }  // namespace attn
