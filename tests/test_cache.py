@@ -220,6 +220,25 @@ def test_rows_of_any_layout_are_written(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [3, 70, 1000])
+@pytest.mark.parametrize("widths", [(32, 256), (256, 32), (96, 160)], ids=str)
+def test_keys_and_values_of_very_different_widths(device, n, widths):
+    """The narrower rows need fewer blocks than the wider ones: those behind the last row do nothing."""
+    x = [rows(3, 2, n, w, 60 + k, BF16) for k, w in enumerate(widths)]
+    cache = empty_cache(3, 2, 1008, *widths, 4, device)
+    s = torch.full((3,), 5, device=device)
+    tp.cache_write_(*cache, *(y.to(device) for y in x), s)
+    got = tp.cache_read(*cache, key_width=widths[0], value_width=widths[1], starts=s, rows=n)
+    for k in (0, 1):
+        codes, scales = ref.encode(x[k], 4)
+        want, want_scales = (torch.full(y.shape, PATTERN, dtype=torch.uint8) for y in cache[2 * k:2 * k + 2])
+        want[:, :, 5:5 + n], want_scales[..., 5:5 + n] = codes, scales.transpose(-1, -2)
+        assert_equal(raw(cache[2 * k]), want)
+        assert_equal(raw(cache[2 * k + 1]), want_scales)
+        assert_equal(got[k], ref.decode(codes, scales, 4, widths[k]).to(BF16))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_a_page_shared_by_sequences_is_read_by_both(device):
     cpu, cache = filled(4, 2, 16, 64, 64, 4, device)
     pages = torch.tensor([[2, 0], [2, 3]], dtype=torch.int32)

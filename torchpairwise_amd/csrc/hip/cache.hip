@@ -21,13 +21,14 @@ struct RowsArgs {
 };
 
 // A block's share: a thread works on 8 features (a piece) of ROWS consecutive rows (whose scales lie side by
-// side: one word); 4 consecutive lanes share a block of 32 features.  What the call does not have is read from somewhere that exists and dropped: without
-// branches between them all of a thread's loads are in flight at once.
+// side: one word); 4 consecutive lanes share a block of 32 features.  What the call does not have is read from
+// somewhere that exists and dropped: without branches between them all of a thread's loads are in flight at once.
+// The narrower side has more rows to a block, and none for the last ones: those return at once.
 template <int ROWS, bool PAGED>
 struct Share {
     int64_t b, h, first;  // first row of the block's
     int piece, r, per;    // the thread's piece and its place among the `per` threads of that
-    int rows;             // of the call's
+    int rows;             // of the call's (0: none left)
     int64_t entry[ROWS];  // where the thread's rows lie: entry of the cache's first dimension
     int row[ROWS];
     bool live[ROWS];      // the call has the row, and it has a place
@@ -42,7 +43,7 @@ struct Share {
         h = bh % a.heads;
         first = (int64_t)(id % a.tiles) * (ROWS * per);
         const int64_t left = a.n - first;
-        rows = left < ROWS * per ? (int)left : ROWS * per;
+        rows = left <= 0 ? 0 : left < ROWS * per ? (int)left : ROWS * per;
         const int64_t start = (a.starts ? a.starts[b] : 0) + first, counted = a.counts ? a.counts[b] - first : rows;
         const int count = counted < 0 ? 0 : counted < rows ? (int)counted : rows;
 #pragma unroll
@@ -96,6 +97,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const RowsArgs a) {
     const int side = blockIdx.y;
     const Side &s = side ? a.c.v : a.c.k;
     const Share<ROWS, PAGED> p(a, s);
+    if (p.rows == 0) return;
     const T *base = reinterpret_cast<const T *>(a.x[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.first * a.xn[side];
     const int f = 8 * p.piece, d = a.width[side];
     T raw[ROWS][8] = {};
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const RowsArgs a) {
     const Share<ROWS, PAGED> p(a, s);
     T *base = reinterpret_cast<T *>(a.y[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.first * a.xn[side];
     const int f = 8 * p.piece, d = a.width[side];
-    if (f >= d || p.r >= p.per) return;
+    if (p.rows == 0 || f >= d || p.r >= p.per) return;
     Eight<BITS> w[ROWS] = {};
     uint32_t byte[ROWS] = {};
     if (a.m > 0 && a.c.first > 0) {
