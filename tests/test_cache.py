@@ -239,6 +239,27 @@ def test_keys_and_values_of_very_different_widths(device, n, widths):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [1, 70])
+def test_starts_and_counts_at_the_ends_of_their_type(device, n):
+    least, most = -2 ** 63, 2 ** 63 - 1
+    starts = torch.tensor([least, least + 1, most, most - 1, 0, 0, 0], device=device)
+    counts = torch.tensor([most, most, most, most, least, least + 1, most], device=device)
+    x = rows(7, 2, n, 64, 70)
+    cache = empty_cache(7, 2, 80, 64, 64, 8, device)
+    before = [raw(y).clone() for y in cache]
+    tp.cache_write_(*cache, x.to(device), x.to(device), starts, counts=counts)
+    codes, scales = ref.encode(x[6:], 8)
+    for k, (y, w) in enumerate(zip(cache, before)):
+        if k % 2:
+            w[6:, :, :, :n] = scales.transpose(-1, -2)
+        else:
+            w[6:, :, :n] = codes
+        assert_equal(raw(y), w)
+    for y in tp.cache_read(*cache, dtype=F32, starts=starts, rows=n, counts=counts):
+        assert (y[:6] == 0).all() and (y[6] != 0).any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_a_page_shared_by_sequences_is_read_by_both(device):
     cpu, cache = filled(4, 2, 16, 64, 64, 4, device)
     pages = torch.tensor([[2, 0], [2, 3]], dtype=torch.int32)
@@ -597,6 +618,27 @@ def test_refusals(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_writing_refuses_tensors_that_share_memory(device):
+    kc, ks, vc, vs = tp.quantized_cache(2, 2, 32, 64, device=device)
+    x, s = torch.zeros(2, 2, 3, 64, device=device), torch.zeros(2, dtype=torch.long, device=device)
+    inside = vc.view(-1)[:768].view(torch.bfloat16).view(2, 2, 3, 32)
+    for cache in ((kc, ks, kc, vs), (kc, ks, vc, ks)):
+        with pytest.raises(RuntimeError, match="overlap|single memory|refer"):
+            tp.cache_write_(*cache, x, x, s)
+    narrow = tp.quantized_cache(2, 2, 32, 32, device=device)
+    with pytest.raises(RuntimeError, match="overlap|single memory|refer"):
+        tp.cache_write_(narrow[0], narrow[1], vc, vs, inside, x.bfloat16(), s)
+    # side by side in one allocation is fine, and so is reading keys as values
+    both = torch.zeros(2, 2, 2, 32, 32, dtype=torch.uint8, device=device)
+    tp.cache_write_(both[0], ks, both[1], vs, x, x + 1, s)
+    both = both.permute(1, 0, 2, 3, 4).contiguous().permute(1, 0, 2, 3, 4)
+    tp.cache_write_(both[0], ks, both[1], vs, x, x + 1, s)
+    k, v = tp.cache_read(both[1], vs, both[1], vs, dtype=F32, rows=3)
+    assert_equal(k, v)
+    assert (k == 1).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_writing_marks_the_cache_as_changed(device):
     cache = tp.quantized_cache(1, 1, 16, 32, device=device)
     x = torch.ones(1, 1, 1, 32, device=device)
@@ -658,6 +700,13 @@ def test_c_entries_refuse():
     assert lib.tpw_cache_attention_workspace_size(None, None) == 0
     a = attention(batch=0)
     assert lib.tpw_cache_attention(C.byref(a), C.byref(desc(first=0)), None, None) == 0
+    # more blocks than a launch has room for
+    for f in (lib.tpw_cache_write, lib.tpw_cache_read):
+        assert write(desc(first=1 << 24), batch=1 << 24, f=f) == 1 and b"too many" in lib.tpw_last_error()
+        assert write(desc(heads=1 << 62), f=f) == 1 and b"too many" in lib.tpw_last_error()
+    a = attention(batch=1 << 24)
+    assert lib.tpw_cache_attention(C.byref(a), C.byref(desc(first=1 << 24)), None, None) == 1
+    assert b"too many" in lib.tpw_last_error()
 
 
 # ---------------------------------------------------------------- on the GPU

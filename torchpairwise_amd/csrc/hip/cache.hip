@@ -44,8 +44,10 @@ struct Share {
         first = (int64_t)(id % a.tiles) * (ROWS * per);
         const int64_t left = a.n - first;
         rows = left <= 0 ? 0 : left < ROWS * per ? (int)left : ROWS * per;
-        const int64_t start = (a.starts ? a.starts[b] : 0) + first, counted = a.counts ? a.counts[b] - first : rows;
-        const int count = counted < 0 ? 0 : counted < rows ? (int)counted : rows;
+        // starts so far out that none of the call's rows has a place count as -n: no sum passes 64 bits
+        const int64_t from = a.starts ? a.starts[b] : 0, start = (from >= a.m || from < -a.n ? -a.n : from) + first;
+        const int64_t counted = a.counts ? a.counts[b] : a.n;
+        const int count = counted <= first ? 0 : counted - first < rows ? (int)(counted - first) : rows;
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
             const int64_t q = start + own(k);
@@ -208,7 +210,7 @@ int launch(RowsArgs &a, bool write, int64_t batch, int64_t blocks, hipStream_t s
         constexpr int ROWS = decltype(rows)::value;
         constexpr bool WHOLE = decltype(whole)::value, PAGED = decltype(paged)::value;
         const int64_t tiles = cdiv(a.n, ROWS * (256 / (4 * blocks))), all = tiles * batch * a.heads;
-        TPW_REQUIRE(all < (int64_t(1) << 31), "cache: too many rows");
+        TPW_REQUIRE(all <= kMostBlocks, "cache: too many rows");
         a.tiles = (uint32_t)tiles;
         const dim3 grid((unsigned)all, 2);
         if (write) {
@@ -270,6 +272,8 @@ int read_cache(const tpw_cache_desc *d, int64_t batch, Cache &c) {
     TPW_REQUIRE(d, "cache: null descriptor");
     TPW_REQUIRE(d->bits == 4 || d->bits == 8, "cache: 4 or 8 bits");
     TPW_REQUIRE(batch >= 0 && d->first >= 0 && d->heads >= 1 && d->rows >= 0, "cache: invalid sizes");
+    TPW_REQUIRE(batch <= kMostBlocks && d->heads <= kMostBlocks && batch * d->heads <= kMostBlocks,
+                "cache: too many sequences and heads");
     TPW_REQUIRE(d->key_blocks >= 1 && d->key_blocks <= 8 && d->value_blocks >= 1 && d->value_blocks <= 8,
                 "cache: rows have 1 to 8 blocks of 32 features");
     TPW_REQUIRE(d->rows % 16 == 0, "cache: rows must come in multiples of 16");

@@ -144,6 +144,9 @@ __device__ __forceinline__ uint2 to_fp8(const float (&x)[8], float scale) {
     return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
 }
 
+// Blocks of 256 threads that one dimension of a launch has room for: 2^32 threads.
+constexpr int64_t kMostBlocks = (int64_t(1) << 24) - 1;
+
 // Host side (cache.hip): checks a cache against its batch and reads it into the kernels' form.
 int read_cache(const tpw_cache_desc *d, int64_t batch, Cache &c);
 

@@ -569,7 +569,7 @@ int rows_by_blocks(const Args &a, const Cache &c, int mode, unsigned blocks, hip
 template <int BITS>
 int rows_by_type(const Args &a, const Cache &c, int dtype, int mode, hipStream_t s) {
     const int64_t blocks = a.batch * a.key_heads * a.splits, rows = a.n * a.group;
-    TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: too many rows");
+    TPW_REQUIRE(blocks <= cache::kMostBlocks, "attention: too many rows");
     if (dtype == TPW_BF16)
         return rows <= 16 ? rows_by_blocks<BITS, 1, 1>(a, c, mode, (unsigned)blocks, s)
                           : rows_by_blocks<BITS, 1, 2>(a, c, mode, (unsigned)blocks, s);

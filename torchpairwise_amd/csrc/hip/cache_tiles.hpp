@@ -156,7 +156,7 @@ int launch_tiles(const Args &a, const Cache &c, int dtype, int mode, hipStream_t
         constexpr int DP = decltype(dp)::value, MM = decltype(mm)::value, W = Tiles<T, DP>::kWidth;
         constexpr int kWaves = Tiles<T, DP>::kWaves, kKeys = Tiles<T, DP>::kKeys;
         const int64_t blocks = a.batch * a.key_heads * a.tiles * a.splits;
-        TPW_REQUIRE(blocks < (int64_t(1) << 31), "attention: too many rows");
+        TPW_REQUIRE(blocks * kWaves <= 4 * cache::kMostBlocks, "attention: too many rows");
         hipLaunchKernelGGL((cache_tiles_kernel<T, W, DP, kKeys, MM, BITS, kWaves>), dim3((unsigned)blocks),
                            dim3(64 * kWaves), 0, s, a, c);
         return check_launch("cache_tiles_kernel");

@@ -167,12 +167,6 @@ at::Tensor rows_at(const at::Tensor &codes, const at::Tensor &scales, int64_t bi
     return x.masked_fill((first < 0).unsqueeze(1).unsqueeze(-1), 0.0);
 }
 
-// Rows that several others share cannot be written.
-void check_written(const CacheTensors &c) {
-    for (const at::Tensor *x : {&c.key_codes, &c.key_scales, &c.value_codes, &c.value_scales})
-        at::assert_no_internal_overlap(*x);
-}
-
 int64_t batch_of(const char *name, const at::Tensor &key, const at::Tensor &value) {
     TORCH_CHECK(key.dim() == 4 && value.dim() == 4, name, ": expected 4-D key and value, got ", key.dim(), " and ",
                 value.dim(), " dimensions");
@@ -201,6 +195,17 @@ RowTensors check_rows(const char *name, const CacheTensors &c, const at::Tensor 
     return {key, value, check_index(name, "starts", starts, c.batch, key), check_index(name, "counts", counts, c.batch, key)};
 }
 
+// Rows that several others share cannot be written, nor keys where the values go, nor what is read meanwhile.
+void check_written(const CacheTensors &c, const RowTensors &r) {
+    const at::Tensor *all[] = {&c.key_codes, &c.key_scales, &c.value_codes, &c.value_scales};
+    for (int i = 0; i < 4; ++i) {
+        at::assert_no_internal_overlap(*all[i]);
+        for (int j = 0; j < i; ++j) at::assert_no_overlap(*all[i], *all[j]);
+        for (const at::Tensor *x : {&r.key, &r.value, &r.starts, &r.counts, &c.pages})
+            if (x->defined()) at::assert_no_overlap(*all[i], *x);
+    }
+}
+
 void cache_write_cpu(at::Tensor &key_codes, at::Tensor &key_scales, at::Tensor &value_codes, at::Tensor &value_scales,
                      const at::Tensor &key, const at::Tensor &value, const at::Tensor &starts, const OptTensor &counts,
                      const OptTensor &pages) {
@@ -208,7 +213,7 @@ void cache_write_cpu(at::Tensor &key_codes, at::Tensor &key_scales, at::Tensor &
     const auto c = check_cache(name, key_codes, key_scales, value_codes, value_scales, pages,
                                batch_of(name, key, value));
     const auto r = check_rows(name, c, key, value, starts, counts);
-    check_written(c);
+    check_written(c, r);
     auto at = places(c, r.starts, r.counts, key.size(2));
     auto live = (at.first >= 0).flatten().nonzero().flatten();
     if (live.numel() == 0) return;
@@ -354,7 +359,7 @@ void cache_write_cuda(at::Tensor &key_codes, at::Tensor &key_scales, at::Tensor 
     const auto c = check_cache(name, key_codes, key_scales, value_codes, value_scales, pages,
                                batch_of(name, key, value));
     auto r = check_rows(name, c, key, value, starts, counts);
-    check_written(c);
+    check_written(c, r);
     if (key.size(0) * key.size(2) == 0 || c.capacity == 0 || key_codes.size(0) == 0) return;
     DeviceGuard guard(key.device());
     r.key = dense_rows(r.key, false);
