@@ -54,6 +54,7 @@ struct Args {
     float gscale;  // scale (backward)
     int causal;
     int whole_q;    // (few rows over a cache) queries are whole pieces of 8 features
+    int whole_rows; // (few rows over a cache) not in parts, by more waves
     int dwords;     // (forward) operands of whole dwords that are not whole pieces, read as they lie
     int64_t tiles;  // row tiles (dk / dv: key tiles) per (batch, key head)
     int splits;     // parts of the summed axis

@@ -37,16 +37,23 @@ size_t parts_bytes(const Args &a) {
     return a.splits > 1 ? (size_t)a.splits * a.batch * a.heads * a.n * (quads4(a.dv) + 2) * 4 : 0;
 }
 
-// As many parts as fill the card's places once: a block's own time (queries, first loads, joining) is that of
-// 16 chunks of 32 keys, so a second round costs more than long parts do.
+// As many parts as fill the card's places once: a block's own time (queries, first loads, joining: 5 to 7 us) is that
+// of many chunks of 32 keys, so a second round costs more than long parts do.  Short caches are left whole, by blocks
+// of twice the waves, where a SIMD's chunks in turn are no more than those of a part and two: what the second launch
+// and the parts' way through memory take (4 bits, 128 features, 16 x 8 heads: 256 keys 7.2 -> 5.7 us, 512 8.5 -> 7.4,
+// 1024 11.6 -> 9.6, where 1664 stay at 13; one sequence: 256 keys 7.0 -> 5.6).
 void plan_rows(Args &a, const cache::Cache &c, int bits, int dtype) {
     const int nb = row_blocks(c.k.blocks > c.v.blocks ? c.k.blocks : c.v.blocks);
     const int64_t rows = a.n * a.group;
-    const int64_t per_cu = rows_per_cu(bits, nb, dtype == TPW_F32 && rows > kPackedRows ? 3 : 1, rows <= 16 ? 1 : 2);
-    const int64_t bk = a.batch * a.key_heads, most = cdiv(cdiv(a.m, 32), kRowWaves);
+    const int np = dtype == TPW_F32 && rows > kPackedRows ? 3 : 1, rt = rows <= 16 ? 1 : 2;
+    const int64_t per_cu = rows_per_cu(bits, nb, np, rt);
+    const int64_t bk = a.batch * a.key_heads, chunks = cdiv(a.m, 32), most = cdiv(chunks, kRowWaves);
     int64_t splits = bk > 0 ? 256 * per_cu / bk : 1;
-    splits = splits > most ? most : splits;
-    a.splits = (int)(splits < 1 ? 1 : splits > kMaxParts ? kMaxParts : splits);
+    splits = splits > most ? most : splits > kMaxParts ? kMaxParts : splits;
+    const int64_t shared = cdiv(bk * splits, 256);  // parts that share a CU, a wave of each on a SIMD
+    a.whole_rows = splits > 1 && may_be_whole(bits, nb, np, rt) &&
+                   kWholeWaves / 4 * cdiv(chunks, kWholeWaves) <= shared * cdiv(chunks, kRowWaves * splits) + 2;
+    a.splits = a.whole_rows || splits < 1 ? 1 : (int)splits;
     a.tiles = 1;
 }
 

@@ -12,11 +12,17 @@ namespace attn {
 // The form for few rows, up to kFewRows a key head (cache_rows.hpp).
 constexpr int64_t kFewRows = 32;
 constexpr int64_t kPackedRows = 4;  // of float32 whose summands share a product
-constexpr int kRowWaves = 4;  // waves of a block
-// Blocks that share a CU, as their registers leave (NP: summands of a probability, RT: 16 rows each): three up
-// to 128 features in 4 bits, one where two rows of sums, wide rows in 8 bits or float32's summands fill them.
+constexpr int kRowWaves = 4;        // waves of a block that does one of several parts
+constexpr int kWholeWaves = 8;      // .. that works alone on a sequence and head
+// Blocks that share a CU, as their registers leave (NP: summands of a probability, RT: 16 rows each).  Four of
+// 64 features would fit, and were slower where they fill the card (1664 keys of 16 x 8 heads 10.8 -> 11.8 us).
 constexpr int rows_per_cu(int bits, int nb, int np, int rt) {
-    return (nb == 8 && (bits == 8 || np > 1 || rt > 1)) || (np > 1 && rt > 1) ? 1 : bits == 4 && np == 1 && rt == 1 ? 3 : 2;
+    if (np > 1 || rt > 1) return nb == 8 || (np > 1 && rt > 1) ? 1 : 2;
+    return nb == 8 ? (bits == 4 ? 2 : 1) : bits == 4 ? 3 : 2;
+}
+// Up to 16 rows of bfloat16, 4 of float32, may be worked on by kWholeWaves (cache_attention.hip).
+constexpr bool may_be_whole(int bits, int nb, int np, int rt) {
+    return np == 1 && rt == 1 && rows_per_cu(bits, nb, np, rt) > 1;
 }
 // 64, 128 or 256 features.
 constexpr int row_blocks(int most) { return most <= 2 ? 2 : most <= 4 ? 4 : 8; }

@@ -545,14 +545,20 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args 
 
 template <int BITS, int NB, int NP, int RT, bool PACK>
 int launch_rows(const Args &a, const Cache &c, int mode, unsigned blocks, hipStream_t s) {
-    const auto go = [&](auto mm, auto halves) {
-        constexpr int MM = decltype(mm)::value, kOcc = rows_per_cu(BITS, NB, PACK ? 1 : NP, RT);
+    const auto go = [&](auto mm, auto halves, auto waves) {
+        constexpr int MM = decltype(mm)::value, WAVES = decltype(waves)::value;
+        constexpr int kOcc = WAVES > kRowWaves ? 1 : rows_per_cu(BITS, NB, PACK ? 1 : NP, RT);
         constexpr bool HALVES = decltype(halves)::value != 0;
-        hipLaunchKernelGGL((cache_rows_kernel<BITS, NB, NP, RT, MM, HALVES, PACK, kRowWaves, 2, kOcc>), dim3(blocks),
-                           dim3(64 * kRowWaves), 0, s, a, c);
+        hipLaunchKernelGGL((cache_rows_kernel<BITS, NB, NP, RT, MM, HALVES, PACK, WAVES, 2, kOcc>), dim3(blocks),
+                           dim3(64 * WAVES), 0, s, a, c);
         return check_launch("cache_rows_kernel");
     };
-    const auto by_page = [&](auto mm) { return c.shift == 4 ? go(mm, Const<1>{}) : go(mm, Const<0>{}); };
+    const auto by_waves = [&](auto mm, auto halves) {
+        if constexpr (may_be_whole(BITS, NB, PACK ? 1 : NP, RT))
+            if (a.whole_rows) return go(mm, halves, Const<kWholeWaves>{});
+        return go(mm, halves, Const<kRowWaves>{});
+    };
+    const auto by_page = [&](auto mm) { return c.shift == 4 ? by_waves(mm, Const<1>{}) : by_waves(mm, Const<0>{}); };
     return mode == kNoMask ? by_page(Const<kNoMask>{}) : mode == kKeep ? by_page(Const<kKeep>{}) : by_page(Const<kBias>{});
 }
 template <int BITS, int NP, int RT, bool PACK = false>
