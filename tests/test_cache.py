@@ -723,7 +723,7 @@ def test_results_repeat_bit_for_bit(n):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("bits,d", [(4, 64), (4, 128), (4, 250), (8, 128), (8, 250)])
-@pytest.mark.parametrize("m", [32, 240, 528, 1024, 1104])
+@pytest.mark.parametrize("m", [240, 1024, 1104])
 def test_short_caches_of_many_heads(dtype, bits, d, m):
     """Up to a length one block works on a sequence and head; past it several, whose parts are joined."""
     lengths = torch.tensor([m - k * m // 15 for k in range(16)])
