@@ -129,6 +129,40 @@ __device__ __forceinline__ void unpack8(const Frag<float> &f, float (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = f.v[i >> 2][i & 3];
 }
 
+// The upper halves of two words.
+__device__ __forceinline__ uint32_t high2(uint32_t lo, uint32_t hi) {
+    return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+}
+// fp32 values as three bf16 summands that hold all 24 bits, each what is left cut off to 8 (products with values that
+// are exact in bf16 then run at its rate).
+__device__ __forceinline__ void split3(float (&x)[8], Frag<uint16_t> (&f)[3]) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            w[e] = __float_as_uint(x[e]);
+            x[e] -= __uint_as_float(w[e] & 0xffff0000u);
+        }
+        f[p].v = make_uint4(high2(w[0], w[1]), high2(w[2], w[3]), high2(w[4], w[5]), high2(w[6], w[7]));
+    }
+}
+// The same where an infinity may be among them: its first summand alone.
+__device__ __forceinline__ void split3_any(float (&x)[8], Frag<uint16_t> (&f)[3]) {
+    uint32_t inf[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const bool is = __builtin_fabsf(x[e]) == INFINITY;
+        inf[e] = is ? __float_as_uint(x[e]) : 0u;
+        x[e] = is ? 0.0f : x[e];
+    }
+    split3(x, f);
+    f[0].v.x |= high2(inf[0], inf[1]);
+    f[0].v.y |= high2(inf[2], inf[3]);
+    f[0].v.z |= high2(inf[4], inf[5]);
+    f[0].v.w |= high2(inf[6], inf[7]);
+}
+
 // ---- LDS tiles -----------------------------------------------------------------------------
 // A tile of ROWS rows of DP features, with room for a power of two of them, lies as 16-byte pieces,
 // piece c of row r at position c ^ swz(r).  Every 16 consecutive rows put one piece into the 16

@@ -8,15 +8,16 @@ namespace tpw {
 namespace attn {
 
 // Per-row running softmax of one wave's W rows and the loop over one key tile.  GAPS: some of a tile's keys
-// may be no keys at all.
-template <typename T, int W, int DP, int BN, int MM, bool DWORDS, bool GAPS = false>
+// may be no keys at all.  QT: the queries' type; float over tiles of bf16 (whose values are exact) takes three products.
+template <typename T, int W, int DP, int BN, int MM, bool DWORDS, bool GAPS = false, typename QT = T>
 struct Forward {
+    static constexpr int NP = sizeof(QT) / sizeof(T) == 2 ? 3 : 1;  // summands of a query and a probability
     using M = Mma<T, W>;
     using Acc = typename M::Acc;
     using CR = ColReader<T, DP, W>;
     static constexpr int NB = BN / W, NQ = NB * M::Q, DB = DP / W, QS = DP / M::KS;
 
-    Frag<T> q[QS];
+    Frag<T> q[QS][NP];
     Acc o[DB];
     float top, sum;  // running maximum (in units of log2 e; kBias: natural) and the lane's part of the sum
     int lim, wlim_min, wlim_max;  // keys seen: this lane's row, over the wave's rows
@@ -39,16 +40,24 @@ struct Forward {
         }
         wlim_max = __builtin_amdgcn_readfirstlane(wlim_max);
         wlim_min = __builtin_amdgcn_readfirstlane(wlim_min);
-        const T *row = live ? reinterpret_cast<const T *>(a.q.p) + b * a.q.b + qh * a.q.h + qi * a.q.n : nullptr;
+        const QT *row = live ? reinterpret_cast<const QT *>(a.q.p) + b * a.q.b + qh * a.q.h + qi * a.q.n : nullptr;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
-            q[s] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d, DWORDS);
-            if (a.qsign != 1.0f) {
+            if constexpr (NP == 1) {
+                q[s][0] = load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d, DWORDS);
+                if (a.qsign != 1.0f) {
+                    float x[8];
+                    unpack8(q[s][0], x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] *= a.qsign;
+                    q[s][0] = pack8(x, T{});
+                }
+            } else {
                 float x[8];
-                unpack8(q[s], x);
+                unpack8(load_row8(row, M::KS * s + 8 * (lane / W), (int)a.d, DWORDS), x);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] *= a.qsign;
-                q[s] = pack8(x, T{});
+                split3_any(x, q[s]);
             }
         }
 #pragma unroll
@@ -80,10 +89,14 @@ struct Forward {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
 #pragma unroll
-                    for (int i = 0; i < NB; ++i) M::mma1(s[i], f[i], q[k], e);
+                    for (int i = 0; i < NB; ++i) M::mma1(s[i], f[i], q[k][0], e);
             } else {
 #pragma unroll
-                for (int i = 0; i < NB; ++i) M::mma(s[i], rr.read(kt, i, k), q[k]);
+                for (int i = 0; i < NB; ++i) {
+                    const Frag<T> f = rr.read(kt, i, k);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) M::mma(s[i], f, q[k][p]);
+                }
             }
         }
 
@@ -185,21 +198,32 @@ struct Forward {
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[4 * u + e] = s[(2 * t + u) / M::Q][4 * ((2 * t + u) % M::Q) + e];
-            const Frag<T> p = pack8(x, T{});
+            if constexpr (NP == 1) {
+                const Frag<T> p = pack8(x, T{});
 #pragma unroll
-            for (int c = 0; c < CR::kPieces; ++c) CR::use(o, c, cr.read(vt, t, c), p);
+                for (int c = 0; c < CR::kPieces; ++c) CR::use(o, c, cr.read(vt, t, c), p);
+            } else {
+                Frag<T> p[NP];
+                split3(x, p);
+#pragma unroll
+                for (int c = 0; c < CR::kPieces; ++c) {
+                    const auto f = cr.read(vt, t, c);
+#pragma unroll
+                    for (int u = NP - 1; u >= 0; --u) CR::use(o, c, f, p[u]);
+                }
+            }
         }
     }
 };
 
-// Sets tiles and splits for the element type and width.
+// Sets tiles and splits for the element type and width, per_cu blocks to a CU.
 template <typename T, int DP>
-void plan(Args &a) {
+void plan(Args &a, int64_t per_cu = Tiles<T, DP>::kPerCu, int products = 2) {
     using L = Tiles<T, DP>;
     constexpr int64_t kOwn = L::kWaves * L::kWidth;
     a.tiles = cdiv(a.n * a.group, kOwn);
-    a.splits = (int)parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, L::kKeys), L::kPerCu, uneven(a),
-                              step_us<T, DP>(kOwn, L::kKeys, 2, L::kPerCu),
+    a.splits = (int)parts_for(a.batch * a.key_heads * a.tiles, cdiv(a.m, L::kKeys), per_cu, uneven(a),
+                              step_us<T, DP>(kOwn, L::kKeys, products, per_cu),
                               part_us(a.batch * a.heads * a.n, quads4(a.dv)));
 }
 

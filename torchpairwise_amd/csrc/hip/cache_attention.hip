@@ -58,8 +58,13 @@ void plan_rows(Args &a, const cache::Cache &c, int bits, int dtype) {
 }
 
 void plan_tiles(Args &a, int dtype) {
-    by_type(a, dtype, kNoMask, [&](auto t, auto dp, auto) {
-        plan<decltype(t), decltype(dp)::value>(a);
+    by_width<uint16_t>(a, kNoMask, [&](auto t, auto dp, auto) {
+        using T = decltype(t);
+        constexpr int DP = decltype(dp)::value;
+        if (dtype == TPW_BF16)
+            plan<T, DP>(a);
+        else
+            plan<T, DP>(a, tiles_per_simd(4, DP), 6);
         return TPW_OK;
     });
 }

@@ -29,7 +29,8 @@ constexpr int row_blocks(int most) { return most <= 2 ? 2 : most <= 4 ? 4 : 8; }
 int cache_rows4(const Args &a, const cache::Cache &c, int dtype, int mode, hipStream_t s);
 int cache_rows8(const Args &a, const cache::Cache &c, int dtype, int mode, hipStream_t s);
 
-// The form for many rows (cache_tiles.hpp).
+// The form for many rows (cache_tiles.hpp): waves that its registers leave a SIMD (blocks of four waves a CU).
+constexpr int tiles_per_simd(int size, int dp) { return size == 4 && dp > 128 ? 1 : 2; }
 int cache_tiles4(const Args &a, const cache::Cache &c, int dtype, int mode, hipStream_t s);
 int cache_tiles8(const Args &a, const cache::Cache &c, int dtype, int mode, hipStream_t s);
 

@@ -119,24 +119,14 @@ struct Rows {
         for (int x = 0; x < kOwn; ++x) {
             const int id = x * kThreads + (int)threadIdx.x, r = id / (4 * NB), f = id % (4 * NB) * 8;
             if (kPieces % kThreads && id >= kPieces) break;
-            float z[8], inf[8];
+            float z[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                z[e] = to_f32(y[x].x[e]) * a.qsign;
-                inf[e] = 0.0f;
-                if (NP > 1 && __builtin_fabsf(z[e]) == INFINITY) {  // its first summand alone
-                    inf[e] = z[e];
-                    z[e] = 0.0f;
-                }
-            }
+            for (int e = 0; e < 8; ++e) z[e] = to_f32(y[x].x[e]) * a.qsign;
             Frag<uint16_t> w[NP];
-            split(z, w);
-            if constexpr (NP > 1) {
-                w[0].v.x |= high(__float_as_uint(inf[0]), __float_as_uint(inf[1]));
-                w[0].v.y |= high(__float_as_uint(inf[2]), __float_as_uint(inf[3]));
-                w[0].v.z |= high(__float_as_uint(inf[4]), __float_as_uint(inf[5]));
-                w[0].v.w |= high(__float_as_uint(inf[6]), __float_as_uint(inf[7]));
-            }
+            if constexpr (NP == 1)
+                w[0] = pack8(z, uint16_t{});
+            else
+                split3_any(z, w);
 #pragma unroll
             for (int p = 0; p < NP; ++p) *reinterpret_cast<uint4 *>(to + p * kPlane + r * kRow + 2 * f) = w[p].v;
         }
@@ -156,24 +146,6 @@ struct Rows {
                 }
     }
 
-    // One summand in bfloat16, rounded (queries: exact); or three that hold all 24 bits, each what is left cut
-    // off to 8.
-    static __device__ __forceinline__ void split(float (&x)[8], Frag<uint16_t> (&f)[NP]) {
-        if constexpr (NP == 1) {
-            f[0] = pack8(x, uint16_t{});
-        } else {
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                uint32_t w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    w[e] = __float_as_uint(x[e]);
-                    x[e] -= __uint_as_float(w[e] & 0xffff0000u);
-                }
-                f[p].v = make_uint4(high(w[0], w[1]), high(w[2], w[3]), high(w[4], w[5]), high(w[6], w[7]));
-            }
-        }
-    }
     // The lane's own summand of its row's eight probabilities (the fourth: nothing is left for it).
     static __device__ __forceinline__ void split_own(float (&x)[8], int i, Frag<uint16_t> &f) {
         uint32_t w[8];
@@ -186,7 +158,7 @@ struct Rows {
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(x[e]);
-        f.v = make_uint4(high(w[0], w[1]), high(w[2], w[3]), high(w[4], w[5]), high(w[6], w[7]));
+        f.v = make_uint4(high2(w[0], w[1]), high2(w[2], w[3]), high2(w[4], w[5]), high2(w[6], w[7]));
     }
     // The sum over a row's four columns (lanes i, i + 4, .. of 16), the same bits in every one of them: 8 apart
     // first, then 4 (the other way round the orders would differ, and with them, now and then, the columns' ideas
@@ -194,9 +166,6 @@ struct Rows {
     static __device__ __forceinline__ float over_columns(float x) {
         x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));  // row_ror:8
         return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x124, 0xf, 0xf, true));  // row_ror:4
-    }
-    static __device__ __forceinline__ uint32_t high(uint32_t lo, uint32_t hi) {
-        return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
     }
 
     // Rows 0 .. n - 1 from a place on: buffers whose range ends with the last of them.
@@ -388,8 +357,10 @@ struct Rows {
             // bfloat16 queries: probabilities rounded to bfloat16 (within 2^-9 of each), their sum is not
             if constexpr (PACK)
                 split_own(x, i, pr[r][0]);
+            else if constexpr (NP == 1)
+                pr[r][0] = pack8(x, uint16_t{});
             else
-                split(x, pr[r]);
+                split3(x, pr[r]);
         }
         float vscale[8];
 #pragma unroll

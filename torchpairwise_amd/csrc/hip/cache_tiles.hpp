@@ -12,12 +12,12 @@ using cache::Cache;
 using cache::Eight;
 using cache::Side;
 
-// Brings tiles of BN keys and their values into LDS as the element type T.  A slot is a block of 32 features
+// Brings tiles of BN keys and their values into LDS in bfloat16, which holds them exactly.  A slot is a block of 32 features
 // of one row: threads of 64 (32) consecutive rows share a block, so that the 16-byte stores of 16 of them
 // fall on 16 different slots of the banks.  Codes wait in registers while the tile before is worked on.
-template <typename T, int DP, int BN, int WAVES, int BITS>
+template <int DP, int BN, int WAVES, int BITS>
 struct Decoder {
-    using L = Tile<T, DP>;
+    using L = Tile<uint16_t, DP>;
     static constexpr int kThreads = 64 * WAVES, kBlocks = L::P / 32, kSlots = 2 * BN * kBlocks / kThreads;
     static_assert(2 * BN * kBlocks % kThreads == 0 && BN * kBlocks % 64 == 0, "whole waves of slots");
     uint4 codes[kSlots][BITS / 4];
@@ -59,7 +59,7 @@ struct Decoder {
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
             const int id = i * kThreads + tid, r = id % BN, block = id / BN;  // blocks of the keys, then the values
-            const int piece = block % kBlocks * (32 / L::E);
+            const int piece = block % kBlocks * 4;
             if (DP < L::P && block % kBlocks * 32 >= DP) continue;
             const uint32_t row = to + (uint32_t)(block / kBlocks * BN * L::kRowBytes + r * L::kRowBytes);
             const float f = cache::scale_of(scale[i]);
@@ -71,14 +71,7 @@ struct Decoder {
                 Eight<BITS> e;
 #pragma unroll
                 for (int y = 0; y < BITS / 4; ++y) e.w[y] = w[x * (BITS / 4) + y];
-                if constexpr (sizeof(T) == 2) {
-                    put(row, r, piece + x, e.bf16(f));
-                } else {
-                    float v[8];
-                    e.f32(f, v);
-                    put(row, r, piece + 2 * x, *reinterpret_cast<uint4 *>(v));
-                    put(row, r, piece + 2 * x + 1, *reinterpret_cast<uint4 *>(v + 4));
-                }
+                put(row, r, piece + x, e.bf16(f));
             }
         }
     }
@@ -89,9 +82,11 @@ struct Decoder {
 };
 
 // One block: kWaves * W query rows of the rows that share a key head, over the keys of one part.
-template <typename T, int W, int DP, int BN, int MM, int BITS, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, 2) void cache_tiles_kernel(const Args a, const Cache c) {
-    using F = Forward<T, W, DP, BN, MM, false, true>;
+template <typename QT, int DP, int MM, int BITS, int kWaves, int kPerSimd>
+__global__ __launch_bounds__(64 * kWaves, kPerSimd) void cache_tiles_kernel(const Args a, const Cache c) {
+    using T = uint16_t;
+    constexpr int W = Tiles<T, DP>::kWidth, BN = Tiles<T, DP>::kKeys;
+    using F = Forward<T, W, DP, BN, MM, false, true, QT>;
     constexpr uint32_t kTileBytes = BN * Tile<T, DP>::kRowBytes;
     // two buffers of a key tile and a value tile
     __shared__ __attribute__((aligned(256))) uint4 smem[4 * kTileBytes / 16];
@@ -114,7 +109,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_tiles_kernel(const Args 
     const int t0 = (int)((int64_t)nt * part / a.splits), t1 = (int)((int64_t)nt * (part + 1) / a.splits);
 
     const uint32_t lds = tile::lds_addr(smem);
-    Decoder<T, DP, BN, kWaves, BITS> d;
+    Decoder<DP, BN, kWaves, BITS> d;
     if (t0 < t1) {
         d.load(c, b, kh, t0 * BN, (int)len, threadIdx.x);
         d.store(lds, threadIdx.x);
@@ -145,22 +140,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_tiles_kernel(const Args 
         F::CR::each(f.o, lane, [&](int at, f32x4 v) { store4(p, at, width, v); });
         return;
     }
-    const OutRow<T> out(a, b, f.qh, f.qi);
+    const OutRow<QT> out(a, b, f.qh, f.qi);
     F::CR::each(f.o, lane, [&](int at, f32x4 v) { out.store(at, v * inv); });
 }
 
-template <int BITS>
-int launch_tiles(const Args &a, const Cache &c, int dtype, int mode, hipStream_t s) {
-    return by_type(a, dtype, mode, [&](auto t, auto dp, auto mm) {
-        using T = decltype(t);
-        constexpr int DP = decltype(dp)::value, MM = decltype(mm)::value, W = Tiles<T, DP>::kWidth;
-        constexpr int kWaves = Tiles<T, DP>::kWaves, kKeys = Tiles<T, DP>::kKeys;
+template <int BITS, typename QT>
+int launch_tiles_of(const Args &a, const Cache &c, int mode, hipStream_t s) {
+    return by_width<QT>(a, mode, [&](auto, auto dp, auto mm) {
+        constexpr int DP = decltype(dp)::value, MM = decltype(mm)::value, kWaves = Tiles<uint16_t, DP>::kWaves;
         const int64_t blocks = a.batch * a.key_heads * a.tiles * a.splits;
         TPW_REQUIRE(blocks * kWaves <= 4 * cache::kMostBlocks, "attention: too many rows");
-        hipLaunchKernelGGL((cache_tiles_kernel<T, W, DP, kKeys, MM, BITS, kWaves>), dim3((unsigned)blocks),
+        constexpr int kPerSimd = tiles_per_simd(sizeof(QT), DP);
+        hipLaunchKernelGGL((cache_tiles_kernel<QT, DP, MM, BITS, kWaves, kPerSimd>), dim3((unsigned)blocks),
                            dim3(64 * kWaves), 0, s, a, c);
         return check_launch("cache_tiles_kernel");
     });
+}
+template <int BITS>
+int launch_tiles(const Args &a, const Cache &c, int dtype, int mode, hipStream_t s) {
+    return dtype == TPW_BF16 ? launch_tiles_of<BITS, uint16_t>(a, c, mode, s) : launch_tiles_of<BITS, float>(a, c, mode, s);
 }
 
 }  // namespace attn
