@@ -366,6 +366,25 @@ def test_pages_that_are_not_there_hold_no_keys(device, dtype, bits, n, mask):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("kind", ["none", "keep", "bias"])
+@pytest.mark.parametrize("n,page", [(9, 0), (16, 16), (17, 0), (30, 64), (32, 0), (33, 0)])
+def test_wide_float32_rows_in_groups(device, bits, kind, n, page):
+    """More than 128 features of float32: 16 rows a block up to 64, then tiles."""
+    b, h, hk, m, d, dv = 2, 4, 2, 320, 200, 136
+    mask = None
+    if kind != "none":
+        mask = torch.randn(b, h, n, m, generator=gen(7))
+        mask = mask > -0.3 if kind == "keep" else mask
+    pages, first = None, b
+    if page:
+        first = b * (m // page) + 1
+        pages = torch.randperm(first, generator=gen(8))[:b * (m // page)].view(b, -1).int()
+    attend(device, rows(b, h, n, d, 90), first, hk, m, dv, bits, mask, causal=kind == "none",
+           lengths=torch.tensor([m - 3, 70]), pages=pages, spoil=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("d", [64, 90, 128, 256])
 @pytest.mark.parametrize("n", [1, 9, 45])

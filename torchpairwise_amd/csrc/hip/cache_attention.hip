@@ -26,11 +26,11 @@ int read_call(const tpw_attention_desc *d, const tpw_cache_desc *cd, tpw_attenti
     return TPW_OK;
 }
 
-// The form for few rows reads a mask's keys side by side, and has no registers left for a second 16 rows of
-// float32 with more than 128 features.
+bool wide_f32(const Args &a, int dtype) { return dtype == TPW_F32 && (a.d > 128 || a.dv > 128); }
+
+// The form for few rows reads a mask's keys side by side.
 bool few_rows(const Args &a, int dtype, int mode) {
-    return a.n * a.group <= (dtype == TPW_F32 && (a.d > 128 || a.dv > 128) ? 16 : kFewRows) &&
-           (mode == kNoMask || a.mm == 1);
+    return a.n * a.group <= (wide_f32(a, dtype) ? kGroupedRows : kFewRows) && (mode == kNoMask || a.mm == 1);
 }
 
 size_t parts_bytes(const Args &a) {
@@ -45,16 +45,16 @@ size_t parts_bytes(const Args &a) {
 void plan_rows(Args &a, const cache::Cache &c, int bits, int dtype) {
     const int nb = row_blocks(c.k.blocks > c.v.blocks ? c.k.blocks : c.v.blocks);
     const int64_t rows = a.n * a.group;
-    const int np = dtype == TPW_F32 && rows > kPackedRows ? 3 : 1, rt = rows <= 16 ? 1 : 2;
+    const int np = dtype == TPW_F32 && rows > kPackedRows ? 3 : 1, rt = rows <= 16 || (nb == 8 && np > 1) ? 1 : 2;
     const int64_t per_cu = rows_per_cu(bits, nb, np, rt);
-    const int64_t bk = a.batch * a.key_heads, chunks = cdiv(a.m, 32), most = cdiv(chunks, kRowWaves);
+    a.tiles = in_groups(nb, np, false) ? cdiv(rows, 16) : 1;
+    const int64_t bk = a.batch * a.key_heads * a.tiles, chunks = cdiv(a.m, 32), most = cdiv(chunks, kRowWaves);
     int64_t splits = bk > 0 ? 256 * per_cu / bk : 1;
     splits = splits > most ? most : splits > kMaxParts ? kMaxParts : splits;
     const int64_t shared = cdiv(bk * splits, 256);  // parts that share a CU, a wave of each on a SIMD
     a.whole_rows = splits > 1 && may_be_whole(bits, nb, np, rt) &&
                    kWholeWaves / 4 * cdiv(chunks, kWholeWaves) <= shared * cdiv(chunks, kRowWaves * splits) + 2;
     a.splits = a.whole_rows || splits < 1 ? 1 : (int)splits;
-    a.tiles = 1;
 }
 
 void plan_tiles(Args &a, int dtype) {

@@ -53,7 +53,9 @@ struct Rows {
     int msize;                // bytes of one of its values
     uint32_t kat[KS], ksat[KS], vat, vsat;  // bytes of the lane's part: codes and scales of its key, its values
 
-    __device__ __forceinline__ void init(const Args &a, const Cache &c, int64_t b, int64_t kh, int64_t len, int lane) {
+    // row0: the block's first of the rows that share the key head
+    __device__ __forceinline__ void init(const Args &a, const Cache &c, int64_t b, int64_t kh, int row0, int64_t len,
+                                         int lane) {
         const int i = lane & 15, g = lane >> 4;
         // Blocks past the row's are not there: block 0 in their place, against queries of zero.
 #pragma unroll
@@ -68,7 +70,7 @@ struct Rows {
         vsat = (uint32_t)(block * c.v.sb + 8 * g);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int r = PACK ? i & 3 : 16 * t + i, n = (int)a.n;
+            const int r = row0 + (PACK ? i & 3 : 16 * t + i), n = (int)a.n;
             const bool in = r < n * (int)a.group;
             const int h = in ? n == 1 ? r : r / n : 0;
             const int64_t qh = kh * a.group + h, qi = in ? r - h * n : 0;
@@ -94,14 +96,14 @@ struct Rows {
     struct Piece {
         T x[8];
     };
-    static __device__ __forceinline__ void load_queries(const Args &a, int64_t b, int64_t kh, Piece (&y)[kOwn]) {
+    static __device__ __forceinline__ void load_queries(const Args &a, int64_t b, int64_t kh, int row0, Piece (&y)[kOwn]) {
         const T *q = reinterpret_cast<const T *>(a.q.p) + b * a.q.b;
         const int rows = (int)(a.n * a.group), n = (int)a.n, d = (int)a.d;
 #pragma unroll
         for (int x = 0; x < kOwn; ++x) {
-            const int id = x * kThreads + (int)threadIdx.x, r = id / (4 * NB), f = id % (4 * NB) * 8;
+            const int id = x * kThreads + (int)threadIdx.x, r = row0 + id / (4 * NB), f = id % (4 * NB) * 8;
             y[x] = {};
-            if (r < rows && f < d) {
+            if (id < kPieces && r < rows && f < d) {
                 const int h = n == 1 ? r : r / n;
                 const T *p = q + (kh * a.group + h) * a.q.h + (r - h * n) * a.q.n + f;
                 if (a.whole_q) {
@@ -416,16 +418,22 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args 
     const int i = lane & 15, g = lane >> 4;
     // 32 bits: divisions in 64 would take as long as several chunks
     const uint32_t all = gridDim.x, id = (all & 7) == 0 ? (blockIdx.x & 7) * (all >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-    const uint32_t part = id % (uint32_t)a.splits, bk = id / (uint32_t)a.splits;
+    const uint32_t part = id % (uint32_t)a.splits;
+    uint32_t bk = id / (uint32_t)a.splits;
+    int row0 = 0;
+    if constexpr (in_groups(NB, NP, PACK)) {
+        row0 = (int)(bk % (uint32_t)a.tiles) * kRows;
+        bk /= (uint32_t)a.tiles;
+    }
     const int64_t b = bk / (uint32_t)a.key_heads, kh = bk % (uint32_t)a.key_heads;
     typename R::Piece y[R::kOwn];
-    R::load_queries(a, b, kh, y);
+    R::load_queries(a, b, kh, row0, y);
     const int len = (int)key_end(a, b);
     const uint32_t chunks = (uint32_t)(len + 31) / 32;  // below 2^26, parts at most 64
     const int c0 = (int)(chunks * part / (uint32_t)a.splits), c1 = (int)(chunks * (part + 1) / (uint32_t)a.splits);
 
     R r;
-    r.init(a, c, b, kh, len, lane);
+    r.init(a, c, b, kh, row0, len, lane);
     // Codes of DEPTH chunks are in flight or worked on, the places of the next one known.
     typename R::C w[DEPTH];
     int x = c0 + wave, ahead = x;
@@ -482,7 +490,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args 
                     f32x4{r.o[q][k][e], r.o[q][k + 1][e], r.o[q][k + 2][e], r.o[q][k + 3][e]};
     }
     __syncthreads();
-    const int live = (int)(a.n * a.group), quads = (int)cdiv_dev(a.dv, 4), width = (int)quads4(a.dv);
+    const int live = (int)(a.n * a.group) - row0, quads = (int)cdiv_dev(a.dv, 4), width = (int)quads4(a.dv);
     for (int id = threadIdx.x; id < kRows * 8 * NB; id += 64 * WAVES) {
         const int q = id / (8 * NB), f = id % (8 * NB);
         if (q >= live || f >= quads) continue;
@@ -497,8 +505,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args 
             sum += w * stat[1][v][q];
             o += *reinterpret_cast<const f32x4 *>(mine + (v * kRows + q) * kWide + 4 * f) * w;
         }
-        const int n = (int)a.n, hi = n == 1 ? q : q / n;
-        const int64_t h = kh * a.group + hi, qi = q - hi * n, row = (b * a.heads + h) * n + qi;
+        const int n = (int)a.n, at_row = row0 + q, hi = n == 1 ? at_row : at_row / n;
+        const int64_t h = kh * a.group + hi, qi = at_row - hi * n, row = (b * a.heads + h) * n + qi;
         if (a.splits > 1) {
             const int64_t all = a.batch * a.heads * n, at = part;
             if (f == 0) {
@@ -536,8 +544,7 @@ template <int BITS, int NP, int RT, bool PACK = false>
 int rows_by_blocks(const Args &a, const Cache &c, int mode, unsigned blocks, hipStream_t s) {
     const int nb = row_blocks(c.k.blocks > c.v.blocks ? c.k.blocks : c.v.blocks);
     if (nb == 2) return launch_rows<BITS, 2, NP, RT, PACK>(a, c, mode, blocks, s);
-    // wider float32 rows come 16 at most
-    if constexpr (NP > 1 && RT > 1)
+    if constexpr (NP > 1 && RT > 1)  // (wider ones: 16 a block)
         return launch_rows<BITS, 4, NP, RT, PACK>(a, c, mode, blocks, s);
     else
         return nb == 4 ? launch_rows<BITS, 4, NP, RT, PACK>(a, c, mode, blocks, s)
@@ -545,14 +552,15 @@ int rows_by_blocks(const Args &a, const Cache &c, int mode, unsigned blocks, hip
 }
 template <int BITS>
 int rows_by_type(const Args &a, const Cache &c, int dtype, int mode, hipStream_t s) {
-    const int64_t blocks = a.batch * a.key_heads * a.splits, rows = a.n * a.group;
+    const int64_t blocks = a.batch * a.key_heads * a.tiles * a.splits, rows = a.n * a.group;
     TPW_REQUIRE(blocks <= cache::kMostBlocks, "attention: too many rows");
     if (dtype == TPW_BF16)
         return rows <= 16 ? rows_by_blocks<BITS, 1, 1>(a, c, mode, (unsigned)blocks, s)
                           : rows_by_blocks<BITS, 1, 2>(a, c, mode, (unsigned)blocks, s);
     return rows <= kPackedRows ? rows_by_blocks<BITS, 3, 1, true>(a, c, mode, (unsigned)blocks, s)
-           : rows <= 16        ? rows_by_blocks<BITS, 3, 1>(a, c, mode, (unsigned)blocks, s)
-                               : rows_by_blocks<BITS, 3, 2>(a, c, mode, (unsigned)blocks, s);
+           : rows <= 16 || a.tiles > 1
+               ? rows_by_blocks<BITS, 3, 1>(a, c, mode, (unsigned)blocks, s)
+               : rows_by_blocks<BITS, 3, 2>(a, c, mode, (unsigned)blocks, s);
 }
 
 }  // namespace attn
