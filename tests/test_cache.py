@@ -741,6 +741,15 @@ def test_results_repeat_bit_for_bit(n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,m", [(1, 8208), (1, 40912), (5, 24704), (20, 24704), (40, 24704)])
+@pytest.mark.parametrize("d", [64, 160])
+def test_one_head_over_a_long_cache(dtype, n, m, d):
+    """More chunks of keys than there may be parts."""
+    attend("cuda", rows(1, 1, n, d, 3, dtype), 1, 1, m, d, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("bits,d", [(4, 64), (4, 128), (4, 250), (8, 128), (8, 250)])
 @pytest.mark.parametrize("m", [240, 1024, 1104])
 def test_short_caches_of_many_heads(dtype, bits, d, m):

@@ -50,7 +50,8 @@ void plan_rows(Args &a, const cache::Cache &c, int bits, int dtype) {
     a.tiles = in_groups(nb, np, false) ? cdiv(rows, 16) : 1;
     const int64_t bk = a.batch * a.key_heads * a.tiles, chunks = cdiv(a.m, 32), most = cdiv(chunks, kRowWaves);
     int64_t splits = bk > 0 ? 256 * per_cu / bk : 1;
-    splits = splits > most ? most : splits > kMaxParts ? kMaxParts : splits;
+    splits = splits > most ? most : splits;
+    splits = splits > kMaxParts ? kMaxParts : splits;
     const int64_t shared = cdiv(bk * splits, 256);  // parts that share a CU, a wave of each on a SIMD
     a.whole_rows = splits > 1 && may_be_whole(bits, nb, np, rt) &&
                    kWholeWaves / 4 * cdiv(chunks, kWholeWaves) <= shared * cdiv(chunks, kRowWaves * splits) + 2;
