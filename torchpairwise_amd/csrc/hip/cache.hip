@@ -20,12 +20,13 @@ struct RowsArgs {
     uint32_t heads, tiles;   // blocks of 256 threads per (sequence, head), those of the wider side
 };
 
-// A block's share: a thread works on 8 features (a piece) of ROWS consecutive rows (whose scales lie side by
-// side: one word); 4 consecutive lanes share a block of 32 features.  What the call does not have is read from
+// A block's share: a thread works on PIECE features (a piece) of ROWS consecutive rows (whose scales lie side by
+// side: one word); 4 (8) consecutive lanes share a block of 32 features.  What the call does not have is read from
 // somewhere that exists and dropped: without branches between them all of a thread's loads are in flight at once.
 // The narrower side has more rows to a block, and none for the last ones: those return at once.
-template <int ROWS, bool PAGED>
+template <int ROWS, bool PAGED, int PIECE>
 struct Share {
+    static constexpr int kPieces = 32 / PIECE;  // of a block of 32 features
     int64_t b, h, first;  // first row of the block's
     int piece, r, per;    // the thread's piece and its place among the `per` threads of that
     int rows;             // of the call's (0: none left)
@@ -34,7 +35,7 @@ struct Share {
     bool live[ROWS];      // the call has the row, and it has a place
     __device__ __forceinline__ Share(const RowsArgs &a, const Side &s) {
         // 32 bits: divisions in 64 would be most of a block's instructions
-        const uint32_t pieces = 4 * s.blocks, t = threadIdx.x;
+        const uint32_t pieces = kPieces * s.blocks, t = threadIdx.x;
         per = (int)(256 / pieces);
         r = (int)(t / pieces);
         piece = (int)(t % pieces);
@@ -80,7 +81,7 @@ struct Share {
         return s.codes + entry[k] * s.cf + h * s.ch + (int64_t)row[k] * s.cr;
     }
     __device__ __forceinline__ uint8_t *scale(const Side &s, int k) const {
-        return s.scales + entry[k] * s.sf + h * s.sh + piece / 4 * s.sb + row[k];
+        return s.scales + entry[k] * s.sf + h * s.sh + piece / kPieces * s.sb + row[k];
     }
     // Row k of the thread's among the call's, and whether it is there.
     __device__ __forceinline__ int own(int k) const { return r * ROWS + k; }
@@ -98,7 +99,7 @@ template <typename T, int BITS, int ROWS, bool WHOLE, bool PAGED>
 __global__ __launch_bounds__(256) void cache_write_kernel(const RowsArgs a) {
     const int side = blockIdx.y;
     const Side &s = side ? a.c.v : a.c.k;
-    const Share<ROWS, PAGED> p(a, s);
+    const Share<ROWS, PAGED, 8> p(a, s);
     if (p.rows == 0) return;
     const T *base = reinterpret_cast<const T *>(a.x[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.first * a.xn[side];
     const int f = 8 * p.piece, d = a.width[side];
@@ -154,49 +155,72 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const RowsArgs a) {
         if (p.live[k]) *p.scale(s, k) = (uint8_t)bytes[k];
 }
 
+// What a thread reads of a row: 16 bytes out, so that a wave's stores cover whole lines.
+constexpr int read_piece(size_t size) { return size == 4 ? 4 : 8; }
+template <int BITS, int P>
+struct Codes;
+template <int BITS>
+struct Codes<BITS, 8> {  // to bfloat16
+    Eight<BITS> w;
+    __device__ __forceinline__ void values(uint32_t byte, uint16_t (&out)[8]) const {
+        const float scale = cache::scale_of(byte);
+        if (__all(byte >= 32)) {  // exact
+            const uint4 y = w.bf16(scale);
+            __builtin_memcpy(out, &y, 16);
+        } else {  // (below bfloat16's normal range: rounded)
+            float x[8];
+            w.f32(scale, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) from_f32(&out[e], x[e]);
+        }
+    }
+};
+template <int BITS>
+struct Codes<BITS, 4> {  // to float32
+    uint32_t w;
+    __device__ __forceinline__ void values(uint32_t byte, float (&out)[4]) const {
+        const float scale = cache::scale_of(byte);
+        const f2 a = f32_pair<BITS, 0>(w, scale), b = f32_pair<BITS, 1>(w, scale);
+        out[0] = a[0], out[1] = a[1], out[2] = b[0], out[3] = b[1];
+    }
+};
+
 // Rows that are not the call's, or that lie nowhere, are zeros.  Bound by memory: 2 x 16 x 2 x 32768 x 128 in 122
 // to 132 us (5 TB/s); one row a thread, with branches around its loads, took 205.
 template <typename T, int BITS, int ROWS, bool WHOLE, bool PAGED>
 __global__ __launch_bounds__(256) void cache_read_kernel(const RowsArgs a) {
     const int side = blockIdx.y;
     const Side &s = side ? a.c.v : a.c.k;
-    const Share<ROWS, PAGED> p(a, s);
+    constexpr int P = read_piece(sizeof(T));
+    const Share<ROWS, PAGED, P> p(a, s);
     T *base = reinterpret_cast<T *>(a.y[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.first * a.xn[side];
-    const int f = 8 * p.piece, d = a.width[side];
+    const int f = P * p.piece, d = a.width[side];
     if (p.rows == 0 || f >= d || p.r >= p.per) return;
-    Eight<BITS> w[ROWS] = {};
+    Codes<BITS, P> w[ROWS] = {};
     uint32_t byte[ROWS] = {};
     if (a.m > 0 && a.c.first > 0) {
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
-            __builtin_memcpy(&w[k], __builtin_assume_aligned(p.codes(s, k) + BITS * p.piece, BITS), sizeof(w[k]));
+            constexpr int kBytes = BITS * P / 8;
+            __builtin_memcpy(&w[k], __builtin_assume_aligned(p.codes(s, k) + kBytes * p.piece, kBytes), kBytes);
             byte[k] = *p.scale(s, k);
         }
     }
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-        T out[8];
-        const float scale = scale_of(byte[k]);
-        if (sizeof(T) == 2 && __all(byte[k] >= 32)) {  // exact
-            const uint4 y = w[k].bf16(scale);
-            __builtin_memcpy(out, &y, 16);
-        } else {  // (bfloat16 below its normal range: rounded)
-            float x[8];
-            w[k].f32(scale, x);
+        T out[P];
+        w[k].values(byte[k], out);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) from_f32(&out[e], x[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) out[e] = p.live[k] ? out[e] : T(0);
+        for (int e = 0; e < P; ++e) out[e] = p.live[k] ? out[e] : T(0);
         if (!p.has(k)) continue;
         T *row = base + p.own(k) * a.xn[side] + f;
         if constexpr (WHOLE) {
             __builtin_memcpy(__builtin_assume_aligned(row, 16), out, sizeof(out));
-        } else if (f + 8 <= d) {  // any alignment
+        } else if (f + P <= d) {  // any alignment
             __builtin_memcpy(row, out, sizeof(out));
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < P; ++e)
                 if (f + e < d) row[e] = out[e];
         }
     }
@@ -209,7 +233,8 @@ int launch(RowsArgs &a, bool write, int64_t batch, int64_t blocks, hipStream_t s
     const auto go = [&](auto rows, auto whole, auto paged) {
         constexpr int ROWS = decltype(rows)::value;
         constexpr bool WHOLE = decltype(whole)::value, PAGED = decltype(paged)::value;
-        const int64_t tiles = cdiv(a.n, ROWS * (256 / (4 * blocks))), all = tiles * batch * a.heads;
+        const int64_t piece = write ? 8 : read_piece(sizeof(T));
+        const int64_t tiles = cdiv(a.n, ROWS * (256 / (32 / piece * blocks))), all = tiles * batch * a.heads;
         TPW_REQUIRE(all <= kMostBlocks, "cache: too many rows");
         a.tiles = (uint32_t)tiles;
         const dim3 grid((unsigned)all, 2);
