@@ -20,11 +20,11 @@ struct RowsArgs {
     uint32_t heads, tiles;   // blocks of 256 threads per (sequence, head), those of the wider side
 };
 
-// A block's share: a thread works on PIECE features (a piece) of ROWS consecutive rows (whose scales lie side by
-// side: one word); 4 (8) consecutive lanes share a block of 32 features.  What the call does not have is read from
+// A block's share: a thread works on PIECE features (a piece) of ROWS rows, consecutive ones (whose scales lie side by
+// side: one word) or spread over the block; 4 (8) consecutive lanes share a block of 32 features.  What the call does not have is read from
 // somewhere that exists and dropped: without branches between them all of a thread's loads are in flight at once.
 // The narrower side has more rows to a block, and none for the last ones: those return at once.
-template <int ROWS, bool PAGED, int PIECE>
+template <int ROWS, bool PAGED, int PIECE, bool SPREAD>
 struct Share {
     static constexpr int kPieces = 32 / PIECE;  // of a block of 32 features
     int64_t b, h, first;  // first row of the block's
@@ -84,7 +84,7 @@ struct Share {
         return s.scales + entry[k] * s.sf + h * s.sh + piece / kPieces * s.sb + row[k];
     }
     // Row k of the thread's among the call's, and whether it is there.
-    __device__ __forceinline__ int own(int k) const { return r * ROWS + k; }
+    __device__ __forceinline__ int own(int k) const { return SPREAD ? k * per + r : r * ROWS + k; }
     __device__ __forceinline__ bool has(int k) const { return r < per && own(k) < rows; }
     // Ids go round-robin over the 8 XCDs: where they divide, each XCD gets a contiguous range, so that the
     // scales of neighbouring rows, a byte each, meet in one L2.
@@ -99,7 +99,7 @@ template <typename T, int BITS, int ROWS, bool WHOLE, bool PAGED>
 __global__ __launch_bounds__(256) void cache_write_kernel(const RowsArgs a) {
     const int side = blockIdx.y;
     const Side &s = side ? a.c.v : a.c.k;
-    const Share<ROWS, PAGED, 8> p(a, s);
+    const Share<ROWS, PAGED, 8, false> p(a, s);
     if (p.rows == 0) return;
     const T *base = reinterpret_cast<const T *>(a.x[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.first * a.xn[side];
     const int f = 8 * p.piece, d = a.width[side];
@@ -185,14 +185,17 @@ struct Codes<BITS, 4> {  // to float32
     }
 };
 
-// Rows that are not the call's, or that lie nowhere, are zeros.  Bound by memory: 2 x 16 x 2 x 32768 x 128 in 122
-// to 132 us (5 TB/s); one row a thread, with branches around its loads, took 205.
+// Rows that are not the call's, or that lie nowhere, are zeros.  Bound by memory: 2 x 16 x 2 x 32768 x 128 bf16 in 122
+// to 132 us (5 TB/s; one row a thread, with branches around its loads, took 205), 2 x 8 x 4 x 10240 x 128 fp32 in 73
+// (5.2; 8 features a thread, a wave's store skipping every other 16 bytes: 106).  Rows that do not lie in 16-byte
+// pieces are spread over the block, so that a store instruction's rows follow one another: 118 bf16 out of 8 bits 72 ->
+// 56, 90 29 -> 26 (whole pieces: 33.6 -> 35.1); of fp32, 90 take 90 (3 TB/s): 16-byte stores at 8-byte addresses.
 template <typename T, int BITS, int ROWS, bool WHOLE, bool PAGED>
 __global__ __launch_bounds__(256) void cache_read_kernel(const RowsArgs a) {
     const int side = blockIdx.y;
     const Side &s = side ? a.c.v : a.c.k;
     constexpr int P = read_piece(sizeof(T));
-    const Share<ROWS, PAGED, P> p(a, s);
+    const Share<ROWS, PAGED, P, !WHOLE> p(a, s);
     T *base = reinterpret_cast<T *>(a.y[side]) + p.b * a.xb[side] + p.h * a.xh[side] + p.first * a.xn[side];
     const int f = P * p.piece, d = a.width[side];
     if (p.rows == 0 || f >= d || p.r >= p.per) return;
@@ -226,7 +229,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const RowsArgs a) {
     }
 }
 
-// Rows of a thread: several where there are blocks enough to fill the card's places all the same.
+// Rows of a thread: several where every CU has a block all the same (4 x 4 x 1664 x 96 out of 8 bits: fp32 11.8 -> 6.9 us,
+// bf16 7.3 -> 5.9, written 7.0 -> 5.6; 2 x 2 x 512 x 64, which have not: 3.1 where they would take 3.9).
 constexpr int kManyRows = 4;
 template <typename T, int BITS>
 int launch(RowsArgs &a, bool write, int64_t batch, int64_t blocks, hipStream_t s) {
@@ -251,8 +255,9 @@ int launch(RowsArgs &a, bool write, int64_t batch, int64_t blocks, hipStream_t s
     const auto by_row = [&](auto rows) {
         return a.whole[0] && a.whole[1] ? by_page(rows, std::true_type{}) : by_page(rows, std::false_type{});
     };
-    const int64_t all = cdiv(a.n, kManyRows * (256 / (4 * blocks))) * batch * a.heads * 2;
-    return all >= 256 * 8 ? by_row(std::integral_constant<int, kManyRows>{}) : by_row(std::integral_constant<int, 1>{});
+    const int64_t piece = write ? 8 : read_piece(sizeof(T));
+    const int64_t all = cdiv(a.n, kManyRows * (256 / (32 / piece * blocks))) * batch * a.heads * 2;
+    return all >= 256 ? by_row(std::integral_constant<int, kManyRows>{}) : by_row(std::integral_constant<int, 1>{});
 }
 
 int move_rows(const tpw_cache_desc *d, bool write, int dtype, int64_t batch, int64_t n, const void *key, int64_t width,
