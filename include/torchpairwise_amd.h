@@ -816,6 +816,9 @@ typedef struct tpw_attention_desc {
     int64_t mask_strides[4];
 } tpw_attention_desc;
 
+/* The sizes of workspaces (here and of the cache below) follow from the types, the sizes, the strides, whether there is an
+ * out_rest, and how the operands' addresses are aligned: a null one counts as 16-byte aligned, so that they can be asked
+ * for before there are any.  Operands that do not lie in 16-byte pieces are copied into the workspace. */
 size_t tpw_attention_workspace_size(const tpw_attention_desc *desc);
 int tpw_attention(const tpw_attention_desc *desc, void *workspace, void *stream);
 /* grad_query, grad_key and grad_value (every element is written) for an upstream grad_out. */

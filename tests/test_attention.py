@@ -444,6 +444,25 @@ print("done")
     assert r.returncode == 0 and "done" in r.stdout, (r.returncode, r.stdout, r.stderr[-2000:])
 
 
+@pytest.mark.parametrize("dtype", [capi.TPW_F32, capi.TPW_BF16])
+@pytest.mark.parametrize("d", [1, 50, 64, 90, 200])
+def test_workspace_sizes_before_and_after_there_are_operands(dtype, d):
+    """Operands without an address count as aligned ones: rows that have to be copied are counted."""
+    lib = capi.lib()
+    for n, m, mask_type in ((1, 1, 0), (1, 1000, 1), (70, 1000, 2), (1000, 1000, 0), (1000, 1000, 1)):
+        sizes = []
+        for address in (None, 4096):
+            a = capi.AttentionDesc(dtype=dtype, batch=2, heads=4, key_heads=2, n=n, m=m, d=d, dv=d, scale=1.0,
+                                   mask_type=mask_type)
+            for name in ("query", "key", "value", "out", "grad_out", "grad_query", "grad_key", "grad_value"):
+                getattr(a, name + "_strides")[:] = [4 * max(n, m) * d, max(n, m) * d, d]
+                setattr(a, name, address)
+            a.mask_strides[:] = [0, 0, m, 1]
+            a.mask = a.stats = a.lengths = address
+            sizes.append((lib.tpw_attention_workspace_size(C.byref(a)), lib.tpw_attention_backward_workspace_size(C.byref(a))))
+        assert sizes[0] == sizes[1], (n, m, mask_type, sizes)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_c_entries_without_statistics(dtype):

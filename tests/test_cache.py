@@ -728,6 +728,38 @@ def test_c_entries_refuse():
     assert b"too many" in lib.tpw_last_error()
 
 
+def c_cache(**more):
+    """A descriptor of one sequence of one head, 16 rows of a block, at addresses that nothing is read from."""
+    d = capi.CacheDesc(bits=4, first=1, heads=1, rows=16, key_blocks=1, value_blocks=1, key_codes=4096, key_scales=4096,
+                       value_codes=4096, value_scales=4096)
+    for side in ("key", "value"):
+        getattr(d, side + "_code_strides")[:] = [256, 256, 16]
+        getattr(d, side + "_scale_strides")[:] = [16, 16, 16]
+    for k, v in more.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("dtype", [capi.TPW_F32, capi.TPW_BF16])
+@pytest.mark.parametrize("d", [1, 50, 64, 90, 200])
+def test_workspace_sizes_before_and_after_there_are_operands(dtype, d):
+    """A query without an address counts as an aligned one: rows that have to be copied are counted."""
+    lib, blocks = capi.lib(), ref.blocks_of(d)
+    for n, m, mask_type in ((1, 16, 0), (1, 1008, 1), (70, 1008, 2), (1000, 1008, 0), (1000, 1008, 1)):
+        c = c_cache(first=2, heads=2, rows=m, key_blocks=blocks, value_blocks=blocks)
+        sizes = []
+        for address in (None, 4096):
+            a = capi.AttentionDesc(dtype=dtype, batch=2, heads=4, key_heads=2, n=n, m=m, d=d, dv=d, scale=1.0,
+                                   mask_type=mask_type, query=address, out=address, mask=address, lengths=address)
+            a.query_strides[:] = a.out_strides[:] = [4 * n * d, n * d, d]
+            a.mask_strides[:] = [0, 0, m, 1]
+            sizes.append(lib.tpw_cache_attention_workspace_size(C.byref(a), C.byref(c)))
+        assert sizes[0] == sizes[1], (n, m, mask_type, sizes)
+        # the copy of the query alone: keys and values have no addresses here, and need no copies
+        copied = 2 * 4 * n * -(-d * (4 if dtype == capi.TPW_F32 else 2) // 16) * 16
+        assert sizes[0] >= copied or d % 8 == 0 or n == 1
+
+
 # ---------------------------------------------------------------- on the GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 8, 60])

@@ -248,7 +248,7 @@ size_t plan_padding(Args &a, int dtype, bool backward, uint8_t *at, PadArgs *p) 
     size_t bytes = 0;
     if (a.dwords) return 0;
     const auto take = [&](View &v, int64_t heads, int64_t rows, int64_t width, bool always = false) {
-        if (!v.p || (!always && whole_pieces(v, width, size)) || a.batch * heads * rows == 0) return;
+        if ((!always && whole_pieces(v, width, size)) || a.batch * heads * rows == 0) return;
         const int64_t pieces = cdiv(width, e), n = a.batch * heads * rows * pieces;
         if (p) {
             const int t = p->count++;
@@ -261,8 +261,10 @@ size_t plan_padding(Args &a, int dtype, bool backward, uint8_t *at, PadArgs *p) 
         bytes += (size_t)n * 16;
     };
     take(a.q, a.heads, a.n, a.d);
-    take(a.k, a.key_heads, a.m, a.d);
-    take(a.v, a.key_heads, a.m, a.dv);
+    if (!a.cached) {
+        take(a.k, a.key_heads, a.m, a.d);
+        take(a.v, a.key_heads, a.m, a.dv);
+    }
     if (backward) {
         take(a.go, a.heads, a.n, a.dv);
         View rest = {a.rest, a.o.b, a.o.h, a.o.n};

@@ -53,6 +53,7 @@ struct Args {
     float qsign;   // -1, 0 or 1: the sign of scale, folded into q as it is loaded
     float gscale;  // scale (backward)
     int causal;
+    int cached;     // keys and values lie in a cache in 4 or 8 bits: k and v are no operands
     int whole_q;    // (few rows over a cache) queries are whole pieces of 8 features
     int whole_rows; // (few rows over a cache) not in parts, by more waves
     int dwords;     // (forward) operands of whole dwords that are not whole pieces, read as they lie

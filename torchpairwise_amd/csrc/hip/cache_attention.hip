@@ -19,6 +19,7 @@ int read_call(const tpw_attention_desc *d, const tpw_cache_desc *cd, tpw_attenti
     TPW_REQUIRE(d->key_heads == cd->heads, "attention: key_heads differ from the cache's heads");
     TPW_REQUIRE(d->m == (cd->pages ? cd->page_count * cd->rows : cd->rows), "attention: m differs from the cache's rows");
     TPW_REQUIRE(d->d <= 32 * cd->key_blocks && d->dv <= 32 * cd->value_blocks, "attention: rows are wider than the cache's");
+    a.cached = 1;
     a.dwords = 0;
     const int64_t size = d->dtype == TPW_F32 ? 4 : 2;
     a.whole_q = a.d % 8 == 0 && aligned16(a.q.p) && (a.q.b | a.q.h | a.q.n) * size % 16 == 0;
