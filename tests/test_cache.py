@@ -760,6 +760,21 @@ def test_workspace_sizes_before_and_after_there_are_operands(dtype, d):
         assert sizes[0] >= copied or d % 8 == 0 or n == 1
 
 
+def test_c_workspace_of_tables_without_pages():
+    """Sizes of a call over no keys: what a mask over them would take is not asked for."""
+    lib = capi.lib()
+    for dtype in (capi.TPW_F32, capi.TPW_BF16):
+        for n in (1, 100):
+            sizes = []
+            for mask_type in (0, 1, 2):
+                a = capi.AttentionDesc(dtype=dtype, batch=2, heads=4, key_heads=2, n=n, m=64, d=90, dv=90, scale=1.0,
+                                       mask_type=mask_type)
+                a.query_strides[:] = a.out_strides[:] = [4 * n * 90, n * 90, 90]
+                c = c_cache(first=0, heads=2, key_blocks=3, value_blocks=3, pages=4096, page_count=4, page_pitch=4)
+                sizes.append(lib.tpw_cache_attention_workspace_size(C.byref(a), C.byref(c)))
+            assert sizes[0] == sizes[1] == sizes[2], (dtype, n, sizes)
+
+
 # ---------------------------------------------------------------- on the GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 8, 60])
@@ -769,6 +784,28 @@ def test_results_repeat_bit_for_bit(n):
     outs = [tp.cache_attention(q, *cache, causal=True) for _ in range(3)]
     for o in outs[1:]:
         assert_equal(o, outs[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [1, 100])
+@pytest.mark.parametrize("mask_type", [0, 1, 2])
+def test_c_entry_over_tables_without_pages(dtype, n, mask_type):
+    """Tables over no pages at all, called through the C entry: zeros, whatever the mask."""
+    b, h, hk, d = 2, 4, 2, 90  # rows that are copied first
+    q, pages = rows(b, h, n, d, 1, dtype).cuda(), torch.zeros(b, 4, dtype=torch.int32, device="cuda")
+    out, mask = torch.full_like(q, 7.0), torch.ones(n, 64, dtype=torch.bool if mask_type == 1 else F32, device="cuda")
+    a = capi.AttentionDesc(dtype=capi.TPW_F32 if dtype == F32 else capi.TPW_BF16, batch=b, heads=h, key_heads=hk, n=n, m=64,
+                           d=d, dv=d, scale=1.0, mask_type=mask_type, query=q.data_ptr(), out=out.data_ptr(),
+                           mask=mask.data_ptr())
+    a.query_strides[:] = a.out_strides[:] = q.stride()[:3]
+    a.mask_strides[:] = [0, 0, 64, 1]
+    c = c_cache(first=0, heads=hk, key_blocks=3, value_blocks=3, key_codes=None, key_scales=None, value_codes=None,
+                value_scales=None, pages=pages.data_ptr(), page_count=4, page_pitch=4)
+    size = capi.lib().tpw_cache_attention_workspace_size(C.byref(a), C.byref(c))
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    capi.call("tpw_cache_attention", C.byref(a), C.byref(c), ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert not out.any()
 
 
 @pytest.mark.gpu

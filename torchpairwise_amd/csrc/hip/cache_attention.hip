@@ -23,7 +23,7 @@ int read_call(const tpw_attention_desc *d, const tpw_cache_desc *cd, tpw_attenti
     a.dwords = 0;
     const int64_t size = d->dtype == TPW_F32 ? 4 : 2;
     a.whole_q = a.d % 8 == 0 && aligned16(a.q.p) && (a.q.b | a.q.h | a.q.n) * size % 16 == 0;
-    if (cd->first == 0) a.m = 0;  // a table without pages
+    if (cd->first == 0) a.m = own.m = 0;  // a table without pages: no keys, and no mask over them
     return TPW_OK;
 }
 
@@ -83,7 +83,7 @@ extern "C" size_t tpw_cache_attention_workspace_size(const tpw_attention_desc *d
     cache::Cache c = {};
     tpw_attention_desc own;
     if (read_call(d, cd, own, a, c) != TPW_OK || a.batch * a.heads * a.n == 0) return 0;
-    if (few_rows(a, d->dtype, mask_mode(d))) {
+    if (few_rows(a, d->dtype, mask_mode(&own))) {
         plan_rows(a, c, cd->bits, d->dtype);
         return parts_bytes(a);
     }
@@ -99,7 +99,7 @@ extern "C" int tpw_cache_attention(const tpw_attention_desc *d, const tpw_cache_
     if (const int rc = read_call(d, cd, own, a, c)) return rc;
     if (a.batch * a.heads * a.n == 0) return TPW_OK;
     TPW_REQUIRE(a.q.p && a.o.p, "attention: null operand");
-    const int mode = mask_mode(d);
+    const int mode = mask_mode(&own);
     TPW_REQUIRE(mode == kNoMask || a.mask, "attention: null mask");
     hipStream_t s = as_stream(stream);
     size_t prepared = 0;
