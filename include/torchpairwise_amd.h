@@ -833,8 +833,8 @@ int tpw_attention_backward(const tpw_attention_desc *desc, void *workspace, void
  * a block that holds NaN or an infinity becomes NaN.
  * codes [first, heads, rows, blocks] of 16 (32) bytes, the bytes of a row dense; scales [first, heads, blocks,
  * rows], rows dense.  Strides are in bytes, of [first, heads, rows] and [first, heads, blocks]; they and the
- * addresses are multiples of 16, and so is rows; rows lie at most 8 MiB apart, a row's scales 256 MiB.  Without a table of pages first is the batch and rows what
- * each sequence has room for; with one (int32, or int64 where pages_wide), row j of sequence b is row j % rows
+ * addresses are multiples of 16, and so is rows; those of rows and of blocks are not negative.  Without a table of
+ * pages first is the batch and rows what each sequence has room for; with one (int32, or int64 where pages_wide), row j of sequence b is row j % rows
  * of page pages[b * page_pitch + j / rows], rows being a power of two.  Entries outside [0, first) stand for no
  * page: their rows are not written, read as zeros, and are no keys. */
 typedef struct tpw_cache_desc {

@@ -507,6 +507,39 @@ def test_queries_of_any_layout(device):
             assert_close(tp.cache_attention(on, *cache), o, rtol=0.0, atol=tol + TINY)
 
 
+def far_apart(x, dim, stride):
+    """x's values in a view whose entries along `dim` lie `stride` bytes apart."""
+    strides = list(x.stride())
+    strides[dim] = stride
+    y = torch.zeros(sum((s - 1) * st for s, st in zip(x.shape, strides)) + 1, dtype=torch.uint8, device=x.device)
+    return y.as_strided(x.shape, strides).view(x.dtype)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("side", ["key", "value"])
+@pytest.mark.parametrize("far", ["codes", "scales"])
+def test_rows_and_scales_that_lie_far_apart(device, bits, side, far):
+    """Strides over rows past 8 MiB and over blocks past 256 MiB: written, read back, attended to by few rows and
+    by many."""
+    hk, m, d = 1, 16, 64
+    cache = list(tp.quantized_cache(1, hk, m, d, bits=bits, device=device))
+    at = 2 * (side == "value") + (far == "scales")
+    cache[at] = far_apart(cache[at], 2, (1 << 23) + 16 if far == "codes" else (1 << 28) + 16)
+    x = [rows(1, hk, m, d, 50 + k) for k in (0, 1)]
+    tp.cache_write_(*cache, *(y.to(device) for y in x), torch.zeros(1, dtype=torch.long, device=device))
+    k, v = (ref.decode(*ref.encode(y, bits), bits, d) for y in x)
+    got = tp.cache_read(*cache, dtype=F32)
+    assert_equal(got[0], k.float())
+    assert_equal(got[1], v.float())
+    for n in (1, 3, 20, 40):
+        for dtype in (F32, BF16):
+            q = rows(1, 2, n, d, 60 + n, dtype)
+            o, tol = ref.reference(q, k, v, torch.ones(1, m, dtype=torch.bool), causal=True)
+            out = tp.cache_attention(q.to(device), *cache, causal=True)
+            assert_close(out, o, rtol=0.0, atol=tol + TINY, what=f"{n} {dtype}")
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_empty_calls(device):
     for b, n, m in ((0, 1, 16), (2, 0, 16), (2, 1, 0), (2, 3, 0)):
@@ -758,6 +791,18 @@ def test_workspace_sizes_before_and_after_there_are_operands(dtype, d):
         # the copy of the query alone: keys and values have no addresses here, and need no copies
         copied = 2 * 4 * n * -(-d * (4 if dtype == capi.TPW_F32 else 2) // 16) * 16
         assert sizes[0] >= copied or d % 8 == 0 or n == 1
+
+
+def test_c_entries_take_rows_and_scales_far_apart():
+    """What a descriptor may hold, seen by calls of no rows."""
+    lib, three = capi.lib(), (C.c_int64 * 3)(32, 32, 32)
+    for row, block, rc in ((1 << 40, 1 << 40, 0), (-16, 16, 1), (16, -16, 1), (24, 16, 1), (16, 24, 1)):
+        c = c_cache(key_blocks=2, value_blocks=2)
+        for side in ("key", "value"):
+            getattr(c, side + "_code_strides")[:] = [0, 0, row]
+            getattr(c, side + "_scale_strides")[:] = [0, 0, block]
+        for f in (lib.tpw_cache_write, lib.tpw_cache_read):
+            assert f(C.byref(c), 0, 1, 0, 4096, 32, three, 4096, 32, three, None, None, None) == rc, (row, block)
 
 
 def test_c_workspace_of_tables_without_pages():

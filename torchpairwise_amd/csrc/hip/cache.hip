@@ -325,6 +325,7 @@ int read_cache(const tpw_cache_desc *d, int64_t batch, Cache &c) {
     c.pitch = d->page_pitch;
     c.first = d->first;
     c.wide = d->pages_wide != 0;
+    c.near = 1;
     const auto side = [&](Side &s, void *codes, void *scales, const int64_t *cs, const int64_t *ss, int64_t blocks) {
         s.codes = reinterpret_cast<uint8_t *>(codes);
         s.scales = reinterpret_cast<uint8_t *>(scales);
@@ -336,16 +337,15 @@ int read_cache(const tpw_cache_desc *d, int64_t batch, Cache &c) {
         s.sf = d->first == 1 ? 0 : ss[0];
         s.sh = d->heads == 1 ? 0 : ss[1];
         s.sb = blocks == 1 ? 0 : ss[2];
-        // rows and scales within the kernels' 32-bit reach
-        if (s.cr < 0 || s.cr > (int64_t(1) << 23) || s.sb < 0 || s.sb > (int64_t(1) << 28)) return false;
-        return aligned16(codes) && aligned16(scales) && (s.cf | s.ch | s.cr | s.sf | s.sh | s.sb) % 16 == 0 &&
+        c.near = c.near && s.cr <= (int64_t(1) << 23) && s.sb <= (int64_t(1) << 28);
+        return s.cr >= 0 && s.sb >= 0 && aligned16(codes) && aligned16(scales) && (s.cf | s.ch | s.cr | s.sf | s.sh | s.sb) % 16 == 0 &&
                (m * d->first == 0 || (codes && scales));
     };
     TPW_REQUIRE(side(c.k, d->key_codes, d->key_scales, d->key_code_strides, d->key_scale_strides, d->key_blocks) &&
                     side(c.v, d->value_codes, d->value_scales, d->value_code_strides, d->value_scale_strides,
                          d->value_blocks),
-                "cache: codes and scales must lie at 16-byte aligned addresses and strides, rows at most 8 MiB and scales of "
-                "a block at most 256 MiB apart");
+                "cache: codes and scales must lie at 16-byte aligned addresses and strides, and those of rows and blocks "
+                "must not be negative");
     return TPW_OK;
 }
 

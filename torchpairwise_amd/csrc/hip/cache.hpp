@@ -36,6 +36,7 @@ struct Cache {
     int64_t first;      // pages there are (without a table: sequences)
     int wide;           // its entries are 64-bit
     int shift, mask;    // rows of a page: 1 << shift, and less one (without a table: 31, all ones)
+    int near;           // rows lie at most 8 MiB apart, the scales of a row's blocks 256 MiB: 32 bits reach over 32 rows
 };
 
 // Where row j of sequence b lies: entry of the first dimension (-1: nowhere) and row.

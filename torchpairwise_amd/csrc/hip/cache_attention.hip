@@ -29,9 +29,10 @@ int read_call(const tpw_attention_desc *d, const tpw_cache_desc *cd, tpw_attenti
 
 bool wide_f32(const Args &a, int dtype) { return dtype == TPW_F32 && (a.d > 128 || a.dv > 128); }
 
-// The form for few rows reads a mask's keys side by side.
-bool few_rows(const Args &a, int dtype, int mode) {
-    return a.n * a.group <= (wide_f32(a, dtype) ? kGroupedRows : kFewRows) && (mode == kNoMask || a.mm == 1);
+// The form for few rows reads a mask's keys side by side, and reaches its 32 rows and their scales by 32-bit offsets (the
+// form for many addresses each row by itself, in 64 bits).
+bool few_rows(const Args &a, const cache::Cache &c, int dtype, int mode) {
+    return c.near && a.n * a.group <= (wide_f32(a, dtype) ? kGroupedRows : kFewRows) && (mode == kNoMask || a.mm == 1);
 }
 
 size_t parts_bytes(const Args &a) {
@@ -83,7 +84,7 @@ extern "C" size_t tpw_cache_attention_workspace_size(const tpw_attention_desc *d
     cache::Cache c = {};
     tpw_attention_desc own;
     if (read_call(d, cd, own, a, c) != TPW_OK || a.batch * a.heads * a.n == 0) return 0;
-    if (few_rows(a, d->dtype, mask_mode(&own))) {
+    if (few_rows(a, c, d->dtype, mask_mode(&own))) {
         plan_rows(a, c, cd->bits, d->dtype);
         return parts_bytes(a);
     }
@@ -103,7 +104,7 @@ extern "C" int tpw_cache_attention(const tpw_attention_desc *d, const tpw_cache_
     TPW_REQUIRE(mode == kNoMask || a.mask, "attention: null mask");
     hipStream_t s = as_stream(stream);
     size_t prepared = 0;
-    const bool few = few_rows(a, d->dtype, mode);
+    const bool few = few_rows(a, c, d->dtype, mode);
     if (few) {
         if (mode == kNoMask) a.mask = nullptr;
         plan_rows(a, c, cd->bits, d->dtype);
