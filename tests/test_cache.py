@@ -855,6 +855,36 @@ def test_c_entry_over_tables_without_pages(dtype, n, mask_type):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("n", [1, 12, 100])
+def test_c_entry_with_fewer_features_than_the_cache(dtype, bits, n):
+    """Blocks behind the features of a call are no part of it, whatever they hold."""
+    h, hk, m, d = 4, 2, 48, 30
+    cpu, cache = filled(1, hk, m, 100, 70, bits, "cuda")
+    cache[1][:, :, 1:] = 255
+    cache[3][:, :, 1:] = 255
+    q = rows(1, h, n, d, 1, dtype).cuda()
+    out = torch.full_like(q, 7.0)
+    a = capi.AttentionDesc(dtype=capi.TPW_F32 if dtype == F32 else capi.TPW_BF16, batch=1, heads=h, key_heads=hk, n=n, m=m,
+                           d=d, dv=d, scale=1.0, query=q.data_ptr(), out=out.data_ptr())
+    a.query_strides[:] = a.out_strides[:] = q.stride()[:3]
+    c = c_cache(bits=bits, heads=hk, rows=m, key_blocks=4, value_blocks=3, **{
+        f"{side}_{what}": cache[2 * k + i].data_ptr()
+        for k, side in enumerate(("key", "value")) for i, what in enumerate(("codes", "scales"))})
+    for k, side in enumerate(("key", "value")):
+        getattr(c, side + "_code_strides")[:] = cache[2 * k].stride()[:3]
+        getattr(c, side + "_scale_strides")[:] = cache[2 * k + 1].stride()[:3]
+    size = capi.lib().tpw_cache_attention_workspace_size(C.byref(a), C.byref(c))
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    capi.call("tpw_cache_attention", C.byref(a), C.byref(c), ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    k, there = ref.whole(cpu[0], cpu[1], bits, d)
+    v, _ = ref.whole(cpu[2], cpu[3], bits, d)
+    o, tol = ref.reference(q.cpu(), k, v, there, scale=1.0)
+    assert_close(out, o, rtol=0.0, atol=tol + TINY)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n,m", [(1, 8208), (1, 40912), (5, 24704), (20, 24704), (40, 24704)])
 @pytest.mark.parametrize("d", [64, 160])
 def test_one_head_over_a_long_cache(dtype, n, m, d):

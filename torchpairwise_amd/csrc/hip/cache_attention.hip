@@ -19,6 +19,9 @@ int read_call(const tpw_attention_desc *d, const tpw_cache_desc *cd, tpw_attenti
     TPW_REQUIRE(d->key_heads == cd->heads, "attention: key_heads differ from the cache's heads");
     TPW_REQUIRE(d->m == (cd->pages ? cd->page_count * cd->rows : cd->rows), "attention: m differs from the cache's rows");
     TPW_REQUIRE(d->d <= 32 * cd->key_blocks && d->dv <= 32 * cd->value_blocks, "attention: rows are wider than the cache's");
+    // blocks behind the call's features are not read: a NaN of theirs would spoil the scores
+    c.k.blocks = (int)cdiv(d->d, 32);
+    c.v.blocks = (int)cdiv(d->dv, 32);
     a.cached = 1;
     a.dwords = 0;
     const int64_t size = d->dtype == TPW_F32 ? 4 : 2;
