@@ -165,3 +165,40 @@ def test_masks_over_pages_of_16(dtype, bits, d, n):
             for causal in (False, True):
                 attend("cuda", rows(b, h, n, d, 1, dtype), first, hk, m, d, bits, mask, causal,
                        lengths=torch.tensor([m - 5, m]), pages=pages, spoil=True, what=f"{m} {what} {causal}")
+
+
+# ---------------------------------------------------------------- the borders of the scale
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bits,border", [(4, 7.0), (8, 464.0)])
+def test_the_power_that_a_border_takes(device, dtype, bits, border):
+    """The first power 2^e with which the largest magnitude is below the border."""
+    below = torch.tensor(border, dtype=dtype)
+    below = (below * (1 - torch.finfo(dtype).eps / 2)).float().item()
+    assert below < border
+    x = torch.zeros(1, 1, 16, 32, dtype=dtype)
+    for i, (top, e) in enumerate(((border, -3), (border, 0), (border, 60), (below, -3), (below, 0), (below, 60))):
+        x[0, 0, i, i] = -top * 2.0 ** e
+        x[0, 0, i, 31] = 2.0 ** (e - 9)  # the smallest of 8 bits with the smaller power, half of it with the larger
+    cache = tp.quantized_cache(1, 1, 16, 32, bits=bits, device=device)
+    tp.cache_write_(*cache, x.to(device), x.to(device), torch.zeros(1, dtype=torch.long, device=device))
+    assert cache[1][0, 0, 0, :6].tolist() == [125, 128, 188, 124, 127, 187]
+    got = tp.cache_read(*cache, dtype=F32)[0].cpu()[0, 0, :, 31]
+    assert got[:3].eq(0).all()
+    assert (got[3:6] == (torch.tensor([2.0 ** -12, 2.0 ** -9, 2.0 ** 51]) if bits == 8 else 0.0)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bits,first", [(4, 3.5 * 2.0 ** 126), (8, 1.9375 * 2.0 ** 127)])
+def test_magnitudes_that_round_past_float32(device, dtype, bits, first):
+    """From `first` on finite magnitudes round to 2^128; the one before stays finite."""
+    before = torch.tensor(first * (1 - torch.finfo(dtype).eps / 2), dtype=torch.float64).to(dtype)
+    assert before.double() < first
+    x = torch.zeros(1, 1, 16, 32, dtype=dtype)
+    x[0, 0, 0, 0], x[0, 0, 1, 0], x[0, 0, 2, 0] = first, -torch.finfo(dtype).max, before
+    cache = tp.quantized_cache(1, 1, 16, 32, bits=bits, device=device)
+    tp.cache_write_(*cache, x.to(device), x.to(device), torch.zeros(1, dtype=torch.long, device=device))
+    for y in (*tp.cache_read(*cache, dtype=F32), *tp.cache_read(*cache)):
+        assert y[0, 0, 0, 0] == math.inf and y[0, 0, 1, 0] == -math.inf and y[0, 0, 2, 0].isfinite()
+        assert (y[..., 1:] == 0).all()

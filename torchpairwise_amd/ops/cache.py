@@ -16,9 +16,11 @@ def quantized_cache(batch: int, heads: int, rows: int, width: int, value_width: 
     ``rows`` rows.  ``rows`` is a multiple of 16 (of pages: a power of two); ``width`` and ``value_width``
     (None: the same) are 1 to 256 features.
 
-    Every 32 features of a row share a power of two, the first with which the largest magnitude does not
-    round past the last code; ``bits=4`` keeps values of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign (uint8 codes, two
-    a byte, the even feature in the low half), ``bits=8`` float8_e4m3fn.  A feature takes ``bits + 0.25`` bits.
+    Every 32 features of a row share a power of two 2^e, the first with which the largest magnitude is below
+    7 * 2^e (``bits=4``) or 464 * 2^e (``bits=8``): halfway past the last code.  ``bits=4`` keeps values of 0, 0.5,
+    1, 1.5, 2, 3, 4, 6 and a sign (uint8 codes, two a byte, the even feature in the low half), ``bits=8``
+    float8_e4m3fn, rounded to nearest, ties to even; magnitudes that round to 2^128 (from 3.5 * 2^126 on, in 8 bits
+    1.9375 * 2^127) read back as infinite.  A feature takes ``bits + 0.25`` bits.
     Codes are ``[batch, heads, rows, bytes of whole blocks]``, scales (exponent + 127; 255: the block is NaN)
     ``[batch, heads, blocks, rows]``; any view of them with strides in multiples of 16 will do.
     """
