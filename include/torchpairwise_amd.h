@@ -816,9 +816,10 @@ typedef struct tpw_attention_desc {
     int64_t mask_strides[4];
 } tpw_attention_desc;
 
-/* The sizes of workspaces (here and of the cache below) follow from the types, the sizes, the strides, whether there is an
- * out_rest, and how the operands' addresses are aligned: a null one counts as 16-byte aligned, so that they can be asked
- * for before there are any.  Operands that do not lie in 16-byte pieces are copied into the workspace. */
+/* The sizes of workspaces (here and of the cache below) follow from the types, the sizes, the strides, whether
+ * there is an out_rest, and how the operands' addresses are aligned: a null one counts as 16-byte aligned, so
+ * that they can be asked for before there are any.  Operands that do not lie in 16-byte pieces are copied into
+ * the workspace. */
 size_t tpw_attention_workspace_size(const tpw_attention_desc *desc);
 int tpw_attention(const tpw_attention_desc *desc, void *workspace, void *stream);
 /* grad_query, grad_key and grad_value (every element is written) for an upstream grad_out. */
@@ -834,9 +835,10 @@ int tpw_attention_backward(const tpw_attention_desc *desc, void *workspace, void
  * 1.9375 2^127) read back as infinite.
  * codes [first, heads, rows, blocks] of 16 (32) bytes, the bytes of a row dense; scales [first, heads, blocks,
  * rows], rows dense.  Strides are in bytes, of [first, heads, rows] and [first, heads, blocks]; they and the
- * addresses are multiples of 16, and so is rows; those of rows and of blocks are not negative.  Without a table of
- * pages first is the batch and rows what each sequence has room for; with one (int32, or int64 where pages_wide), row j of sequence b is row j % rows
- * of page pages[b * page_pitch + j / rows], rows being a power of two.  Entries outside [0, first) stand for no
+ * addresses are multiples of 16, and so is rows; those of rows and of blocks are not negative.  Without a table
+ * of pages first is the batch and rows what each sequence has room for; with one (int32, or int64 where
+ * pages_wide), row j of sequence b is row j % rows of page pages[b * page_pitch + j / rows], rows being a power
+ * of two.  Entries outside [0, first) stand for no
  * page: their rows are not written, read as zeros, and are no keys. */
 typedef struct tpw_cache_desc {
     int32_t bits; /* 4 or 8 */

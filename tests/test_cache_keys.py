@@ -142,21 +142,24 @@ def test_every_bit_of_a_float32_probability_counts(device, bits, d, n):
     assert_close(out, o, rtol=0.0, atol=tol)
 
 
-# ---------------------------------------------------------------- masks over pages of 16 rows
+# ---------------------------------------------------------------- masks, over pages of 16 rows too
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("d", [50, 128, 224])
-@pytest.mark.parametrize("n", [1, 3, 8, 10, 16])
-def test_masks_over_pages_of_16(dtype, bits, d, n):
-    """Two heads a key head, short caches and long ones, a sequence with holes, lengths that end inside a page."""
+@pytest.mark.parametrize("n", [1, 3, 8, 10, 16, 40])
+@pytest.mark.parametrize("paged", [True, False])
+def test_masks_by_widths_and_pages(dtype, bits, d, n, paged):
+    """Two heads a key head, short caches and long ones, a sequence with holes, lengths that end inside a page; and
+    the same rows in one piece."""
     b, h, hk = 2, 4, 2
     for m in (48, 240, 1104):
-        first = b * (m // 16) + 1
-        pages = torch.randperm(first, generator=gen(m))[:b * (m // 16)].view(b, -1).int()
-        pages[1, ::3] = -1
-        pages[1, 1] = first
-        g = gen(m + n)
+        first, pages, g = b, None, gen(m + n)
+        if paged:
+            first = b * (m // 16) + 1
+            pages = torch.randperm(first, generator=gen(m))[:b * (m // 16)].view(b, -1).int()
+            pages[1, ::3] = -1
+            pages[1, 1] = first
         keep = torch.rand(b, h, n, m, generator=g) < 0.5
         keep[0, 0, 0] = False
         bias = torch.randn(b, h, n, m, generator=g)

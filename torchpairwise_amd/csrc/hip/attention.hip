@@ -85,15 +85,16 @@ __global__ __launch_bounds__(64 * kWaves, OCC) void attention_kernel(const Args 
     F::CR::each(f.o, lane, [&](int at, f32x4 v) { out.store(at, v * inv); });
 }
 
-// Joins the parts of every row: m = max m_s, l = sum l_s 2^(m_s - m), o = sum o_s 2^(m_s - m) / l.
-// One block per row: lane s of every wave holds part s's weight; then LANES lanes of four features
-// each, 256 / LANES parts at a time, in an order that the sizes fix.
-// Row r's entry, head and row.  Rows are below 2^31: divisions in 64 bits would be a third of the kernel's time.
+// Row r's entry, head and row.  Rows are below 2^31: divisions in 64 bits would be a third of the joining kernels' time.
 template <typename T>
 __device__ __forceinline__ OutRow<T> joined_row(const Args &a, uint32_t r) {
     const uint32_t n = (uint32_t)a.n, i = r % n, bh = r / n;
     return OutRow<T>(a, bh / (uint32_t)a.heads, bh % (uint32_t)a.heads, i);
 }
+
+// Joins the parts of every row: m = max m_s, l = sum l_s 2^(m_s - m), o = sum o_s 2^(m_s - m) / l.
+// One block per row: lane s of every wave holds part s's weight; then LANES lanes of four features
+// each, 256 / LANES parts at a time, in an order that the sizes fix.
 template <typename T, bool BIAS, int LANES>
 __global__ __launch_bounds__(256) void attention_join_kernel(const Args a) {
     constexpr int G = 256 / LANES, U = kMaxParts / G < 8 ? kMaxParts / G : 8;

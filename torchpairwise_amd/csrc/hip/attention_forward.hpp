@@ -1,5 +1,5 @@
 // The forward's work on one tile of keys, shared by the kernels that bring tiles of keys and values into LDS
-// (attention.hip: by DMA; cache_attention.hpp: out of a cache in 4 or 8 bits), and their launch's plan.
+// (attention.hip: by DMA; cache_tiles.hpp: out of a cache in 4 or 8 bits), and their launch's plan.
 #pragma once
 
 #include "attention.hpp"

@@ -20,10 +20,11 @@ struct RowsArgs {
     uint32_t heads, tiles;   // blocks of 256 threads per (sequence, head), those of the wider side
 };
 
-// A block's share: a thread works on PIECE features (a piece) of ROWS rows, consecutive ones (whose scales lie side by
-// side: one word) or spread over the block; 4 (8) consecutive lanes share a block of 32 features.  What the call does not have is read from
-// somewhere that exists and dropped: without branches between them all of a thread's loads are in flight at once.
-// The narrower side has more rows to a block, and none for the last ones: those return at once.
+// A block's share: a thread works on PIECE features (a piece) of ROWS rows, consecutive ones (whose scales lie
+// side by side: one word) or spread over the block; 4 (8) consecutive lanes share a block of 32 features.  What
+// the call does not have is read from somewhere that exists and dropped: without branches between them all of a
+// thread's loads are in flight at once.  The narrower side has more rows to a block, and none for the last ones:
+// those return at once.
 template <int ROWS, bool PAGED, int PIECE, bool SPREAD>
 struct Share {
     static constexpr int kPieces = 32 / PIECE;  // of a block of 32 features

@@ -170,7 +170,10 @@ struct Rows {
         return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x124, 0xf, 0xf, true));  // row_ror:4
     }
 
-    // Rows 0 .. n - 1 from a place on: buffers whose range ends with the last of them.
+    // Rows 0 .. n - 1 from a place on: buffers whose range ends with the last of them.  The hardware counts a load's
+    // scalar offset into the range without wrapping round (ranges of 0 to 4096 bytes, offsets of 0 to 8192: read is
+    // exactly what ends inside), so rows from n on are neither read nor paid for, and no row where n is 0.  Were it
+    // left out of the check, a load would reach at most the last row of its 8, which is there: rows come in 16s.
     struct Buffers {
         __amdgpu_buffer_rsrc_t codes, scales;
     };
@@ -356,7 +359,8 @@ struct Rows {
                             : __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale, -b0));
                 sum[r] += x[e];
             }
-            // bfloat16 queries: probabilities rounded to bfloat16 (within 2^-9 of each), their sum is not
+            // bfloat16 queries: probabilities rounded to bfloat16 (within 2^-8 of each, as the dense form's are
+            // and as the output is), their sum is not
             if constexpr (PACK)
                 split_own(x, i, pr[r][0]);
             else if constexpr (NP == 1)
