@@ -142,6 +142,27 @@ def test_every_bit_of_a_float32_probability_counts(device, bits, d, n):
     assert_close(out, o, rtol=0.0, atol=tol)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("n", [x for x in ROWS if x <= 16])
+def test_few_bfloat16_rows_are_rounded_once(device, bits, d, n):
+    """The same of bfloat16: probabilities are off by 2^-17 (two summands), and the output is rounded, half a step."""
+    cache = two_keys(bits, d, d, [1.0], device)
+    t = torch.rand(1, 32, n, generator=gen(n + 70)).to(BF16)
+    q = torch.zeros(1, 32, n, d, dtype=BF16)
+    q.scatter_(3, torch.randint(0, d, (1, 32, n, 1), generator=gen(n)), -t[..., None])
+    out = torch.cat([tp.cache_attention(q[:, h:h + 1].to(device), *cache, scale=1.0, lengths=torch.tensor([2], device=device))
+                     for h in range(32)], 1)
+    o, tol = (x[..., None].expand(1, 32, n, d) for x in share(-t.double()))
+    tol = tol + 2.0 ** -17 * o + torch.ldexp(torch.ones_like(o), torch.frexp(o)[1] - 9)  # half a step of o's binade
+    # one summand would be seen: rounded twice
+    p = torch.exp(-t.double())
+    once = (p.to(BF16).double() / (1 + p)).to(BF16).double()[..., None]
+    assert n < 3 or ((once - o[..., :1]).abs() > tol[..., :1]).any()
+    assert_close(out, o, rtol=0.0, atol=tol)
+
+
 # ---------------------------------------------------------------- masks, over pages of 16 rows too
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -148,7 +148,16 @@ __device__ __forceinline__ void split3(float (&x)[8], Frag<uint16_t> (&f)[3]) {
         f[p].v = make_uint4(high2(w[0], w[1]), high2(w[2], w[3]), high2(w[4], w[5]), high2(w[6], w[7]));
     }
 }
-// The same where an infinity may be among them: its first summand alone.
+// As two: rounded, and what that left, rounded.
+__device__ __forceinline__ void split2(float (&x)[8], Frag<uint16_t> (&f)[2]) {
+    f[0] = pack8(x, uint16_t{});
+    float y[8];
+    unpack8(f[0], y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] -= y[e];
+    f[1] = pack8(x, uint16_t{});
+}
+// As three, where an infinity may be among them: its first summand alone.
 __device__ __forceinline__ void split3_any(float (&x)[8], Frag<uint16_t> (&f)[3]) {
     uint32_t inf[8];
 #pragma unroll

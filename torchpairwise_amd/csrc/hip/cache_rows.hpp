@@ -33,13 +33,20 @@ struct Codes {
     uint32_t m[RT][MM == kBias ? 8 : MM == kKeep ? 2 : 1];  // the mask's values for the lane's eight keys
 };
 
-// NP: summands in bfloat16 of a query and a probability (float32: three).  PACK: at most 4 rows, whose summands
-// take 4 columns of a product each: one product for all three, where 16 rows take three (float32, 8 x 16 (4) heads
-// over 16000 of 90: 19.3 -> 16.9 us).
+// NP: summands in bfloat16 of a query and a probability (float32: three).  Up to 16 rows of bfloat16 have two summands of
+// a probability (within 2^-17 of it), so that the output's rounding is the only one to count: single tokens over 8192 to
+// 32768 are off by 1.6e-3 of their norm, where one summand makes it 2.3e-3, for 1 to 5 % of the time (16 x 16 (2) heads
+// over 32768 of 128 28.7 -> 29.3 us, 16 x 32 (8) over 8192 in 8 bits 47.6 -> 48.1; 16 x 8 x 4 rows over 8192 of 64 21.9
+// -> 23.0).  17 to 32 rows, and many
+// (attention_forward.hpp), have one (within 2^-8, as the output's rounding is): two would cost 4 to 16 % (16 x 8 heads
+// over 4096: 32 rows of 128 25.5 -> 27.8 us, of 256 in 8 bits 85 -> 99), in tiles 20 to 31 (8192^2 causal 603 -> 791).
+// PACK: at most 4 rows, whose summands take 4 columns of a product each: one product for all three, where 16 rows take
+// three (float32, 8 x 16 (4) heads over 16000 of 90: 19.3 -> 16.9 us).
 template <int BITS, int NB, int NP, int RT, int MM, bool HALVES, bool PACK, int WAVES>
 struct Rows {
     static_assert(!PACK || (NP == 3 && RT == 1), "three summands of 4 rows");
-    static constexpr int NM = PACK ? 1 : NP;  // products for a tile of 16 rows
+    static constexpr int NM = PACK ? 1 : NP;  // products for a tile of 16 rows: of the scores,
+    static constexpr int NV = PACK ? 1 : NP == 1 && RT == 1 ? 2 : NP;  // of the values
     using C = Codes<BITS, NB, RT, MM>;
     static constexpr bool BIAS = MM == kBias;
     using T = std::conditional_t<NP == 1, uint16_t, float>;
@@ -325,7 +332,7 @@ struct Rows {
                                                                           s[t][r], 0, 0, 0);
             }
         }
-        Frag<uint16_t> pr[RT][NM];
+        Frag<uint16_t> pr[RT][NV];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             float x[8];
@@ -359,12 +366,12 @@ struct Rows {
                             : __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale, -b0));
                 sum[r] += x[e];
             }
-            // bfloat16 queries: probabilities rounded to bfloat16 (within 2^-8 of each, as the dense form's are
-            // and as the output is), their sum is not
             if constexpr (PACK)
                 split_own(x, i, pr[r][0]);
-            else if constexpr (NP == 1)
+            else if constexpr (NV == 1)
                 pr[r][0] = pack8(x, uint16_t{});
+            else if constexpr (NV == 2)
+                split2(x, pr[r]);
             else
                 split3(x, pr[r]);
         }
@@ -378,13 +385,13 @@ struct Rows {
     static constexpr float kSlack = BIAS ? 5.0f : 8.0f;
 
     template <int... P>
-    __device__ __forceinline__ void values(const C &w, const float (&scale)[8], const Frag<uint16_t> (&pr)[RT][NM],
+    __device__ __forceinline__ void values(const C &w, const float (&scale)[8], const Frag<uint16_t> (&pr)[RT][NV],
                                            std::integer_sequence<int, P...>) {
         (pair<P>(w, scale, pr), ...);
     }
     // Features 2 P and 2 P + 1 of the lane's.
     template <int P>
-    __device__ __forceinline__ void pair(const C &w, const float (&scale)[8], const Frag<uint16_t> (&pr)[RT][NM]) {
+    __device__ __forceinline__ void pair(const C &w, const float (&scale)[8], const Frag<uint16_t> (&pr)[RT][NV]) {
         constexpr int kWord = BITS == 4 ? P / 4 : P / 2, kPart = BITS == 4 ? P % 4 : P % 2;
         uint32_t x[8];
 #pragma unroll
@@ -398,7 +405,7 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int p = NM - 1; p >= 0; --p) {
+            for (int p = NV - 1; p >= 0; --p) {
                 const bf16x8 f = __builtin_bit_cast(bf16x8, pr[r][p].v);
                 o[r][2 * P] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                     __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3])), f, o[r][2 * P], 0, 0, 0);
