@@ -832,7 +832,7 @@ int tpw_attention_backward(const tpw_attention_desc *desc, void *workspace, void
  * two features a byte, the even one in the low half; 8 bits: sign, 4, 3 (float8 e4m3, largest 448).  Writing
  * takes the first e >= -127 with max |x| < 7 2^e (464 2^e), then rounds x / 2^e to nearest, ties to even;
  * a block that holds NaN or an infinity becomes NaN.  Magnitudes that round to 2^128 (from 3.5 2^126 on, in 8 bits
- * 1.9375 2^127) read back as infinite.
+ * 1.9375 2^127) read back as infinite, and attention makes infinities or NaN of them.
  * codes [first, heads, rows, blocks] of 16 (32) bytes, the bytes of a row dense; scales [first, heads, blocks,
  * rows], rows dense.  Strides are in bytes, of [first, heads, rows] and [first, heads, blocks]; they and the
  * addresses are multiples of 16, and so is rows; those of rows and of blocks are not negative.  Without a table

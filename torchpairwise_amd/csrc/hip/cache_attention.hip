@@ -46,7 +46,8 @@ size_t parts_bytes(const Args &a) {
 // of many chunks of 32 keys, so a second round costs more than long parts do.  Short caches are left whole, by blocks
 // of twice the waves, where a SIMD's chunks in turn are no more than those of a part and two: what the second launch
 // and the parts' way through memory take (4 bits, 128 features, 16 x 8 heads: 256 keys 7.2 -> 5.7 us, 512 8.5 -> 7.4,
-// 1024 11.6 -> 9.6, where 1664 stay at 13; one sequence: 256 keys 7.0 -> 5.6).
+// 1024 11.6 -> 9.6, where 1664 stay at 13; one sequence: 256 keys 7.0 -> 5.6; both with one summand of a probability,
+// with two the whole ones take 5.8, 7.6, 10.1 and 5.6).
 void plan_rows(Args &a, const cache::Cache &c, int bits, int dtype) {
     const int nb = row_blocks(c.k.blocks > c.v.blocks ? c.k.blocks : c.v.blocks);
     const int64_t rows = a.n * a.group;

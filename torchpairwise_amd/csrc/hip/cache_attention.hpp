@@ -20,8 +20,9 @@ constexpr int64_t kGroupedRows = 64;
 constexpr bool in_groups(int nb, int np, bool pack) { return nb == 8 && np > 1 && !pack; }
 constexpr int kRowWaves = 4;        // waves of a block that does one of several parts
 constexpr int kWholeWaves = 8;      // .. that works alone on a sequence and head
-// Blocks that share a CU, as their registers leave (NP: summands of a probability, RT: 16 rows each).  Four of
-// 64 features would fit, and were slower where they fill the card (1664 keys of 16 x 8 heads 10.8 -> 11.8 us).
+// Blocks that share a CU, as their registers leave (NP: summands of a query, RT: 16 rows each).  Four of 64
+// features would fit, and were slower where they fill the card (1664 keys of 16 x 8 heads 10.8 -> 11.8 us, with one
+// summand of a probability; three with two of them: 11.4).
 constexpr int rows_per_cu(int bits, int nb, int np, int rt) {
     if (np > 1 || rt > 1) return nb == 8 || (np > 1 && rt > 1) ? 1 : 2;
     return nb == 8 ? (bits == 4 ? 2 : 1) : bits == 4 ? 3 : 2;

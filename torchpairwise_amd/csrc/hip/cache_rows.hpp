@@ -418,8 +418,8 @@ struct Rows {
 // One block: the rows of a (sequence, key head), over the keys of one part; its waves take 32 keys in turn and
 // are joined at the end, in an order that the sizes fix.  Long caches are bound by memory: 16 x 32 (8) heads over
 // 8192 of 128 in 8 bits, 230 MB, 37 us one after the other (a call whose cache is in no level of cache: 47.7); in
-// 4 bits, 16 x 16 (2) over 32768, lengths from a half up, 24 us for 114 MB (4.7 TB/s), where some 200 vector
-// instructions a step (a third of them conversions) keep the SIMDs busy two thirds of the time.  Short ones by what a
+// 4 bits, 16 x 16 (2) over 32768, lengths from a half up, 23 to 25 us for 114 MB (4.5 to 4.9 TB/s), where some 240 vector
+// instructions a step (a third of them conversions) take 0.36 of the SIMDs' cycles.  Short ones by what a
 // block does once: 208 blocks of one step a wave take 5.8 us, an empty kernel with these arguments 2.9.
 template <int BITS, int NB, int NP, int RT, int MM, bool HALVES, bool PACK, int WAVES, int DEPTH, int OCC>
 __global__ __launch_bounds__(64 * WAVES, OCC) void cache_rows_kernel(const Args a, const Cache c) {
