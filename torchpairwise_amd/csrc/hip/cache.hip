@@ -339,8 +339,8 @@ int read_cache(const tpw_cache_desc *d, int64_t batch, Cache &c) {
         s.sh = d->heads == 1 ? 0 : ss[1];
         s.sb = blocks == 1 ? 0 : ss[2];
         c.near = c.near && s.cr <= (int64_t(1) << 23) && s.sb <= (int64_t(1) << 28);
-        return s.cr >= 0 && s.sb >= 0 && aligned16(codes) && aligned16(scales) && (s.cf | s.ch | s.cr | s.sf | s.sh | s.sb) % 16 == 0 &&
-               (m * d->first == 0 || (codes && scales));
+        return s.cr >= 0 && s.sb >= 0 && aligned16(codes) && aligned16(scales) &&
+               (s.cf | s.ch | s.cr | s.sf | s.sh | s.sb) % 16 == 0 && (m * d->first == 0 || (codes && scales));
     };
     TPW_REQUIRE(side(c.k, d->key_codes, d->key_scales, d->key_code_strides, d->key_scale_strides, d->key_blocks) &&
                     side(c.v, d->value_codes, d->value_scales, d->value_code_strides, d->value_scale_strides,

@@ -4,13 +4,13 @@
 // A block of 32 features of a row shares a power of two 2^e, the first, from e = -127 on, with which the block's
 // largest magnitude a is less than halfway from the last code to the one that would follow it:
 //   4 bits: sign, 2 exponent and 1 mantissa bit, 0 .5 1 1.5 2 3 4 6;  a < 7 2^e
-//   8 bits: sign, 4 and 3, largest 448;  a < 464 2^e  (464 itself would round to 448, as ties do: it takes the next power)
+//   8 bits: sign, 4 and 3, largest 448;  a < 464 2^e  (464, a tie, would still round to 448: it takes the next power)
 // so no value rounds past the last code, and each is off by at most half a step of its own binade, or of the block's
 // smallest codes.  x / 2^e is exact, its rounding (to nearest, ties to even) the only one: the codes are the same on
-// every machine.  (Magnitudes from 3.5 2^126, in 8 bits 1.9375 2^127 on round to 2^128, which float32 reads as infinity.)  The scale is kept as the
-// byte e + 127, whose place in a float's bits is its exponent: gfx950's conversions (v_cvt_scalef32_*) take
-// that float, read 0 as 2^-127 and 255 as NaN, whatever the code.  A block that holds NaN or an infinity
-// has scale 255 and codes of zero.
+// every machine.  (Magnitudes from 3.5 2^126, in 8 bits 1.9375 2^127 on round to 2^128, which float32 reads as
+// infinity.)  The scale is kept as the byte e + 127, whose place in a float's bits is its exponent: gfx950's
+// conversions (v_cvt_scalef32_*) take that float, read 0 as 2^-127 and 255 as NaN, whatever the code.  A block that
+// holds NaN or an infinity has scale 255 and codes of zero.
 // Every value is exact in bfloat16 (2 or 4 significant bits).
 //
 // Codes: [batch | pages, heads, rows, blocks] of 16 bytes (two features a byte, the even one low) or 32.

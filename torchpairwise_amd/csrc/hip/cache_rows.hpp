@@ -37,9 +37,9 @@ struct Codes {
 // a probability (within 2^-17 of it), so that the output's rounding is the only one to count: single tokens over 8192 to
 // 32768 are off by 1.6e-3 of their norm, where one summand makes it 2.3e-3, for 1 to 5 % of the time (16 x 16 (2) heads
 // over 32768 of 128 28.7 -> 29.3 us, 16 x 32 (8) over 8192 in 8 bits 47.6 -> 48.1; 16 x 8 x 4 rows over 8192 of 64 21.9
-// -> 23.0).  17 to 32 rows, and many
-// (attention_forward.hpp), have one (within 2^-8, as the output's rounding is): two would cost 4 to 16 % (16 x 8 heads
-// over 4096: 32 rows of 128 25.5 -> 27.8 us, of 256 in 8 bits 85 -> 99), in tiles 20 to 31 (8192^2 causal 603 -> 791).
+// -> 23.0).  17 to 32 rows, and many (attention_forward.hpp), have one (within 2^-8, as the output's rounding is): two
+// would cost 4 to 16 % (16 x 8 heads over 4096: 32 rows of 128 25.5 -> 27.8 us, of 256 in 8 bits 85 -> 99), in tiles 20
+// to 31 (8192^2 causal 603 -> 791).
 // PACK: at most 4 rows, whose summands take 4 columns of a product each: one product for all three, where 16 rows take
 // three (float32, 8 x 16 (4) heads over 16000 of 90: 19.3 -> 16.9 us).
 template <int BITS, int NB, int NP, int RT, int MM, bool HALVES, bool PACK, int WAVES>

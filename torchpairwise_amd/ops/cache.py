@@ -20,7 +20,8 @@ def quantized_cache(batch: int, heads: int, rows: int, width: int, value_width: 
     7 * 2^e (``bits=4``) or 464 * 2^e (``bits=8``): halfway past the last code.  ``bits=4`` keeps values of 0, 0.5,
     1, 1.5, 2, 3, 4, 6 and a sign (uint8 codes, two a byte, the even feature in the low half), ``bits=8``
     float8_e4m3fn, rounded to nearest, ties to even; magnitudes that round to 2^128 (from 3.5 * 2^126 on, in 8 bits
-    1.9375 * 2^127) read back as infinite, and attention makes infinities or NaN of them.  A feature takes ``bits + 0.25`` bits.
+    1.9375 * 2^127) read back as infinite, and attention makes infinities or NaN of them.  A feature takes
+    ``bits + 0.25`` bits.
     Codes are ``[batch, heads, rows, bytes of whole blocks]``, scales (exponent + 127; 255: the block is NaN)
     ``[batch, heads, blocks, rows]``; any view of them with strides in multiples of 16 will do.
     """
